@@ -153,7 +153,8 @@ int qlin_workspace_query(const qlin_workspace* ws, qlin_workspace_info* out);
 
 /* Sticky error word of asynchronous runs on this workspace: returns QLIN_OK or
  * QLIN_ERR_NONFINITE if any activation row seen since the last clear held Inf/NaN.
- * Synchronizes the workspace's last stream.  clear != 0 resets it. */
+ * Synchronizes the workspace's last stream.  clear != 0 resets it.  QLIN_ERR_PARAM: a key/value cache
+ * call found row starts, lengths or pages outside its batch's limits (see qlin_kv_batch). */
 int qlin_workspace_status(qlin_workspace* ws, int32_t clear);
 
 /* ---- host-buffer runs: the drop-in for the reference's synchronous calls ----
@@ -348,6 +349,96 @@ int qlin_chain_stage_output(const qlin_chain* chain, int32_t stage, void** ptr, 
  * Synchronizes the last run's stream.  clear != 0 resets the word.  A run that gave up
  * leaves no state behind: the next run is correct without any reset. */
 int qlin_chain_status(qlin_chain* chain, int32_t clear);
+
+/* ---- key/value cache in 8 bits, and attention over it ----
+ * The reference keeps its keys and values in FP16 and runs attention as a unit of the native
+ * library (src/npu/attention.rs); these calls keep a decoder layer on the device between its qkv
+ * and o projections.  Keys and values are quantized by the per-token rule of the activations, one scale per
+ * token and KV head:
+ *   s = max(absmax_d |x[d]| / 127, 2^-64),  code[d] = clamp(round(x[d] * (1/s)), -127, 127)
+ * A row with Inf or NaN gets the scale NaN (whoever reads it gets NaN) and sets
+ * QLIN_ERR_NONFINITE in the workspace's error word.
+ *
+ * Tokens lie in pages of page_tokens; a sequence's tokens p .. p + page_tokens - 1 are the page named
+ * by column p / page_tokens of its row of the page table.  Who owns which page is the caller's
+ * business: pages may be shared by sequences for reading, but no two rows of one append may be the
+ * same slot.
+ *
+ * The workspace of these calls gives its error word and its scratch for partial results (64 MiB; its
+ * max_rows, max_k and max_n set no limit here).  They allocate nothing and can be captured into a graph: the
+ * arrays of a batch are read when the kernels run, so lengths and tables may change between
+ * replays within max_new and max_len.  Cache and workspace belong to the device that is current when
+ * they are created, which has to be the current one in every call. */
+typedef struct qlin_kv_cache qlin_kv_cache;
+
+typedef struct qlin_kv_config {
+    int32_t kv_heads;    /* 1..1024 */
+    int32_t head_dim;    /* 1..256; stored as 64, 128 or 256 columns */
+    int32_t page_tokens; /* a power of two, 16..4096 */
+    int32_t pages;
+} qlin_kv_config;
+
+typedef struct qlin_kv_info {
+    int32_t kv_heads, head_dim, page_tokens, pages;
+    int32_t head_dim_padded; /* columns stored per row */
+    int32_t device;
+    uint64_t device_bytes; /* codes and scales of keys and values */
+} qlin_kv_info;
+
+/* New rows of some sequences.  Rows row_start[i] .. row_start[i + 1] - 1 of the row tensors (none: an
+ * idle slot) are the last tokens of sequence i, whose length with them is length[i]: the t-th of n is token
+ * length[i] - n + t.  Rows at and behind row_start[seqs] belong to nobody and are left as they are.
+ * A row whose token is negative (n > length[i]) is not stored, reads as zeros and attends to nothing.
+ * What the device arrays hold is checked by the kernels: row starts that decrease or pass `rows`, more than
+ * max_new rows, a length below 0 or above max_len, or a page outside the cache set QLIN_ERR_PARAM in
+ * the workspace's error word; no such value is followed out of a buffer, a row on such a page is
+ * not stored and reads as NaN, and the other results of that sequence are unspecified. */
+typedef struct qlin_kv_batch {
+    int32_t seqs;    /* sequences, 1..2^20 */
+    int32_t rows;    /* rows of the row tensors, 0..2^24 */
+    int32_t max_new; /* at least the new rows of any sequence; at most rows */
+    int32_t max_len; /* at least the length of any sequence, up to 2^30; what the launch is cut by */
+    const int32_t* row_start;  /* device [seqs + 1], not decreasing */
+    const int32_t* length;     /* device [seqs] */
+    const int32_t* page_table; /* device [seqs, page_ld] */
+    int64_t page_ld;           /* at least ceil(max_len / page_tokens) */
+} qlin_kv_batch;
+
+/* Geometry outside the limits above: QLIN_ERR_UNSUPPORTED.  Rows never written read as zeros. */
+int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out);
+void qlin_kv_free(qlin_kv_cache* cache);
+int qlin_kv_query(const qlin_kv_cache* cache, qlin_kv_info* out);
+
+/* Quantizes the batch's new rows into their pages.  K: device [rows, ldk] of dtype, head h in columns
+ * h * head_dim .. h * head_dim + head_dim - 1 (e.g. the k columns of qkv rows), V likewise.
+ * flags: QLIN_ROUND_HALF_EVEN.  No row of K or V may lie in memory the cache owns. */
+int qlin_kv_append(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const void* K,
+                   int64_t ldk, const void* V, int64_t ldv, int32_t dtype, uint32_t flags, void* stream);
+
+/* Reads the same rows back: x[d] = code[d] * s, one f32 rounding, then dtype. */
+int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K,
+                 int64_t ldk, void* V, int64_t ldv, int32_t dtype, void* stream);
+
+/* Causal attention of the batch's new rows over their sequences' tokens, which the cache holds
+ * already (the rows' own among them): row t of n sees tokens 0 .. length[i] - n + t.
+ *   l[j] = scale * (Q . K[j]),  O = sum_j softmax(l)[j] * V[j];  a row that sees no token gives zeros
+ * Q: device [rows, ldq] of q_dtype, query head h in columns h * head_dim ..; q_heads is a multiple of
+ * kv_heads, and KV head h serves query heads h * q_heads / kv_heads ..  O: device [rows, ldo] of
+ * o_dtype; it must not overlap Q.  Sums and the softmax are held in f32.  With fp16 rows in and
+ * out, probabilities (scaled into fp16's range) are rounded to fp16 before they meet V; if either
+ * is f32, queries and probabilities are kept to 22 bits. */
+int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
+                      int32_t q_heads, const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,
+                      int32_t o_dtype, int64_t ldo, void* stream);
+
+/* The same for sequences that share their first prefix_tokens tokens (a multiple of page_tokens):
+ * their pages are taken from prefix_pages (device, prefix_tokens / page_tokens ids) and read once
+ * for all rows, and the tables' columns of the prefix are not read.  Lengths count the prefix; a
+ * sequence shorter than it sees its first tokens. */
+int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
+                             int32_t prefix_tokens, const int32_t* prefix_pages, int32_t q_heads,
+                             const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,
+                             int32_t o_dtype, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

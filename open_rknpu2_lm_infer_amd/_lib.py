@@ -79,6 +79,13 @@ SIGNATURES = {
     "qlin_run_noalloc": (ctypes.c_int, [_P, _I32, _P, _I32, _I64, _P, _F, _P, _I32, _I64, _U32, _P, _P]),
     "qlin_swiglu": (ctypes.c_int, [_I32, _I32, _P, _I32, _I64, _P, _I32, _I64, _P]),
     "qlin_run_plan": (ctypes.c_int, [_P, _P, _I32, _P, _I64, _P, _U32, _P]),
+    "qlin_kv_create": (ctypes.c_int, [_P, _P]),
+    "qlin_kv_free": (None, [_P]),
+    "qlin_kv_query": (ctypes.c_int, [_P, _P]),
+    "qlin_kv_append": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _I64, _I32, _U32, _P]),
+    "qlin_kv_read": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _I64, _I32, _P]),
+    "qlin_kv_attention": (ctypes.c_int, [_P, _P, _P, _I32, _P, _I32, _I64, _F, _P, _I32, _I64, _P]),
+    "qlin_kv_attention_prefix": (ctypes.c_int, [_P, _P, _P, _I32, _P, _I32, _P, _I32, _I64, _F, _P, _I32, _I64, _P]),
 }
 
 
@@ -110,6 +117,20 @@ class ChainStage(ctypes.Structure):
     _fields_ = [("weights", _P), ("flags", _U32), ("gamma", _P), ("eps", _F), ("input", _I32),
                 ("input_offset", _I32), ("residual", _I32), ("residual_offset", _I32),
                 ("residual_multiplier", _F)]
+
+
+class KVConfig(ctypes.Structure):
+    _fields_ = [("kv_heads", _I32), ("head_dim", _I32), ("page_tokens", _I32), ("pages", _I32)]
+
+
+class KVInfo(ctypes.Structure):
+    _fields_ = [("kv_heads", _I32), ("head_dim", _I32), ("page_tokens", _I32), ("pages", _I32),
+                ("head_dim_padded", _I32), ("device", _I32), ("device_bytes", ctypes.c_uint64)]
+
+
+class KVBatch(ctypes.Structure):
+    _fields_ = [("seqs", _I32), ("rows", _I32), ("max_new", _I32), ("max_len", _I32), ("row_start", _P),
+                ("length", _P), ("page_table", _P), ("page_ld", _I64)]
 
 
 class QlinError(RuntimeError):

@@ -374,6 +374,18 @@ bool gemv_ok(const qlin_workspace* ws, const qlin_weights* w, int rows) {
 
 }  // namespace
 
+namespace qlin {
+
+int workspace_device(const qlin_workspace* ws) { return ws->device; }
+
+WorkspaceParts workspace_begin(qlin_workspace* ws, hipStream_t stream) {
+    ws->last = stream;
+    ws->err_used = true;
+    return {ws->cu_count, reinterpret_cast<float*>(ws->gemm_part), ws->part_ints, ws->err};
+}
+
+}  // namespace qlin
+
 extern "C" {
 
 const char* qlin_strerror(int rc) {
@@ -628,7 +640,7 @@ int qlin_workspace_status(qlin_workspace* ws, int32_t clear) {
     if (hipStreamSynchronize(ws->last) != hipSuccess) return QLIN_ERR_DEVICE;
     if (hipMemcpy(&e, ws->err, sizeof(e), hipMemcpyDeviceToHost) != hipSuccess) return QLIN_ERR_DEVICE;
     if (clear && e && hipMemset(ws->err, 0, sizeof(uint32_t)) != hipSuccess) return QLIN_ERR_DEVICE;
-    return e ? QLIN_ERR_NONFINITE : QLIN_OK;
+    return e & kErrBatch ? QLIN_ERR_PARAM : e ? QLIN_ERR_NONFINITE : QLIN_OK;
 }
 
 int qlin_quantize(int32_t rows, int32_t K, const void* A, int32_t a_dtype, int64_t lda, const float* gamma,

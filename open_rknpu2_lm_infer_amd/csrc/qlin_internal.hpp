@@ -127,6 +127,23 @@ __device__ __forceinline__ float residual_add(const void* R, int64_t ldr, int r_
     return h + p;
 }
 
+// What entry points outside qlin_capi.hip take from a workspace, and the begin of a run on it (the
+// stream is remembered for qlin_workspace_status).
+struct WorkspaceParts {
+    int cu_count;
+    float* part;          // scratch for partial results, shared with the GEMM's split-K sums
+    int64_t part_floats;
+    uint32_t* err;        // sticky error word
+};
+}  // namespace qlin
+struct qlin_workspace;
+namespace qlin {
+int workspace_device(const qlin_workspace* ws);
+WorkspaceParts workspace_begin(qlin_workspace* ws, hipStream_t stream);
+
+// Bits of a workspace's sticky error word.
+enum : uint32_t { kErrNonfinite = 0x1u, kErrBatch = 0x2u };
+
 // Launchers (return hipError_t of the launch).
 hipError_t launch_quant(const QuantParams& p, int rows, hipStream_t stream);
 hipError_t launch_gemv(const GemvParams& p, int bits, int waves, hipStream_t stream);

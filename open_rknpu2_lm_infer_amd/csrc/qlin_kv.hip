@@ -1,0 +1,156 @@
+// Key/value cache in 8 bits: new rows quantized into their pages, and read back.
+//
+// A row is the key (or value) of one token and one head, dim values x.  With the rule of the
+// per-token activation quantization, s = max(absmax |x| / 127, 2^-64) and
+// code = clamp(round(x * (1 / s)), -127, 127), every operation one f32 rounding.  A row that holds
+// Inf or NaN gets codes 0 and the scale NaN: whoever reads it gets NaN, and the error word says so.
+//
+// Both kernels move their bytes once and do a few operations a value, so memory bounds them (and
+// the launch, for a few tokens).  A group of dim_padded / 8 lanes holds a row, 8 values a lane: 16 bytes of
+// fp16 in, 8 bytes of codes out, and the absmax is a few lane exchanges.
+#include "qlin_kv.hpp"
+#include "qlin_rows.hpp"
+
+namespace qlin {
+namespace {
+
+// Unit of work u of a sequence: keys (0) or values (1) of head h of new row t.
+struct Unit {
+    KvSeq s;
+    int t, h, which;
+    bool ok;       // there is such a row
+    int64_t at;    // row of the cache, -1: no such token or a bad page
+    bool bad;
+};
+
+template <int LPU>
+__device__ __forceinline__ Unit find_unit(const KvRows& p) {
+    const int per_seq = p.b.max_new * p.c.heads * 2;
+    const int upb = 256 / LPU;
+    const int bps = (per_seq + upb - 1) / upb;
+    const int i = blockIdx.x / bps;
+    const int u = (blockIdx.x - i * bps) * upb + threadIdx.x / LPU;
+    Unit r;
+    r.s = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
+    // keys and values of a row's heads side by side: their columns are neighbours in memory
+    r.t = u / (p.c.heads * 2);
+    r.which = (u / p.c.heads) & 1;
+    r.h = u % p.c.heads;
+    r.ok = r.t < r.s.rows;
+    r.bad = r.s.bad;
+    r.at = -1;
+    const int pos = r.s.len - r.s.rows + r.t;
+    if (r.ok && pos >= 0) {
+        bool bad = false;
+        const int page = kv_page(p.b.table[i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
+        if (!bad) r.at = kv_row(page, p.c.heads, r.h, p.c.shift, pos & ((1 << p.c.shift) - 1));
+        r.bad |= bad;
+    }
+    return r;
+}
+
+template <int DP, typename T, bool VEC>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
+    constexpr int LPU = DP / 8;
+    const Unit u = find_unit<LPU>(p);
+    const int d0 = (threadIdx.x % LPU) * 8;
+    float x[8] = {};
+    if (u.ok && u.at >= 0) {
+        const T* src = reinterpret_cast<const T*>(u.which ? p.v : p.k) +
+                       (u.s.row0 + u.t) * (u.which ? p.ldv : p.ldk) + (int64_t)u.h * p.c.dim;
+        load8<T, VEC>(src, d0, p.c.dim, x);
+    }
+    uint32_t m = 0;  // largest bit pattern of |x|: for non-negative floats their order, Inf and NaN on top
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LPU / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    const bool finite = m < 0x7f800000u;
+    const float s = finite ? fmaxf(__uint_as_float(m) / 127.0f, kKvScaleMin) : __uint_as_float(0x7fc00000u);
+    const float inv = finite ? 1.0f / s : 0.0f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = finite ? x[i] : 0.0f;
+        const int c = p.rne ? quant_finite<true>(v, inv) : quant_finite<false>(v, inv);
+        w[i / 4] |= (uint32_t)(c + 128) << (8 * (i % 4));
+    }
+    if (u.ok && u.at >= 0) {
+        *reinterpret_cast<uint2*>((u.which ? p.c.v : p.c.k) + u.at * DP + d0) = make_uint2(w[0], w[1]);
+        if (d0 == 0) (u.which ? p.c.vs : p.c.ks)[u.at] = s;
+    }
+    const uint32_t e = (u.bad ? kErrBatch : 0u) | (finite ? 0u : kErrNonfinite);
+    if (e) atomicOr(p.err, e);
+}
+
+template <int DP, typename T, bool VEC>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
+    constexpr int LPU = DP / 8;
+    const Unit u = find_unit<LPU>(p);
+    const int d0 = (threadIdx.x % LPU) * 8;
+    if (u.bad) atomicOr(p.err, kErrBatch);
+    if (!u.ok) return;
+    T* dst = reinterpret_cast<T*>(u.which ? p.v : p.k) + (u.s.row0 + u.t) * (u.which ? p.ldv : p.ldk) +
+             (int64_t)u.h * p.c.dim;
+    uint2 w = make_uint2(0x80808080u, 0x80808080u);
+    // no such token: zeros; a page outside the cache: NaN
+    float s = u.s.len - u.s.rows + u.t < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+    if (u.at >= 0) {
+        w = *reinterpret_cast<const uint2*>((u.which ? p.c.v : p.c.k) + u.at * DP + d0);
+        s = (u.which ? p.c.vs : p.c.ks)[u.at];
+    }
+    alignas(16) T y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = (float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i % 4))) & 0xffu) - 128) * s;
+        if constexpr (sizeof(T) == 2) y[i] = __builtin_bit_cast(T, f16_of_f32(x));
+        else y[i] = x;
+    }
+    if constexpr (VEC) {
+        if (d0 < p.c.dim) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                reinterpret_cast<uint4*>(dst + d0)[i] = reinterpret_cast<const uint4*>(y)[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (d0 + i < p.c.dim) dst[d0 + i] = y[i];
+    }
+}
+
+template <int DP, typename T, bool VEC>
+hipError_t launch_rows(const KvRows& p, bool append, hipStream_t st) {
+    const int64_t per_seq = (int64_t)p.b.max_new * p.c.heads * 2, upb = 256 / (DP / 8);
+    const int64_t blocks = (per_seq + upb - 1) / upb * p.b.seqs;
+    if (append) kv_append_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    else kv_read_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int DP>
+hipError_t launch_dp(const KvRows& p, bool append, hipStream_t st) {
+    // 16-byte accesses: every row and head 16-byte aligned, heads of whole groups of 8
+    const int per16 = p.f16 ? 8 : 4;
+    const bool vec = p.c.dim % 8 == 0 && p.ldk % per16 == 0 && p.ldv % per16 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
+    if (p.f16) {
+        return vec ? launch_rows<DP, __half, true>(p, append, st) : launch_rows<DP, __half, false>(p, append, st);
+    }
+    return vec ? launch_rows<DP, float, true>(p, append, st) : launch_rows<DP, float, false>(p, append, st);
+}
+
+hipError_t launch_any(const KvRows& p, bool append, hipStream_t st) {
+    switch (p.c.dim_padded) {
+        case 64: return launch_dp<64>(p, append, st);
+        case 128: return launch_dp<128>(p, append, st);
+        default: return launch_dp<256>(p, append, st);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const KvRows& p, hipStream_t st) { return launch_any(p, true, st); }
+hipError_t launch_kv_read(const KvRows& p, hipStream_t st) { return launch_any(p, false, st); }
+
+}  // namespace qlin

@@ -1,0 +1,223 @@
+// C ABI of the key/value cache: its handle, the argument checks, and how an attention call is cut
+// into parts.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "../../include/qlinear.h"
+#include "qlin_kv.hpp"
+
+using namespace qlin;
+
+struct qlin_kv_cache {
+    KvCache c;
+    int device;
+    uint64_t device_bytes;
+};
+
+namespace {
+
+bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Checks a batch against its cache, the workspace and the current device, and begins a run on the workspace.
+int begin(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* b, void* stream, KvBatch* out,
+          WorkspaceParts* parts) {
+    if (!ws || !cache || !b || b->seqs <= 0 || b->rows < 0 || b->max_new < 0 || b->max_len < 0 || !b->row_start ||
+        !b->length || (b->max_len > 0 && !b->page_table) || b->max_new > b->rows ||
+        b->page_ld < ceil_div(b->max_len, (int64_t)1 << cache->c.shift) || b->page_ld < 0)
+        return QLIN_ERR_PARAM;
+    if (b->seqs > kKvMaxSeqs || b->rows > kKvMaxRows || b->max_len > kKvMaxLen) return QLIN_ERR_UNSUPPORTED;
+    if (workspace_device(ws) != cache->device) return QLIN_ERR_PARAM;
+    int dev;
+    if (hipGetDevice(&dev) != hipSuccess) return QLIN_ERR_NODEVICE;
+    if (dev != cache->device) return QLIN_ERR_PARAM;
+    *out = KvBatch{b->seqs, b->rows, b->max_new, b->max_len, b->row_start, b->length, b->page_table, b->page_ld};
+    *parts = workspace_begin(ws, (hipStream_t)stream);
+    return QLIN_OK;
+}
+
+bool is_dtype(int32_t t) { return t == QLIN_F32 || t == QLIN_F16; }
+
+int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K, int64_t ldk, void* V,
+              int64_t ldv, int32_t dtype, uint32_t flags, void* stream, bool append) {
+    if (!cache || !batch || (batch->rows > 0 && (!K || !V)) || !is_dtype(dtype) || (flags & ~QLIN_ROUND_HALF_EVEN)) return QLIN_ERR_PARAM;
+    const int64_t cols = (int64_t)cache->c.heads * cache->c.dim;
+    if (ldk < cols || ldv < cols) return QLIN_ERR_PARAM;
+    KvRows p{};
+    WorkspaceParts parts;
+    if (int rc = begin(ws, cache, batch, stream, &p.b, &parts)) return rc;
+    if (p.b.max_new == 0) return QLIN_OK;
+    // a row and head takes dim_padded / 8 lanes of 256-thread workgroups
+    if ((int64_t)p.b.max_new * cache->c.heads * 2 * cache->c.dim_padded / 8 > (int64_t)1 << 30 ||
+        ceil_div((int64_t)p.b.max_new * cache->c.heads * 2 * cache->c.dim_padded / 8, 256) * p.b.seqs > kKvMaxGrid)
+        return QLIN_ERR_UNSUPPORTED;
+    p.c = cache->c;
+    p.k = K;
+    p.v = V;
+    p.ldk = ldk;
+    p.ldv = ldv;
+    p.f16 = dtype == QLIN_F16;
+    p.rne = (flags & QLIN_ROUND_HALF_EVEN) != 0;
+    p.err = parts.err;
+    const hipError_t e = append ? launch_kv_append(p, (hipStream_t)stream) : launch_kv_read(p, (hipStream_t)stream);
+    return e == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
+}
+
+bool fill_scales(float* p, uint64_t n) {
+    constexpr int bits = 0x1f800000;  // kKvScaleMin
+    static_assert(kKvScaleMin == 0x1p-64f, "its bit pattern");
+    return hipMemsetD32(p, bits, n) == hipSuccess;
+}
+
+// Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part: enough parts that
+// the launch covers the CUs some times over (a workgroup's loads alone do not keep its CU's share of
+// the HBM busy, and ragged sequences end at different times), at least one step of a workgroup each,
+// at most `cap` of them.
+void cut(int64_t tokens, int64_t blocks, int cus, int64_t cap, int* parts, int* chunk) {
+    const int64_t steps = std::max<int64_t>(1, ceil_div(tokens, kAttendStep));
+    const int64_t want = std::max<int64_t>(1, std::min({steps, ceil_div((int64_t)cus * 4, blocks), cap}));
+    const int64_t per = ceil_div(steps, want);
+    *chunk = (int)(per * kAttendStep);
+    *parts = (int)ceil_div(steps, per);
+}
+
+int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, int32_t prefix,
+              const int32_t* prefix_pages, int32_t q_heads, const void* Q, int32_t q_dtype, int64_t ldq, float scale,
+              void* O, int32_t o_dtype, int64_t ldo, void* stream) {
+    if (!cache || !batch || (batch->rows > 0 && (!Q || !O)) || !is_dtype(q_dtype) || !is_dtype(o_dtype) || !std::isfinite(scale) ||
+        q_heads <= 0 || q_heads % cache->c.heads != 0 || prefix < 0 || (prefix > 0 && !prefix_pages))
+        return QLIN_ERR_PARAM;
+    if (prefix & ((1 << cache->c.shift) - 1)) return QLIN_ERR_PARAM;
+    const int64_t cols = (int64_t)q_heads * cache->c.dim;
+    if (ldq < cols || ldo < cols) return QLIN_ERR_PARAM;
+    AttendParams p{};
+    WorkspaceParts wp;
+    if (q_heads > kKvMaxHeads || prefix > kKvMaxLen || (int64_t)batch->rows * q_heads > 1 << 30) return QLIN_ERR_UNSUPPORTED;
+    if (int rc = begin(ws, cache, batch, stream, &p.b, &wp)) return rc;
+    if (p.b.max_new == 0) return QLIN_OK;
+    p.c = cache->c;
+    p.q = Q;
+    p.ldq = ldq;
+    p.q_f16 = q_dtype == QLIN_F16;
+    p.q_heads = q_heads;
+    p.group = q_heads / cache->c.heads;
+    p.scale2 = scale * 1.44269504f;
+    p.o = O;
+    p.ldo = ldo;
+    p.o_f16 = o_dtype == QLIN_F16;
+    p.prefix = prefix;
+    p.prefix_pages = prefix_pages;
+    p.err = wp.err;
+    // parts that the workspace's scratch holds results of
+    const int64_t vectors = (int64_t)p.b.rows * q_heads;
+    const int64_t cap = wp.part_floats / (vectors * (cache->c.dim_padded + 2));
+    const int64_t tile = attend_tile(p);
+    const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * ceil_div((int64_t)p.b.max_new * p.group, tile);
+    const int64_t prefix_blocks = (int64_t)cache->c.heads * ceil_div((int64_t)p.b.rows * p.group, tile);
+    // The prefix gets parts of its own where the scratch can hold its results; else every sequence reads it itself.
+    const bool apart = prefix > 0 && cap >= 2;
+    p.own_from = apart ? prefix : 0;
+    int parts = 1;
+    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, wp.cu_count, apart ? cap / 2 : cap, &parts, &p.chunk);
+    if (apart) cut(prefix, prefix_blocks, wp.cu_count, cap - parts, &p.prefix_parts, &p.prefix_chunk);
+    p.parts = parts + p.prefix_parts;
+    if (own_blocks * parts + prefix_blocks * p.prefix_parts > kKvMaxGrid) return QLIN_ERR_UNSUPPORTED;
+    p.part_o = wp.part;
+    p.part_ml = wp.part + vectors * p.parts * cache->c.dim_padded;
+    return launch_attend(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) {
+    if (!out) return QLIN_ERR_PARAM;
+    *out = nullptr;
+    if (!config || config->kv_heads <= 0 || config->head_dim <= 0 || config->pages <= 0 ||
+        !power_of_two(config->page_tokens))
+        return QLIN_ERR_PARAM;
+    if (config->head_dim > kKvMaxDim || config->kv_heads > kKvMaxHeads || config->page_tokens < kKvMinPage ||
+        config->page_tokens > kKvMaxPage)
+        return QLIN_ERR_UNSUPPORTED;
+    int dev;
+    if (hipGetDevice(&dev) != hipSuccess) return QLIN_ERR_NODEVICE;
+    auto* x = new (std::nothrow) qlin_kv_cache();
+    if (!x) return QLIN_ERR_NOMEM;
+    KvCache& c = x->c;
+    c.pages = config->pages;
+    c.heads = config->kv_heads;
+    c.dim = config->head_dim;
+    c.dim_padded = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    while ((1 << c.shift) < config->page_tokens) ++c.shift;
+    x->device = dev;
+    const uint64_t rows = (uint64_t)c.pages * c.heads * config->page_tokens;
+    x->device_bytes = rows * (2 * (uint64_t)c.dim_padded + 2 * sizeof(float));
+    // rows never written hold code 0 and the smallest scale: they read as zeros
+    bool ok = hipMalloc(&c.k, rows * c.dim_padded) == hipSuccess && hipMalloc(&c.v, rows * c.dim_padded) == hipSuccess &&
+              hipMalloc(&c.ks, rows * sizeof(float)) == hipSuccess && hipMalloc(&c.vs, rows * sizeof(float)) == hipSuccess;
+    if (!ok) {
+        (void)hipGetLastError();
+        qlin_kv_free(x);
+        return QLIN_ERR_NOMEM;
+    }
+    ok = hipMemset(c.k, 0x80, rows * c.dim_padded) == hipSuccess && hipMemset(c.v, 0x80, rows * c.dim_padded) == hipSuccess &&
+         fill_scales(c.ks, rows) && fill_scales(c.vs, rows) &&
+         hipDeviceSynchronize() == hipSuccess;
+    if (!ok) {
+        qlin_kv_free(x);
+        return QLIN_ERR_DEVICE;
+    }
+    *out = x;
+    return QLIN_OK;
+}
+
+void qlin_kv_free(qlin_kv_cache* x) {
+    if (!x) return;
+    (void)hipFree(x->c.k);
+    (void)hipFree(x->c.v);
+    (void)hipFree(x->c.ks);
+    (void)hipFree(x->c.vs);
+    delete x;
+}
+
+int qlin_kv_query(const qlin_kv_cache* x, qlin_kv_info* out) {
+    if (!x || !out) return QLIN_ERR_PARAM;
+    out->kv_heads = x->c.heads;
+    out->head_dim = x->c.dim;
+    out->page_tokens = 1 << x->c.shift;
+    out->pages = x->c.pages;
+    out->head_dim_padded = x->c.dim_padded;
+    out->device = x->device;
+    out->device_bytes = x->device_bytes;
+    return QLIN_OK;
+}
+
+int qlin_kv_append(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const void* K, int64_t ldk,
+                   const void* V, int64_t ldv, int32_t dtype, uint32_t flags, void* stream) {
+    return rows_call(ws, cache, batch, const_cast<void*>(K), ldk, const_cast<void*>(V), ldv, dtype, flags, stream, true);
+}
+
+int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K, int64_t ldk, void* V,
+                 int64_t ldv, int32_t dtype, void* stream) {
+    return rows_call(ws, cache, batch, K, ldk, V, ldv, dtype, 0, stream, false);
+}
+
+int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, int32_t q_heads,
+                      const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O, int32_t o_dtype, int64_t ldo,
+                      void* stream) {
+    return attention(ws, cache, batch, 0, nullptr, q_heads, Q, q_dtype, ldq, scale, O, o_dtype, ldo, stream);
+}
+
+int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
+                             int32_t prefix_tokens, const int32_t* prefix_pages, int32_t q_heads, const void* Q,
+                             int32_t q_dtype, int64_t ldq, float scale, void* O, int32_t o_dtype, int64_t ldo,
+                             void* stream) {
+    return attention(ws, cache, batch, prefix_tokens, prefix_pages, q_heads, Q, q_dtype, ldq, scale, O, o_dtype, ldo,
+                     stream);
+}
+
+}  // extern "C"

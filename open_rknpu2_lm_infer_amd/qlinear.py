@@ -293,6 +293,107 @@ def run_quantized(ws: Workspace, w: Weights, q: torch.Tensor, s: torch.Tensor, o
     return out
 
 
+class KVCache:
+    """Keys and values of kv_heads heads of head_dim in 8 bits, in `pages` pages of page_tokens tokens (qlin_kv_cache)."""
+
+    def __init__(self, kv_heads: int, head_dim: int, pages: int, page_tokens: int = 64):
+        self.handle = ctypes.c_void_p()
+        cfg = _lib.KVConfig(kv_heads, head_dim, page_tokens, pages)
+        check(_lib.load().qlin_kv_create(ctypes.byref(cfg), ctypes.byref(self.handle)), "qlin_kv_create")
+        info = _lib.KVInfo()
+        check(_lib.load().qlin_kv_query(self.handle, ctypes.byref(info)), "qlin_kv_query")
+        self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
+        self.device_bytes = info.device_bytes
+
+    def close(self):
+        if self.handle:
+            _lib.load().qlin_kv_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVBatch:
+    """New rows of some sequences (qlin_kv_batch): device int32 row_start [seqs + 1], length [seqs] and page_table
+    [seqs, columns]; rows of the row tensors, the most new rows and the greatest length of a sequence as numbers,
+    since the device arrays are read only by the kernels (and may change between replays of a captured graph)."""
+
+    def __init__(self, row_start: torch.Tensor, length: torch.Tensor, page_table: torch.Tensor, rows: int, max_new: int,
+                 max_len: int):
+        assert row_start.dtype == length.dtype == page_table.dtype == torch.int32
+        assert row_start.is_cuda and length.is_cuda and page_table.is_cuda
+        assert row_start.is_contiguous() and length.is_contiguous() and page_table.dim() == 2
+        assert page_table.shape[1] <= 1 or page_table.stride(1) == 1
+        seqs = length.numel()
+        assert row_start.numel() == seqs + 1 and page_table.shape[0] == seqs
+        # a table of one row has no row stride of its own
+        ld = page_table.stride(0) if seqs > 1 else max(page_table.shape[1], 1)
+        assert seqs <= 1 or ld >= page_table.shape[1]
+        self.columns, self.rows = page_table.shape[1], rows
+        self.c = _lib.KVBatch(seqs, rows, max_new, max_len, row_start.data_ptr(), length.data_ptr(), page_table.data_ptr(),
+                              ld)
+        self._keep = (row_start, length, page_table)
+
+
+def _kv_batch(cache: KVCache, batch: KVBatch, *rows: torch.Tensor):
+    assert batch.columns * cache.page_tokens >= batch.c.max_len, "the page table is too narrow for max_len"
+    for t in rows:
+        assert t.is_cuda and t.dim() == 2 and t.shape[0] >= batch.rows and (t.shape[1] <= 1 or t.stride(1) == 1)
+    return ctypes.byref(batch.c)
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def kv_append(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor, V: torch.Tensor, flags: int = 0) -> None:
+    """Quantizes the batch's new rows K, V [rows, kv_heads * head_dim] into their pages (qlin_kv_append)."""
+    b = _kv_batch(cache, batch, K, V)
+    assert K.dtype == V.dtype and K.shape[1] == V.shape[1] == cache.kv_heads * cache.head_dim
+    check(_lib.load().qlin_kv_append(ws.handle, cache.handle, b, _ptr(K), _ld(K), _ptr(V), _ld(V), _DT[K.dtype], flags,
+                                     _stream()), "qlin_kv_append")
+
+
+def kv_read(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor | None = None, V: torch.Tensor | None = None,
+            out_dtype=torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The batch's new rows as the cache holds them, K, V [rows, kv_heads * head_dim] (qlin_kv_read)."""
+    shape, dev = (batch.rows, cache.kv_heads * cache.head_dim), batch._keep[0].device
+    K = torch.empty(shape, dtype=out_dtype, device=dev) if K is None else K
+    V = torch.empty(shape, dtype=K.dtype, device=dev) if V is None else V
+    b = _kv_batch(cache, batch, K, V)
+    assert K.dtype == V.dtype and K.shape[1] == V.shape[1] == shape[1]
+    check(_lib.load().qlin_kv_read(ws.handle, cache.handle, b, _ptr(K), _ld(K), _ptr(V), _ld(V), _DT[K.dtype], _stream()),
+          "qlin_kv_read")
+    return K, V
+
+
+def kv_attention(ws: Workspace, cache: KVCache, batch: KVBatch, Q: torch.Tensor, out: torch.Tensor | None = None,
+                 out_dtype=None, scale: float | None = None, prefix_pages: torch.Tensor | None = None,
+                 prefix_tokens: int = 0) -> torch.Tensor:
+    """Causal attention of the batch's new rows Q [rows, q_heads * head_dim] over the cache (qlin_kv_attention; with
+    prefix_tokens, qlin_kv_attention_prefix: the tokens that all sequences begin with, in prefix_pages).  scale
+    defaults to head_dim ** -0.5, out_dtype to Q's."""
+    D = cache.head_dim
+    if out is None:
+        out = torch.empty((Q.shape[0], Q.shape[1]), dtype=out_dtype or Q.dtype, device=Q.device)
+    b = _kv_batch(cache, batch, Q, out)
+    assert Q.shape[1] == out.shape[1] and Q.shape[1] % D == 0
+    args = (Q.shape[1] // D, _ptr(Q), _DT[Q.dtype], _ld(Q), D ** -0.5 if scale is None else scale, _ptr(out),
+            _DT[out.dtype], _ld(out), _stream())
+    if prefix_tokens:
+        assert prefix_pages is not None and prefix_pages.dtype == torch.int32 and prefix_pages.is_cuda
+        assert prefix_pages.is_contiguous() and prefix_pages.numel() * cache.page_tokens >= prefix_tokens
+        check(_lib.load().qlin_kv_attention_prefix(ws.handle, cache.handle, b, prefix_tokens, _ptr(prefix_pages), *args),
+              "qlin_kv_attention_prefix")
+    else:
+        check(_lib.load().qlin_kv_attention(ws.handle, cache.handle, b, *args), "qlin_kv_attention")
+    return out
+
+
 def run_host_f32(ws: Workspace, w: Weights, A: np.ndarray, swiglu: bool = False) -> np.ndarray:
     """The synchronous host-buffer entry (drop-in for rk_npu_w4a8_run_f32 / _run_swiglu_f32)."""
     A = np.ascontiguousarray(A, dtype=np.float32)
