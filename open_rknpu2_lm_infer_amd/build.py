@@ -46,7 +46,8 @@ COMMON = [
 # registers on every iteration.
 FILE_FLAGS = {"qlin_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "qlin_gemm_ks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-              "qlin_gemm_pp.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+              "qlin_gemm_pp.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "qlin_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 ROOT = os.path.dirname(HERE)
 TEST_SRC = os.path.join(ROOT, "tests", "cpp", "npu_backend_test.cpp")

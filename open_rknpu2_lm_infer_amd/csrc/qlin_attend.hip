@@ -52,22 +52,45 @@ struct Bytes {
     uint32_t w[N / 4];
 };
 
-// N consecutive bytes, N-byte aligned (16-byte aligned beyond 16).
+typedef const __attribute__((address_space(4))) int32_t* const_ids;
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+
+// Where a wave finds 16 tokens: their keys, values and scales as buffers of exactly that size, so
+// that an absent tile (past the end, or on a page outside the cache) reads zeros without an access.
+struct Tile {
+    __amdgpu_buffer_rsrc_t k, v, ks, vs;
+    bool bad;  // the page id was outside the cache
+};
+
+template <int DP>
+__device__ __forceinline__ Tile find_tile(const KvCache& c, int id, int head, int off, bool there) {
+    Tile t;
+    t.bad = false;
+    const int page = kv_page(id, c.pages, &t.bad);
+    there = there && !t.bad;
+    const KvBlock<DP> b(c, page, head);
+    constexpr int flags = 0x00027000;  // raw, 32-bit elements
+    t.k = __builtin_amdgcn_make_buffer_rsrc(b.k(off), (short)0, there ? 16 * DP : 0, flags);
+    t.v = __builtin_amdgcn_make_buffer_rsrc(b.v(off), (short)0, there ? 16 * DP : 0, flags);
+    t.ks = __builtin_amdgcn_make_buffer_rsrc(b.ks(off), (short)0, there ? 64 : 0, flags);
+    t.vs = __builtin_amdgcn_make_buffer_rsrc(b.vs(off), (short)0, there ? 64 : 0, flags);
+    return t;
+}
+
+// N consecutive bytes of a buffer.
 template <int N>
-__device__ __forceinline__ void load_bytes(Bytes<N>& r, const uint8_t* p) {
-    if constexpr (N == 4) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+__device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at) {
+    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
     else if constexpr (N == 8) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        r.w[0] = x.x;
-        r.w[1] = x.y;
+        const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
+        r.w[0] = x[0];
+        r.w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N / 16; ++i) {
-            const uint4 x = reinterpret_cast<const uint4*>(p)[i];
-            r.w[4 * i] = x.x;
-            r.w[4 * i + 1] = x.y;
-            r.w[4 * i + 2] = x.z;
-            r.w[4 * i + 3] = x.w;
+            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, 0, 0));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
         }
     }
 }
@@ -79,20 +102,27 @@ template <int DP>
 struct StepData {
     Bytes<DP / 4> k[2];
     Bytes<DP / 16> v[8];
-    float4 ks[2], vs[2];  // scales of tokens 4g .. 4g + 3
+    float4v ks[2], vs[2];  // scales of tokens 4g .. 4g + 3
+    bool bad;
 };
 
 template <int DP>
-__device__ __forceinline__ void load_step(StepData<DP>& r, const KvCache& c, int64_t row0, int64_t row1, int n, int g) {
+__device__ __forceinline__ void load_tile(StepData<DP>& r, const Tile& b, int t, int n, int g) {
+    load_bytes<DP / 4>(r.k[t], b.k, n * DP + g * (DP / 4));
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int64_t row = t ? row1 : row0;
-        load_bytes<DP / 4>(r.k[t], c.k + (row + n) * DP + g * (DP / 4));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_bytes<DP / 16>(r.v[4 * t + i], c.v + (row + 4 * g + i) * DP + n * (DP / 16));
-        r.ks[t] = *reinterpret_cast<const float4*>(c.ks + row + 4 * g);
-        r.vs[t] = *reinterpret_cast<const float4*>(c.vs + row + 4 * g);
-    }
+    for (int i = 0; i < 4; ++i) load_bytes<DP / 16>(r.v[4 * t + i], b.v, (4 * g + i) * DP + n * (DP / 16));
+    r.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(b.ks, 16 * g, 0, 0));
+    r.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(b.vs, 16 * g, 0, 0));
+}
+
+// Sum and maximum over the four lanes n, n + 16, n + 32, n + 48.
+template <bool MAX>
+__device__ __forceinline__ float over_groups(float x) {
+    typedef unsigned int pair __attribute__((ext_vector_type(2)));
+    pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // fp16 high part, and the rest (exact in fp16 unless it underflows) where f32 is asked for.
@@ -102,99 +132,152 @@ __device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
     if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
 }
 
+// Eight columns of a query row, d0 on, as f32; columns past the head's are zeros.
+__device__ __forceinline__ void load_query(const AttendParams& p, int64_t at, int d0, float x[8]) {
+    const int left = p.c.dim - d0;
+    if (p.q_vec) {  // 16-byte aligned heads of whole groups of 8
+        if (p.q_f16) load8<__half, true>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
+        else load8<float, true>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
+    } else if (p.q_f16) load8<__half, false>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
+    else load8<float, false>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
+}
+
+// N consecutive columns of an output row.
+template <int N>
+__device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int d0, const float* y) {
+    if (p.o_vec && N % 4 == 0) {  // 16-byte aligned heads of whole groups of 8
+        if (d0 >= p.c.dim) return;
+#pragma unroll
+        for (int i = 0; i + 4 <= N; i += 4) {
+            if (p.o_f16) {
+                typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+                const half4v h = {(_Float16)y[i], (_Float16)y[i + 1], (_Float16)y[i + 2], (_Float16)y[i + 3]};
+                *reinterpret_cast<half4v*>(reinterpret_cast<_Float16*>(p.o) + at + d0 + i) = h;
+            } else {
+                *reinterpret_cast<float4v*>(reinterpret_cast<float*>(p.o) + at + d0 + i) = float4v{y[i], y[i + 1], y[i + 2], y[i + 3]};
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (d0 + i >= p.c.dim) continue;
+        if (p.o_f16) reinterpret_cast<_Float16*>(p.o)[at + d0 + i] = (_Float16)y[i];
+        else reinterpret_cast<float*>(p.o)[at + d0 + i] = y[i];
+    }
+}
+
 // Workgroup: 4 waves, R tiles of 16 vectors of one KV head, one part of the tokens.  The waves take
 // steps of 32 tokens in turn, each with a running maximum, sum and output of its own, and join
-// them at the end.  LIMBS = 2 (f32 rows in or out): queries and P as a sum of two fp16 values,
-// 22 bits; fp16 queries are exact with one, and P rounded to 11 bits is off by as much as an fp16 output.
-template <int DP, int R, int LIMBS>
-__global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_blocks) {
+// them at the end: nothing is shared before that, and a step's loads are issued a step ahead.
+// LIMBS = 2 (f32 rows in or out): queries and P as a sum of two fp16 values, 22 bits; fp16 queries are
+// exact with one, and P rounded to 11 bits is off by as much as an fp16 output.
+// SHARED: the part of the prefix, for the rows of all sequences at once.
+template <int DP, int R, int LIMBS, bool SHARED>
+__global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
     constexpr int KS = DP / 32;   // matrix steps of a q . k
     constexpr int DT = DP / 16;   // tiles of 16 output columns
     constexpr int VT = 16 * R;    // vectors of the workgroup
-    __shared__ float lds_o[2][VT][DP];
+    constexpr int LD = DP + 4;    // a row of outputs in the LDS: 16 lanes' rows in different banks
+    __shared__ __align__(16) float lds_o[2][VT][LD];
     __shared__ float lds_m[4][VT], lds_l[4][VT];
-    __shared__ int lds_seen[VT];  // tokens that each vector sees
-    __shared__ int lds_range;     // the most of them
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const bool shared_part = (int)blockIdx.x < prefix_blocks;
-    int b = shared_part ? blockIdx.x : blockIdx.x - prefix_blocks;
-    const int parts = shared_part ? p.prefix_parts : p.parts - p.prefix_parts;
+    const int parts = SHARED ? p.prefix_parts : p.parts - p.prefix_parts;
+    const int chunk = SHARED ? p.prefix_chunk : p.chunk;
+    int b = blockIdx.x;
     const int part = b % parts;
     b /= parts;
     const int h = b % p.c.heads;
     b /= p.c.heads;
 
-    // the vectors: (row, head) pairs from first_row on
-    int first_row, rows_left, seq = 0;
-    KvSeq s{};
-    if (shared_part) {
+    // the vectors: (row, head) pairs from first_row on, and how many tokens each sees (-1: no vector)
+    int first_row, seq = 0, cap, end;
+    const int j0 = (SHARED ? 0 : p.own_from) + part * chunk;
+    int seen[R];
+    if constexpr (SHARED) {
+        __shared__ int lds_seen[VT], lds_most;
         first_row = 0;
-        rows_left = p.b.rows;
+        cap = min(p.prefix, j0 + chunk);
+        if (tid == 0) lds_most = 0;
+        if (tid < VT) lds_seen[tid] = -1;
+        __syncthreads();
+        const int v0 = b * VT, r_lo = v0 / p.group, r_hi = min((v0 + VT - 1) / p.group + 1, p.b.rows);
+        for (int i = tid; i < p.b.seqs; i += 256) {
+            const KvSeq q = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
+            for (int r = max(q.row0, r_lo); r < min(q.row0 + q.rows, r_hi); ++r) {
+                const int y = kv_visible(q, r - q.row0);
+                for (int x = max(r * p.group, v0); x < min((r + 1) * p.group, v0 + VT); ++x) lds_seen[x - v0] = y;
+                atomicMax(&lds_most, y);
+            }
+        }
+        __syncthreads();
+        end = min(cap, lds_most);
+#pragma unroll
+        for (int r = 0; r < R; ++r) seen[r] = lds_seen[16 * r + n];
     } else {
         const int tiles = (p.b.max_new * p.group + VT - 1) / VT;
         seq = b / tiles;
         b -= seq * tiles;
-        s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
+        const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
         if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
+        if (b * VT >= s.rows * p.group) return;
+        if (part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
         first_row = s.row0;
-        rows_left = s.rows;
-    }
-    const int v0 = b * VT;
-    if (v0 >= rows_left * p.group) return;
-    const int j0 = (shared_part ? 0 : p.own_from) + part * (shared_part ? p.prefix_chunk : p.chunk);
-    if (!shared_part && part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
-    const int cap = shared_part ? min(p.prefix, j0 + p.prefix_chunk) : min(s.len, j0 + p.chunk);
-
-    // tokens that each vector sees
-    if (tid == 0) lds_range = 0;
-    if (tid < VT) lds_seen[tid] = -1;
-    __syncthreads();
-    if (shared_part) {
-        const int r_lo = v0 / p.group, r_hi = min((v0 + VT - 1) / p.group + 1, p.b.rows);
-        for (int i = tid; i < p.b.seqs; i += 256) {
-            const KvSeq q = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
-            for (int r = max(q.row0, r_lo); r < min(q.row0 + q.rows, r_hi); ++r) {
-                const int seen = kv_visible(q, r - q.row0);
-                for (int x = max(r * p.group, v0); x < min((r + 1) * p.group, v0 + VT); ++x) lds_seen[x - v0] = seen;
-            }
+        cap = min(s.len, j0 + chunk);
+        end = min(cap, kv_visible(s, min(b * VT + VT - 1, s.rows * p.group - 1) / p.group));  // its last row sees most
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int v = b * VT + 16 * r + n;
+            seen[r] = v < s.rows * p.group ? kv_visible(s, v / p.group) : -1;
         }
-    } else if (tid < VT && v0 + tid < rows_left * p.group) {
-        lds_seen[tid] = kv_visible(s, (v0 + tid) / p.group);
     }
-    __syncthreads();
-    if (tid < VT && lds_seen[tid] >= 0) atomicMax(&lds_range, lds_seen[tid]);
-    __syncthreads();
-    const int end = __builtin_amdgcn_readfirstlane(min(cap, lds_range));  // no vector sees more
+    end = __builtin_amdgcn_readfirstlane(end);
+    const int v0 = b * VT;
+
+    // page ids through the scalar cache: nothing writes them while the kernel runs
+    const const_ids table = (const_ids)(uintptr_t)(p.b.table + seq * p.b.table_ld);
+    const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
+    const int off_mask = (1 << p.c.shift) - 1;
+    bool bad_page = false;
+    auto load_step = [&](StepData<DP>& d, int j) {
+        d.bad = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int jt = j + 16 * t, jj = min(jt, end - 1);
+            int id = -1;
+            if (end > 0) id = SHARED || jj < p.prefix ? prefix[jj >> p.c.shift] : table[jj >> p.c.shift];
+            const Tile x = find_tile<DP>(p.c, id, h, jt & off_mask, jt < end);
+            load_tile<DP>(d, x, t, n, g);
+            if (jt < end) d.bad |= x.bad;
+        }
+        bad_page |= d.bad;
+    };
+    int j = j0 + 32 * wave;
+    StepData<DP> d0, d1;
+    load_step(d0, j);
 
     // queries, as the B operand: lane (n, g) holds columns g * DP/4 + 8 s .. + 7 of vector n
     half8v qf[R][KS][LIMBS];
     float unit[R];  // what the f16 operands were divided by, times scale2
-    int seen[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int v = v0 + 16 * r + n;
-        seen[r] = lds_seen[16 * r + n];
         const bool ok = seen[r] >= 0;
         const int row = first_row + (ok ? v / p.group : 0), head = h * p.group + (ok ? v % p.group : 0);
         const int64_t at = (int64_t)row * p.ldq + (int64_t)head * p.c.dim;
         unit[r] = p.scale2 * kCodeUnit;
-        float x[DP / 4];
+        float x[DP / 4] = {};
 #pragma unroll
-        for (int i = 0; i < DP / 4; ++i) {
-            const int d = g * (DP / 4) + i;
-            x[i] = !ok || d >= p.c.dim ? 0.0f
-                   : p.q_f16           ? (float)reinterpret_cast<const _Float16*>(p.q)[at + d]
-                                       : reinterpret_cast<const float*>(p.q)[at + d];
-        }
+        for (int k = 0; k < KS; ++k)
+            if (ok) load_query(p, at, g * (DP / 4) + 8 * k, x + 8 * k);
         if constexpr (LIMBS == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float m = 0.0f;
 #pragma unroll
             for (int i = 0; i < DP / 4; ++i) m = fmaxf(m, fabsf(x[i]));
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            m = over_groups<true>(m);
             const int e = kv_clamp((int)((__float_as_uint(m) >> 23) & 0xff) - 127, -100, 126);
             const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
             unit[r] *= __uint_as_float((uint32_t)(e - 13 + 127) << 23);
@@ -222,21 +305,7 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
         for (int t = 0; t < DT; ++t) o[r][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int32_t* table = p.b.table + seq * p.b.table_ld;
-    const int off_mask = (1 << p.c.shift) - 1;
-    bool bad_page = false;
-    // tokens of a tile past the end are read from the last page (never past the cache) and masked
-    auto tile_row = [&](int j, bool* bad) {
-        const int jj = min(j, end - 1);
-        const int page = kv_page((jj < p.prefix ? p.prefix_pages : table)[jj >> p.c.shift], p.c.pages, bad);
-        return kv_row(page, p.c.heads, h, p.c.shift, j & off_mask);
-    };
-    for (int j = j0 + 32 * wave; j < end; j += kAttendStep) {
-        bool bad = false;
-        StepData<DP> d;
-        const int64_t row0 = tile_row(j, &bad), row1 = tile_row(j + 16, &bad);
-        load_step<DP>(d, p.c, row0, row1, n, g);
-        bad_page |= bad;
+    auto work = [&](const StepData<DP>& d, int j) {
         // S^T: tokens 16 t + 4 g + i of vector n
         float4v sc[2][R];
 #pragma unroll
@@ -253,38 +322,43 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
                         sc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[r][k][q], sc[t][r], 0, 0, 0);
             }
         }
+        float lv[8], iv[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lv[4 * t + i] = d.bad ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
+                iv[4 * t + i] = __builtin_amdgcn_rcpf(d.vs[t][i]);
+            }
         half8v pf[R][LIMBS];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float x[8], inv[8];
+            const int left = min(seen[r], cap) - j - 4 * g;
+            float x[8];
             float top = -__builtin_inff();
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const float ks[4] = {d.ks[t].x, d.ks[t].y, d.ks[t].z, d.ks[t].w};
-                const float vs[4] = {d.vs[t].x, d.vs[t].y, d.vs[t].z, d.vs[t].w};
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float y = __builtin_fmaf(sc[t][r][i] * unit[r], bad ? kNan : ks[i], __builtin_amdgcn_logf(vs[i]));
-                    const bool in = j + 16 * t + 4 * g + i < min(seen[r], cap);
+                    const float y = __builtin_fmaf(sc[t][r][i] * unit[r], d.ks[t][i], lv[4 * t + i]);
                     // masked tokens are chosen away, whatever their scales hold
-                    x[4 * t + i] = in ? y : -__builtin_inff();
-                    inv[4 * t + i] = in ? __builtin_amdgcn_rcpf(vs[i]) : 0.0f;
+                    x[4 * t + i] = 16 * t + i < left ? y : -__builtin_inff();
                     top = fmaxf(top, x[4 * t + i]);
                 }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float m_new = fmaxf(m[r], top);
-            const float base = m_new == -__builtin_inff() ? 0.0f : m_new;
-            const float fade = __builtin_amdgcn_exp2f(m[r] - base);
-            m[r] = m_new;
-            l[r] *= fade;
+            top = over_groups<true>(top);
+            if (__builtin_amdgcn_ballot_w64(top > m[r])) {
+                const float m_new = fmaxf(m[r], top);
+                const float fade = m[r] == m_new ? 1.0f : __builtin_amdgcn_exp2f(m[r] - m_new);
+                m[r] = m_new;
+                l[r] *= fade;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) o[r][t] *= fade;
+                for (int t = 0; t < DT; ++t) o[r][t] *= fade;
+            }
+            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - kPShift;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float e = __builtin_amdgcn_exp2f(x[i] - base + kPShift);
-                l[r] = __builtin_fmaf(e, inv[i], l[r]);
+                const float e = __builtin_amdgcn_exp2f(x[i] - base);
+                l[r] = 16 * (i / 4) + i % 4 < left ? __builtin_fmaf(e, iv[i], l[r]) : l[r];
                 _Float16 y[LIMBS];
                 split_f16<LIMBS>(e, y);
 #pragma unroll
@@ -304,14 +378,23 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
                 for (int q = 0; q < LIMBS; ++q)
                     o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r][q], o[r][t], 0, 0, 0);
         }
+    };
+    for (;;) {
+        if (j >= end) break;
+        load_step(d1, j + kAttendStep);
+        work(d0, j);
+        j += kAttendStep;
+        if (j >= end) break;
+        load_step(d0, j + kAttendStep);
+        work(d1, j);
+        j += kAttendStep;
     }
     if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
 
     // join the waves: a common maximum, then 3 -> 1 and 2 -> 0, then 1 -> 0
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        l[r] += __shfl_xor(l[r], 16, 64);
-        l[r] += __shfl_xor(l[r], 32, 64);
+        l[r] = over_groups<false>(l[r]);
         if (g == 0) {
             lds_m[wave][16 * r + n] = m[r];
             lds_l[wave][16 * r + n] = l[r];
@@ -331,21 +414,30 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[r][t] *= fade;
     }
+    // columns (4 g + i) * DT + t of a vector, t = 4 u .. 4 u + 3
+    auto four = [&](int r, int i, int u) -> float4v {
+        return {o[r][4 * u][i], o[r][4 * u + 1][i], o[r][4 * u + 2][i], o[r][4 * u + 3][i]};
+    };
     auto put = [&](int slot) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds_o[slot][16 * r + n][(4 * g + i) * DT + t] = o[r][t][i];
+                for (int u = 0; u < DT / 4; ++u)
+                    *reinterpret_cast<float4v*>(&lds_o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]) = four(r, i, u);
     };
     auto add = [&](int slot) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[r][t][i] += lds_o[slot][16 * r + n][(4 * g + i) * DT + t];
+                for (int u = 0; u < DT / 4; ++u) {
+                    const float4v y = *reinterpret_cast<const float4v*>(&lds_o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[r][4 * u + c][i] += y[c];
+                }
     };
     if (wave >= 2) put(wave - 2);
     __syncthreads();
@@ -367,20 +459,18 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    const int d = (4 * g + i) * DT + t;
-                    if (d >= p.c.dim) continue;
-                    const float y = o[r][t][i] * f;
-                    const int64_t at = row * p.ldo + (int64_t)head * p.c.dim + d;
-                    if (p.o_f16) reinterpret_cast<_Float16*>(p.o)[at] = (_Float16)y;
-                    else reinterpret_cast<float*>(p.o)[at] = y;
+                for (int u = 0; u < DT / 4; ++u) {
+                    const float4v y = four(r, i, u) * f;
+                    const float z[4] = {y[0], y[1], y[2], y[3]};
+                    store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, (4 * g + i) * DT + 4 * u, z);
                 }
         } else {
-            const int64_t slot = (row * p.q_heads + head) * p.parts + (shared_part ? 0 : p.prefix_parts) + part;
+            const int64_t slot = (row * p.q_heads + head) * p.parts + (SHARED ? 0 : p.prefix_parts) + part;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int t = 0; t < DT; ++t) p.part_o[slot * DP + (4 * g + i) * DT + t] = o[r][t][i];
+                for (int u = 0; u < DT / 4; ++u)
+                    *reinterpret_cast<float4v*>(p.part_o + slot * DP + (4 * g + i) * DT + 4 * u) = four(r, i, u);
             if (g == 0) {
                 p.part_ml[2 * slot] = m_all[r];
                 p.part_ml[2 * slot + 1] = l_all[r];
@@ -389,63 +479,86 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p, int prefix_
     }
 }
 
-// Joins the parts of every vector: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes a
-// vector, four columns each.
+// Joins the parts of a vector, one workgroup each: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// Groups of DP / 4 lanes take the parts in turn, four columns a lane, and are added up in the LDS.
 template <int DP>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
-    constexpr int LPV = DP / 4, VPB = 256 / LPV;
-    const int per_seq = (p.b.max_new * p.q_heads + VPB - 1) / VPB;
-    const int seq = blockIdx.x / per_seq;
-    const int x = (blockIdx.x - seq * per_seq) * VPB + threadIdx.x / LPV;
+    constexpr int LPV = DP / 4, GROUPS = 256 / LPV;
+    __shared__ __align__(16) float lds_o[GROUPS][DP];
+    __shared__ float lds_l[GROUPS];
+    const int per_seq = p.b.max_new * p.q_heads;
+    const int seq = blockIdx.x / per_seq, x = blockIdx.x - seq * per_seq;
     const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
-    const int t = x / p.q_heads, head = x % p.q_heads;
+    const int t = x / p.q_heads, head = x - t * p.q_heads;
     if (t >= s.rows) return;
     const int parts = p.prefix_parts + kv_parts(s.len - p.own_from, p.chunk);
-    const int d = (threadIdx.x % LPV) * 4;
+    const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4, lane = threadIdx.x & 63;
     const int64_t row = s.row0 + t, slot = (row * p.q_heads + head) * p.parts;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot;
     float m = -__builtin_inff();
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[2 * (slot + i)]);
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[i].x);
+    m = wave_max(m);
     const float base = m == -__builtin_inff() ? 0.0f : m;
     float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < parts; ++i) {
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * (slot + i)] - base);
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (slot + i) * DP + d);
-        l = __builtin_fmaf(f, p.part_ml[2 * (slot + i) + 1], l);
-        o.x = __builtin_fmaf(f, y.x, o.x);
-        o.y = __builtin_fmaf(f, y.y, o.y);
-        o.z = __builtin_fmaf(f, y.z, o.z);
-        o.w = __builtin_fmaf(f, y.w, o.w);
+    float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = group; i < parts; i += GROUPS) {
+        const float2 y = ml[i];
+        const float f = __builtin_amdgcn_exp2f(y.x - base);
+        l = __builtin_fmaf(f, y.y, l);
+        const float4v z = *reinterpret_cast<const float4v*>(p.part_o + (slot + i) * DP + d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[c], o[c]);
+    }
+    *reinterpret_cast<float4v*>(&lds_o[group][d]) = o;
+    if (d == 0) lds_l[group] = l;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) {
+        o += *reinterpret_cast<const float4v*>(&lds_o[i][d]);
+        l += lds_l[i];
     }
     const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
-    const float y[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
-    const int64_t at = row * p.ldo + (int64_t)head * p.c.dim + d;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (d + i >= p.c.dim) continue;
-        if (p.o_f16) reinterpret_cast<_Float16*>(p.o)[at + i] = (_Float16)y[i];
-        else reinterpret_cast<float*>(p.o)[at + i] = y[i];
-    }
+    const float y[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+    store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, d, y);
+}
+
+// Vectors of a workgroup, given how many share its tokens.  Two tiles of 256 columns would not fit
+// the registers.
+int tile_of(int64_t vectors, int dim_padded) { return vectors <= 16 || dim_padded > 128 ? 16 : 32; }
+
+template <int DP, int R, int LIMBS, bool SHARED>
+hipError_t launch_r(const AttendParams& p, hipStream_t st) {
+    const int64_t vectors = (int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group;
+    const int64_t blocks = (int64_t)(SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs) *
+                           p.c.heads * ((vectors + 16 * R - 1) / (16 * R));
+    attend_kernel<DP, R, LIMBS, SHARED><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int DP, int LIMBS, bool SHARED>
+hipError_t launch_part(const AttendParams& p, hipStream_t st) {
+    const int tile = SHARED ? attend_tile_prefix(p) : attend_tile(p);
+    if constexpr (DP <= 128)
+        if (tile == 32) return launch_r<DP, 2, LIMBS, SHARED>(p, st);
+    return launch_r<DP, 1, LIMBS, SHARED>(p, st);
 }
 
 template <int DP, int LIMBS>
 hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
-    constexpr int R = 1;
-    const int64_t tiles = ((int64_t)p.b.max_new * p.group + 16 * R - 1) / (16 * R);
-    const int64_t own = (int64_t)(p.parts - p.prefix_parts) * p.c.heads * tiles * p.b.seqs;
-    const int64_t shared = p.prefix_parts * (int64_t)p.c.heads * (((int64_t)p.b.rows * p.group + 16 * R - 1) / (16 * R));
-    attend_kernel<DP, R, LIMBS><<<dim3((uint32_t)(own + shared)), 256, 0, st>>>(p, (int)shared);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (p.prefix_parts)
+        if (hipError_t e = launch_part<DP, LIMBS, true>(p, st)) return e;
+    if (hipError_t e = launch_part<DP, LIMBS, false>(p, st)) return e;
     if (p.parts == 1) return hipSuccess;
-    constexpr int VPB = 256 / (DP / 4);
-    const int64_t per_seq = ((int64_t)p.b.max_new * p.q_heads + VPB - 1) / VPB;
-    attend_join_kernel<DP><<<dim3((uint32_t)(per_seq * p.b.seqs)), 256, 0, st>>>(p);
+    attend_join_kernel<DP><<<dim3((uint32_t)((int64_t)p.b.max_new * p.q_heads * p.b.seqs)), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int attend_tile(const AttendParams&) { return 16; }
+int attend_tile(const AttendParams& p) { return tile_of((int64_t)p.b.max_new * p.group, p.c.dim_padded); }
+int attend_tile_prefix(const AttendParams& p) { return tile_of((int64_t)p.b.rows * p.group, p.c.dim_padded); }
 
 hipError_t launch_attend(const AttendParams& p, hipStream_t st) {
     const bool two = !p.q_f16 || !p.o_f16;

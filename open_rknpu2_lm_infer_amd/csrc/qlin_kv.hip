@@ -14,70 +14,78 @@
 namespace qlin {
 namespace {
 
-// Unit of work u of a sequence: keys (0) or values (1) of head h of new row t.
+// Unit of work u of a sequence: head h of new row t, its key and its value.
 struct Unit {
     KvSeq s;
-    int t, h, which;
-    bool ok;       // there is such a row
-    int64_t at;    // row of the cache, -1: no such token or a bad page
+    int i, t, h;
+    bool ok;  // there is such a row
     bool bad;
 };
 
 template <int LPU>
 __device__ __forceinline__ Unit find_unit(const KvRows& p) {
-    const int per_seq = p.b.max_new * p.c.heads * 2;
-    const int upb = 256 / LPU;
-    const int bps = (per_seq + upb - 1) / upb;
-    const int i = blockIdx.x / bps;
-    const int u = (blockIdx.x - i * bps) * upb + threadIdx.x / LPU;
+    constexpr int UPB = 256 / LPU;
+    const int bps = (p.b.max_new * p.c.heads + UPB - 1) / UPB;
     Unit r;
-    r.s = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
-    // keys and values of a row's heads side by side: their columns are neighbours in memory
-    r.t = u / (p.c.heads * 2);
-    r.which = (u / p.c.heads) & 1;
-    r.h = u % p.c.heads;
+    r.i = blockIdx.x / bps;
+    const int u = (blockIdx.x - r.i * bps) * UPB + threadIdx.x / LPU;
+    r.s = kv_seq(p.b.row_start, p.b.length, r.i, p.b.rows, p.b.max_new, p.b.max_len);
+    r.t = u / p.c.heads;
+    r.h = u - r.t * p.c.heads;
     r.ok = r.t < r.s.rows;
     r.bad = r.s.bad;
-    r.at = -1;
-    const int pos = r.s.len - r.s.rows + r.t;
-    if (r.ok && pos >= 0) {
-        bool bad = false;
-        const int page = kv_page(p.b.table[i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
-        if (!bad) r.at = kv_row(page, p.c.heads, r.h, p.c.shift, pos & ((1 << p.c.shift) - 1));
-        r.bad |= bad;
-    }
     return r;
+}
+
+// The slot of a unit's token: its page (-1: no such token, or a page outside the cache) and place in it.
+__device__ __forceinline__ int find_page(const KvRows& p, Unit& u, int* off) {
+    const int pos = u.s.len - u.s.rows + u.t;
+    *off = pos & ((1 << p.c.shift) - 1);
+    if (!u.ok || pos < 0) return -1;
+    bool bad = false;
+    const int page = kv_page(p.b.table[u.i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
+    u.bad |= bad;
+    return bad ? -1 : page;
 }
 
 template <int DP, typename T, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
     constexpr int LPU = DP / 8;
-    const Unit u = find_unit<LPU>(p);
+    Unit u = find_unit<LPU>(p);
     const int d0 = (threadIdx.x % LPU) * 8;
-    float x[8] = {};
-    if (u.ok && u.at >= 0) {
-        const T* src = reinterpret_cast<const T*>(u.which ? p.v : p.k) +
-                       (u.s.row0 + u.t) * (u.which ? p.ldv : p.ldk) + (int64_t)u.h * p.c.dim;
-        load8<T, VEC>(src, d0, p.c.dim, x);
+    // the rows' loads do not wait for the page's
+    float x[2][8] = {};
+    if (u.ok) {
+        const int64_t row = u.s.row0 + u.t, col = (int64_t)u.h * p.c.dim;
+        load8<T, VEC>(reinterpret_cast<const T*>(p.k) + row * p.ldk + col, d0, p.c.dim, x[0]);
+        load8<T, VEC>(reinterpret_cast<const T*>(p.v) + row * p.ldv + col, d0, p.c.dim, x[1]);
     }
-    uint32_t m = 0;  // largest bit pattern of |x|: for non-negative floats their order, Inf and NaN on top
+    int off;
+    const int page = find_page(p, u, &off);
+    const KvBlock<DP> blk(p.c, max(page, 0), u.h);
+    bool finite = true;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int y = 0; y < 2; ++y) {
+        uint32_t m = 0;  // largest bit pattern of |x|: for non-negative floats their order, Inf and NaN on top
 #pragma unroll
-    for (int o = LPU / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    const bool finite = m < 0x7f800000u;
-    const float s = finite ? fmaxf(__uint_as_float(m) / 127.0f, kKvScaleMin) : __uint_as_float(0x7fc00000u);
-    const float inv = finite ? 1.0f / s : 0.0f;
-    uint32_t w[2] = {0, 0};
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[y][i]) & 0x7fffffffu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = finite ? x[i] : 0.0f;
-        const int c = p.rne ? quant_finite<true>(v, inv) : quant_finite<false>(v, inv);
-        w[i / 4] |= (uint32_t)(c + 128) << (8 * (i % 4));
-    }
-    if (u.ok && u.at >= 0) {
-        *reinterpret_cast<uint2*>((u.which ? p.c.v : p.c.k) + u.at * DP + d0) = make_uint2(w[0], w[1]);
-        if (d0 == 0) (u.which ? p.c.vs : p.c.ks)[u.at] = s;
+        for (int o = LPU / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+        const bool fin = m < 0x7f800000u;
+        const float s = fin ? fmaxf(__uint_as_float(m) / 127.0f, kKvScaleMin) : __uint_as_float(0x7fc00000u);
+        const float inv = fin ? 1.0f / s : 0.0f;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = fin ? x[y][i] : 0.0f;
+            const int c = p.rne ? quant_finite<true>(v, inv) : quant_finite<false>(v, inv);
+            w[i / 4] |= (uint32_t)(c + 128) << (8 * (i % 4));
+        }
+        if (page >= 0) {
+            *reinterpret_cast<uint2*>((y ? blk.v(off) : blk.k(off)) + d0) = make_uint2(w[0], w[1]);
+            if (d0 == 0) *(y ? blk.vs(off) : blk.ks(off)) = s;
+            finite &= fin;
+        }
     }
     const uint32_t e = (u.bad ? kErrBatch : 0u) | (finite ? 0u : kErrNonfinite);
     if (e) atomicOr(p.err, e);
@@ -86,42 +94,55 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
 template <int DP, typename T, bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     constexpr int LPU = DP / 8;
-    const Unit u = find_unit<LPU>(p);
+    Unit u = find_unit<LPU>(p);
     const int d0 = (threadIdx.x % LPU) * 8;
+    int off;
+    const int page = find_page(p, u, &off);
     if (u.bad) atomicOr(p.err, kErrBatch);
     if (!u.ok) return;
-    T* dst = reinterpret_cast<T*>(u.which ? p.v : p.k) + (u.s.row0 + u.t) * (u.which ? p.ldv : p.ldk) +
-             (int64_t)u.h * p.c.dim;
-    uint2 w = make_uint2(0x80808080u, 0x80808080u);
+    const KvBlock<DP> blk(p.c, max(page, 0), u.h);
+    uint2 w[2] = {make_uint2(0x80808080u, 0x80808080u), make_uint2(0x80808080u, 0x80808080u)};
     // no such token: zeros; a page outside the cache: NaN
-    float s = u.s.len - u.s.rows + u.t < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
-    if (u.at >= 0) {
-        w = *reinterpret_cast<const uint2*>((u.which ? p.c.v : p.c.k) + u.at * DP + d0);
-        s = (u.which ? p.c.vs : p.c.ks)[u.at];
+    const float none = u.s.len - u.s.rows + u.t < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+    float s[2] = {none, none};
+    if (page >= 0) {
+        w[0] = *reinterpret_cast<const uint2*>(blk.k(off) + d0);
+        w[1] = *reinterpret_cast<const uint2*>(blk.v(off) + d0);
+        s[0] = *blk.ks(off);
+        s[1] = *blk.vs(off);
     }
-    alignas(16) T y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = (float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i % 4))) & 0xffu) - 128) * s;
-        if constexpr (sizeof(T) == 2) y[i] = __builtin_bit_cast(T, f16_of_f32(x));
-        else y[i] = x;
-    }
-    if constexpr (VEC) {
-        if (d0 < p.c.dim) {
+    for (int z = 0; z < 2; ++z) {
+        T* dst = reinterpret_cast<T*>(z ? p.v : p.k) + (u.s.row0 + u.t) * (z ? p.ldv : p.ldk) + (int64_t)u.h * p.c.dim;
+        alignas(16) T y[8];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                reinterpret_cast<uint4*>(dst + d0)[i] = reinterpret_cast<const uint4*>(y)[i];
+        for (int i = 0; i < 8; ++i) {
+            const float x = (float)((int)(((i < 4 ? w[z].x : w[z].y) >> (8 * (i % 4))) & 0xffu) - 128) * s[z];
+            if constexpr (sizeof(T) == 2) y[i] = __builtin_bit_cast(T, f16_of_f32(x));
+            else y[i] = x;
         }
-    } else {
+        if constexpr (VEC) {
+            if (d0 < p.c.dim) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (d0 + i < p.c.dim) dst[d0 + i] = y[i];
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                    reinterpret_cast<uint4*>(dst + d0)[i] = reinterpret_cast<const uint4*>(y)[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d0 + i < p.c.dim) dst[d0 + i] = y[i];
+        }
     }
+}
+
+__global__ __launch_bounds__(256) void kv_clear_kernel(uint32_t* data, int64_t words, int64_t block_words, int64_t code_words) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256)
+        data[i] = i % block_words < code_words ? 0x80808080u : __float_as_uint(kKvScaleMin);
 }
 
 template <int DP, typename T, bool VEC>
 hipError_t launch_rows(const KvRows& p, bool append, hipStream_t st) {
-    const int64_t per_seq = (int64_t)p.b.max_new * p.c.heads * 2, upb = 256 / (DP / 8);
+    const int64_t per_seq = (int64_t)p.b.max_new * p.c.heads, upb = 256 / (DP / 8);
     const int64_t blocks = (per_seq + upb - 1) / upb * p.b.seqs;
     if (append) kv_append_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
     else kv_read_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
@@ -150,6 +171,12 @@ hipError_t launch_any(const KvRows& p, bool append, hipStream_t st) {
 
 }  // namespace
 
+hipError_t launch_kv_clear(const KvCache& c, hipStream_t st) {
+    const int64_t block = kv_block_bytes(c.dim_padded, c.shift) / 4;
+    kv_clear_kernel<<<dim3(4096), 256, 0, st>>>(reinterpret_cast<uint32_t*>(c.data), block * c.heads * c.pages, block,
+                                                 ((int64_t)c.dim_padded << c.shift) / 2);
+    return hipGetLastError();
+}
 hipError_t launch_kv_append(const KvRows& p, hipStream_t st) { return launch_any(p, true, st); }
 hipError_t launch_kv_read(const KvRows& p, hipStream_t st) { return launch_any(p, false, st); }
 

@@ -17,11 +17,27 @@ constexpr int64_t kKvMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads of o
 
 // The cache in device memory.  Codes are stored as code + 128, one byte each: a byte b between two
 // zero bytes is the fp16 subnormal b * 2^-24, so one byte permute and one packed FMA make two exact
-// fp16 codes of four bytes.  Columns dim .. dim_padded - 1 hold code 0.
+// fp16 codes of two bytes.  Columns dim .. dim_padded - 1 hold code 0.
+//
+// A block of a page and head is contiguous: keys [page tokens][dim_padded], values alike, then the
+// key scales f32 [page tokens] and the value scales.  One address leads to all of it.
 struct KvCache {
-    uint8_t *k, *v;  // [pages][heads][page tokens][dim_padded]
-    float *ks, *vs;  // [pages][heads][page tokens]
+    uint8_t* data;  // [pages][heads] blocks
     int pages, heads, dim, dim_padded, shift;  // 1 << shift tokens a page
+};
+__host__ __device__ __forceinline__ int64_t kv_block_bytes(int dim_padded, int shift) {
+    return (int64_t)(2 * dim_padded + 8) << shift;
+}
+template <int DP>
+struct KvBlock {
+    uint8_t* base;
+    int shift;
+    __device__ KvBlock(const KvCache& c, int page, int head)
+        : base(c.data + ((int64_t)page * c.heads + head) * kv_block_bytes(DP, c.shift)), shift(c.shift) {}
+    __device__ uint8_t* k(int off) const { return base + off * DP; }
+    __device__ uint8_t* v(int off) const { return base + (((int64_t)DP << shift) + off * DP); }
+    __device__ float* ks(int off) const { return reinterpret_cast<float*>(base + ((int64_t)(2 * DP) << shift)) + off; }
+    __device__ float* vs(int off) const { return ks(off + (1 << shift)); }
 };
 
 struct KvBatch {
@@ -43,18 +59,19 @@ struct KvRows {
 };
 hipError_t launch_kv_append(const KvRows& p, hipStream_t stream);
 hipError_t launch_kv_read(const KvRows& p, hipStream_t stream);
+hipError_t launch_kv_clear(const KvCache& c, hipStream_t stream);  // every row: code 0, the smallest scale
 
 struct AttendParams {
     KvCache c;
     KvBatch b;
     const void* q;  // [rows, ldq]
     int64_t ldq;
-    int q_f16;
+    int q_f16, q_vec;    // q_vec, o_vec: heads of whole groups of 8, 16-byte aligned
     int q_heads, group;  // group = q_heads / kv heads
     float scale2;        // scale * log2 e
     void* o;             // [rows, ldo]
     int64_t ldo;
-    int o_f16;
+    int o_f16, o_vec;
     int prefix;                   // tokens of the shared prefix, a multiple of the page; 0: none
     const int32_t* prefix_pages;  // its pages
     int own_from;                 // first token that a sequence's own parts cover: prefix, or 0 (no parts of the prefix)
@@ -68,7 +85,9 @@ struct AttendParams {
 };
 // Tokens worked on at once by a workgroup of the attention kernel: chunks are multiples of it.
 constexpr int kAttendStep = 128;
-int attend_tile(const AttendParams& p);  // vectors of a workgroup
+// Vectors of a workgroup: over a sequence's own tokens, over the prefix.
+int attend_tile(const AttendParams& p);
+int attend_tile_prefix(const AttendParams& p);
 hipError_t launch_attend(const AttendParams& p, hipStream_t stream);
 
 }  // namespace qlin

@@ -39,6 +39,11 @@ int begin(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* b
     return QLIN_OK;
 }
 
+// Rows whose heads are whole groups of 8 columns, each 16-byte aligned.
+bool aligned(const void* p, int64_t ld, int dtype, int dim) {
+    return dim % 8 == 0 && ld % (dtype == QLIN_F16 ? 8 : 4) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
 bool is_dtype(int32_t t) { return t == QLIN_F32 || t == QLIN_F16; }
 
 int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K, int64_t ldk, void* V,
@@ -51,8 +56,8 @@ int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     if (int rc = begin(ws, cache, batch, stream, &p.b, &parts)) return rc;
     if (p.b.max_new == 0) return QLIN_OK;
     // a row and head takes dim_padded / 8 lanes of 256-thread workgroups
-    if ((int64_t)p.b.max_new * cache->c.heads * 2 * cache->c.dim_padded / 8 > (int64_t)1 << 30 ||
-        ceil_div((int64_t)p.b.max_new * cache->c.heads * 2 * cache->c.dim_padded / 8, 256) * p.b.seqs > kKvMaxGrid)
+    const int64_t lanes = (int64_t)p.b.max_new * cache->c.heads * cache->c.dim_padded / 8;
+    if (lanes > (int64_t)1 << 30 || ceil_div(lanes, 256) * p.b.seqs > kKvMaxGrid)
         return QLIN_ERR_UNSUPPORTED;
     p.c = cache->c;
     p.k = K;
@@ -64,12 +69,6 @@ int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.err = parts.err;
     const hipError_t e = append ? launch_kv_append(p, (hipStream_t)stream) : launch_kv_read(p, (hipStream_t)stream);
     return e == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
-}
-
-bool fill_scales(float* p, uint64_t n) {
-    constexpr int bits = 0x1f800000;  // kKvScaleMin
-    static_assert(kKvScaleMin == 0x1p-64f, "its bit pattern");
-    return hipMemsetD32(p, bits, n) == hipSuccess;
 }
 
 // Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part: enough parts that
@@ -101,12 +100,14 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.c = cache->c;
     p.q = Q;
     p.ldq = ldq;
+    p.q_vec = aligned(Q, ldq, q_dtype, cache->c.dim);
     p.q_f16 = q_dtype == QLIN_F16;
     p.q_heads = q_heads;
     p.group = q_heads / cache->c.heads;
     p.scale2 = scale * 1.44269504f;
     p.o = O;
     p.ldo = ldo;
+    p.o_vec = aligned(O, ldo, o_dtype, cache->c.dim);
     p.o_f16 = o_dtype == QLIN_F16;
     p.prefix = prefix;
     p.prefix_pages = prefix_pages;
@@ -114,9 +115,8 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     // parts that the workspace's scratch holds results of
     const int64_t vectors = (int64_t)p.b.rows * q_heads;
     const int64_t cap = wp.part_floats / (vectors * (cache->c.dim_padded + 2));
-    const int64_t tile = attend_tile(p);
-    const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * ceil_div((int64_t)p.b.max_new * p.group, tile);
-    const int64_t prefix_blocks = (int64_t)cache->c.heads * ceil_div((int64_t)p.b.rows * p.group, tile);
+    const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * ceil_div((int64_t)p.b.max_new * p.group, attend_tile(p));
+    const int64_t prefix_blocks = (int64_t)cache->c.heads * ceil_div((int64_t)p.b.rows * p.group, attend_tile_prefix(p));
     // The prefix gets parts of its own where the scratch can hold its results; else every sequence reads it itself.
     const bool apart = prefix > 0 && cap >= 2;
     p.own_from = apart ? prefix : 0;
@@ -124,7 +124,8 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, wp.cu_count, apart ? cap / 2 : cap, &parts, &p.chunk);
     if (apart) cut(prefix, prefix_blocks, wp.cu_count, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
-    if (own_blocks * parts + prefix_blocks * p.prefix_parts > kKvMaxGrid) return QLIN_ERR_UNSUPPORTED;
+    if (std::max({own_blocks * parts, prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs}) > kKvMaxGrid)
+        return QLIN_ERR_UNSUPPORTED;
     p.part_o = wp.part;
     p.part_ml = wp.part + vectors * p.parts * cache->c.dim_padded;
     return launch_attend(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
@@ -154,20 +155,13 @@ int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) {
     c.dim_padded = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     while ((1 << c.shift) < config->page_tokens) ++c.shift;
     x->device = dev;
-    const uint64_t rows = (uint64_t)c.pages * c.heads * config->page_tokens;
-    x->device_bytes = rows * (2 * (uint64_t)c.dim_padded + 2 * sizeof(float));
-    // rows never written hold code 0 and the smallest scale: they read as zeros
-    bool ok = hipMalloc(&c.k, rows * c.dim_padded) == hipSuccess && hipMalloc(&c.v, rows * c.dim_padded) == hipSuccess &&
-              hipMalloc(&c.ks, rows * sizeof(float)) == hipSuccess && hipMalloc(&c.vs, rows * sizeof(float)) == hipSuccess;
-    if (!ok) {
+    x->device_bytes = (uint64_t)c.pages * c.heads * kv_block_bytes(c.dim_padded, c.shift);
+    if (hipMalloc(&c.data, x->device_bytes) != hipSuccess) {
         (void)hipGetLastError();
-        qlin_kv_free(x);
+        delete x;
         return QLIN_ERR_NOMEM;
     }
-    ok = hipMemset(c.k, 0x80, rows * c.dim_padded) == hipSuccess && hipMemset(c.v, 0x80, rows * c.dim_padded) == hipSuccess &&
-         fill_scales(c.ks, rows) && fill_scales(c.vs, rows) &&
-         hipDeviceSynchronize() == hipSuccess;
-    if (!ok) {
+    if (launch_kv_clear(c, nullptr) != hipSuccess || hipDeviceSynchronize() != hipSuccess) {
         qlin_kv_free(x);
         return QLIN_ERR_DEVICE;
     }
@@ -177,10 +171,7 @@ int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) {
 
 void qlin_kv_free(qlin_kv_cache* x) {
     if (!x) return;
-    (void)hipFree(x->c.k);
-    (void)hipFree(x->c.v);
-    (void)hipFree(x->c.ks);
-    (void)hipFree(x->c.vs);
+    (void)hipFree(x->c.data);
     delete x;
 }
 

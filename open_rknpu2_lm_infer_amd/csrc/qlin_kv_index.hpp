@@ -46,11 +46,6 @@ QLIN_HD int kv_page(int id, int pages, bool* bad) {
     return 0;
 }
 
-// Index of (page, head, token) among the rows of the cache: [pages][heads][page tokens].
-QLIN_HD int64_t kv_row(int page, int heads, int head, int shift, int off) {
-    return (((static_cast<int64_t>(page) * heads + head) << shift) + off);
-}
-
 // Parts of `chunk` tokens that a sequence of `tokens` tokens is worked on in (one at least).
 QLIN_HD int kv_parts(int tokens, int chunk) { return tokens <= chunk ? 1 : (tokens - 1) / chunk + 1; }
 
