@@ -14,38 +14,10 @@
 // transposed, S^T = K Q^T and O^T = V^T P^T: then the matrix core's result layout (a lane holds
 // four consecutive tokens of one vector) is the operand layout of the second product with its k
 // axis permuted, and P never leaves its lane.
-#include "qlin_kv.hpp"
-#include "qlin_rows.hpp"
+#include "qlin_attend.hpp"
 
 namespace qlin {
 namespace {
-
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef _Float16 half8v __attribute__((ext_vector_type(8)));
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-
-constexpr float kNan = __builtin_nanf("");
-
-// P is scaled by 2^kPShift before it is rounded to fp16 (11 bits), so that it stays normal down to
-// 2^-22 and non-zero down to 2^-32 of the largest; the factor is in the sum too and cancels.
-constexpr float kPShift = 8.0f;
-
-// Two fp16 codes times 2^-9 from bytes i and j of the cache (code + 128) that sel picks from
-// (hi, lo): the permuted pair is (b_i, b_j) * 2^-24, both exact; * 2^15 - 128 * 2^-9 is exact.
-__device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t sel) {
-    const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(hi, lo, sel));
-    const half2v m = {(_Float16)32768.0f, (_Float16)32768.0f}, a = {(_Float16)-0.25f, (_Float16)-0.25f};
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, m, a));
-}
-constexpr float kCodeUnit = 512.0f;  // 1 / 2^-9
-
-// Eight codes of consecutive columns, bytes of (w0, w1).
-__device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
-    const uint4v r = {codes2(w0, w0, 0x0c010c00u), codes2(w0, w0, 0x0c030c02u), codes2(w1, w1, 0x0c010c00u),
-                      codes2(w1, w1, 0x0c030c02u)};
-    return __builtin_bit_cast(half8v, r);
-}
 
 template <int N>
 struct Bytes {
@@ -123,48 +95,6 @@ __device__ __forceinline__ float over_groups(float x) {
     x = MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
     r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
     return MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// fp16 high part, and the rest (exact in fp16 unless it underflows) where f32 is asked for.
-template <int LIMBS>
-__device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
-    out[0] = (_Float16)x;
-    if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
-}
-
-// Eight columns of a query row, d0 on, as f32; columns past the head's are zeros.
-__device__ __forceinline__ void load_query(const AttendParams& p, int64_t at, int d0, float x[8]) {
-    const int left = p.c.dim - d0;
-    if (p.q_vec) {  // 16-byte aligned heads of whole groups of 8
-        if (p.q_f16) load8<__half, true>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
-        else load8<float, true>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
-    } else if (p.q_f16) load8<__half, false>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
-    else load8<float, false>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
-}
-
-// N consecutive columns of an output row.
-template <int N>
-__device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int d0, const float* y) {
-    if (p.o_vec && N % 4 == 0) {  // 16-byte aligned heads of whole groups of 8
-        if (d0 >= p.c.dim) return;
-#pragma unroll
-        for (int i = 0; i + 4 <= N; i += 4) {
-            if (p.o_f16) {
-                typedef _Float16 half4v __attribute__((ext_vector_type(4)));
-                const half4v h = {(_Float16)y[i], (_Float16)y[i + 1], (_Float16)y[i + 2], (_Float16)y[i + 3]};
-                *reinterpret_cast<half4v*>(reinterpret_cast<_Float16*>(p.o) + at + d0 + i) = h;
-            } else {
-                *reinterpret_cast<float4v*>(reinterpret_cast<float*>(p.o) + at + d0 + i) = float4v{y[i], y[i + 1], y[i + 2], y[i + 3]};
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (d0 + i >= p.c.dim) continue;
-        if (p.o_f16) reinterpret_cast<_Float16*>(p.o)[at + d0 + i] = (_Float16)y[i];
-        else reinterpret_cast<float*>(p.o)[at + d0 + i] = y[i];
-    }
 }
 
 // Workgroup: 4 waves, R tiles of 16 vectors of one KV head, one part of the tokens.  The waves take
@@ -299,7 +229,7 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
     float4v o[R][DT];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        m[r] = -__builtin_inff();
+        m[r] = kNegInf;
         l[r] = 0.0f;
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[r][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -335,18 +265,18 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
         for (int r = 0; r < R; ++r) {
             const int left = min(seen[r], cap) - j - 4 * g;
             float x[8];
-            float top = -__builtin_inff();
+            float top = kNegInf;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float y = __builtin_fmaf(sc[t][r][i] * unit[r], d.ks[t][i], lv[4 * t + i]);
                     // masked tokens are chosen away, whatever their scales hold
-                    x[4 * t + i] = 16 * t + i < left ? y : -__builtin_inff();
+                    x[4 * t + i] = 16 * t + i < left ? y : kNegInf;
                     top = fmaxf(top, x[4 * t + i]);
                 }
             top = over_groups<true>(top);
-            if (__builtin_amdgcn_ballot_w64(top > m[r])) {
+            if (__builtin_amdgcn_ballot_w64(top > m[r] + kSlack)) {
                 const float m_new = fmaxf(m[r], top);
                 const float fade = m[r] == m_new ? 1.0f : __builtin_amdgcn_exp2f(m[r] - m_new);
                 m[r] = m_new;
@@ -354,7 +284,7 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) o[r][t] *= fade;
             }
-            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r] - kPShift;
+            const float base = m[r] == kNegInf ? 0.0f : m[r] - kPShift;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float e = __builtin_amdgcn_exp2f(x[i] - base);
@@ -406,7 +336,7 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
     for (int r = 0; r < R; ++r) {
         const int v = 16 * r + n;
         m_all[r] = fmaxf(fmaxf(lds_m[0][v], lds_m[1][v]), fmaxf(lds_m[2][v], lds_m[3][v]));
-        const float base = m_all[r] == -__builtin_inff() ? 0.0f : m_all[r];
+        const float base = m_all[r] == kNegInf ? 0.0f : m_all[r];
         l_all[r] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) l_all[r] += lds_l[w][v] * __builtin_amdgcn_exp2f(lds_m[w][v] - base);
@@ -495,10 +425,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4, lane = threadIdx.x & 63;
     const int64_t row = s.row0 + t, slot = (row * p.q_heads + head) * p.parts;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot;
-    float m = -__builtin_inff();
+    float m = kNegInf;
     for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[i].x);
     m = wave_max(m);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
+    const float base = m == kNegInf ? 0.0f : m;
     float l = 0.0f;
     float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -524,9 +454,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, d, y);
 }
 
-// Vectors of a workgroup, given how many share its tokens.  Two tiles of 256 columns would not fit
-// the registers.
-int tile_of(int64_t vectors, int dim_padded) { return vectors <= 16 || dim_padded > 128 ? 16 : 32; }
+// Vectors of a workgroup, given how many share its tokens: this file's kernel for up to two tiles (two
+// of 256 columns would not fit the registers), else the wide one.
+int tile_of(int64_t vectors, int dim_padded) {
+    if (vectors <= 16) return 16;
+    return vectors <= 32 && dim_padded <= 128 ? 32 : kAttendWide;
+}
 
 template <int DP, int R, int LIMBS, bool SHARED>
 hipError_t launch_r(const AttendParams& p, hipStream_t st) {
@@ -540,6 +473,7 @@ hipError_t launch_r(const AttendParams& p, hipStream_t st) {
 template <int DP, int LIMBS, bool SHARED>
 hipError_t launch_part(const AttendParams& p, hipStream_t st) {
     const int tile = SHARED ? attend_tile_prefix(p) : attend_tile(p);
+    if (tile == kAttendWide) return launch_attend_wide(p, SHARED, st);
     if constexpr (DP <= 128)
         if (tile == 32) return launch_r<DP, 2, LIMBS, SHARED>(p, st);
     return launch_r<DP, 1, LIMBS, SHARED>(p, st);

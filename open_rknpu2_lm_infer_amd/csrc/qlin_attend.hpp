@@ -1,0 +1,83 @@
+// Parts that the attention kernels share: exact fp16 codes from the cache's bytes, query rows, output rows.
+#pragma once
+
+#include "qlin_kv.hpp"
+#include "qlin_rows.hpp"
+
+namespace qlin {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+constexpr float kNan = __builtin_nanf("");
+constexpr float kNegInf = -__builtin_inff();
+
+// P is scaled by 2^kPShift before it is rounded to fp16 (11 bits), so that it stays normal down to
+// 2^-22 and non-zero down to 2^-32 of the largest; the factor is in the sum too and cancels.
+constexpr float kPShift = 8.0f;
+
+// Two fp16 codes times 2^-9 from bytes i and j of the cache (code + 128) that sel picks from
+// (hi, lo): the permuted pair is (b_i, b_j) * 2^-24, both exact; * 2^15 - 128 * 2^-9 is exact.
+__device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t sel) {
+    const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(hi, lo, sel));
+    const half2v m = {(_Float16)32768.0f, (_Float16)32768.0f}, a = {(_Float16)-0.25f, (_Float16)-0.25f};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, m, a));
+}
+constexpr float kCodeUnit = 512.0f;  // 1 / 2^-9
+
+// Eight codes of consecutive columns, bytes of (w0, w1).
+__device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
+    const uint4v r = {codes2(w0, w0, 0x0c010c00u), codes2(w0, w0, 0x0c030c02u), codes2(w1, w1, 0x0c010c00u),
+                      codes2(w1, w1, 0x0c030c02u)};
+    return __builtin_bit_cast(half8v, r);
+}
+
+// The running maximum of a vector is raised only when a token passes it by more than this (bits): most
+// steps leave the output as it is.  P stays at or below 2^(kPShift + kSlack), inside fp16.
+constexpr float kSlack = 5.0f;
+
+// fp16 high part, and the rest (exact in fp16 unless it underflows) where f32 is asked for.
+template <int LIMBS>
+__device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
+    out[0] = (_Float16)x;
+    if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
+}
+
+// Eight columns of a query row, d0 on, as f32; columns past the head's are zeros.
+__device__ __forceinline__ void load_query(const AttendParams& p, int64_t at, int d0, float x[8]) {
+    const int left = p.c.dim - d0;
+    if (p.q_vec) {  // 16-byte aligned heads of whole groups of 8
+        if (p.q_f16) load8<__half, true>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
+        else load8<float, true>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
+    } else if (p.q_f16) load8<__half, false>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
+    else load8<float, false>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
+}
+
+// N consecutive columns of an output row.
+template <int N>
+__device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int d0, const float* y) {
+    if (p.o_vec && N % 4 == 0) {  // 16-byte aligned heads of whole groups of 8
+        if (d0 >= p.c.dim) return;
+#pragma unroll
+        for (int i = 0; i + 4 <= N; i += 4) {
+            if (p.o_f16) {
+                typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+                const half4v h = {(_Float16)y[i], (_Float16)y[i + 1], (_Float16)y[i + 2], (_Float16)y[i + 3]};
+                *reinterpret_cast<half4v*>(reinterpret_cast<_Float16*>(p.o) + at + d0 + i) = h;
+            } else {
+                *reinterpret_cast<float4v*>(reinterpret_cast<float*>(p.o) + at + d0 + i) = float4v{y[i], y[i + 1], y[i + 2], y[i + 3]};
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (d0 + i >= p.c.dim) continue;
+        if (p.o_f16) reinterpret_cast<_Float16*>(p.o)[at + d0 + i] = (_Float16)y[i];
+        else reinterpret_cast<float*>(p.o)[at + d0 + i] = y[i];
+    }
+}
+
+}  // namespace qlin

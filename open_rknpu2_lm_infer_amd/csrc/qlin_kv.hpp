@@ -88,6 +88,8 @@ constexpr int kAttendStep = 128;
 // Vectors of a workgroup: over a sequence's own tokens, over the prefix.
 int attend_tile(const AttendParams& p);
 int attend_tile_prefix(const AttendParams& p);
+constexpr int kAttendWide = 128;  // of the kernel for many vectors
 hipError_t launch_attend(const AttendParams& p, hipStream_t stream);
+hipError_t launch_attend_wide(const AttendParams& p, bool prefix, hipStream_t stream);
 
 }  // namespace qlin

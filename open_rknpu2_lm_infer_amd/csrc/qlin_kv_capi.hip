@@ -71,13 +71,17 @@ int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     return e == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
 }
 
-// Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part: enough parts that
-// the launch covers the CUs some times over (a workgroup's loads alone do not keep its CU's share of
-// the HBM busy, and ragged sequences end at different times), at least one step of a workgroup each,
-// at most `cap` of them.
-void cut(int64_t tokens, int64_t blocks, int cus, int64_t cap, int* parts, int* chunk) {
+// Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part of `tile` vectors each:
+// enough parts that the launch covers the CUs some times over (a workgroup's loads alone do not keep
+// its CU's share of the HBM busy), at least one step of a workgroup each, at most `cap`.
+// Parts of the kernel for few vectors hold at most kMaxChunk tokens: ragged sequences then end in many
+// workgroups of one size, and the results kept for the join stay under 2% of the bytes read.
+constexpr int kMaxChunk = 512;
+void cut(int64_t tokens, int64_t blocks, int tile, int cus, int64_t cap, int* parts, int* chunk) {
     const int64_t steps = std::max<int64_t>(1, ceil_div(tokens, kAttendStep));
-    const int64_t want = std::max<int64_t>(1, std::min({steps, ceil_div((int64_t)cus * 4, blocks), cap}));
+    int64_t want = ceil_div((int64_t)cus * (tile == kAttendWide ? 2 : 4), blocks);
+    if (tile != kAttendWide) want = std::max(want, ceil_div(tokens, kMaxChunk));
+    want = std::max<int64_t>(1, std::min({steps, want, cap}));
     const int64_t per = ceil_div(steps, want);
     *chunk = (int)(per * kAttendStep);
     *parts = (int)ceil_div(steps, per);
@@ -121,8 +125,9 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     const bool apart = prefix > 0 && cap >= 2;
     p.own_from = apart ? prefix : 0;
     int parts = 1;
-    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, wp.cu_count, apart ? cap / 2 : cap, &parts, &p.chunk);
-    if (apart) cut(prefix, prefix_blocks, wp.cu_count, cap - parts, &p.prefix_parts, &p.prefix_chunk);
+    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, attend_tile(p), wp.cu_count, apart ? cap / 2 : cap, &parts,
+        &p.chunk);
+    if (apart) cut(prefix, prefix_blocks, attend_tile_prefix(p), wp.cu_count, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
     if (std::max({own_blocks * parts, prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs}) > kKvMaxGrid)
         return QLIN_ERR_UNSUPPORTED;
