@@ -75,17 +75,7 @@ struct StepData {
     Bytes<DP / 4> k[2];
     Bytes<DP / 16> v[8];
     float4v ks[2], vs[2];  // scales of tokens 4g .. 4g + 3
-    bool bad;
 };
-
-template <int DP>
-__device__ __forceinline__ void load_tile(StepData<DP>& r, const Tile& b, int t, int n, int g) {
-    load_bytes<DP / 4>(r.k[t], b.k, n * DP + g * (DP / 4));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load_bytes<DP / 16>(r.v[4 * t + i], b.v, (4 * g + i) * DP + n * (DP / 16));
-    r.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(b.ks, 16 * g, 0, 0));
-    r.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(b.vs, 16 * g, 0, 0));
-}
 
 // Sum and maximum over the four lanes n, n + 16, n + 32, n + 48.
 template <bool MAX>
@@ -99,12 +89,12 @@ __device__ __forceinline__ float over_groups(float x) {
 
 // Workgroup: 4 waves, R tiles of 16 vectors of one KV head, one part of the tokens.  The waves take
 // steps of 32 tokens in turn, each with a running maximum, sum and output of its own, and join
-// them at the end: nothing is shared before that, and a step's loads are issued a step ahead.
+// them at the end: nothing is shared before that.
 // LIMBS = 2 (f32 rows in or out): queries and P as a sum of two fp16 values, 22 bits; fp16 queries are
 // exact with one, and P rounded to 11 bits is off by as much as an fp16 output.
 // SHARED: the part of the prefix, for the rows of all sequences at once.
-template <int DP, int R, int LIMBS, bool SHARED>
-__global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
+template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
+__global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 128 ? 3 : 1) void attend_kernel(AttendParams p) {
     constexpr int KS = DP / 32;   // matrix steps of a q . k
     constexpr int DT = DP / 16;   // tiles of 16 output columns
     constexpr int VT = 16 * R;    // vectors of the workgroup
@@ -114,16 +104,20 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int parts = SHARED ? p.prefix_parts : p.parts - p.prefix_parts;
     const int chunk = SHARED ? p.prefix_chunk : p.chunk;
+    // heads fastest, parts slowest: workgroups go to the 8 XCDs in turn, and the later parts of ragged
+    // sequences are empty.  (With the parts fastest, 64 sequences of 1024 tokens in a batch cut for
+    // 4096 in four parts ran on two XCDs: 68 us against 26.)
     int b = blockIdx.x;
-    const int part = b % parts;
-    b /= parts;
-    const int h = b % p.c.heads;
-    b /= p.c.heads;
+    const int h = p.by_heads.mod(b);
+    b = p.by_heads.div(b);
+    const int tile = (SHARED ? p.by_prefix_tiles : p.by_tiles).mod(b);
+    b = (SHARED ? p.by_prefix_tiles : p.by_tiles).div(b);
+    const int seq = SHARED ? 0 : p.by_seqs.mod(b), part = SHARED ? b : p.by_seqs.div(b), v0 = tile * VT;
+    const int group = p.group.d;
 
     // the vectors: (row, head) pairs from first_row on, and how many tokens each sees (-1: no vector)
-    int first_row, seq = 0, cap, end;
+    int first_row, cap, end;
     const int j0 = (SHARED ? 0 : p.own_from) + part * chunk;
     int seen[R];
     if constexpr (SHARED) {
@@ -133,12 +127,12 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
         if (tid == 0) lds_most = 0;
         if (tid < VT) lds_seen[tid] = -1;
         __syncthreads();
-        const int v0 = b * VT, r_lo = v0 / p.group, r_hi = min((v0 + VT - 1) / p.group + 1, p.b.rows);
+        const int r_lo = p.group.div(v0), r_hi = min(p.group.div(v0 + VT - 1) + 1, p.b.rows);
         for (int i = tid; i < p.b.seqs; i += 256) {
             const KvSeq q = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
             for (int r = max(q.row0, r_lo); r < min(q.row0 + q.rows, r_hi); ++r) {
                 const int y = kv_visible(q, r - q.row0);
-                for (int x = max(r * p.group, v0); x < min((r + 1) * p.group, v0 + VT); ++x) lds_seen[x - v0] = y;
+                for (int x = max(r * group, v0); x < min((r + 1) * group, v0 + VT); ++x) lds_seen[x - v0] = y;
                 atomicMax(&lds_most, y);
             }
         }
@@ -147,61 +141,83 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) seen[r] = lds_seen[16 * r + n];
     } else {
-        const int tiles = (p.b.max_new * p.group + VT - 1) / VT;
-        seq = b / tiles;
-        b -= seq * tiles;
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
         if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
-        if (b * VT >= s.rows * p.group) return;
+        if (v0 >= s.rows * group) return;
         if (part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
         first_row = s.row0;
         cap = min(s.len, j0 + chunk);
-        end = min(cap, kv_visible(s, min(b * VT + VT - 1, s.rows * p.group - 1) / p.group));  // its last row sees most
+        end = min(cap, kv_visible(s, p.group.div(min(v0 + VT - 1, s.rows * group - 1))));  // its last row sees most
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int v = b * VT + 16 * r + n;
-            seen[r] = v < s.rows * p.group ? kv_visible(s, v / p.group) : -1;
+            const int v = v0 + 16 * r + n;
+            seen[r] = v < s.rows * group ? kv_visible(s, p.group.div(v)) : -1;
         }
     }
     end = __builtin_amdgcn_readfirstlane(end);
-    const int v0 = b * VT;
+
+    // the queries' loads first: they do not wait for page ids (vectors that are none take the first row's)
+    QueryRow<KS, Q16> qr[R];
+    int64_t out_row[R];
+    int head[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int v = seen[r] >= 0 ? v0 + 16 * r + n : 0;
+        out_row[r] = first_row + p.group.div(v);
+        head[r] = h * group + p.group.mod(v);
+        load_query<KS, 8, Q16>(p, qr[r], out_row[r] * p.ldq + (int64_t)head[r] * p.c.dim, g * (DP / 4));
+    }
 
     // page ids through the scalar cache: nothing writes them while the kernel runs
     const const_ids table = (const_ids)(uintptr_t)(p.b.table + seq * p.b.table_ld);
     const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
-    bool bad_page = false;
-    auto load_step = [&](StepData<DP>& d, int j) {
-        d.bad = false;
+    bool bad_page = false, bad = false, bad_next = false;
+    StepData<DP> d;
+    Tile next[2];
+    auto find_step = [&](int j) {
+        bad_next = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int jt = j + 16 * t, jj = min(jt, end - 1);
             int id = -1;
             if (end > 0) id = SHARED || jj < p.prefix ? prefix[jj >> p.c.shift] : table[jj >> p.c.shift];
-            const Tile x = find_tile<DP>(p.c, id, h, jt & off_mask, jt < end);
-            load_tile<DP>(d, x, t, n, g);
-            if (jt < end) d.bad |= x.bad;
+            next[t] = find_tile<DP>(p.c, id, h, jt & off_mask, jt < end);
+            if (jt < end) bad_next |= next[t].bad;
         }
-        bad_page |= d.bad;
+        bad_page |= bad_next;
+    };
+    auto load_k = [&] {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) load_bytes<DP / 4>(d.k[t], next[t].k, n * DP + g * (DP / 4));
+    };
+    auto load_scales = [&] {
+        bad = bad_next;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            d.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].ks, 16 * g, 0, 0));
+            d.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].vs, 16 * g, 0, 0));
+        }
+    };
+    auto load_v = [&] {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_bytes<DP / 16>(d.v[i], next[i / 4].v, (4 * g + i % 4) * DP + n * (DP / 16));
     };
     int j = j0 + 32 * wave;
-    StepData<DP> d0, d1;
-    load_step(d0, j);
+    find_step(j);
+    load_k();
+    load_scales();
+    load_v();
 
     // queries, as the B operand: lane (n, g) holds columns g * DP/4 + 8 s .. + 7 of vector n
     half8v qf[R][KS][LIMBS];
     float unit[R];  // what the f16 operands were divided by, times scale2
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int v = v0 + 16 * r + n;
-        const bool ok = seen[r] >= 0;
-        const int row = first_row + (ok ? v / p.group : 0), head = h * p.group + (ok ? v % p.group : 0);
-        const int64_t at = (int64_t)row * p.ldq + (int64_t)head * p.c.dim;
         unit[r] = p.scale2 * kCodeUnit;
-        float x[DP / 4] = {};
+        float x[DP / 4];
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-            if (ok) load_query(p, at, g * (DP / 4) + 8 * k, x + 8 * k);
+        for (int i = 0; i < DP / 4; ++i) x[i] = query_at<KS, Q16>(qr[r], i / 8, i % 8);
         if constexpr (LIMBS == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float m = 0.0f;
@@ -235,7 +251,10 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
         for (int t = 0; t < DT; ++t) o[r][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto work = [&](const StepData<DP>& d, int j) {
+    // The next step's keys are loaded over this one's when those are used, then its scales, then its values:
+    // one set of registers, and some loads are in flight at any time.
+    for (; j < end; j += kAttendStep) {
+        find_step(j + kAttendStep);
         // S^T: tokens 16 t + 4 g + i of vector n
         float4v sc[2][R];
 #pragma unroll
@@ -252,12 +271,14 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
                         sc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[r][k][q], sc[t][r], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k();
         float lv[8], iv[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                lv[4 * t + i] = d.bad ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
+                lv[4 * t + i] = bad ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
                 iv[4 * t + i] = __builtin_amdgcn_rcpf(d.vs[t][i]);
             }
         half8v pf[R][LIMBS];
@@ -295,6 +316,8 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
                 for (int q = 0; q < LIMBS; ++q) pf[r][q][i] = y[q];
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_scales();
         // O^T: columns n * DP/16 + t (row n of the operand) over tokens 4g + i of both tiles
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -308,16 +331,8 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
                 for (int q = 0; q < LIMBS; ++q)
                     o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r][q], o[r][t], 0, 0, 0);
         }
-    };
-    for (;;) {
-        if (j >= end) break;
-        load_step(d1, j + kAttendStep);
-        work(d0, j);
-        j += kAttendStep;
-        if (j >= end) break;
-        load_step(d0, j + kAttendStep);
-        work(d1, j);
-        j += kAttendStep;
+        __builtin_amdgcn_sched_barrier(0);
+        load_v();
     }
     if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
 
@@ -381,9 +396,6 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (seen[r] < 0) continue;
-        const int v = v0 + 16 * r + n;
-        const int64_t row = first_row + v / p.group;
-        const int head = h * p.group + v % p.group;
         if (p.parts == 1) {
             const float f = l_all[r] == 0.0f ? 0.0f : kCodeUnit / l_all[r];
 #pragma unroll
@@ -392,10 +404,10 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendParams p) {
                 for (int u = 0; u < DT / 4; ++u) {
                     const float4v y = four(r, i, u) * f;
                     const float z[4] = {y[0], y[1], y[2], y[3]};
-                    store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, (4 * g + i) * DT + 4 * u, z);
+                    store_out<4>(p, out_row[r] * p.ldo + (int64_t)head[r] * p.c.dim, (4 * g + i) * DT + 4 * u, z);
                 }
         } else {
-            const int64_t slot = (row * p.q_heads + head) * p.parts + (SHARED ? 0 : p.prefix_parts) + part;
+            const int64_t slot = (out_row[r] * p.q_heads + head[r]) * p.parts + (SHARED ? 0 : p.prefix_parts) + part;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -461,45 +473,51 @@ int tile_of(int64_t vectors, int dim_padded) {
     return vectors <= 32 && dim_padded <= 128 ? 32 : kAttendWide;
 }
 
-template <int DP, int R, int LIMBS, bool SHARED>
+template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_r(const AttendParams& p, hipStream_t st) {
-    const int64_t vectors = (int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group;
+    const int64_t vectors = (int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group.d;
     const int64_t blocks = (int64_t)(SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs) *
                            p.c.heads * ((vectors + 16 * R - 1) / (16 * R));
-    attend_kernel<DP, R, LIMBS, SHARED><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    attend_kernel<DP, R, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
-template <int DP, int LIMBS, bool SHARED>
+template <int DP, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_part(const AttendParams& p, hipStream_t st) {
     const int tile = SHARED ? attend_tile_prefix(p) : attend_tile(p);
     if (tile == kAttendWide) return launch_attend_wide(p, SHARED, st);
     if constexpr (DP <= 128)
-        if (tile == 32) return launch_r<DP, 2, LIMBS, SHARED>(p, st);
-    return launch_r<DP, 1, LIMBS, SHARED>(p, st);
+        if (tile == 32) return launch_r<DP, 2, LIMBS, Q16, SHARED>(p, st);
+    return launch_r<DP, 1, LIMBS, Q16, SHARED>(p, st);
 }
 
-template <int DP, int LIMBS>
-hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
+template <int DP, int LIMBS, bool Q16>
+hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     if (p.prefix_parts)
-        if (hipError_t e = launch_part<DP, LIMBS, true>(p, st)) return e;
-    if (hipError_t e = launch_part<DP, LIMBS, false>(p, st)) return e;
-    if (p.parts == 1) return hipSuccess;
+        if (hipError_t e = launch_part<DP, LIMBS, Q16, true>(p, st)) return e;
+    return launch_part<DP, LIMBS, Q16, false>(p, st);
+}
+
+template <int DP>
+hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
+    const hipError_t e = !p.q_f16 ? launch_typed<DP, 2, false>(p, st)
+                         : p.o_f16 ? launch_typed<DP, 1, true>(p, st)
+                                   : launch_typed<DP, 2, true>(p, st);
+    if (e != hipSuccess || p.parts == 1) return e;
     attend_join_kernel<DP><<<dim3((uint32_t)((int64_t)p.b.max_new * p.q_heads * p.b.seqs)), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int attend_tile(const AttendParams& p) { return tile_of((int64_t)p.b.max_new * p.group, p.c.dim_padded); }
-int attend_tile_prefix(const AttendParams& p) { return tile_of((int64_t)p.b.rows * p.group, p.c.dim_padded); }
+int attend_tile(const AttendParams& p) { return tile_of((int64_t)p.b.max_new * p.group.d, p.c.dim_padded); }
+int attend_tile_prefix(const AttendParams& p) { return tile_of((int64_t)p.b.rows * p.group.d, p.c.dim_padded); }
 
 hipError_t launch_attend(const AttendParams& p, hipStream_t st) {
-    const bool two = !p.q_f16 || !p.o_f16;
     switch (p.c.dim_padded) {
-        case 64: return two ? launch_dp<64, 2>(p, st) : launch_dp<64, 1>(p, st);
-        case 128: return two ? launch_dp<128, 2>(p, st) : launch_dp<128, 1>(p, st);
-        default: return two ? launch_dp<256, 2>(p, st) : launch_dp<256, 1>(p, st);
+        case 64: return launch_dp<64>(p, st);
+        case 128: return launch_dp<128>(p, st);
+        default: return launch_dp<256>(p, st);
     }
 }
 

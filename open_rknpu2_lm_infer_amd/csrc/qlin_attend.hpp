@@ -45,14 +45,49 @@ __device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
     if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
 }
 
-// Eight columns of a query row, d0 on, as f32; columns past the head's are zeros.
-__device__ __forceinline__ void load_query(const AttendParams& p, int64_t at, int d0, float x[8]) {
-    const int left = p.c.dim - d0;
-    if (p.q_vec) {  // 16-byte aligned heads of whole groups of 8
-        if (p.q_f16) load8<__half, true>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
-        else load8<float, true>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
-    } else if (p.q_f16) load8<__half, false>(reinterpret_cast<const __half*>(p.q) + at + d0, 0, left, x);
-    else load8<float, false>(reinterpret_cast<const float*>(p.q) + at + d0, 0, left, x);
+// Columns of a query row on their way to the matrix core: KS groups of eight from column first on, STEP
+// apart, as they lie in memory; columns past the head's are zeros.  All loads are issued before any is used.
+template <int KS, bool Q16>
+struct QueryRow {
+    uint4v w[KS][Q16 ? 1 : 2];
+};
+template <int KS, int STEP, bool Q16>
+__device__ __forceinline__ void load_query(const AttendParams& p, QueryRow<KS, Q16>& r, int64_t at, int first) {
+    constexpr int W = Q16 ? 1 : 2;
+    if (p.q_vec) {  // heads of whole groups of 8, 16-byte aligned
+        const uint8_t* q = reinterpret_cast<const uint8_t*>(p.q) + (at + first) * (2 * W);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const bool in = first + k * STEP < p.c.dim;
+#pragma unroll
+            for (int i = 0; i < W; ++i) r.w[k][i] = *reinterpret_cast<const uint4v*>(q + (in ? k * STEP * 2 * W : -first * 2 * W) + 16 * i);
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < W; ++i) r.w[k][i] = first + k * STEP < p.c.dim ? r.w[k][i] : uint4v{0, 0, 0, 0};
+    } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4 * W; ++i) {
+                const int d = first + k * STEP + (Q16 ? 2 * i : i), last = p.c.dim - 1;
+                uint32_t x;
+                if constexpr (Q16) {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + at;
+                    x = (d <= last ? (uint32_t)q[min(d, last)] : 0) | (d < last ? (uint32_t)q[min(d + 1, last)] : 0) << 16;
+                } else {
+                    x = d <= last ? reinterpret_cast<const uint32_t*>(p.q)[at + d] : 0;
+                }
+                r.w[k][i / 4][i % 4] = x;
+            }
+    }
+}
+// Element i of group k.
+template <int KS, bool Q16>
+__device__ __forceinline__ float query_at(const QueryRow<KS, Q16>& r, int k, int i) {
+    if constexpr (Q16) return (float)__builtin_bit_cast(half8v, r.w[k][0])[i];
+    else return __uint_as_float(r.w[k][i / 4][i % 4]);
 }
 
 // N consecutive columns of an output row.

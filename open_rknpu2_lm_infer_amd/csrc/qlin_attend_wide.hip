@@ -44,7 +44,7 @@ __device__ __forceinline__ int key_row(int i) { return (threadIdx.x + i * kThrea
 template <int DP>
 __device__ __forceinline__ int value_group(int i) { return (threadIdx.x + i * kThreads) / (DP / 4); }  // 2 c + h
 
-template <int DP, int LIMBS, bool SHARED>
+template <int DP, int LIMBS, bool Q16, bool SHARED>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
     using L = TileLds<DP>;
     using Sh = Share<DP>;
@@ -52,17 +52,18 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int parts = SHARED ? p.prefix_parts : p.parts - p.prefix_parts;
+    const int group = p.group.d;
     const int chunk = SHARED ? p.prefix_chunk : p.chunk;
-    // heads fastest: with 8 of them, neighbours in the launch order (8 XCDs in turn) read the same
-    // head's tokens from the same XCD's L2; then the vectors, those that see most first
+    // heads fastest: with 8 of them, neighbours in the launch order (8 XCDs in turn) read the same head's
+    // tokens from the same XCD's L2; then the vectors, those that see most first; parts slowest, as the
+    // later ones of ragged sequences are empty
     int b = blockIdx.x;
-    const int h = b % p.c.heads;
-    b /= p.c.heads;
-    const int tiles = ((SHARED ? p.b.rows : p.b.max_new) * p.group + kAttendWide - 1) / kAttendWide;
-    const int v0 = (tiles - 1 - b % tiles) * kAttendWide;
-    b /= tiles;
-    const int part = b % parts, seq = b / parts;
+    const int h = p.by_heads.mod(b);
+    b = p.by_heads.div(b);
+    const FastDiv& by_tiles = SHARED ? p.by_prefix_tiles : p.by_tiles;
+    const int v0 = ((int)by_tiles.d - 1 - by_tiles.mod(b)) * kAttendWide;
+    b = by_tiles.div(b);
+    const int seq = SHARED ? 0 : p.by_seqs.mod(b), part = SHARED ? b : p.by_seqs.div(b);
 
     // how many tokens each vector sees (-1: no vector)
     int first_row = 0, cap, end, seen;
@@ -73,12 +74,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         cap = min(p.prefix, j0 + chunk);
         if (tid < kAttendWide) lds_seen[tid] = -1;
         __syncthreads();
-        const int r_lo = v0 / p.group, r_hi = min((v0 + kAttendWide - 1) / p.group + 1, p.b.rows);
+        const int r_lo = p.group.div(v0), r_hi = min(p.group.div(v0 + kAttendWide - 1) + 1, p.b.rows);
         for (int i = tid; i < p.b.seqs; i += kThreads) {
             const KvSeq q = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
             for (int r = max(q.row0, r_lo); r < min(q.row0 + q.rows, r_hi); ++r) {
                 const int y = kv_visible(q, r - q.row0);
-                for (int x = max(r * p.group, v0); x < min((r + 1) * p.group, v0 + kAttendWide); ++x) lds_seen[x - v0] = y;
+                for (int x = max(r * group, v0); x < min((r + 1) * group, v0 + kAttendWide); ++x) lds_seen[x - v0] = y;
             }
         }
         __syncthreads();
@@ -91,12 +92,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
         if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
-        if (v0 >= s.rows * p.group) return;
+        if (v0 >= s.rows * group) return;
         if (part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
         first_row = s.row0;
         cap = min(s.len, j0 + chunk);
-        end = min(cap, kv_visible(s, min(v0 + kAttendWide - 1, s.rows * p.group - 1) / p.group));
-        seen = v < s.rows * p.group ? kv_visible(s, v / p.group) : -1;
+        end = min(cap, kv_visible(s, p.group.div(min(v0 + kAttendWide - 1, s.rows * group - 1))));
+        seen = v < s.rows * group ? kv_visible(s, p.group.div(v)) : -1;
     }
     end = __builtin_amdgcn_readfirstlane(end);
     int most = seen, least = seen < 0 ? 0x7fffffff : seen;  // over the wave's vectors
@@ -182,42 +183,38 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         }
     };
 
-    // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of vector n
+    // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of vector n (vectors that are
+    // none take the first row's)
     half8v qf[KS][LIMBS];
     float unit = 1.0f;
     const bool ok = seen >= 0;
-    const int64_t row = first_row + (ok ? v / p.group : 0);
-    const int head = h * p.group + (ok ? v % p.group : 0);
+    const int64_t row = first_row + p.group.div(ok ? v : 0);
+    const int head = h * group + p.group.mod(ok ? v : 0);
     {
-        const int64_t at = row * p.ldq + (int64_t)head * p.c.dim;
+        QueryRow<KS, Q16> qr;
+        load_query<KS, 16, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
         float up = 1.0f;
         if constexpr (LIMBS == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float m = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                float x[8] = {};
-                if (ok) load_query(p, at, 16 * k + 8 * hi, x);
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-            }
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(query_at<KS, Q16>(qr, k, i)));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const int e = kv_clamp((int)((__float_as_uint(m) >> 23) & 0xff) - 127, -100, 126);
             up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
             unit = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
         }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            float x[8] = {};
-            if (ok) load_query(p, at, 16 * k + 8 * hi, x);
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 _Float16 y[LIMBS];
-                split_f16<LIMBS>(x[i] * up, y);
+                split_f16<LIMBS>(query_at<KS, Q16>(qr, k, i) * up, y);
 #pragma unroll
                 for (int q = 0; q < LIMBS; ++q) qf[k][q][i] = y[q];
             }
-        }
     }
 
     float m = kNegInf, l = 0.0f;
@@ -343,22 +340,27 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     }
 }
 
-template <int DP, int LIMBS, bool SHARED>
+template <int DP, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_one(const AttendParams& p, hipStream_t st) {
     constexpr int bytes = 2 * TileLds<DP>::BYTES;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, SHARED>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, Q16, SHARED>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (attr != hipSuccess) return attr;
-    const int64_t tiles = ((int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group + kAttendWide - 1) / kAttendWide;
+    const int64_t tiles = ((int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group.d + kAttendWide - 1) / kAttendWide;
     const int64_t blocks = tiles * p.c.heads * (SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs);
-    attend_wide_kernel<DP, LIMBS, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
+    attend_wide_kernel<DP, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
     return hipGetLastError();
+}
+
+template <int DP, bool SHARED>
+hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
+    if (!p.q_f16) return launch_one<DP, 2, false, SHARED>(p, st);
+    return p.o_f16 ? launch_one<DP, 1, true, SHARED>(p, st) : launch_one<DP, 2, true, SHARED>(p, st);
 }
 
 template <int DP>
 hipError_t launch_dp(const AttendParams& p, bool prefix, hipStream_t st) {
-    if (p.q_f16 && p.o_f16) return prefix ? launch_one<DP, 1, true>(p, st) : launch_one<DP, 1, false>(p, st);
-    return prefix ? launch_one<DP, 2, true>(p, st) : launch_one<DP, 2, false>(p, st);
+    return prefix ? launch_typed<DP, true>(p, st) : launch_typed<DP, false>(p, st);
 }
 
 }  // namespace

@@ -67,7 +67,8 @@ struct AttendParams {
     const void* q;  // [rows, ldq]
     int64_t ldq;
     int q_f16, q_vec;    // q_vec, o_vec: heads of whole groups of 8, 16-byte aligned
-    int q_heads, group;  // group = q_heads / kv heads
+    int q_heads;
+    FastDiv group;       // by q_heads / kv heads
     float scale2;        // scale * log2 e
     void* o;             // [rows, ldo]
     int64_t ldo;
@@ -79,6 +80,7 @@ struct AttendParams {
     // outputs each, then (running maximum, sum) pairs.
     int parts, prefix_parts;  // in all; of the prefix (they come first)
     int chunk, prefix_chunk;  // tokens a part
+    FastDiv by_heads, by_seqs, by_tiles, by_prefix_tiles;  // of workgroup indexes; tiles of vectors
     float* part_o;
     float* part_ml;
     uint32_t* err;

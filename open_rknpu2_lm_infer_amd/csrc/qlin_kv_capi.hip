@@ -107,7 +107,8 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.q_vec = aligned(Q, ldq, q_dtype, cache->c.dim);
     p.q_f16 = q_dtype == QLIN_F16;
     p.q_heads = q_heads;
-    p.group = q_heads / cache->c.heads;
+    const int group = q_heads / cache->c.heads;
+    p.group = fast_div(group);
     p.scale2 = scale * 1.44269504f;
     p.o = O;
     p.ldo = ldo;
@@ -119,8 +120,9 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     // parts that the workspace's scratch holds results of
     const int64_t vectors = (int64_t)p.b.rows * q_heads;
     const int64_t cap = wp.part_floats / (vectors * (cache->c.dim_padded + 2));
-    const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * ceil_div((int64_t)p.b.max_new * p.group, attend_tile(p));
-    const int64_t prefix_blocks = (int64_t)cache->c.heads * ceil_div((int64_t)p.b.rows * p.group, attend_tile_prefix(p));
+    const int64_t tiles = ceil_div((int64_t)p.b.max_new * group, attend_tile(p));
+    const int64_t prefix_tiles = ceil_div((int64_t)p.b.rows * group, attend_tile_prefix(p));
+    const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * tiles, prefix_blocks = cache->c.heads * prefix_tiles;
     // The prefix gets parts of its own where the scratch can hold its results; else every sequence reads it itself.
     const bool apart = prefix > 0 && cap >= 2;
     p.own_from = apart ? prefix : 0;
@@ -131,6 +133,10 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.parts = parts + p.prefix_parts;
     if (std::max({own_blocks * parts, prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs}) > kKvMaxGrid)
         return QLIN_ERR_UNSUPPORTED;
+    p.by_seqs = fast_div(p.b.seqs);
+    p.by_heads = fast_div(cache->c.heads);
+    p.by_tiles = fast_div((int)tiles);
+    p.by_prefix_tiles = fast_div((int)prefix_tiles);
     p.part_o = wp.part;
     p.part_ml = wp.part + vectors * p.parts * cache->c.dim_padded;
     return launch_attend(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;

@@ -13,6 +13,20 @@
 
 namespace qlin {
 
+// n / d and n % d for 0 <= n < 2^31 with one multiplication: with 2^(L-1) < d <= 2^L and
+// mul = floor(2^(31+L) / d) + 1, the product n * mul / 2^(31+L) exceeds n / d by less than 1 / d.
+struct FastDiv {
+    uint32_t mul, d;
+    int shift;
+    QLIN_HD int div(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift); }
+    QLIN_HD int mod(int n) const { return n - div(n) * static_cast<int>(d); }
+};
+inline FastDiv fast_div(int d) {
+    int l = 0;
+    while ((static_cast<int64_t>(1) << l) < d) ++l;
+    return {static_cast<uint32_t>((static_cast<uint64_t>(1) << (31 + l)) / d + 1), static_cast<uint32_t>(d), 31 + l};
+}
+
 // One sequence of a batch: its new rows are row0 .. row0 + rows - 1 of the row tensors, and the
 // t-th of them is position len - rows + t of the sequence (negative: no such token).
 struct KvSeq {

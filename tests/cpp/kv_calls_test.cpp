@@ -90,6 +90,12 @@ void index() {
         const int page = qlin::kv_page(id, 8, &bad);
         expect(page >= 0 && page < 8 && bad == (id < 0 || id >= 8), "pages in the cache");
     }
+    for (int d : {1, 2, 3, 4, 5, 7, 8, 12, 31, 32, 33, 100, 127, 1000, 1 << 16, (1 << 16) + 1, (1 << 30) - 1, 1 << 30, big}) {
+        const qlin::FastDiv f = qlin::fast_div(d);
+        for (int64_t n : {0, 1, 2, 3, 30, 31, 32, 99, 100, 101, 4095, 4096, 1 << 20, (1 << 30) - 1, 1 << 30, big - 1, big})
+            for (int64_t x : {n, n / d * d, n / d * d - 1, n / d * d + d - 1})
+                if (x >= 0 && x <= big) expect(f.div((int)x) == x / d && f.mod((int)x) == x % d, "division by multiplication");
+    }
     for (int tokens : {low, -5, 0, 1, 128, 129, 256, 1 << 30})
         expect(qlin::kv_parts(tokens, 128) == (tokens <= 128 ? 1 : (int)(((int64_t)tokens + 127) / 128)), "parts");
 }
