@@ -19,54 +19,6 @@
 namespace qlin {
 namespace {
 
-template <int N>
-struct Bytes {
-    uint32_t w[N / 4];
-};
-
-typedef const __attribute__((address_space(4))) int32_t* const_ids;
-typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
-
-// Where a wave finds 16 tokens: their keys, values and scales as buffers of exactly that size, so
-// that an absent tile (past the end, or on a page outside the cache) reads zeros without an access.
-struct Tile {
-    __amdgpu_buffer_rsrc_t k, v, ks, vs;
-    bool bad;  // the page id was outside the cache
-};
-
-template <int DP>
-__device__ __forceinline__ Tile find_tile(const KvCache& c, int id, int head, int off, bool there) {
-    Tile t;
-    t.bad = false;
-    const int page = kv_page(id, c.pages, &t.bad);
-    there = there && !t.bad;
-    const KvBlock<DP> b(c, page, head);
-    constexpr int flags = 0x00027000;  // raw, 32-bit elements
-    t.k = __builtin_amdgcn_make_buffer_rsrc(b.k(off), (short)0, there ? 16 * DP : 0, flags);
-    t.v = __builtin_amdgcn_make_buffer_rsrc(b.v(off), (short)0, there ? 16 * DP : 0, flags);
-    t.ks = __builtin_amdgcn_make_buffer_rsrc(b.ks(off), (short)0, there ? 64 : 0, flags);
-    t.vs = __builtin_amdgcn_make_buffer_rsrc(b.vs(off), (short)0, there ? 64 : 0, flags);
-    return t;
-}
-
-// N consecutive bytes of a buffer.
-template <int N>
-__device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at) {
-    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
-    else if constexpr (N == 8) {
-        const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
-        r.w[0] = x[0];
-        r.w[1] = x[1];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 16; ++i) {
-            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, 0, 0));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
-        }
-    }
-}
-
 // What a wave loads for one step of 32 tokens: two tiles of 16.  Lane l (n = l % 16, g = l / 16)
 // holds, as the matrix core's A operand, columns g * DP/4 .. + DP/4 - 1 of key n of each tile, and
 // columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
@@ -467,10 +419,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 }
 
 // Vectors of a workgroup, given how many share its tokens: this file's kernel for up to two tiles (two
-// of 256 columns would not fit the registers), else the wide one.
-int tile_of(int64_t vectors, int dim_padded) {
+// of 256 columns would not fit the registers), else the wide one, with two tiles a wave (fp16
+// rows of up to 128 columns) from where its workgroups are filled.
+int tile_of(const AttendParams& p, int64_t vectors) {
     if (vectors <= 16) return 16;
-    return vectors <= 32 && dim_padded <= 128 ? 32 : kAttendWide;
+    if (vectors <= 32 && p.c.dim_padded <= 128) return 32;
+    return kAttendWide;
 }
 
 template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
@@ -485,7 +439,7 @@ hipError_t launch_r(const AttendParams& p, hipStream_t st) {
 template <int DP, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_part(const AttendParams& p, hipStream_t st) {
     const int tile = SHARED ? attend_tile_prefix(p) : attend_tile(p);
-    if (tile == kAttendWide) return launch_attend_wide(p, SHARED, st);
+    if (tile >= kAttendWide) return launch_attend_wide(p, SHARED, st);
     if constexpr (DP <= 128)
         if (tile == 32) return launch_r<DP, 2, LIMBS, Q16, SHARED>(p, st);
     return launch_r<DP, 1, LIMBS, Q16, SHARED>(p, st);
@@ -510,8 +464,8 @@ hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
 
 }  // namespace
 
-int attend_tile(const AttendParams& p) { return tile_of((int64_t)p.b.max_new * p.group.d, p.c.dim_padded); }
-int attend_tile_prefix(const AttendParams& p) { return tile_of((int64_t)p.b.rows * p.group.d, p.c.dim_padded); }
+int attend_tile(const AttendParams& p) { return tile_of(p, (int64_t)p.b.max_new * p.group.d); }
+int attend_tile_prefix(const AttendParams& p) { return tile_of(p, (int64_t)p.b.rows * p.group.d); }
 
 hipError_t launch_attend(const AttendParams& p, hipStream_t st) {
     switch (p.c.dim_padded) {

@@ -115,4 +115,52 @@ __device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int
     }
 }
 
+template <int N>
+struct Bytes {
+    uint32_t w[N / 4];
+};
+
+typedef const __attribute__((address_space(4))) int32_t* const_ids;
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+
+// Where a wave finds 16 tokens: their keys, values and scales as buffers of exactly that size, so
+// that an absent tile (past the end, or on a page outside the cache) reads zeros without an access.
+struct Tile {
+    __amdgpu_buffer_rsrc_t k, v, ks, vs;
+    bool bad;  // the page id was outside the cache
+};
+
+template <int DP>
+__device__ __forceinline__ Tile find_tile(const KvCache& c, int id, int head, int off, bool there) {
+    Tile t;
+    t.bad = false;
+    const int page = kv_page(id, c.pages, &t.bad);
+    there = there && !t.bad;
+    const KvBlock<DP> b(c, page, head);
+    constexpr int flags = 0x00027000;  // raw, 32-bit elements
+    t.k = __builtin_amdgcn_make_buffer_rsrc(b.k(off), (short)0, there ? 16 * DP : 0, flags);
+    t.v = __builtin_amdgcn_make_buffer_rsrc(b.v(off), (short)0, there ? 16 * DP : 0, flags);
+    t.ks = __builtin_amdgcn_make_buffer_rsrc(b.ks(off), (short)0, there ? 64 : 0, flags);
+    t.vs = __builtin_amdgcn_make_buffer_rsrc(b.vs(off), (short)0, there ? 64 : 0, flags);
+    return t;
+}
+
+// N consecutive bytes of a buffer.
+template <int N>
+__device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at) {
+    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
+    else if constexpr (N == 8) {
+        const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
+        r.w[0] = x[0];
+        r.w[1] = x[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i) {
+            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, 0, 0));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
+        }
+    }
+}
+
 }  // namespace qlin

@@ -79,8 +79,8 @@ int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
 constexpr int kMaxChunk = 512;
 void cut(int64_t tokens, int64_t blocks, int tile, int cus, int64_t cap, int* parts, int* chunk) {
     const int64_t steps = std::max<int64_t>(1, ceil_div(tokens, kAttendStep));
-    int64_t want = ceil_div((int64_t)cus * (tile == kAttendWide ? 2 : 4), blocks);
-    if (tile != kAttendWide) want = std::max(want, ceil_div(tokens, kMaxChunk));
+    int64_t want = ceil_div((int64_t)cus * (tile >= kAttendWide ? 2 : 4), blocks);
+    if (tile < kAttendWide) want = std::max(want, ceil_div(tokens, kMaxChunk));
     want = std::max<int64_t>(1, std::min({steps, want, cap}));
     const int64_t per = ceil_div(steps, want);
     *chunk = (int)(per * kAttendStep);
