@@ -46,7 +46,7 @@ template <int DP, int NT, int LIMBS, bool Q16, bool SHARED>
 __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
     using L = TileLds<DP>;
     using Sh = Share<DP>;
-    constexpr int KS = DP / 16, ND = DP / 32, VT = 128 * NT;
+    constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide * NT;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -63,11 +63,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
     b = by_tiles.div(b);
     const int seq = SHARED ? 0 : p.by_seqs.mod(b), part = SHARED ? b : p.by_seqs.div(b);
 
-    // how many tokens each vector sees (-1: no vector); vectors v0 + 32 NT wave + 32 y + n
+    // how many tokens each vector sees (-1: no vector); vectors v0 + 32 (NT wave + y) + n
     int first_row = 0, cap, end, least;  // no vector sees end or more; all see the first `least`
     int seen[NT];
     const int j0 = (SHARED ? 0 : p.own_from) + part * chunk;
-    const int vw = v0 + 32 * NT * wave + n;
+    const int v = v0 + 32 * NT * wave + n;
     if constexpr (SHARED) {
         int* lds_seen = reinterpret_cast<int*>(lds);  // before the first tile
         cap = min(p.prefix, j0 + chunk);
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         }
         end = min(cap, end);
 #pragma unroll
-        for (int y = 0; y < NT; ++y) seen[y] = lds_seen[32 * NT * wave + 32 * y + n];
+        for (int y = 0; y < NT; ++y) seen[y] = lds_seen[32 * (NT * wave + y) + n];
         __syncthreads();
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
@@ -110,52 +110,48 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         end = min(cap, kv_visible(s, p.group.div(min(v0 + VT, vectors) - 1)));
         least = min(cap, kv_visible(s, p.group.div(v0)));
 #pragma unroll
-        for (int y = 0; y < NT; ++y) seen[y] = vw + 32 * y < vectors ? kv_visible(s, p.group.div(vw + 32 * y)) : -1;
+        for (int y = 0; y < NT; ++y) seen[y] = v + 32 * y < vectors ? kv_visible(s, p.group.div(v + 32 * y)) : -1;
     }
     end = __builtin_amdgcn_readfirstlane(end);
     least = __builtin_amdgcn_readfirstlane(least);
 
-    // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of a vector (vectors that are
-    // none take the first row's)
+    // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of its vector (vectors that
+    // are none take the first row's)
     half8v qf[NT][KS][LIMBS];
     float unit[NT];
     int64_t row[NT];
     int head[NT];
-    auto load_queries = [&] {
-        QueryRow<KS, Q16> qr[NT];
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            const int v = seen[y] >= 0 ? vw + 32 * y : 0;
-            row[y] = first_row + p.group.div(v);
-            head[y] = h * group + p.group.mod(v);
-            load_query<KS, 16, Q16>(p, qr[y], row[y] * p.ldq + (int64_t)head[y] * p.c.dim, 8 * hi);
-        }
-#pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            float up = 1.0f;
-            unit[y] = 1.0f;
-            if constexpr (LIMBS == 2) {
-                // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
-                float m = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(query_at<KS, Q16>(qr[y], k, i)));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
-                const int e = kv_clamp((int)((__float_as_uint(m) >> 23) & 0xff) - 127, -100, 126);
-                up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
-                unit[y] = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
-            }
+    for (int y = 0; y < NT; ++y) {
+        row[y] = first_row + p.group.div(seen[y] >= 0 ? v + 32 * y : 0);
+        head[y] = h * group + p.group.mod(seen[y] >= 0 ? v + 32 * y : 0);
+    }
+    auto load_queries = [&](int y) {
+        QueryRow<KS, Q16> qr;
+        load_query<KS, 16, Q16>(p, qr, row[y] * p.ldq + (int64_t)head[y] * p.c.dim, 8 * hi);
+        float up = 1.0f;
+        unit[y] = 1.0f;
+        if constexpr (LIMBS == 2) {
+            // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
+            float top = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    _Float16 z[LIMBS];
-                    split_f16<LIMBS>(query_at<KS, Q16>(qr[y], k, i) * up, z);
-#pragma unroll
-                    for (int q = 0; q < LIMBS; ++q) qf[y][k][q][i] = z[q];
-                }
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(query_at<KS, Q16>(qr, k, i)));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const int e = kv_clamp((int)((__float_as_uint(top) >> 23) & 0xff) - 127, -100, 126);
+            up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
+            unit[y] = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
         }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                _Float16 z[LIMBS];
+                split_f16<LIMBS>(query_at<KS, Q16>(qr, k, i) * up, z);
+#pragma unroll
+                for (int q = 0; q < LIMBS; ++q) qf[y][k][q][i] = z[q];
+            }
     };
 
     // a wave's shares lie in 16-token half `half(i)` of a tile; 64 columns take two waves only
@@ -166,150 +162,203 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
     const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false;
-    Sh sh;
     const int k_row = DP == 256 ? tid / 16 : tid % 128 / Sh::KCOLS % 16, k_at = k_row * DP + tid % Sh::KCOLS * 16;
     const int v_quad = DP == 256 ? wave : tid / Sh::VCOLS % 4, v_at = 4 * v_quad * DP + tid % Sh::VCOLS * 4;
-    auto load_share = [&](int j) {  // the tile at token j; past the end: zeros without an access
+    // A tile on its way: the page ids (loaded a step ahead of their use), the buffers, the bytes.
+    int ids[Sh::SUBS];
+    auto load_ids = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < Sh::SUBS; ++i) {
+            const int jt = min(j + 16 * half(i), end - 1);
+            ids[i] = (SHARED || jt < p.prefix ? prefix : table)[jt >> p.c.shift];
+        }
+    };
+    Tile at[Sh::SUBS];
+    bool there[Sh::SUBS];
+    auto find = [&](int j) {  // past the end: zeros without an access
 #pragma unroll
         for (int i = 0; i < Sh::SUBS; ++i) {
             const int jt = j + 16 * half(i);
-            const bool there = helps && jt < end;
-            int id = -1;
-            if (there) id = SHARED || jt < p.prefix ? prefix[jt >> p.c.shift] : table[jt >> p.c.shift];
-            const Tile t = find_tile<DP>(p.c, id, h, jt & off_mask, there);
-            sh.bad[i] = there && t.bad;
-            bad_page |= sh.bad[i];
-            sh.k[i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(t.k, k_at, 0, 0));
+            there[i] = helps && jt < end;
+            at[i] = find_tile<DP>(p.c, ids[i], h, jt & off_mask, there[i]);
+        }
+    };
+    auto load_share = [&](Sh& sh) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(t.v, v_at + x * DP, 0, 0);
-            if (scales) {  // lanes from 16 on lie outside the buffer
-                sh.ks[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(t.ks, 4 * lane, 0, 0));
-                sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(t.vs, 4 * lane, 0, 0));
-            }
+        for (int i = 0; i < Sh::SUBS; ++i) {
+            sh.bad[i] = there[i] && at[i].bad;
+            bad_page |= sh.bad[i];
+            sh.k[i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(at[i].k, k_at, 0, 0));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(at[i].v, v_at + x * DP, 0, 0);
+            // lanes from 16 on lie outside the buffer
+            sh.ks[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].ks, 4 * lane, 0, 0));
+            sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].vs, 4 * lane, 0, 0));
         }
     };
     const float key_unit = LIMBS == 2 ? 1.0f : p.scale2 * kCodeUnit;
-    auto store_share = [&](uint8_t* buf) {
-        if (!helps) return;
-#pragma unroll
-        for (int i = 0; i < Sh::SUBS; ++i) {
-            uint8_t* at = buf + (16 * half(i) + k_row) * L::KROW + tid % Sh::KCOLS * 32;
-            *reinterpret_cast<half8v*>(at) = codes8(sh.k[i][0], sh.k[i][1]);
-            *reinterpret_cast<half8v*>(at + 16) = codes8(sh.k[i][2], sh.k[i][3]);
+    // a share's way into the LDS, in pieces: 16 bytes of keys are two, four columns of values one each, then the scales
+    constexpr int PIECES = 6 * Sh::SUBS;
+    auto store_piece = [&](const Sh& sh, uint8_t* buf, int piece) {
+        if (DP == 64 && !helps) return;
+        const int i = piece / 6, x = piece % 6 - 2;
+        if (x < 0) {
+            uint8_t* to = buf + (16 * half(i) + k_row) * L::KROW + tid % Sh::KCOLS * 32 + 16 * (x + 2);
+            *reinterpret_cast<half8v*>(to) = codes8(sh.k[i][2 * (x + 2)], sh.k[i][2 * (x + 2) + 1]);
+        } else {
             // tokens 4 quad + 0..3 of the half: quad 2 b + h goes to place 8 h + 4 b of 16
             const int place = 16 * half(i) + 8 * (v_quad & 1) + 4 * (v_quad >> 1);
+            const uint32_t sel = 0x0c000c00u | (4 + x) << 16 | x;
+            const uint2v w = {codes2(sh.v[i][1], sh.v[i][0], sel), codes2(sh.v[i][3], sh.v[i][2], sel)};
+            // column d is row d / ND of tile d % ND: a lane's columns of all tiles are neighbours
+            const int d = tid % Sh::VCOLS * 4 + x;
+            *reinterpret_cast<uint2v*>(buf + L::V + (d % ND * 32 + d / ND) * L::VROW + 2 * place) = w;
+        }
+    };
+    auto store_scales = [&](const Sh& sh, uint8_t* buf) {
+        if (!scales || lane >= 16) return;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t sel = 0x0c000c00u | (4 + x) << 16 | x;
-                const uint2v w = {codes2(sh.v[i][1], sh.v[i][0], sel), codes2(sh.v[i][3], sh.v[i][2], sel)};
-                // column d is row d / ND of tile d % ND: a lane's columns of all tiles are neighbours
-                const int d = tid % Sh::VCOLS * 4 + x;
-                *reinterpret_cast<uint2v*>(buf + L::V + (d % ND * 32 + d / ND) * L::VROW + 2 * place) = w;
-            }
-            if (scales && lane < 16) {
-                float* s = reinterpret_cast<float*>(buf + L::S) + 16 * half(i) + lane;
-                const float inv = __builtin_amdgcn_rcpf(sh.vs[i]);
-                s[0] = sh.bad[i] ? kNan : sh.ks[i] * key_unit;
-                s[kTokens] = __builtin_amdgcn_logf(sh.vs[i]);
-                s[2 * kTokens] = inv < __builtin_inff() ? inv : 0.0f;  // a token that is none adds 0 * 0, not 0 * inf
-            }
+        for (int i = 0; i < Sh::SUBS; ++i) {
+            float* s = reinterpret_cast<float*>(buf + L::S) + 16 * half(i) + lane;
+            const float inv = __builtin_amdgcn_rcpf(sh.vs[i]);
+            s[0] = sh.bad[i] ? kNan : sh.ks[i] * key_unit;
+            s[kTokens] = __builtin_amdgcn_logf(sh.vs[i]);
+            s[2 * kTokens] = inv < __builtin_inff() ? inv : 0.0f;  // a token that is none adds 0 * 0, not 0 * inf
         }
     };
 
     float m[NT], l[NT], top[NT];
-    float16v s[NT], o[NT][ND];
+    float16v x[NT], o[NT][ND];  // exponents of a tile: tokens 8 c + 4 hi + i of vector n; outputs
     half8v pf[NT][2][LIMBS];
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
-        m[y] = kNegInf;
+        m[y] = top[y] = kNegInf;
         l[y] = 0.0f;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[y][t][i] = 0.0f;
     }
-    // S^T of a tile: tokens 8 c + 4 hi + i of vector n
-    auto keys = [&](const uint8_t* buf) {
-        const uint8_t* kb = buf + n * L::KROW + 16 * hi;
+
+    // The two phases of a step are written in the order that the instructions are to be issued in, held by
+    // scheduling barriers: LDS reads early, and after each matrix instruction the vector work that runs beside it.
+    auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+    // P of elements 2 i and 2 i + 1 of x
+    auto exponents = [&](int y, int i, float base, const float4v* iv) {
+        typedef float float2v __attribute__((ext_vector_type(2)));
+        const float2v e = {__builtin_amdgcn_exp2f(x[y][2 * i] - base), __builtin_amdgcn_exp2f(x[y][2 * i + 1] - base)};
+        l[y] = __builtin_fmaf(e[0], iv[i / 2][2 * i % 4], l[y]);
+        l[y] = __builtin_fmaf(e[1], iv[i / 2][2 * i % 4 + 1], l[y]);
+        const half2v z = __builtin_convertvector(e, half2v);
+        pf[y][i / 4][0][2 * i % 8] = z[0];
+        pf[y][i / 4][0][2 * i % 8 + 1] = z[1];
+        if constexpr (LIMBS == 2) {
+            const half2v w = __builtin_convertvector(e - __builtin_convertvector(z, float2v), half2v);
+            pf[y][i / 4][1][2 * i % 8] = w[0];
+            pf[y][i / 4][1][2 * i % 8 + 1] = w[1];
+        }
+    };
+    // exponents from products, elements 2 i and 2 i + 1; MASK where some vector does not see all of the tile
+    auto scale = [&](const float16v& s, int y, int i, int left, const float4v* ks, const float4v* lv, auto mask) {
 #pragma unroll
-        for (int y = 0; y < NT; ++y)
+        for (int e = 2 * i; e < 2 * i + 2; ++e) {
+            float z = s[e];
+            if constexpr (LIMBS == 2) z *= unit[y];
+            z = __builtin_fmaf(z, ks[e / 4][e % 4], lv[e / 4][e % 4]);
+            // masked tokens are chosen away, whatever their scales hold
+            if constexpr (decltype(mask)::value) z = 8 * (e / 4) + e % 4 < left ? z : kNegInf;
+            asm volatile("" : "+v"(z));  // computed here, not where it is used next
+            x[y][e] = z;
+            top[y] = fmaxf(top[y], z);
+        }
+    };
+    auto key = [&](const uint8_t* buf, int k) { return *reinterpret_cast<const half8v*>(buf + n * L::KROW + 16 * hi + 32 * k); };
+    auto value = [&](const uint8_t* buf, int c, int t) {
+        return *reinterpret_cast<const half8v*>(buf + L::V + (32 * t + n) * L::VROW + 16 * hi + 32 * c);
+    };
+    auto factors = [&](const uint8_t* buf, int which, float4v* f) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[y][i] = 0.0f;
+        for (int c = 0; c < 4; ++c)
+            f[c] = *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(buf + L::S) + which * kTokens + 8 * c + 4 * hi);
+    };
+    // First P of tile u (its values lie in bu) beside the products of tile u + 1 (NEXT: its keys in bk). Then
+    // the outputs of tile u beside the exponents of tile u + 1, at token j, and the way of tile u + 2 into bn.
+    auto advance = [&](const uint8_t* bu, const uint8_t* bk, uint8_t* bn, const Sh& sh, int j, auto next, auto mask) {
+        constexpr bool NEXT = decltype(next)::value;
+        constexpr int SV = 2 * ND;                                  // matrix steps of O
+        constexpr int EP = (8 + KS - 1) / KS;                       // pairs of exponents beside a matrix step of S
+        constexpr int FROM = SV >= 8 ? 1 : 0;                       // the products are on their way until then
+        constexpr int SP = (8 + SV - FROM - 1) / (SV - FROM);       // pairs beside a matrix step of O
+        constexpr int PP = (PIECES + SV - 1) / SV;
+        float4v iv[4], ks[4], lv[4];
+        half8v kf[KS], vf[SV];
+        float16v s[NT];
+        float base[NT];
+        if constexpr (NEXT) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const half8v a = *reinterpret_cast<const half8v*>(kb + 32 * k);
+            for (int k = 0; k < KS / 2; ++k) kf[k] = key(bk, k);
 #pragma unroll
             for (int y = 0; y < NT; ++y)
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) s[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[y][k][q], s[y], 0, 0, 0);
+                for (int i = 0; i < 16; ++i) s[y][i] = 0.0f;
         }
-    };
-    // P of the tile whose S is at hand
-    auto exponents = [&](const uint8_t* buf) {
-        const float* sc = reinterpret_cast<const float*>(buf + L::S) + 2 * kTokens + 4 * hi;
-        float base[NT];
+        factors(bu, 2, iv);
+        pin();
 #pragma unroll
         for (int y = 0; y < NT; ++y) base[y] = m[y] == kNegInf ? 0.0f : m[y] - kPShift;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float4v iv = *reinterpret_cast<const float4v*>(sc + 8 * c);
-#pragma unroll
-            for (int y = 0; y < NT; ++y)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(s[y][4 * c + i] - base[y]);
-                    l[y] = __builtin_fmaf(e, iv[i], l[y]);
-                    _Float16 z[LIMBS];
-                    split_f16<LIMBS>(e, z);
-#pragma unroll
-                    for (int q = 0; q < LIMBS; ++q) pf[y][c / 2][q][4 * (c % 2) + i] = z[q];
-                }
-        }
-    };
-    auto values = [&](const uint8_t* buf) {
-        const uint8_t* vb = buf + L::V + n * L::VROW + 16 * hi;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int t = 0; t < ND; ++t) {
-                const half8v a = *reinterpret_cast<const half8v*>(vb + 32 * t * L::VROW + 32 * c);
-#pragma unroll
-                for (int y = 0; y < NT; ++y)
-#pragma unroll
-                    for (int q = 0; q < LIMBS; ++q) o[y][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pf[y][c][q], o[y][t], 0, 0, 0);
-            }
-    };
-    // exponents of the tile at token j whose products are in s, and their maximum; MASK where some vector
-    // does not see all of the tile
-    auto scale = [&](const uint8_t* buf, int j, auto mask) {
-        constexpr bool MASK = decltype(mask)::value;
-        const float* sc = reinterpret_cast<const float*>(buf + L::S) + 4 * hi;
-#pragma unroll
-        for (int y = 0; y < NT; ++y) top[y] = kNegInf;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float4v ks = *reinterpret_cast<const float4v*>(sc + 8 * c), lv = *reinterpret_cast<const float4v*>(sc + kTokens + 8 * c);
+        for (int k = 0; k < KS; ++k) {
 #pragma unroll
             for (int y = 0; y < NT; ++y) {
-                const int left = min(seen[y], cap) - j - 4 * hi;
+                if constexpr (NEXT)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = s[y][4 * c + i];
-                    if constexpr (LIMBS == 2) x *= unit[y];
-                    x = __builtin_fmaf(x, ks[i], lv[i]);
-                    // masked tokens are chosen away, whatever their scales hold
-                    if constexpr (MASK) x = 8 * c + i < left ? x : kNegInf;
-                    s[y][4 * c + i] = x;
-                    top[y] = fmaxf(top[y], x);
+                    for (int q = 0; q < LIMBS; ++q) s[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[y][k][q], s[y], 0, 0, 0);
+#pragma unroll
+                for (int i = k * EP; i < (k + 1) * EP; ++i)
+                    if (i < 8) exponents(y, i, base[y], iv);
+                if (y == 0) {
+                    if (NEXT && k < KS / 2) kf[k + KS / 2] = key(bk, k + KS / 2);
+                    if (k >= KS - ND) vf[k - (KS - ND)] = value(bu, 0, k - (KS - ND));
                 }
+                pin();
             }
         }
+        if constexpr (NEXT) {
+            factors(bk, 0, ks);
+            factors(bk, 1, lv);
+        }
+        int left[NT];
+#pragma unroll
+        for (int y = 0; y < NT; ++y) {
+            top[y] = kNegInf;
+            left[y] = min(seen[y], cap) - j - 4 * hi;
+        }
+#pragma unroll
+        for (int t = 0; t < SV; ++t) {
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+#pragma unroll
+                for (int q = 0; q < LIMBS; ++q) o[y][t % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t], pf[y][t / ND][q], o[y][t % ND], 0, 0, 0);
+                if constexpr (NEXT) {
+#pragma unroll
+                    for (int i = (t - FROM) * SP; i < (t - FROM + 1) * SP; ++i)
+                        if (i >= 0 && i < 8) scale(s[y], y, i, left[y], ks, lv, mask);
+                }
+                if (y == 0 && t < ND) vf[t + ND] = value(bu, 1, t);
+                if (NEXT && y == NT - 1)
+#pragma unroll
+                    for (int i = t * PP; i < (t + 1) * PP; ++i)
+                        if (i < PIECES) store_piece(sh, bn, i);
+                pin();
+            }
+        }
+        if constexpr (NEXT) store_scales(sh, bn);
     };
     auto raise = [&] {
+        typedef unsigned int pair __attribute__((ext_vector_type(2)));
         bool up = false;
 #pragma unroll
         for (int y = 0; y < NT; ++y) {
-            typedef unsigned int pair __attribute__((ext_vector_type(2)));
             const pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(top[y]), __float_as_uint(top[y]), false, false));
             top[y] = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
             up |= top[y] > m[y] + kSlack;
@@ -327,28 +376,55 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
     };
 
     if (j0 < end) {
-        load_share(j0);
-        load_queries();
+        Sh sh;
+        load_ids(j0);
+        find(j0);
+        load_share(sh);
+        load_ids(j0 + kTokens);
+#pragma unroll
+        for (int y = 0; y < NT; ++y) load_queries(y);
+        auto store_share = [&](uint8_t* buf) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) store_piece(sh, buf, i);
+            store_scales(sh, buf);
+        };
         store_share(lds);
-        load_share(j0 + kTokens);
+        find(j0 + kTokens);
+        load_share(sh);
+        load_ids(j0 + 2 * kTokens);
         store_share(lds + L::BYTES);
-        load_share(j0 + 2 * kTokens);
+        find(j0 + 2 * kTokens);
+        load_share(sh);
+        load_ids(j0 + 3 * kTokens);
         __syncthreads();
-        keys(lds);
-        scale(lds, j0, std::true_type{});
+        {
+            float4v ks[4], lv[4];
+            factors(lds, 0, ks);
+            factors(lds, 1, lv);
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+                float16v s;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(lds, k), qf[y][k][q], s, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) scale(s, y, i, min(seen[y], cap) - j0 - 4 * hi, ks, lv, std::true_type{});
+            }
+        }
         raise();
         // tile u's values, tile u + 1's keys, tile u + 2's place
         int bu = 0, bk = L::BYTES, bn = 2 * L::BYTES;
         int j = j0;
         auto step = [&](auto mask) {
-            exponents(lds + bu);
-            keys(lds + bk);
-            values(lds + bu);
-            scale(lds + bk, j + kTokens, mask);
-            store_share(lds + bn);
-            load_share(j + 3 * kTokens);
+            find(j + 3 * kTokens);
+            advance(lds + bu, lds + bk, lds + bn, sh, j + kTokens, std::true_type{}, mask);
+            load_share(sh);
+            load_ids(j + 4 * kTokens);
             raise();
-            __syncthreads();
+            lds_barrier();  // the bytes of later tiles stay on their way
             const int t = bu;
             bu = bk;
             bk = bn;
@@ -356,10 +432,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         };
         for (; j + 2 * kTokens <= least; j += kTokens) step(std::false_type{});
         for (; j + kTokens < end; j += kTokens) step(std::true_type{});
-        exponents(lds + bu);
-        values(lds + bu);
-    } else {
-        load_queries();  // for the places of the results
+        advance(lds + bu, nullptr, nullptr, sh, 0, std::false_type{}, std::false_type{});
     }
     if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
 
