@@ -303,7 +303,7 @@ class KVCache:
         info = _lib.KVInfo()
         check(_lib.load().qlin_kv_query(self.handle, ctypes.byref(info)), "qlin_kv_query")
         self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
-        self.device_bytes = info.device_bytes
+        self.columns, self.device_bytes = kv_heads * head_dim, info.device_bytes
 
     def close(self):
         if self.handle:
@@ -333,41 +333,58 @@ class KVBatch:
         # a table of one row has no row stride of its own
         ld = page_table.stride(0) if seqs > 1 else max(page_table.shape[1], 1)
         assert seqs <= 1 or ld >= page_table.shape[1]
-        self.columns, self.rows = page_table.shape[1], rows
+        self.columns, self.rows, self.max_len, self.device = page_table.shape[1], rows, max_len, row_start.device
         self.c = _lib.KVBatch(seqs, rows, max_new, max_len, row_start.data_ptr(), length.data_ptr(), page_table.data_ptr(),
                               ld)
+        self.ref = ctypes.byref(self.c)
         self._keep = (row_start, length, page_table)
 
 
-def _kv_batch(cache: KVCache, batch: KVBatch, *rows: torch.Tensor):
+# The calls below are made once a layer and token: they take a current stream, a pointer and a row stride as plain
+# integers (2 us a call on the host, where stream objects and ctypes pointers took 6).
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _kv_ld(batch: KVBatch, t: torch.Tensor, cols: int) -> int:
+    """Row stride of row tensor t, which has to hold the batch's rows of `cols` columns."""
+    (rows, n), (ld, step) = t.shape, t.stride()
+    assert n == cols and rows >= batch.c.rows and (step == 1 or n == 1) and t.device == batch.device
+    return ld if rows > 1 else n
+
+
+def _kv_check(cache: KVCache, batch: KVBatch) -> None:
     assert batch.columns * cache.page_tokens >= batch.c.max_len, "the page table is too narrow for max_len"
-    for t in rows:
-        assert t.is_cuda and t.dim() == 2 and t.shape[0] >= batch.rows and (t.shape[1] <= 1 or t.stride(1) == 1)
-    return ctypes.byref(batch.c)
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
 def kv_append(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor, V: torch.Tensor, flags: int = 0) -> None:
     """Quantizes the batch's new rows K, V [rows, kv_heads * head_dim] into their pages (qlin_kv_append)."""
-    b = _kv_batch(cache, batch, K, V)
-    assert K.dtype == V.dtype and K.shape[1] == V.shape[1] == cache.kv_heads * cache.head_dim
-    check(_lib.load().qlin_kv_append(ws.handle, cache.handle, b, _ptr(K), _ld(K), _ptr(V), _ld(V), _DT[K.dtype], flags,
-                                     _stream()), "qlin_kv_append")
+    _kv_check(cache, batch)
+    dtype = K.dtype
+    assert V.dtype == dtype
+    rc = _lib.load().qlin_kv_append(ws.handle, cache.handle, batch.ref, K.data_ptr(), _kv_ld(batch, K, cache.columns),
+                                    V.data_ptr(), _kv_ld(batch, V, cache.columns), _DT[dtype], flags,
+                                    _raw_stream(batch.device))
+    if rc:
+        check(rc, "qlin_kv_append")
 
 
 def kv_read(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor | None = None, V: torch.Tensor | None = None,
             out_dtype=torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """The batch's new rows as the cache holds them, K, V [rows, kv_heads * head_dim] (qlin_kv_read)."""
-    shape, dev = (batch.rows, cache.kv_heads * cache.head_dim), batch._keep[0].device
-    K = torch.empty(shape, dtype=out_dtype, device=dev) if K is None else K
-    V = torch.empty(shape, dtype=K.dtype, device=dev) if V is None else V
-    b = _kv_batch(cache, batch, K, V)
-    assert K.dtype == V.dtype and K.shape[1] == V.shape[1] == shape[1]
-    check(_lib.load().qlin_kv_read(ws.handle, cache.handle, b, _ptr(K), _ld(K), _ptr(V), _ld(V), _DT[K.dtype], _stream()),
-          "qlin_kv_read")
+    _kv_check(cache, batch)
+    if K is None:
+        K = torch.empty((batch.rows, cache.columns), dtype=out_dtype, device=batch.device)
+    if V is None:
+        V = torch.empty((batch.rows, cache.columns), dtype=K.dtype, device=batch.device)
+    dtype = K.dtype
+    assert V.dtype == dtype
+    rc = _lib.load().qlin_kv_read(ws.handle, cache.handle, batch.ref, K.data_ptr(), _kv_ld(batch, K, cache.columns),
+                                  V.data_ptr(), _kv_ld(batch, V, cache.columns), _DT[dtype], _raw_stream(batch.device))
+    if rc:
+        check(rc, "qlin_kv_read")
     return K, V
 
 
@@ -377,20 +394,28 @@ def kv_attention(ws: Workspace, cache: KVCache, batch: KVBatch, Q: torch.Tensor,
     """Causal attention of the batch's new rows Q [rows, q_heads * head_dim] over the cache (qlin_kv_attention; with
     prefix_tokens, qlin_kv_attention_prefix: the tokens that all sequences begin with, in prefix_pages).  scale
     defaults to head_dim ** -0.5, out_dtype to Q's."""
+    _kv_check(cache, batch)
     D = cache.head_dim
+    cols = Q.shape[1]
+    heads = cols // D
+    assert heads * D == cols
     if out is None:
-        out = torch.empty((Q.shape[0], Q.shape[1]), dtype=out_dtype or Q.dtype, device=Q.device)
-    b = _kv_batch(cache, batch, Q, out)
-    assert Q.shape[1] == out.shape[1] and Q.shape[1] % D == 0
-    args = (Q.shape[1] // D, _ptr(Q), _DT[Q.dtype], _ld(Q), D ** -0.5 if scale is None else scale, _ptr(out),
-            _DT[out.dtype], _ld(out), _stream())
+        out = torch.empty((Q.shape[0], cols), dtype=out_dtype or Q.dtype, device=Q.device)
+    if scale is None:
+        scale = D ** -0.5
     if prefix_tokens:
-        assert prefix_pages is not None and prefix_pages.dtype == torch.int32 and prefix_pages.is_cuda
+        assert prefix_pages is not None and prefix_pages.dtype == torch.int32 and prefix_pages.device == batch.device
         assert prefix_pages.is_contiguous() and prefix_pages.numel() * cache.page_tokens >= prefix_tokens
-        check(_lib.load().qlin_kv_attention_prefix(ws.handle, cache.handle, b, prefix_tokens, _ptr(prefix_pages), *args),
-              "qlin_kv_attention_prefix")
+        rc = _lib.load().qlin_kv_attention_prefix(
+            ws.handle, cache.handle, batch.ref, prefix_tokens, prefix_pages.data_ptr(), heads, Q.data_ptr(), _DT[Q.dtype],
+            _kv_ld(batch, Q, cols), scale, out.data_ptr(), _DT[out.dtype], _kv_ld(batch, out, cols),
+            _raw_stream(batch.device))
     else:
-        check(_lib.load().qlin_kv_attention(ws.handle, cache.handle, b, *args), "qlin_kv_attention")
+        rc = _lib.load().qlin_kv_attention(
+            ws.handle, cache.handle, batch.ref, heads, Q.data_ptr(), _DT[Q.dtype], _kv_ld(batch, Q, cols), scale,
+            out.data_ptr(), _DT[out.dtype], _kv_ld(batch, out, cols), _raw_stream(batch.device))
+    if rc:
+        check(rc, "qlin_kv_attention")
     return out
 
 
