@@ -45,14 +45,17 @@ __device__ __forceinline__ float over_groups(float x) {
 // LIMBS = 2 (f32 rows in or out): queries and P as a sum of two fp16 values, 22 bits; fp16 queries are
 // exact with one, and P rounded to 11 bits is off by as much as an fp16 output.
 // SHARED: the part of the prefix, for the rows of all sequences at once.
+template <int DP, int R>
+struct AttendLds {
+    alignas(16) float o[2][16 * R][DP + 4];  // rows padded: 16 lanes' rows start in different banks
+    float m[4][16 * R], l[4][16 * R];
+    int seen[16 * R], most;  // SHARED: tokens that each vector sees, the most of them
+};
 template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
-__global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 128 ? 3 : 1) void attend_kernel(AttendParams p) {
+__device__ __forceinline__ void attend_part(const AttendParams& p, int block, AttendLds<DP, R>& lds) {
     constexpr int KS = DP / 32;   // matrix steps of a q . k
     constexpr int DT = DP / 16;   // tiles of 16 output columns
     constexpr int VT = 16 * R;    // vectors of the workgroup
-    constexpr int LD = DP + 4;    // a row of outputs in the LDS: 16 lanes' rows in different banks
-    __shared__ __align__(16) float lds_o[2][VT][LD];
-    __shared__ float lds_m[4][VT], lds_l[4][VT];
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -60,7 +63,7 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
     // heads fastest, parts slowest: workgroups go to the 8 XCDs in turn, and the later parts of ragged
     // sequences are empty.  (With the parts fastest, 64 sequences of 1024 tokens in a batch cut for
     // 4096 in four parts ran on two XCDs: 68 us against 26.)
-    int b = blockIdx.x;
+    int b = block;
     const int h = p.by_heads.mod(b);
     b = p.by_heads.div(b);
     const int tile = (SHARED ? p.by_prefix_tiles : p.by_tiles).mod(b);
@@ -73,25 +76,24 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
     const int j0 = (SHARED ? 0 : p.own_from) + part * chunk;
     int seen[R];
     if constexpr (SHARED) {
-        __shared__ int lds_seen[VT], lds_most;
         first_row = 0;
         cap = min(p.prefix, j0 + chunk);
-        if (tid == 0) lds_most = 0;
-        if (tid < VT) lds_seen[tid] = -1;
+        if (tid == 0) lds.most = 0;
+        if (tid < VT) lds.seen[tid] = -1;
         __syncthreads();
         const int r_lo = p.group.div(v0), r_hi = min(p.group.div(v0 + VT - 1) + 1, p.b.rows);
         for (int i = tid; i < p.b.seqs; i += 256) {
             const KvSeq q = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
             for (int r = max(q.row0, r_lo); r < min(q.row0 + q.rows, r_hi); ++r) {
                 const int y = kv_visible(q, r - q.row0);
-                for (int x = max(r * group, v0); x < min((r + 1) * group, v0 + VT); ++x) lds_seen[x - v0] = y;
-                atomicMax(&lds_most, y);
+                for (int x = max(r * group, v0); x < min((r + 1) * group, v0 + VT); ++x) lds.seen[x - v0] = y;
+                atomicMax(&lds.most, y);
             }
         }
         __syncthreads();
-        end = min(cap, lds_most);
+        end = min(cap, lds.most);
 #pragma unroll
-        for (int r = 0; r < R; ++r) seen[r] = lds_seen[16 * r + n];
+        for (int r = 0; r < R; ++r) seen[r] = lds.seen[16 * r + n];
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
         if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
@@ -293,8 +295,8 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
     for (int r = 0; r < R; ++r) {
         l[r] = over_groups<false>(l[r]);
         if (g == 0) {
-            lds_m[wave][16 * r + n] = m[r];
-            lds_l[wave][16 * r + n] = l[r];
+            lds.m[wave][16 * r + n] = m[r];
+            lds.l[wave][16 * r + n] = l[r];
         }
     }
     __syncthreads();
@@ -302,11 +304,11 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int v = 16 * r + n;
-        m_all[r] = fmaxf(fmaxf(lds_m[0][v], lds_m[1][v]), fmaxf(lds_m[2][v], lds_m[3][v]));
+        m_all[r] = fmaxf(fmaxf(lds.m[0][v], lds.m[1][v]), fmaxf(lds.m[2][v], lds.m[3][v]));
         const float base = m_all[r] == kNegInf ? 0.0f : m_all[r];
         l_all[r] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) l_all[r] += lds_l[w][v] * __builtin_amdgcn_exp2f(lds_m[w][v] - base);
+        for (int w = 0; w < 4; ++w) l_all[r] += lds.l[w][v] * __builtin_amdgcn_exp2f(lds.m[w][v] - base);
         const float fade = __builtin_amdgcn_exp2f(m[r] - base);
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[r][t] *= fade;
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int u = 0; u < DT / 4; ++u)
-                    *reinterpret_cast<float4v*>(&lds_o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]) = four(r, i, u);
+                    *reinterpret_cast<float4v*>(&lds.o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]) = four(r, i, u);
     };
     auto add = [&](int slot) {
 #pragma unroll
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int u = 0; u < DT / 4; ++u) {
-                    const float4v y = *reinterpret_cast<const float4v*>(&lds_o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]);
+                    const float4v y = *reinterpret_cast<const float4v*>(&lds.o[slot][16 * r + n][(4 * g + i) * DT + 4 * u]);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[r][4 * u + c][i] += y[c];
                 }
@@ -373,30 +375,49 @@ __global__ __launch_bounds__(256, DP * R * LIMBS <= 64 ? 4 : DP * R * LIMBS <= 1
     }
 }
 
-// Joins the parts of a vector, one workgroup each: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
-// Groups of DP / 4 lanes take the parts in turn, four columns a lane, and are added up in the LDS.
-template <int DP>
+// A launch: the first `shared` workgroups work on the prefix with RS tiles (0: there is none), the others on the
+// sequences' own tokens with RO.
+template <int DP, int RS, int RO, int LIMBS, bool Q16>
+__global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * LIMBS <= 64 ? 4 : DP * (RS > RO ? RS : RO) * LIMBS <= 128 ? 3 : 1)
+void attend_kernel(AttendParams p, int shared) {
+    __shared__ union {
+        AttendLds<DP, (RS > 0 ? RS : RO)> prefix;
+        AttendLds<DP, RO> own;
+    } lds;
+    if constexpr (RS > 0) {
+        if ((int)blockIdx.x < shared) {
+            attend_part<DP, RS, LIMBS, Q16, true>(p, blockIdx.x, lds.prefix);
+            return;
+        }
+    }
+    attend_part<DP, RO, LIMBS, Q16, false>(p, blockIdx.x - shared, lds.own);
+}
+
+// Joins the parts of vectors: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes hold a vector's
+// columns, four each.  MANY parts: a workgroup per vector, its groups of lanes take the parts in turn
+// and are added up in the LDS.  Few: a group per vector.
+template <int DP, bool MANY>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
-    constexpr int LPV = DP / 4, GROUPS = 256 / LPV;
-    __shared__ __align__(16) float lds_o[GROUPS][DP];
+    constexpr int LPV = DP / 4, GROUPS = 256 / LPV, STEP = MANY ? GROUPS : 1;
+    __shared__ __align__(16) float lds_o[MANY ? GROUPS : 1][DP];
     __shared__ float lds_l[GROUPS];
-    const int per_seq = p.b.max_new * p.q_heads;
-    const int seq = blockIdx.x / per_seq, x = blockIdx.x - seq * per_seq;
+    const int seq = p.by_join.div(blockIdx.x);
+    const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4, lane = threadIdx.x & 63;
+    const int x = MANY ? p.by_join.mod(blockIdx.x) : p.by_join.mod(blockIdx.x) * GROUPS + group;
     const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
-    const int t = x / p.q_heads, head = x - t * p.q_heads;
+    const int t = p.by_q_heads.div(x), head = p.by_q_heads.mod(x);
     if (t >= s.rows) return;
     const int parts = p.prefix_parts + kv_parts(s.len - p.own_from, p.chunk);
-    const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4, lane = threadIdx.x & 63;
     const int64_t row = s.row0 + t, slot = (row * p.q_heads + head) * p.parts;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot;
     float m = kNegInf;
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, ml[i].x);
-    m = wave_max(m);
+    for (int i = MANY ? lane : 0; i < parts; i += MANY ? 64 : 1) m = fmaxf(m, ml[i].x);
+    if constexpr (MANY) m = wave_max(m);
     const float base = m == kNegInf ? 0.0f : m;
     float l = 0.0f;
     float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int i = group; i < parts; i += GROUPS) {
+    for (int i = MANY ? group : 0; i < parts; i += STEP) {
         const float2 y = ml[i];
         const float f = __builtin_amdgcn_exp2f(y.x - base);
         l = __builtin_fmaf(f, y.y, l);
@@ -404,52 +425,59 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[c], o[c]);
     }
-    *reinterpret_cast<float4v*>(&lds_o[group][d]) = o;
-    if (d == 0) lds_l[group] = l;
-    __syncthreads();
-    if (group != 0) return;
+    if constexpr (MANY) {
+        *reinterpret_cast<float4v*>(&lds_o[group][d]) = o;
+        if (d == 0) lds_l[group] = l;
+        __syncthreads();
+        if (group != 0) return;
 #pragma unroll
-    for (int i = 1; i < GROUPS; ++i) {
-        o += *reinterpret_cast<const float4v*>(&lds_o[i][d]);
-        l += lds_l[i];
+        for (int i = 1; i < GROUPS; ++i) {
+            o += *reinterpret_cast<const float4v*>(&lds_o[i][d]);
+            l += lds_l[i];
+        }
     }
     const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
     const float y[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
     store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, d, y);
 }
 
-// Vectors of a workgroup, given how many share its tokens: this file's kernel for up to two tiles (two
-// of 256 columns would not fit the registers), else the wide one, with two tiles a wave (fp16
-// rows of up to 128 columns) from where its workgroups are filled.
+// Vectors of a workgroup, given how many share its tokens: one or two tiles here (two of 256 columns would
+// not fit the registers), or the wide kernel's.  That one reads a token's bytes once for 128 vectors but
+// waits at a barrier for every 32 tokens: with up to 256 vectors (512 in two limbs) more workgroups of this one
+// are faster.  (4096 tokens, 8 KV heads of 128, us here and there: fp16 64 vectors 15.5 / 17.8, 128 18.1 / 23.2,
+// 256 23.2 / 31.7, 512 33.9 / 37.8, a prefix for 512 45.2 / 44.3; f32 256 27.5 / 40.6, 512 41.3 / 51.1.)
 int tile_of(const AttendParams& p, int64_t vectors) {
-    if (vectors <= 16) return 16;
-    if (vectors <= 32 && p.c.dim_padded <= 128) return 32;
-    return kAttendWide;
-}
-
-template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
-hipError_t launch_r(const AttendParams& p, hipStream_t st) {
-    const int64_t vectors = (int64_t)(SHARED ? p.b.rows : p.b.max_new) * p.group.d;
-    const int64_t blocks = (int64_t)(SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs) *
-                           p.c.heads * ((vectors + 16 * R - 1) / (16 * R));
-    attend_kernel<DP, R, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
-    return hipGetLastError();
-}
-
-template <int DP, int LIMBS, bool Q16, bool SHARED>
-hipError_t launch_part(const AttendParams& p, hipStream_t st) {
-    const int tile = SHARED ? attend_tile_prefix(p) : attend_tile(p);
-    if (tile >= kAttendWide) return launch_attend_wide(p, SHARED, st);
-    if constexpr (DP <= 128)
-        if (tile == 32) return launch_r<DP, 2, LIMBS, Q16, SHARED>(p, st);
-    return launch_r<DP, 1, LIMBS, Q16, SHARED>(p, st);
+    if (vectors > (p.q_f16 && p.o_f16 ? 256 : 512)) return kAttendWide;
+    return vectors <= 16 || p.c.dim_padded > 128 ? 16 : 32;
 }
 
 template <int DP, int LIMBS, bool Q16>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
-    if (p.prefix_parts)
-        if (hipError_t e = launch_part<DP, LIMBS, Q16, true>(p, st)) return e;
-    return launch_part<DP, LIMBS, Q16, false>(p, st);
+    const int own = attend_tile(p), shared = p.prefix_parts ? attend_tile_prefix(p) : 0;
+    const uint32_t own_blocks = (uint32_t)((p.parts - p.prefix_parts) * (int64_t)p.b.seqs * p.c.heads * p.by_tiles.d);
+    const uint32_t shared_blocks = (uint32_t)(p.prefix_parts * (int64_t)p.c.heads * p.by_prefix_tiles.d);
+    if (shared == kAttendWide)
+        if (hipError_t e = launch_attend_wide(p, true, st)) return e;
+    if (own == kAttendWide) return launch_attend_wide(p, false, st);
+    const uint32_t first = shared == kAttendWide ? 0 : shared_blocks;
+    const dim3 grid(first + own_blocks);
+    if (first == 0) {
+        if constexpr (DP <= 128)
+            if (own == 32) {
+                attend_kernel<DP, 0, 2, LIMBS, Q16><<<grid, 256, 0, st>>>(p, 0);
+                return hipGetLastError();
+            }
+        attend_kernel<DP, 0, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, 0);
+        return hipGetLastError();
+    }
+    if constexpr (DP <= 128) {  // the prefix's rows are those of all sequences: at least as many
+        if (own == 32) attend_kernel<DP, 2, 2, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+        else if (shared == 32) attend_kernel<DP, 2, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+        else attend_kernel<DP, 1, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+    } else {
+        attend_kernel<DP, 1, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+    }
+    return hipGetLastError();
 }
 
 template <int DP>
@@ -458,7 +486,14 @@ hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
                          : p.o_f16 ? launch_typed<DP, 1, true>(p, st)
                                    : launch_typed<DP, 2, true>(p, st);
     if (e != hipSuccess || p.parts == 1) return e;
-    attend_join_kernel<DP><<<dim3((uint32_t)((int64_t)p.b.max_new * p.q_heads * p.b.seqs)), 256, 0, st>>>(p);
+    // few parts: fewer than the groups of lanes a workgroup has for them
+    AttendParams j = p;
+    const int64_t vectors = (int64_t)p.b.max_new * p.q_heads, groups = 256 / (DP / 4);
+    const bool many = p.parts >= groups;
+    const int64_t blocks = many ? vectors : (vectors + groups - 1) / groups;
+    j.by_join = fast_div((int)blocks);
+    if (many) attend_join_kernel<DP, true><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
+    else attend_join_kernel<DP, false><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
     return hipGetLastError();
 }
 

@@ -376,26 +376,27 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
     };
 
     if (j0 < end) {
-        Sh sh;
+        // the first three tiles' bytes are asked for together
+        Sh sh, sh0, sh1;
         load_ids(j0);
         find(j0);
-        load_share(sh);
+        load_share(sh0);
         load_ids(j0 + kTokens);
+        find(j0 + kTokens);
+        load_share(sh1);
+        load_ids(j0 + 2 * kTokens);
+        find(j0 + 2 * kTokens);
+        load_share(sh);
+        load_ids(j0 + 3 * kTokens);
 #pragma unroll
         for (int y = 0; y < NT; ++y) load_queries(y);
-        auto store_share = [&](uint8_t* buf) {
+        auto store_share = [&](const Sh& sh, uint8_t* buf) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) store_piece(sh, buf, i);
             store_scales(sh, buf);
         };
-        store_share(lds);
-        find(j0 + kTokens);
-        load_share(sh);
-        load_ids(j0 + 2 * kTokens);
-        store_share(lds + L::BYTES);
-        find(j0 + 2 * kTokens);
-        load_share(sh);
-        load_ids(j0 + 3 * kTokens);
+        store_share(sh0, lds);
+        store_share(sh1, lds + L::BYTES);
         __syncthreads();
         {
             float4v ks[4], lv[4];

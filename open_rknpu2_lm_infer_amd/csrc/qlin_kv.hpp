@@ -81,6 +81,7 @@ struct AttendParams {
     int parts, prefix_parts;  // in all; of the prefix (they come first)
     int chunk, prefix_chunk;  // tokens a part
     FastDiv by_heads, by_seqs, by_tiles, by_prefix_tiles;  // of workgroup indexes; tiles of vectors
+    FastDiv by_q_heads, by_join;                           // of the join's
     float* part_o;
     float* part_ml;
     uint32_t* err;

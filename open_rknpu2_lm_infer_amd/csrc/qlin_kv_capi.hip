@@ -71,17 +71,16 @@ int rows_call(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     return e == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
 }
 
-// Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part of `tile` vectors each:
-// enough parts that the launch covers the CUs some times over (a workgroup's loads alone do not keep
-// its CU's share of the HBM busy), at least one step of a workgroup each, at most `cap`.
-// Parts of the kernel for few vectors hold at most kMaxChunk tokens: ragged sequences then end in many
-// workgroups of one size, and the results kept for the join stay under 2% of the bytes read.
-constexpr int kMaxChunk = 512;
-void cut(int64_t tokens, int64_t blocks, int tile, int cus, int64_t cap, int* parts, int* chunk) {
+// Tokens a part and the parts of `tokens` tokens, for `blocks` workgroups a part: `cover` workgroups for
+// every CU, at least one step of a workgroup each, at most `cap` parts of at most `most` tokens.  A context of
+// up to kOnePart tokens is not cut: a workgroup takes 1.1 us for a step of 128, the join 2.7 us and its launch.
+// (One token, 8 KV heads of 128: 300 tokens 7.9 against 8.7 us in two parts and more, 512 8.8 against 8.3, 768
+// 10.6 against 9.1.)
+constexpr int kOnePart = 512;
+void cut(int64_t tokens, int64_t blocks, int cover, int most, int64_t cap, int* parts, int* chunk) {
     const int64_t steps = std::max<int64_t>(1, ceil_div(tokens, kAttendStep));
-    int64_t want = ceil_div((int64_t)cus * (tile >= kAttendWide ? 2 : 4), blocks);
-    if (tile < kAttendWide) want = std::max(want, ceil_div(tokens, kMaxChunk));
-    want = std::max<int64_t>(1, std::min({steps, want, cap}));
+    int64_t want = std::max(ceil_div(cover, blocks), ceil_div(tokens, most));
+    want = tokens <= kOnePart ? 1 : std::max<int64_t>(1, std::min({steps, want, cap}));
     const int64_t per = ceil_div(steps, want);
     *chunk = (int)(per * kAttendStep);
     *parts = (int)ceil_div(steps, per);
@@ -126,14 +125,20 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     // The prefix gets parts of its own where the scratch can hold its results; else every sequence reads it itself.
     const bool apart = prefix > 0 && cap >= 2;
     p.own_from = apart ? prefix : 0;
+    // The kernel for few vectors runs best with one workgroup a CU (64 sequences of up to 4096 tokens: 73 us
+    // uncut, 76 and 80 us in parts of 1024 and 512); parts of 2048 tokens bound what a single long sequence of a
+    // ragged batch costs.  The one for many vectors has two workgroups a CU, of which the second hides the first's
+    // waits; the prefix, whose results are all joined, one.
+    const bool few = attend_tile(p) < kAttendWide;
     int parts = 1;
-    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, attend_tile(p), wp.cu_count, apart ? cap / 2 : cap, &parts,
-        &p.chunk);
-    if (apart) cut(prefix, prefix_blocks, attend_tile_prefix(p), wp.cu_count, cap - parts, &p.prefix_parts, &p.prefix_chunk);
+    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, few ? wp.cu_count : 2 * wp.cu_count, few ? 2048 : kKvMaxLen,
+        apart ? cap / 2 : cap, &parts, &p.chunk);
+    if (apart) cut(prefix, prefix_blocks, wp.cu_count, kKvMaxLen, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
-    if (std::max({own_blocks * parts, prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs}) > kKvMaxGrid)
+    if (std::max(own_blocks * parts + prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs) > kKvMaxGrid)
         return QLIN_ERR_UNSUPPORTED;
     p.by_seqs = fast_div(p.b.seqs);
+    p.by_q_heads = fast_div(q_heads);
     p.by_heads = fast_div(cache->c.heads);
     p.by_tiles = fast_div((int)tiles);
     p.by_prefix_tiles = fast_div((int)prefix_tiles);
