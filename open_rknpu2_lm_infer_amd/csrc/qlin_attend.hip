@@ -128,7 +128,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false, bad = false, bad_next = false;
     StepData<DP> d;
-    Tile next[2];
+    Half16<DP> next[2];
     auto find_step = [&](int j) {
         bad_next = false;
 #pragma unroll
@@ -136,26 +136,26 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
             const int jt = j + 16 * t, jj = min(jt, end - 1);
             int id = -1;
             if (end > 0) id = SHARED || jj < p.prefix ? prefix[jj >> p.c.shift] : table[jj >> p.c.shift];
-            next[t] = find_tile<DP>(p.c, id, h, jt & off_mask, jt < end);
+            next[t] = find_half<DP>(p.c, id, h, jt & off_mask, jt < end);
             if (jt < end) bad_next |= next[t].bad;
         }
         bad_page |= bad_next;
     };
     auto load_k = [&] {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) load_bytes<DP / 4>(d.k[t], next[t].k, n * DP + g * (DP / 4));
+        for (int t = 0; t < 2; ++t) load_bytes<DP / 4>(d.k[t], next[t].block, n * DP + g * (DP / 4), next[t].k);
     };
     auto load_scales = [&] {
         bad = bad_next;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            d.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].ks, 16 * g, 0, 0));
-            d.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].vs, 16 * g, 0, 0));
+            d.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].block, 16 * g, next[t].ks, 0));
+            d.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].block, 16 * g, next[t].vs, 0));
         }
     };
     auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_bytes<DP / 16>(d.v[i], next[i / 4].v, (4 * g + i % 4) * DP + n * (DP / 16));
+        for (int i = 0; i < 8; ++i) load_bytes<DP / 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * DP + n * (DP / 16), next[i / 4].v);
     };
     int j = j0 + 32 * wave;
     find_step(j);
@@ -456,10 +456,10 @@ hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     const int own = attend_tile(p), shared = p.prefix_parts ? attend_tile_prefix(p) : 0;
     const uint32_t own_blocks = (uint32_t)((p.parts - p.prefix_parts) * (int64_t)p.b.seqs * p.c.heads * p.by_tiles.d);
     const uint32_t shared_blocks = (uint32_t)(p.prefix_parts * (int64_t)p.c.heads * p.by_prefix_tiles.d);
-    if (shared == kAttendWide)
+    if (shared >= kAttendWide)
         if (hipError_t e = launch_attend_wide(p, true, st)) return e;
-    if (own == kAttendWide) return launch_attend_wide(p, false, st);
-    const uint32_t first = shared == kAttendWide ? 0 : shared_blocks;
+    if (own >= kAttendWide) return launch_attend_wide(p, false, st);
+    const uint32_t first = shared >= kAttendWide ? 0 : shared_blocks;
     const dim3 grid(first + own_blocks);
     if (first == 0) {
         if constexpr (DP <= 128)

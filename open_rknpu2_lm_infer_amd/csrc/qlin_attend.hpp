@@ -123,40 +123,41 @@ struct Bytes {
 typedef const __attribute__((address_space(4))) int32_t* const_ids;
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
-// Where a wave finds 16 tokens: their keys, values and scales as buffers of exactly that size, so
-// that an absent tile (past the end, or on a page outside the cache) reads zeros without an access.
-struct Tile {
-    __amdgpu_buffer_rsrc_t k, v, ks, vs;
-    bool bad;  // the page id was outside the cache
-};
-
+// Where a wave finds 16 tokens: the block of their page and head as a buffer, and the offsets of their keys,
+// values and scales.  An id outside the cache leads to page 0 (bad); a group that is not there is a
+// buffer of no bytes, which reads without an access.
 template <int DP>
-__device__ __forceinline__ Tile find_tile(const KvCache& c, int id, int head, int off, bool there) {
-    Tile t;
-    t.bad = false;
-    const int page = kv_page(id, c.pages, &t.bad);
-    there = there && !t.bad;
-    const KvBlock<DP> b(c, page, head);
-    constexpr int flags = 0x00027000;  // raw, 32-bit elements
-    t.k = __builtin_amdgcn_make_buffer_rsrc(b.k(off), (short)0, there ? 16 * DP : 0, flags);
-    t.v = __builtin_amdgcn_make_buffer_rsrc(b.v(off), (short)0, there ? 16 * DP : 0, flags);
-    t.ks = __builtin_amdgcn_make_buffer_rsrc(b.ks(off), (short)0, there ? 64 : 0, flags);
-    t.vs = __builtin_amdgcn_make_buffer_rsrc(b.vs(off), (short)0, there ? 64 : 0, flags);
-    return t;
+struct Half16 {
+    __amdgpu_buffer_rsrc_t block;
+    int k, v, ks, vs;
+    bool bad;
+};
+template <int DP>
+__device__ __forceinline__ Half16<DP> find_half(const KvCache& c, int id, int head, int off, bool there) {
+    Half16<DP> x;
+    x.bad = false;
+    const int page = kv_page(id, c.pages, &x.bad), values = DP << c.shift, bytes = (2 * DP + 8) << c.shift;
+    x.block = __builtin_amdgcn_make_buffer_rsrc(c.data + ((int64_t)page * c.heads + head) * bytes, (short)0,
+                                                there ? bytes : 0, 0x00027000);  // raw, 32-bit elements
+    x.k = off * DP;
+    x.v = values + off * DP;
+    x.ks = 2 * values + 4 * off;
+    x.vs = x.ks + (4 << c.shift);
+    return x;
 }
 
-// N consecutive bytes of a buffer.
+// N consecutive bytes of a buffer, at a lane's offset from `from` on.
 template <int N>
-__device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at) {
-    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
+__device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at, int from) {
+    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
     else if constexpr (N == 8) {
-        const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
+        const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, from, 0));
         r.w[0] = x[0];
         r.w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N / 16; ++i) {
-            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, 0, 0));
+            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, from, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
         }

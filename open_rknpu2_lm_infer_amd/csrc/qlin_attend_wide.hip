@@ -1,7 +1,7 @@
 // Attention of many rows over the 8-bit key/value cache: prompts, chunks of prompts, and the shared
 // prefix of a batch.  The formulas are those of qlin_attend.hip.
 //
-// A workgroup holds 128 or 256 vectors, 32 or 64 a wave, and walks over its tokens 32 at a time.  The
+// A workgroup holds 128 vectors, 32 a wave, and walks over its tokens 32 at a time.  The
 // bytes of a tile are loaded two tiles ahead, made into fp16 codes once for the four waves and laid down
 // in the LDS: keys as they are, values transposed.  The matrix core's result layout of S^T = K Q^T (a
 // lane holds four tokens of every eight of one vector) is the operand layout of O^T = V^T P^T with its
@@ -42,11 +42,11 @@ struct Share {
     bool bad[SUBS];
 };
 
-template <int DP, int NT, int LIMBS, bool Q16, bool SHARED>
-__global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
+template <int DP, int LIMBS, bool Q16, bool SHARED>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
     using L = TileLds<DP>;
     using Sh = Share<DP>;
-    constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide * NT;
+    constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -63,11 +63,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
     b = by_tiles.div(b);
     const int seq = SHARED ? 0 : p.by_seqs.mod(b), part = SHARED ? b : p.by_seqs.div(b);
 
-    // how many tokens each vector sees (-1: no vector); vectors v0 + 32 (NT wave + y) + n
+    // how many tokens each vector sees (-1: no vector); vector v0 + 32 wave + n
     int first_row = 0, cap, end, least;  // no vector sees end or more; all see the first `least`
-    int seen[NT];
+    int seen;
     const int j0 = (SHARED ? 0 : p.own_from) + part * chunk;
-    const int v = v0 + 32 * NT * wave + n;
+    const int v = v0 + 32 * wave + n;
     if constexpr (SHARED) {
         int* lds_seen = reinterpret_cast<int*>(lds);  // before the first tile
         cap = min(p.prefix, j0 + chunk);
@@ -96,8 +96,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
             least = min(least, __shfl_xor(least, o, 64));
         }
         end = min(cap, end);
-#pragma unroll
-        for (int y = 0; y < NT; ++y) seen[y] = lds_seen[32 * (NT * wave + y) + n];
+        seen = lds_seen[32 * wave + n];
         __syncthreads();
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
@@ -109,28 +108,21 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         cap = min(s.len, j0 + chunk);
         end = min(cap, kv_visible(s, p.group.div(min(v0 + VT, vectors) - 1)));
         least = min(cap, kv_visible(s, p.group.div(v0)));
-#pragma unroll
-        for (int y = 0; y < NT; ++y) seen[y] = v + 32 * y < vectors ? kv_visible(s, p.group.div(v + 32 * y)) : -1;
+        seen = v < vectors ? kv_visible(s, p.group.div(v)) : -1;
     }
     end = __builtin_amdgcn_readfirstlane(end);
     least = __builtin_amdgcn_readfirstlane(least);
 
     // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of its vector (vectors that
     // are none take the first row's)
-    half8v qf[NT][KS][LIMBS];
-    float unit[NT];
-    int64_t row[NT];
-    int head[NT];
-#pragma unroll
-    for (int y = 0; y < NT; ++y) {
-        row[y] = first_row + p.group.div(seen[y] >= 0 ? v + 32 * y : 0);
-        head[y] = h * group + p.group.mod(seen[y] >= 0 ? v + 32 * y : 0);
-    }
-    auto load_queries = [&](int y) {
+    half8v qf[KS][LIMBS];
+    float unit = 1.0f;
+    const int64_t row = first_row + p.group.div(seen >= 0 ? v : 0);
+    const int head = h * group + p.group.mod(seen >= 0 ? v : 0);
+    auto load_queries = [&] {
         QueryRow<KS, Q16> qr;
-        load_query<KS, 16, Q16>(p, qr, row[y] * p.ldq + (int64_t)head[y] * p.c.dim, 8 * hi);
+        load_query<KS, 16, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
         float up = 1.0f;
-        unit[y] = 1.0f;
         if constexpr (LIMBS == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float top = 0.0f;
@@ -141,7 +133,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const int e = kv_clamp((int)((__float_as_uint(top) >> 23) & 0xff) - 127, -100, 126);
             up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
-            unit[y] = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+            unit = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -150,7 +142,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
                 _Float16 z[LIMBS];
                 split_f16<LIMBS>(query_at<KS, Q16>(qr, k, i) * up, z);
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) qf[y][k][q][i] = z[q];
+                for (int q = 0; q < LIMBS; ++q) qf[k][q][i] = z[q];
             }
     };
 
@@ -173,27 +165,30 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
             ids[i] = (SHARED || jt < p.prefix ? prefix : table)[jt >> p.c.shift];
         }
     };
-    Tile at[Sh::SUBS];
-    bool there[Sh::SUBS];
-    auto find = [&](int j) {  // past the end: zeros without an access
+    // Past the end the last page is read again, an id outside the cache reads page 0: all of that is masked or
+    // made NaN.
+    Half16<DP> at[Sh::SUBS];
+    auto find = [&](int j) {
 #pragma unroll
         for (int i = 0; i < Sh::SUBS; ++i) {
             const int jt = j + 16 * half(i);
-            there[i] = helps && jt < end;
-            at[i] = find_tile<DP>(p.c, ids[i], h, jt & off_mask, there[i]);
+            at[i] = find_half<DP>(p.c, ids[i], h, jt & off_mask, true);
+            at[i].bad = at[i].bad && jt < end;
+            bad_page |= at[i].bad;
         }
     };
     auto load_share = [&](Sh& sh) {
+        if (DP == 64 && !helps) return;
 #pragma unroll
         for (int i = 0; i < Sh::SUBS; ++i) {
-            sh.bad[i] = there[i] && at[i].bad;
-            bad_page |= sh.bad[i];
-            sh.k[i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(at[i].k, k_at, 0, 0));
+            sh.bad[i] = at[i].bad;
+            sh.k[i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(at[i].block, k_at, at[i].k, 0));
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(at[i].v, v_at + x * DP, 0, 0);
-            // lanes from 16 on lie outside the buffer
-            sh.ks[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].ks, 4 * lane, 0, 0));
-            sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].vs, 4 * lane, 0, 0));
+            for (int x = 0; x < 4; ++x)
+                sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(at[i].block, v_at + x * DP, at[i].v, 0);
+            const int s = 4 * (lane & 15);
+            sh.ks[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].block, s, at[i].ks, 0));
+            sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].block, s, at[i].vs, 0));
         }
     };
     const float key_unit = LIMBS == 2 ? 1.0f : p.scale2 * kCodeUnit;
@@ -227,152 +222,143 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         }
     };
 
-    float m[NT], l[NT], top[NT];
-    float16v x[NT], o[NT][ND];  // exponents of a tile: tokens 8 c + 4 hi + i of vector n; outputs
-    half8v pf[NT][2][LIMBS];
+    float m = kNegInf, l = 0.0f, top = kNegInf;
+    float16v x, o[ND];  // exponents of a tile: tokens 8 c + 4 hi + i of vector n; outputs
+    half8v pf[2][LIMBS];
 #pragma unroll
-    for (int y = 0; y < NT; ++y) {
-        m[y] = top[y] = kNegInf;
-        l[y] = 0.0f;
+    for (int t = 0; t < ND; ++t)
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[y][t][i] = 0.0f;
-    }
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
 
     // The two phases of a step are written in the order that the instructions are to be issued in, held by
     // scheduling barriers: LDS reads early, and after each matrix instruction the vector work that runs beside it.
     auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
     // P of elements 2 i and 2 i + 1 of x
-    auto exponents = [&](int y, int i, float base, const float4v* iv) {
+    auto exponents = [&](int i, float base, const float4v* iv) {
         typedef float float2v __attribute__((ext_vector_type(2)));
-        const float2v e = {__builtin_amdgcn_exp2f(x[y][2 * i] - base), __builtin_amdgcn_exp2f(x[y][2 * i + 1] - base)};
-        l[y] = __builtin_fmaf(e[0], iv[i / 2][2 * i % 4], l[y]);
-        l[y] = __builtin_fmaf(e[1], iv[i / 2][2 * i % 4 + 1], l[y]);
+        const float2v e = {__builtin_amdgcn_exp2f(x[2 * i] - base), __builtin_amdgcn_exp2f(x[2 * i + 1] - base)};
+        l = __builtin_fmaf(e[0], iv[i / 2][2 * i % 4], l);
+        l = __builtin_fmaf(e[1], iv[i / 2][2 * i % 4 + 1], l);
         const half2v z = __builtin_convertvector(e, half2v);
-        pf[y][i / 4][0][2 * i % 8] = z[0];
-        pf[y][i / 4][0][2 * i % 8 + 1] = z[1];
+        pf[i / 4][0][2 * i % 8] = z[0];
+        pf[i / 4][0][2 * i % 8 + 1] = z[1];
         if constexpr (LIMBS == 2) {
             const half2v w = __builtin_convertvector(e - __builtin_convertvector(z, float2v), half2v);
-            pf[y][i / 4][1][2 * i % 8] = w[0];
-            pf[y][i / 4][1][2 * i % 8 + 1] = w[1];
+            pf[i / 4][1][2 * i % 8] = w[0];
+            pf[i / 4][1][2 * i % 8 + 1] = w[1];
         }
     };
     // exponents from products, elements 2 i and 2 i + 1; MASK where some vector does not see all of the tile
-    auto scale = [&](const float16v& s, int y, int i, int left, const float4v* ks, const float4v* lv, auto mask) {
+    auto scale = [&](const float16v& s, int i, int left, const float4v* ks, const float4v* lv, auto mask) {
 #pragma unroll
         for (int e = 2 * i; e < 2 * i + 2; ++e) {
             float z = s[e];
-            if constexpr (LIMBS == 2) z *= unit[y];
+            if constexpr (LIMBS == 2) z *= unit;
             z = __builtin_fmaf(z, ks[e / 4][e % 4], lv[e / 4][e % 4]);
             // masked tokens are chosen away, whatever their scales hold
             if constexpr (decltype(mask)::value) z = 8 * (e / 4) + e % 4 < left ? z : kNegInf;
-            asm volatile("" : "+v"(z));  // computed here, not where it is used next
-            x[y][e] = z;
-            top[y] = fmaxf(top[y], z);
+            x[e] = z;
         }
+        // the exponents are computed here, not where they are used next
+        float t = top, a = x[2 * i], b = x[2 * i + 1];
+        asm volatile("v_max3_f32 %0, %1, %2, %0" : "+v"(t), "+v"(a), "+v"(b));
+        top = t;
+        x[2 * i] = a;
+        x[2 * i + 1] = b;
     };
     auto key = [&](const uint8_t* buf, int k) { return *reinterpret_cast<const half8v*>(buf + n * L::KROW + 16 * hi + 32 * k); };
     auto value = [&](const uint8_t* buf, int c, int t) {
         return *reinterpret_cast<const half8v*>(buf + L::V + (32 * t + n) * L::VROW + 16 * hi + 32 * c);
     };
-    auto factors = [&](const uint8_t* buf, int which, float4v* f) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            f[c] = *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(buf + L::S) + which * kTokens + 8 * c + 4 * hi);
+    // scale factors of tokens 8 c + 4 hi + 0..3: 0 of the keys, 1 logarithms of the values', 2 their inverses
+    auto factor = [&](const uint8_t* buf, int which, int c) {
+        return *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(buf + L::S) + which * kTokens + 8 * c + 4 * hi);
     };
     // First P of tile u (its values lie in bu) beside the products of tile u + 1 (NEXT: its keys in bk). Then
     // the outputs of tile u beside the exponents of tile u + 1, at token j, and the way of tile u + 2 into bn.
-    auto advance = [&](const uint8_t* bu, const uint8_t* bk, uint8_t* bn, const Sh& sh, int j, auto next, auto mask) {
+    auto advance = [&](const uint8_t* bu, const uint8_t* bk, uint8_t* bn, Sh& sh, int j, auto next, auto mask) {
         constexpr bool NEXT = decltype(next)::value;
         constexpr int SV = 2 * ND;                                  // matrix steps of O
         constexpr int EP = (8 + KS - 1) / KS;                       // pairs of exponents beside a matrix step of S
         constexpr int FROM = SV >= 8 ? 1 : 0;                       // the products are on their way until then
         constexpr int SP = (8 + SV - FROM - 1) / (SV - FROM);       // pairs beside a matrix step of O
         constexpr int PP = (PIECES + SV - 1) / SV;
-        float4v iv[4], ks[4], lv[4];
+        constexpr int AHEAD = KS / 2 < ND ? KS / 2 : ND;            // operands on their way
+        float4v iv[5], ks[5], lv[5];
         half8v kf[KS], vf[SV];
-        float16v s[NT];
-        float base[NT];
+        float16v s;
         if constexpr (NEXT) {
 #pragma unroll
-            for (int k = 0; k < KS / 2; ++k) kf[k] = key(bk, k);
+            for (int k = 0; k < AHEAD; ++k) kf[k] = key(bk, k);
 #pragma unroll
-            for (int y = 0; y < NT; ++y)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[y][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[i] = 0.0f;
         }
-        factors(bu, 2, iv);
+        iv[0] = factor(bu, 2, 0);
         pin();
-#pragma unroll
-        for (int y = 0; y < NT; ++y) base[y] = m[y] == kNegInf ? 0.0f : m[y] - kPShift;
+        // the first pairs run while the keys are on their way
+        const float base = m == kNegInf ? 0.0f : m - kPShift;
+        exponents(0, base, iv);
+        pin();
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                if constexpr (NEXT)
-#pragma unroll
-                    for (int q = 0; q < LIMBS; ++q) s[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[y][k][q], s[y], 0, 0, 0);
-#pragma unroll
-                for (int i = k * EP; i < (k + 1) * EP; ++i)
-                    if (i < 8) exponents(y, i, base[y], iv);
-                if (y == 0) {
-                    if (NEXT && k < KS / 2) kf[k + KS / 2] = key(bk, k + KS / 2);
-                    if (k >= KS - ND) vf[k - (KS - ND)] = value(bu, 0, k - (KS - ND));
-                }
-                pin();
+            for (int i = k * EP; i < (k + 1) * EP; ++i)
+                if (i < 8 && i % 2 == 0 && i / 2 < 3) iv[i / 2 + 1] = factor(bu, 2, i / 2 + 1);  // two pairs ahead
+            if (NEXT && k + AHEAD < KS) kf[k + AHEAD] = key(bk, k + AHEAD);
+            if (k >= KS - AHEAD) vf[k - (KS - AHEAD)] = value(bu, (k - (KS - AHEAD)) / ND, (k - (KS - AHEAD)) % ND);
+            if (NEXT && k == KS - 1) {
+                ks[0] = factor(bk, 0, 0);
+                lv[0] = factor(bk, 1, 0);
             }
-        }
-        if constexpr (NEXT) {
-            factors(bk, 0, ks);
-            factors(bk, 1, lv);
-        }
-        int left[NT];
+            if constexpr (NEXT)
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            top[y] = kNegInf;
-            left[y] = min(seen[y], cap) - j - 4 * hi;
+                for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[k][q], s, 0, 0, 0);
+#pragma unroll
+            for (int i = k * EP + 1; i < (k + 1) * EP + 1; ++i)
+                if (i < 8) exponents(i, base, iv);
+            pin();
         }
+        if constexpr (NEXT) find(j + 2 * kTokens);
+        top = kNegInf;
+        const int left = min(seen, cap) - j - 4 * hi;
 #pragma unroll
         for (int t = 0; t < SV; ++t) {
+            if (t + AHEAD < SV) vf[t + AHEAD] = value(bu, (t + AHEAD) / ND, (t + AHEAD) % ND);
+            if constexpr (NEXT) {
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-#pragma unroll
-                for (int q = 0; q < LIMBS; ++q) o[y][t % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t], pf[y][t / ND][q], o[y][t % ND], 0, 0, 0);
-                if constexpr (NEXT) {
-#pragma unroll
-                    for (int i = (t - FROM) * SP; i < (t - FROM + 1) * SP; ++i)
-                        if (i >= 0 && i < 8) scale(s[y], y, i, left[y], ks, lv, mask);
-                }
-                if (y == 0 && t < ND) vf[t + ND] = value(bu, 1, t);
-                if (NEXT && y == NT - 1)
-#pragma unroll
-                    for (int i = t * PP; i < (t + 1) * PP; ++i)
-                        if (i < PIECES) store_piece(sh, bn, i);
-                pin();
+                for (int i = (t - FROM) * SP; i < (t - FROM + 1) * SP; ++i)
+                    if (i >= 0 && i < 8 && i % 2 == 0 && i / 2 < 3) {
+                        ks[i / 2 + 1] = factor(bk, 0, i / 2 + 1);
+                        lv[i / 2 + 1] = factor(bk, 1, i / 2 + 1);
+                    }
             }
+#pragma unroll
+            for (int q = 0; q < LIMBS; ++q) o[t % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t], pf[t / ND][q], o[t % ND], 0, 0, 0);
+            if constexpr (NEXT) {
+#pragma unroll
+                for (int i = (t - FROM) * SP; i < (t - FROM + 1) * SP; ++i)
+                    if (i >= 0 && i < 8) scale(s, i, left, ks, lv, mask);
+#pragma unroll
+                for (int i = t * PP; i < (t + 1) * PP; ++i)
+                    if (i < PIECES) store_piece(sh, bn, i);
+            }
+            pin();
         }
         if constexpr (NEXT) store_scales(sh, bn);
     };
-    auto raise = [&] {
+    auto passed = [&] {  // some vector's maximum is to be raised
         typedef unsigned int pair __attribute__((ext_vector_type(2)));
-        bool up = false;
+        const pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false));
+        top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        return __builtin_amdgcn_ballot_w64(top > m + kSlack) != 0;
+    };
+    auto raise = [&] {
+        const float m_new = fmaxf(m, top);
+        const float fade = m == m_new ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= fade;
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            const pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(top[y]), __float_as_uint(top[y]), false, false));
-            top[y] = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-            up |= top[y] > m[y] + kSlack;
-        }
-        if (!__builtin_amdgcn_ballot_w64(up)) return;
-#pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            const float m_new = fmaxf(m[y], top[y]);
-            const float fade = m[y] == m_new ? 1.0f : __builtin_amdgcn_exp2f(m[y] - m_new);
-            m[y] = m_new;
-            l[y] *= fade;
-#pragma unroll
-            for (int t = 0; t < ND; ++t) o[y][t] *= fade;
-        }
+        for (int t = 0; t < ND; ++t) o[t] *= fade;
     };
 
     if (j0 < end) {
@@ -388,8 +374,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         find(j0 + 2 * kTokens);
         load_share(sh);
         load_ids(j0 + 3 * kTokens);
-#pragma unroll
-        for (int y = 0; y < NT; ++y) load_queries(y);
+        load_queries();
         auto store_share = [&](const Sh& sh, uint8_t* buf) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) store_piece(sh, buf, i);
@@ -400,89 +385,93 @@ __global__ __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 1 : 2) void attend
         __syncthreads();
         {
             float4v ks[4], lv[4];
-            factors(lds, 0, ks);
-            factors(lds, 1, lv);
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                float16v s;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(lds, k), qf[y][k][q], s, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) scale(s, y, i, min(seen[y], cap) - j0 - 4 * hi, ks, lv, std::true_type{});
+            for (int c = 0; c < 4; ++c) {
+                ks[c] = factor(lds, 0, c);
+                lv[c] = factor(lds, 1, c);
             }
+            float16v s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(lds, k), qf[k][q], s, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) scale(s, i, min(seen, cap) - j0 - 4 * hi, ks, lv, std::true_type{});
         }
-        raise();
+        if (passed()) raise();
         // tile u's values, tile u + 1's keys, tile u + 2's place
         int bu = 0, bk = L::BYTES, bn = 2 * L::BYTES;
         int j = j0;
         auto step = [&](auto mask) {
-            find(j + 3 * kTokens);
             advance(lds + bu, lds + bk, lds + bn, sh, j + kTokens, std::true_type{}, mask);
             load_share(sh);
             load_ids(j + 4 * kTokens);
-            raise();
             lds_barrier();  // the bytes of later tiles stay on their way
             const int t = bu;
             bu = bk;
             bk = bn;
             bn = t;
+            j += kTokens;
         };
-        for (; j + 2 * kTokens <= least; j += kTokens) step(std::false_type{});
-        for (; j + kTokens < end; j += kTokens) step(std::true_type{});
+        // raising a maximum is rare and kept out of the loop, which leaves the outputs to the matrix core
+        auto walk = [&](int stop, auto mask) {
+            while (j < stop) {
+                bool up;
+                do {
+                    step(mask);
+                    up = passed();
+                } while (!up && j < stop);
+                if (up) raise();
+            }
+        };
+        walk(least - 2 * kTokens + 1, std::false_type{});
+        walk(end - kTokens, std::true_type{});
         advance(lds + bu, nullptr, nullptr, sh, 0, std::false_type{}, std::false_type{});
     }
     if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
 
+    l += __shfl_xor(l, 32, 64);
+    if (seen < 0) return;
+    if (p.parts == 1) {
+        const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
 #pragma unroll
-    for (int y = 0; y < NT; ++y) {
-        l[y] += __shfl_xor(l[y], 32, 64);
-        if (seen[y] < 0) continue;
-        if (p.parts == 1) {
-            const float f = l[y] == 0.0f ? 0.0f : kCodeUnit / l[y];
+        for (int i = 0; i < 16; ++i) {
+            float z[ND];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float z[ND];
+            for (int t = 0; t < ND; ++t) z[t] = o[t][i] * f;
+            store_out<ND>(p, row * p.ldo + (int64_t)head * p.c.dim, (8 * (i / 4) + 4 * hi + i % 4) * ND, z);
+        }
+    } else {
+        const int64_t slot = (row * p.q_heads + head) * p.parts + (SHARED ? 0 : p.prefix_parts) + part;
 #pragma unroll
-                for (int t = 0; t < ND; ++t) z[t] = o[y][t][i] * f;
-                store_out<ND>(p, row[y] * p.ldo + (int64_t)head[y] * p.c.dim, (8 * (i / 4) + 4 * hi + i % 4) * ND, z);
-            }
-        } else {
-            const int64_t slot = (row[y] * p.q_heads + head[y]) * p.parts + (SHARED ? 0 : p.prefix_parts) + part;
+        for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                for (int t = 0; t < ND; ++t) p.part_o[slot * DP + (8 * (i / 4) + 4 * hi + i % 4) * ND + t] = o[y][t][i];
-            if (hi == 0) {
-                p.part_ml[2 * slot] = m[y];
-                p.part_ml[2 * slot + 1] = l[y];
-            }
+            for (int t = 0; t < ND; ++t) p.part_o[slot * DP + (8 * (i / 4) + 4 * hi + i % 4) * ND + t] = o[t][i];
+        if (hi == 0) {
+            p.part_ml[2 * slot] = m;
+            p.part_ml[2 * slot + 1] = l;
         }
     }
 }
 
-template <int DP, int NT, int LIMBS, bool Q16, bool SHARED>
+template <int DP, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_one(const AttendParams& p, hipStream_t st) {
     constexpr int bytes = 3 * TileLds<DP>::BYTES;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, NT, LIMBS, Q16, SHARED>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, Q16, SHARED>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (attr != hipSuccess) return attr;
     const int64_t tiles = SHARED ? p.by_prefix_tiles.d : p.by_tiles.d;
     const int64_t blocks = tiles * p.c.heads * (SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs);
-    attend_wide_kernel<DP, NT, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
+    attend_wide_kernel<DP, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
     return hipGetLastError();
 }
 
 template <int DP, bool SHARED>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
-    if (!p.q_f16) return launch_one<DP, 1, 2, false, SHARED>(p, st);
-    if (!p.o_f16) return launch_one<DP, 1, 2, true, SHARED>(p, st);
-    if constexpr (DP <= 128)
-        if ((SHARED ? attend_tile_prefix(p) : attend_tile(p)) == 2 * kAttendWide) return launch_one<DP, 2, 1, true, SHARED>(p, st);
-    return launch_one<DP, 1, 1, true, SHARED>(p, st);
+    if (!p.q_f16) return launch_one<DP, 2, false, SHARED>(p, st);
+    return p.o_f16 ? launch_one<DP, 1, true, SHARED>(p, st) : launch_one<DP, 2, true, SHARED>(p, st);
 }
 
 template <int DP>
