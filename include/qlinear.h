@@ -353,9 +353,9 @@ int qlin_chain_status(qlin_chain* chain, int32_t clear);
 /* ---- key/value cache in 8 bits, and attention over it ----
  * The reference keeps its keys and values in FP16 and runs attention as a unit of the native
  * library (src/npu/attention.rs); these calls keep a decoder layer on the device between its qkv
- * and o projections.  Keys and values are quantized by the per-token rule of the activations, one scale per
- * token and KV head:
- *   s = max(absmax_d |x[d]| / 127, 2^-64),  code[d] = clamp(round(x[d] * (1/s)), -127, 127)
+ * and o projections.  Keys and values are quantized like the activations, one scale per token and KV head:
+ *   s = max(absmax_d |x[d]| * (1/127), 2^-64),  code[d] = clamp(round(x[d] * (1/s)), -127, 127)
+ * each operation one f32 rounding and 1/127 the nearest f32 (the scale is within one f32 step of the quotient).
  * A row with Inf or NaN gets the scale NaN (whoever reads it gets NaN) and sets
  * QLIN_ERR_NONFINITE in the workspace's error word.
  *

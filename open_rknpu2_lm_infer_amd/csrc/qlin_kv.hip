@@ -1,8 +1,10 @@
 // Key/value cache in 8 bits: new rows quantized into their pages, and read back.
 //
-// A row is the key (or value) of one token and one head, dim values x.  With the rule of the
-// per-token activation quantization, s = max(absmax |x| / 127, 2^-64) and
-// code = clamp(round(x * (1 / s)), -127, 127), every operation one f32 rounding.  A row that holds
+// A row is the key (or value) of one token and one head, dim values x:
+//   s = max(absmax |x| * (1/127), 2^-64),  code = clamp(round(x * (1/s)), -127, 127),
+// every operation one f32 rounding, 1/127 the f32 nearest to it.  That is the rule of the per-token
+// activation quantization but for its division by 127, whose place a multiplication takes: the
+// scales agree to one step of f32.  A row that holds
 // Inf or NaN gets codes 0 and the scale NaN: whoever reads it gets NaN, and the error word says so.
 //
 // Both kernels move their bytes once and do a few operations a value, so memory bounds them (and
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
 #pragma unroll
         for (int o = LPU / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
         const bool fin = m < 0x7f800000u;
-        const float s = fin ? fmaxf(__uint_as_float(m) / 127.0f, kKvScaleMin) : __uint_as_float(0x7fc00000u);
+        const float s = fin ? fmaxf(__uint_as_float(m) * (1.0f / 127.0f), kKvScaleMin) : __uint_as_float(0x7fc00000u);
         const float inv = fin ? 1.0f / s : 0.0f;
         uint32_t w[2] = {0, 0};
 #pragma unroll

@@ -10,7 +10,7 @@ def quantize(x, half_even=False):
     x = np.asarray(x, np.float32)
     finite = np.isfinite(x).all(-1)
     x = np.where(finite[..., None], x, np.float32(0))
-    s = np.maximum(np.abs(x).max(-1) / np.float32(127), SCALE_MIN).astype(np.float32)
+    s = np.maximum(np.abs(x).max(-1) * (np.float32(1) / np.float32(127)), SCALE_MIN).astype(np.float32)
     y = (x * (np.float32(1) / s)[..., None]).astype(np.float32).astype(np.float64)
     c = np.rint(y) if half_even else np.trunc(y + np.copysign(0.5, y))
     return np.clip(c, -127, 127), np.where(finite, s, np.float32(np.nan))

@@ -26,13 +26,17 @@ def test_structs_match_header_sizes():
 
 
 def test_reference_quantize_matches_oracle(oracle):
-    """The cache's rule is the activations' rule where that one's scale is above the cache's smallest."""
+    """The cache's rule is the activations' rule, but for a multiplication by 1/127 in the place of the division: scales
+    differ by one step of f32 at most (the factor is off by half a step and the product rounded once more), and
+    where they are equal so are the codes."""
     x = np.random.default_rng(1).standard_normal((40, 96)).astype(np.float32) * 10.0 ** np.arange(-10, 10).repeat(2)[:, None]
     x = x.astype(np.float32)
     for even in (False, True):
         c, s = kvref.quantize(x, even)
         q, so, bad = oracle.quantize(x, oracle.ROUND_EVEN if even else oracle.ROUND_AWAY)
-        assert bad == 0 and np.array_equal(c, q) and np.array_equal(s.view(np.uint32), so.view(np.uint32))
+        same = s.view(np.int32) == so.view(np.int32)
+        assert bad == 0 and (np.abs(s.view(np.int32) - so.view(np.int32)) <= 1).all() and same.sum() >= 20
+        assert np.array_equal(c[same], q[same]) and np.abs(c - q).max() <= 1
     c, s = kvref.quantize(np.array([[0.0, 0.0], [2.0 ** -70, 0.0], [np.nan, 1.0]], np.float32))
     assert s[0] == s[1] == 2.0 ** -64 and np.isnan(s[2]) and not c[0].any() and c[1, 0] == 0 and not c[2].any()
 
