@@ -20,8 +20,8 @@ namespace qlin {
 namespace {
 
 // What a wave loads for one step of 32 tokens: two tiles of 16.  Lane l (n = l % 16, g = l / 16)
-// holds, as the matrix core's A operand, columns g * DP/4 .. + DP/4 - 1 of key n of each tile, and
-// columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
+// holds, as the matrix core's A operand, columns 64 c + 16 g .. + 15 of key n of each tile (a load covers 64
+// bytes of each of 16 keys), and columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
 template <int DP>
 struct StepData {
     Bytes<DP / 4> k[2];
@@ -119,7 +119,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         const int v = seen[r] >= 0 ? v0 + 16 * r + n : 0;
         out_row[r] = first_row + p.group.div(v);
         head[r] = h * group + p.group.mod(v);
-        load_query<KS, 8, Q16>(p, qr[r], out_row[r] * p.ldq + (int64_t)head[r] * p.c.dim, g * (DP / 4));
+        load_query<KS, 64, true, Q16>(p, qr[r], out_row[r] * p.ldq + (int64_t)head[r] * p.c.dim, 16 * g);
     }
 
     // page ids through the scalar cache: nothing writes them while the kernel runs
@@ -143,7 +143,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     };
     auto load_k = [&] {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) load_bytes<DP / 4>(d.k[t], next[t].block, n * DP + g * (DP / 4), next[t].k);
+        for (int t = 0; t < 2; ++t) load_bytes<DP / 4, 64>(d.k[t], next[t].block, n * DP + 16 * g, next[t].k);
     };
     auto load_scales = [&] {
         bad = bad_next;
@@ -155,7 +155,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     };
     auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_bytes<DP / 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * DP + n * (DP / 16), next[i / 4].v);
+        for (int i = 0; i < 8; ++i) load_bytes<DP / 16, 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * DP + n * (DP / 16), next[i / 4].v);
     };
     int j = j0 + 32 * wave;
     find_step(j);
@@ -163,7 +163,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     load_scales();
     load_v();
 
-    // queries, as the B operand: lane (n, g) holds columns g * DP/4 + 8 s .. + 7 of vector n
+    // queries, as the B operand: lane (n, g) holds columns 64 c + 16 g .. + 15 of vector n, two matrix steps each
     half8v qf[R][KS][LIMBS];
     float unit[R];  // what the f16 operands were divided by, times scale2
 #pragma unroll

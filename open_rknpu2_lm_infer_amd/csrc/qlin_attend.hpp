@@ -45,33 +45,35 @@ __device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
     if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
 }
 
-// Columns of a query row on their way to the matrix core: KS groups of eight from column first on, STEP
-// apart, as they lie in memory; columns past the head's are zeros.  All loads are issued before any is used.
+// Columns of a query row on their way to the matrix core: KS groups of eight as they lie in memory, two
+// (PAIR: one 16-byte chunk of a key's bytes) or one at column first and every STEP columns; columns past the
+// head's are zeros.  All loads are issued before any is used.
 template <int KS, bool Q16>
 struct QueryRow {
     uint4v w[KS][Q16 ? 1 : 2];
 };
-template <int KS, int STEP, bool Q16>
+template <int KS, int STEP, bool PAIR, bool Q16>
 __device__ __forceinline__ void load_query(const AttendParams& p, QueryRow<KS, Q16>& r, int64_t at, int first) {
     constexpr int W = Q16 ? 1 : 2;
+    auto column = [](int k) { return PAIR ? k / 2 * STEP + k % 2 * 8 : k * STEP; };
     if (p.q_vec) {  // heads of whole groups of 8, 16-byte aligned
         const uint8_t* q = reinterpret_cast<const uint8_t*>(p.q) + (at + first) * (2 * W);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            const bool in = first + k * STEP < p.c.dim;
+            const bool in = first + column(k) < p.c.dim;
 #pragma unroll
-            for (int i = 0; i < W; ++i) r.w[k][i] = *reinterpret_cast<const uint4v*>(q + (in ? k * STEP * 2 * W : -first * 2 * W) + 16 * i);
+            for (int i = 0; i < W; ++i) r.w[k][i] = *reinterpret_cast<const uint4v*>(q + (in ? column(k) * 2 * W : -first * 2 * W) + 16 * i);
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int i = 0; i < W; ++i) r.w[k][i] = first + k * STEP < p.c.dim ? r.w[k][i] : uint4v{0, 0, 0, 0};
+            for (int i = 0; i < W; ++i) r.w[k][i] = first + column(k) < p.c.dim ? r.w[k][i] : uint4v{0, 0, 0, 0};
     } else {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 4 * W; ++i) {
-                const int d = first + k * STEP + (Q16 ? 2 * i : i), last = p.c.dim - 1;
+                const int d = first + column(k) + (Q16 ? 2 * i : i), last = p.c.dim - 1;
                 uint32_t x;
                 if constexpr (Q16) {
                     const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + at;
@@ -146,8 +148,8 @@ __device__ __forceinline__ Half16<DP> find_half(const KvCache& c, int id, int he
     return x;
 }
 
-// N consecutive bytes of a buffer, at a lane's offset from `from` on.
-template <int N>
+// N bytes of a buffer, at a lane's offset from `from` on: up to 16 of them, or 16 every STEP.
+template <int N, int STEP>
 __device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at, int from) {
     if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
     else if constexpr (N == 8) {
@@ -157,7 +159,7 @@ __device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b
     } else {
 #pragma unroll
         for (int i = 0; i < N / 16; ++i) {
-            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, from, 0));
+            const uint4v x = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(b, at + STEP * i, from, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
         }

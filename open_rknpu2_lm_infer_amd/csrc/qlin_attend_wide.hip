@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     const int head = h * group + p.group.mod(seen >= 0 ? v : 0);
     auto load_queries = [&] {
         QueryRow<KS, Q16> qr;
-        load_query<KS, 16, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
+        load_query<KS, 16, false, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
         float up = 1.0f;
         if constexpr (LIMBS == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit

@@ -116,12 +116,16 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.prefix = prefix;
     p.prefix_pages = prefix_pages;
     p.err = wp.err;
-    // parts that the workspace's scratch holds results of
-    const int64_t vectors = (int64_t)p.b.rows * q_heads;
-    const int64_t cap = wp.part_floats / (vectors * (cache->c.dim_padded + 2));
     const int64_t tiles = ceil_div((int64_t)p.b.max_new * group, attend_tile(p));
     const int64_t prefix_tiles = ceil_div((int64_t)p.b.rows * group, attend_tile_prefix(p));
     const int64_t own_blocks = (int64_t)p.b.seqs * cache->c.heads * tiles, prefix_blocks = cache->c.heads * prefix_tiles;
+    if (own_blocks > kKvMaxGrid) return QLIN_ERR_UNSUPPORTED;
+    // Parts that the workspace's scratch holds results of, that one launch covers, and that one can join (a
+    // workgroup for each vector of a batch of which all sequences had max_new rows).
+    const int64_t vectors = (int64_t)p.b.rows * q_heads;
+    const bool joins = (int64_t)p.b.max_new * q_heads * p.b.seqs <= kKvMaxGrid;
+    const int64_t cap = joins ? std::min(wp.part_floats / (vectors * (cache->c.dim_padded + 2)),
+                                         kKvMaxGrid / (own_blocks + prefix_blocks)) : 1;
     // The prefix gets parts of its own where the scratch can hold its results; else every sequence reads it itself.
     const bool apart = prefix > 0 && cap >= 2;
     p.own_from = apart ? prefix : 0;
@@ -135,8 +139,6 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
         apart ? cap / 2 : cap, &parts, &p.chunk);
     if (apart) cut(prefix, prefix_blocks, wp.cu_count, kKvMaxLen, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
-    if (std::max(own_blocks * parts + prefix_blocks * p.prefix_parts, (int64_t)p.b.max_new * q_heads * p.b.seqs) > kKvMaxGrid)
-        return QLIN_ERR_UNSUPPORTED;
     p.by_seqs = fast_div(p.b.seqs);
     p.by_q_heads = fast_div(q_heads);
     p.by_heads = fast_div(cache->c.heads);

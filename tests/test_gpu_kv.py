@@ -302,6 +302,61 @@ def test_nan_query_stays_in_its_row(ws):
     check(ql.kv_attention(ws, s.cache, s.batch(), q.to(DEV)), want, tol)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_nonfinite_f32_query_stays_in_its_row(ws, value):
+    """The same for f32 queries, which are scaled by their largest value; few rows and many."""
+    for seqs in ([(90, 3), (50, 2)], [(400, 300)]):
+        s = Setup(ws, seqs, 2, 72, 16, F32, seed=9, q_heads=4)
+        k, v = s.history()
+        s.fill(k, v)
+        q = s.rand(s.rows, 288)
+        want, tol = s.expected(q, k, v, F32)
+        q[1, 73] = value  # row 1, head 1
+        want[1, 72:144] = np.nan
+        check(ql.kv_attention(ws, s.cache, s.batch(), q.to(DEV)), want, tol)
+
+
+def test_loose_bounds(ws):
+    """Many sequences with one row each in a batch whose max_new and max_len promise far more: too many workgroups
+    for results kept apart, so nothing is cut."""
+    seqs = [(1 + 7 * i % 61, 1) for i in range(290)]
+    s = Setup(ws, seqs, 1, 40, 16, F16, seed=14, q_heads=32, max_len=2560)
+    k, v = s.history()
+    s.fill(k, v)
+    q = torch.zeros((2048, 32 * 40), dtype=F16)
+    q[:290] = s.rand(290, 32 * 40)
+    b = s.batch(max_new=2048)
+    b.c.rows = 2048
+    out = torch.full((2048, 32 * 40), 7.0, dtype=F16, device=DEV)
+    ql.kv_attention(ws, s.cache, b, q.to(DEV), out=out)
+    check(out[:290], *s.expected(q, k, v, F16))
+    assert (out[290:] == 7).all() and ws.status() == 0
+
+
+def test_prefix_without_room_for_its_results(ws):
+    """More vectors than the scratch holds two results of: every sequence reads the prefix itself."""
+    s = Setup(ws, [(2400, 2100), (2300, 2100)], 1, 64, 32, F16, seed=15, q_heads=32)
+    k, v = s.history()
+    k[2400:2400 + 192], v[2400:2400 + 192] = k[:192], v[:192]
+    s.fill(k, v)
+    q = s.rand(s.rows, 2048).to(DEV)
+    plain = ql.kv_attention(ws, s.cache, s.batch(), q)
+    pages, table = i32(s.table[0, :6]), s.table.copy()
+    table[:, :6] = -1
+    got = ql.kv_attention(ws, s.cache, s.batch(table=table), q, prefix_tokens=192, prefix_pages=pages)
+    assert torch.equal(got, plain) and ws.status() == 0
+    few = [0, 1, 2099, 2100, 4199]
+    qs = q.cpu()
+    for r in few:
+        i, t = divmod(r, 2100)
+        n = [2400, 2300][i]
+        at = [0, 2400][i]
+        kc, ks = kvref.quantize(k[at:at + n].float().numpy().reshape(n, 1, 64))
+        vc, vs = kvref.quantize(v[at:at + n].float().numpy().reshape(n, 1, 64))
+        o, tol = kvref.attend(qs[r:r + 1].double().numpy().reshape(1, 32, 64), kc, ks, vc, vs, [n - 2100 + t + 1], 0.125, 1, EPS[F16])
+        check(got[r:r + 1], o.reshape(1, -1), tol.reshape(1, -1))
+
+
 def test_bad_batches_are_flagged(ws):
     """Values in the device arrays outside the limits: flagged, nothing outside the buffers is touched, and
     sequences without fault get their results."""
