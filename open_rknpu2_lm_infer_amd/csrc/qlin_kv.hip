@@ -9,7 +9,11 @@
 //
 // Both kernels move their bytes once and do a few operations a value, so memory bounds them (and
 // the launch, for a few tokens).  A group of dim_padded / 8 lanes holds a row, 8 values a lane: 16 bytes of
-// fp16 in, 8 bytes of codes out, and the absmax is a few lane exchanges.
+// fp16 in, 8 bytes of codes out, and the absmax is a few lane exchanges.  One row a group and many
+// workgroups: two or four rows a group, their loads in flight together, are slower (both kernels over
+// 4096 tokens of 8 heads of 128: 15.9 us with one, 16.3 with two, 19.2 with four).  At that size the
+// append moves 25 MB in 9.3 us (2.7 TB/s) and the read as much in 6.7 (3.8 TB/s); one token takes them
+// 3.1 and 2.6 us, most of it the dependent loads of its place in the batch and in the page table.
 #include "qlin_kv.hpp"
 #include "qlin_rows.hpp"
 
@@ -27,13 +31,12 @@ struct Unit {
 template <int LPU>
 __device__ __forceinline__ Unit find_unit(const KvRows& p) {
     constexpr int UPB = 256 / LPU;
-    const int bps = (p.b.max_new * p.c.heads + UPB - 1) / UPB;
     Unit r;
-    r.i = blockIdx.x / bps;
-    const int u = (blockIdx.x - r.i * bps) * UPB + threadIdx.x / LPU;
+    r.i = p.by_blocks.div(blockIdx.x);
+    const int u = p.by_blocks.mod(blockIdx.x) * UPB + threadIdx.x / LPU;
     r.s = kv_seq(p.b.row_start, p.b.length, r.i, p.b.rows, p.b.max_new, p.b.max_len);
-    r.t = u / p.c.heads;
-    r.h = u - r.t * p.c.heads;
+    r.t = p.by_heads.div(u);
+    r.h = p.by_heads.mod(u);
     r.ok = r.t < r.s.rows;
     r.bad = r.s.bad;
     return r;
@@ -143,11 +146,13 @@ __global__ __launch_bounds__(256) void kv_clear_kernel(uint32_t* data, int64_t w
 }
 
 template <int DP, typename T, bool VEC>
-hipError_t launch_rows(const KvRows& p, bool append, hipStream_t st) {
+hipError_t launch_rows(KvRows p, bool append, hipStream_t st) {
     const int64_t per_seq = (int64_t)p.b.max_new * p.c.heads, upb = 256 / (DP / 8);
-    const int64_t blocks = (per_seq + upb - 1) / upb * p.b.seqs;
-    if (append) kv_append_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
-    else kv_read_kernel<DP, T, VEC><<<dim3((uint32_t)blocks), 256, 0, st>>>(p);
+    p.by_blocks = fast_div((int)((per_seq + upb - 1) / upb));
+    p.by_heads = fast_div(p.c.heads);
+    const dim3 grid((uint32_t)(p.by_blocks.d * (int64_t)p.b.seqs));
+    if (append) kv_append_kernel<DP, T, VEC><<<grid, 256, 0, st>>>(p);
+    else kv_read_kernel<DP, T, VEC><<<grid, 256, 0, st>>>(p);
     return hipGetLastError();
 }
 

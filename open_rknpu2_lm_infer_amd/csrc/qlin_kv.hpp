@@ -56,6 +56,7 @@ struct KvRows {
     int f16;
     int rne;
     uint32_t* err;
+    FastDiv by_blocks, by_heads;  // of workgroup and unit indexes
 };
 hipError_t launch_kv_append(const KvRows& p, hipStream_t stream);
 hipError_t launch_kv_read(const KvRows& p, hipStream_t stream);
