@@ -426,7 +426,9 @@ int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_b
  * kv_heads, and KV head h serves query heads h * q_heads / kv_heads ..  O: device [rows, ldo] of
  * o_dtype; it must not overlap Q.  Sums and the softmax are held in f32.  With fp16 rows in and
  * out, probabilities (scaled into fp16's range) are rounded to fp16 before they meet V; if either
- * is f32, queries and probabilities are kept to 22 bits. */
+ * is f32, queries and probabilities are kept to 22 bits.  The scales of the value rows that a row sees may lie
+ * up to 2^96 apart (a row of zeros has 2^-64, so any values below 2^39 will do); past that,
+ * tokens of the smallest values begin to lose their weight. */
 int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
                       int32_t q_heads, const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,
                       int32_t o_dtype, int64_t ldo, void* stream);

@@ -43,7 +43,8 @@ COMMON = [
 
 # Per-file additions.  The GEMM keeps its MFMA accumulators in VGPRs: with the
 # compiler's AGPR heuristics the two-tile unrolled k loop re-shuffled the accumulator
-# registers on every iteration.
+# registers on every iteration.  So does the attention of few rows, whose outputs are faded and joined
+# by vector instructions; that of many rows leaves them to the matrix core in its loop.
 FILE_FLAGS = {"qlin_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "qlin_gemm_ks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "qlin_gemm_pp.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
