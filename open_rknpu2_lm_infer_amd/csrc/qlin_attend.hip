@@ -135,15 +135,14 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     bool bad_page = false, bad = false, bad_next = false;
     StepData<DP> d;
     Half16<DP> next[2];
-    auto find_step = [&](int j) {
+    auto find_step = [&](int j) {  // end > 0
         bad_next = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int jt = j + 16 * t, jj = min(jt, end - 1);
-            int id = -1;
-            if (end > 0) id = SHARED || jj < p.prefix ? prefix[jj >> p.c.shift] : table[jj >> p.c.shift];
+            const int id = (SHARED || jj < p.prefix ? prefix : table)[jj >> p.c.shift];
             next[t] = find_half<DP>(p.c, id, h, jt & off_mask, jt < end);
-            if (jt < end) bad_next |= next[t].bad;
+            bad_next |= next[t].bad && jt < end;
         }
         bad_page |= bad_next;
     };
@@ -164,10 +163,12 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         for (int i = 0; i < 8; ++i) load_bytes<DP / 16, 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * DP + n * (DP / 16), next[i / 4].v);
     };
     int j = j0 + 32 * wave;
-    find_step(j);
-    load_k();
-    load_scales();
-    load_v();
+    if (end > 0) {
+        find_step(j);
+        load_k();
+        load_scales();
+        load_v();
+    }
 
     // queries, as the B operand: lane (n, g) holds columns 64 c + 16 g .. + 15 of vector n, two matrix steps each
     half8v qf[R][KS][LIMBS];
