@@ -16,9 +16,9 @@
 // axis permuted, and P never leaves its lane.
 //
 // What bounds it, 8 KV heads of 128, 4 query heads each: with few rows a token's bytes, 2 * 128 + 8 a head (64
-// sequences of up to 4096 tokens, 263 MB: 66 us, 4.0 TB/s; one of 32768, 69 MB in 256 parts of 1024: 14.3 us,
-// 4.8 TB/s, and 4.6 us for the join), with one short sequence the chain of dependent loads, steps and the
-// waves' join (300 tokens: 7.6 us).  A prefix of 8192 tokens for 32 rows, 128 vectors a KV head in tiles of 32, takes 20 us
+// sequences of up to 4096 tokens, 263 MB: 64 us, 4.1 TB/s; one of 32768, 69 MB in 256 parts of 1024: 14.2 us,
+// 4.9 TB/s, and 4.2 us for the join), with one short sequence the chain of dependent loads, steps and the
+// waves' join (300 tokens: 7.5 us).  A prefix of 8192 tokens for 32 rows, 128 vectors a KV head in tiles of 32, takes 20 us
 // with the rows' own tokens: the vector units' exponents and byte permutes (28% of their time, waits for loads 48%).
 #include "qlin_attend.hpp"
 

@@ -303,7 +303,7 @@ class KVCache:
         info = _lib.KVInfo()
         check(_lib.load().qlin_kv_query(self.handle, ctypes.byref(info)), "qlin_kv_query")
         self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
-        self.columns, self.device_bytes = kv_heads * head_dim, info.device_bytes
+        self.columns, self.device_bytes, self.device = kv_heads * head_dim, info.device_bytes, info.device
 
     def close(self):
         if self.handle:
@@ -357,6 +357,7 @@ def _kv_ld(batch: KVBatch, t: torch.Tensor, cols: int) -> int:
 
 def _kv_check(cache: KVCache, batch: KVBatch) -> None:
     assert batch.columns * cache.page_tokens >= batch.c.max_len, "the page table is too narrow for max_len"
+    assert batch.device.index == cache.device, "the batch and the cache are on different devices"
 
 
 def kv_append(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor, V: torch.Tensor, flags: int = 0) -> None:

@@ -429,6 +429,34 @@ def test_shared_prefix(ws, dtype, prefix, seqs, hq, hk, D, P):
     s.cache.close()
 
 
+@pytest.mark.parametrize("new", [2, 150])
+def test_rows_before_the_first_sequence(ws, new):
+    """row_start[0] > 0: the rows before it are nobody's, with a prefix and without, few vectors and many."""
+    hq, hk, D, P, skip = 8, 2, 64, 32, 5
+    s = Setup(ws, [(200, new), (230, 1)], hk, D, P, F16, seed=new, q_heads=hq)
+    k, v = s.history()
+    k[200:328], v[200:328] = k[:128], v[:128]
+    s.fill(k, v)
+    q = s.rand(s.rows, hq * D)
+    want, tol = s.expected(q, k, v, F16)
+    b = ql.KVBatch(i32(s.starts + skip), i32([200, 230]), i32(s.table), s.rows + skip + 3, new, 230)
+    qs = torch.full((b.rows, hq * D), float("nan"), dtype=F16)
+    qs[skip:skip + s.rows] = q
+    pages = i32(s.table[0, :4])
+    for kw in ({}, dict(prefix_tokens=128, prefix_pages=pages)):
+        out = torch.full((b.rows, hq * D), 7.0, dtype=F16, device=DEV)
+        ql.kv_attention(ws, s.cache, b, qs.to(DEV), out=out, **kw)
+        check(out[skip:skip + s.rows], want, tol)
+        assert (out[:skip] == 7).all() and (out[skip + s.rows:] == 7).all()
+    ko = torch.full((b.rows, hk * D), 7.0, dtype=F16, device=DEV)
+    vo = ko.clone()
+    ql.kv_read(ws, s.cache, b, ko, vo)
+    for o in (ko, vo):
+        assert (o[:skip] == 7).all() and (o[skip + s.rows:] == 7).all() and not (o[skip:skip + s.rows] == 7).all(1).any()
+    assert ws.status() == 0
+    s.cache.close()
+
+
 # ------------------------------------------------------------------ as a program uses them
 
 
