@@ -402,14 +402,15 @@ void attend_kernel(AttendParams p, int shared) {
 
 // Joins the parts of vectors: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes hold a vector's
 // columns, four each.  MANY parts: a workgroup per vector, its groups of lanes take the parts in turn
-// and are added up in the LDS.  Few: a group per vector.
+// and are joined in the LDS.  Few: a group per vector.  Maxima and outputs of four parts are loaded together
+// and the maximum runs along: what is short here is the chain of loads (sequence, parts), not their bytes.
 template <int DP, bool MANY>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     constexpr int LPV = DP / 4, GROUPS = 256 / LPV, STEP = MANY ? GROUPS : 1;
     __shared__ __align__(16) float lds_o[MANY ? GROUPS : 1][DP];
-    __shared__ float lds_l[GROUPS];
+    __shared__ float lds_m[GROUPS], lds_l[GROUPS];
     const int seq = p.by_join.div(blockIdx.x);
-    const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4, lane = threadIdx.x & 63;
+    const int group = threadIdx.x / LPV, d = (threadIdx.x % LPV) * 4;
     const int x = MANY ? p.by_join.mod(blockIdx.x) : p.by_join.mod(blockIdx.x) * GROUPS + group;
     const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
     const int t = p.by_q_heads.div(x), head = p.by_q_heads.mod(x);
@@ -417,30 +418,54 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     const int parts = p.prefix_parts + kv_parts(s.len - p.own_from, p.chunk);
     const int64_t row = s.row0 + t, slot = (row * p.q_heads + head) * p.parts;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot;
-    float m = kNegInf;
-    for (int i = MANY ? lane : 0; i < parts; i += MANY ? 64 : 1) m = fmaxf(m, ml[i].x);
-    if constexpr (MANY) m = wave_max(m);
-    const float base = m == kNegInf ? 0.0f : m;
-    float l = 0.0f;
+    float m = kNegInf, l = 0.0f;
     float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = MANY ? group : 0; i < parts; i += STEP) {
-        const float2 y = ml[i];
-        const float f = __builtin_amdgcn_exp2f(y.x - base);
-        l = __builtin_fmaf(f, y.y, l);
-        const float4v z = *reinterpret_cast<const float4v*>(p.part_o + (slot + i) * DP + d);
+    for (int i = MANY ? group : 0; i < parts; i += 4 * STEP) {
+        float2 y[4];
+        float4v z[4];
+        float top = m;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[c], o[c]);
+        for (int k = 0; k < 4; ++k) {
+            const int at = min(i + k * STEP, parts - 1);
+            y[k] = ml[at];
+            z[k] = *reinterpret_cast<const float4v*>(p.part_o + (slot + at) * DP + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * STEP < parts) top = fmaxf(top, y[k].x);
+        const float base = top == kNegInf ? 0.0f : top, fade = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= fade;
+        o *= fade;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k * STEP >= parts) continue;
+            const float f = __builtin_amdgcn_exp2f(y[k].x - base);
+            l = __builtin_fmaf(f, y[k].y, l);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[k][c], o[c]);
+        }
     }
     if constexpr (MANY) {
         *reinterpret_cast<float4v*>(&lds_o[group][d]) = o;
-        if (d == 0) lds_l[group] = l;
+        if (d == 0) {
+            lds_m[group] = m;
+            lds_l[group] = l;
+        }
         __syncthreads();
         if (group != 0) return;
 #pragma unroll
-        for (int i = 1; i < GROUPS; ++i) {
-            o += *reinterpret_cast<const float4v*>(&lds_o[i][d]);
-            l += lds_l[i];
+        for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, lds_m[i]);
+        const float base = m == kNegInf ? 0.0f : m;
+        l = 0.0f;
+        o = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float f = __builtin_amdgcn_exp2f(lds_m[i] - base);
+            l = __builtin_fmaf(f, lds_l[i], l);
+            const float4v z = *reinterpret_cast<const float4v*>(&lds_o[i][d]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[c], o[c]);
         }
     }
     const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
