@@ -11,9 +11,9 @@
 // made, then O of tile u while the maximum of tile u + 1 is found.  Three tiles lie in the LDS: the values of u,
 // the keys of u + 1, and u + 2 on its way in.
 //
-// What bounds it (a prompt of 4096 tokens, 32 query and 8 KV heads of 128, 137 GFLOP: 190 us, 720 TFLOP/s):
-// the LDS, busy 45% of the time, the vector units, 44%, and the matrix cores, 32%, each of which the two waves of a SIMD
-// leave idle in turn.  For 16 matrix instructions of 32 x 32 x 16 a wave reads 16 KB of operands and 12 KB of scale
+// What bounds it (a prompt of 4096 tokens, 32 query and 8 KV heads of 128, 137 GFLOP: 178 us, 770 TFLOP/s):
+// the LDS, busy 45% of the time, the vector units, 44%, and the matrix cores, 32% (measured at 190 us), each of which the
+// two waves of a SIMD leave idle in turn.  For 16 matrix instructions of 32 x 32 x 16 a wave reads 16 KB of operands and 12 KB of scale
 // factors; the matrix instructions, their operands' reads and the barriers alone take 124 us.  64 vectors a wave would halve the reads, but their
 // registers leave one wave a SIMD (198 to 247 us).
 #include <type_traits>
@@ -282,6 +282,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     };
     // First P of tile u (its values lie in bu) beside the products of tile u + 1 (NEXT: its keys in bk). Then
     // the outputs of tile u beside the exponents of tile u + 1, at token j, and the way of tile u + 2 into bn.
+    // The wave in the second goes first where both of a SIMD could issue, so that they do not run the same phase side
+    // by side (the prompt of 4096 tokens 193 -> 178 us; in the first instead 182, in both 184).
     auto advance = [&](const uint8_t* bu, const uint8_t* bk, uint8_t* bn, Sh& sh, int j, auto next, auto mask) {
         constexpr bool NEXT = decltype(next)::value;
         constexpr int SV = 2 * ND;                                  // matrix steps of O
@@ -324,6 +326,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
                 if (i < 8) exponents(i, base, iv);
             pin();
         }
+        __builtin_amdgcn_s_setprio(1);
         if constexpr (NEXT) find(j + 2 * kTokens);
         top = kNegInf;
         const int left = min(seen, cap) - j - 4 * hi;
@@ -351,6 +354,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
             pin();
         }
         if constexpr (NEXT) store_scales(sh, bn);
+        __builtin_amdgcn_s_setprio(0);
     };
     auto passed = [&] {  // some vector's maximum is to be raised
         typedef unsigned int pair __attribute__((ext_vector_type(2)));
