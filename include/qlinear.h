@@ -391,8 +391,9 @@ typedef struct qlin_kv_info {
  * A row whose token is negative (n > length[i]) is not stored, reads as zeros and attends to nothing.
  * What the device arrays hold is checked by the kernels: row starts that decrease or pass `rows`, more than
  * max_new rows, a length below 0 or above max_len, or a page outside the cache set QLIN_ERR_PARAM in
- * the workspace's error word; no such value is followed out of a buffer, a row on such a page is
- * not stored and reads as NaN, and the other results of that sequence are unspecified. */
+ * the workspace's error word; no such value is followed out of a buffer, no row of a sequence whose starts
+ * or length are at fault is stored, a row on such a page is not stored and reads as NaN, and the other
+ * results of that sequence are unspecified. */
 typedef struct qlin_kv_batch {
     int32_t seqs;    /* sequences, 1..2^20 */
     int32_t rows;    /* rows of the row tensors, 0..2^24 */

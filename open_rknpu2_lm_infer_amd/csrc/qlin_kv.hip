@@ -65,8 +65,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
         load8<T, VEC>(reinterpret_cast<const T*>(p.k) + row * p.ldk + col, d0, p.c.dim, x[0]);
         load8<T, VEC>(reinterpret_cast<const T*>(p.v) + row * p.ldv + col, d0, p.c.dim, x[1]);
     }
-    int off;
-    const int page = find_page(p, u, &off);
+    // the positions of a sequence whose row starts or length are out of bounds are clamped ones, other tokens' slots
+    // on pages that other sequences may read: nothing of it is stored
+    int off = 0;
+    const int page = u.bad ? -1 : find_page(p, u, &off);
     const KvBlock<DP> blk(p.c, max(page, 0), u.h);
     bool finite = true;
 #pragma unroll

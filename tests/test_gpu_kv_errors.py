@@ -1,0 +1,69 @@
+"""Key/value cache calls with faults in a batch's device arrays: what is stored, what is reported, and which results
+stay right."""
+import numpy as np
+import pytest
+import torch
+
+from open_rknpu2_lm_infer_amd import _lib
+from open_rknpu2_lm_infer_amd import qlinear as ql
+from tests.test_gpu_kv import DEV, F16, F32, Setup, i32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ws():
+    w = ql.Workspace(1, 256, 256)
+    yield w
+    w.close()
+
+
+def whole_cache(s):
+    """Every slot of the cache, [pages, page * columns] each of keys and values: every page as a full sequence."""
+    n, P = s.cache.pages, s.P
+    b = ql.KVBatch(i32(np.arange(n + 1) * P), i32([P] * n), i32(np.arange(n).reshape(n, 1)), n * P, P, P)
+    return [x.view(n, -1) for x in ql.kv_read(s.ws, s.cache, b, out_dtype=F32)]
+
+
+BAD = [  # row starts, lengths, rows of the tensors, max_new, max_len, the sequences at fault
+    ([0, 2, 4, 6], [40, 49, 40], 6, 2, 40, [1]),     # past max_len: clamped, its rows would be tokens 38 and 39
+    ([0, 2, 4, 6], [40, -1, 40], 6, 2, 40, [1]),
+    ([0, 1, 3, 4], [40, 40, 40], 4, 1, 40, [1]),     # more rows than max_new: clamped, a row would take another's slot
+    ([0, 3, 2, 4], [40, 40, 40], 4, 3, 40, [1]),     # decreasing
+    ([0, 2, 5, 9], [40, 40, 40], 5, 3, 40, [2]),     # past the rows
+    ([-1, 2, 4, 6], [40, 40, 40], 6, 3, 40, [0]),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("starts,lens,rows,max_new,max_len,bad", BAD)
+def test_append_stores_nothing_for_a_sequence_at_fault(ws, dtype, starts, lens, rows, max_new, max_len, bad):
+    """The pages of a sequence whose row starts or length are out of the batch's limits keep what they held (they may
+    be shared with others); the other sequences' rows are stored."""
+    s = Setup(ws, [(40, 2)] * 3, 2, 72, 16, dtype, seed=21)
+    k, v = s.history()
+    s.fill(k, v)
+    assert ws.status() == 0
+    before = whole_cache(s)
+    b = ql.KVBatch(i32(starts), i32(lens), i32(s.table), rows, max_new, max_len)
+    new = s.rand(rows, 144, size=9.0).to(DEV), s.rand(rows, 144, size=9.0).to(DEV)
+    ql.kv_append(ws, s.cache, b, *new)
+    assert ws.status() == _lib.QLIN_ERR_PARAM
+    after = whole_cache(s)
+    good = [i for i in range(3) if i not in bad]
+    owned = np.zeros(s.cache.pages, bool)
+    owned[s.table[good].ravel()] = True
+    for x, y in zip(before, after):
+        assert torch.equal(x[~owned], y[~owned])
+    # the good sequences hold what an append of theirs alone stores
+    ref = Setup(ws, [(40, 2)] * 3, 2, 72, 16, dtype, seed=21)
+    ref.fill(k, v)
+    for i in good:
+        n = starts[i + 1] - starts[i]
+        one = ql.KVBatch(i32([0, n]), i32([lens[i]]), i32(s.table[i:i + 1]), n, n, max_len)
+        ql.kv_append(ws, ref.cache, one, *(x[starts[i]:starts[i + 1]] for x in new))
+    for x, y in zip(whole_cache(ref), after):
+        assert torch.equal(x, y)
+    assert ws.status() == 0
+    s.cache.close()
+    ref.cache.close()
