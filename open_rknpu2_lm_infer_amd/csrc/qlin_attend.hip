@@ -102,7 +102,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         for (int r = 0; r < R; ++r) seen[r] = lds.seen[16 * r + n];
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
-        if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
+        if (s.bad && tid == 0) atomicOr(p.err + kErrBatch, 1u);
         if (v0 >= s.rows * group) return;
         if (part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
         first_row = s.row0;
@@ -295,7 +295,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         __builtin_amdgcn_sched_barrier(0);
         load_v();
     }
-    if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
+    if (bad_page && lane == 0) atomicOr(p.err + kErrBatch, 1u);
 
     // join the waves: a common maximum, then 3 -> 1 and 2 -> 0, then 1 -> 0
 #pragma unroll

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         __syncthreads();
     } else {
         const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
-        if (s.bad && tid == 0) atomicOr(p.err, kErrBatch);
+        if (s.bad && tid == 0) atomicOr(p.err + kErrBatch, 1u);
         const int vectors = s.rows * group;
         if (v0 >= vectors) return;
         if (part > 0 && j0 >= s.len) return;  // the join knows how many parts there are
@@ -440,7 +440,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         walk(end - kTokens, std::true_type{});
         advance(lds + bu, nullptr, nullptr, sh, 0, std::false_type{}, std::false_type{});
     }
-    if (bad_page && lane == 0) atomicOr(p.err, kErrBatch);
+    if (bad_page && lane == 0) atomicOr(p.err + kErrBatch, 1u);
 
     l += __shfl_xor(l, 32, 64);
     if (seen < 0) return;

@@ -636,11 +636,11 @@ int qlin_workspace_query(const qlin_workspace* ws, qlin_workspace_info* out) {
 
 int qlin_workspace_status(qlin_workspace* ws, int32_t clear) {
     if (!ws) return QLIN_ERR_PARAM;
-    uint32_t e = 0;
+    uint32_t e[kErrWords] = {};
     if (hipStreamSynchronize(ws->last) != hipSuccess) return QLIN_ERR_DEVICE;
-    if (hipMemcpy(&e, ws->err, sizeof(e), hipMemcpyDeviceToHost) != hipSuccess) return QLIN_ERR_DEVICE;
-    if (clear && e && hipMemset(ws->err, 0, sizeof(uint32_t)) != hipSuccess) return QLIN_ERR_DEVICE;
-    return e & kErrBatch ? QLIN_ERR_PARAM : e ? QLIN_ERR_NONFINITE : QLIN_OK;
+    if (hipMemcpy(e, ws->err, sizeof(e), hipMemcpyDeviceToHost) != hipSuccess) return QLIN_ERR_DEVICE;
+    if (clear && (e[kErrNonfinite] || e[kErrBatch]) && hipMemset(ws->err, 0, sizeof(e)) != hipSuccess) return QLIN_ERR_DEVICE;
+    return e[kErrBatch] ? QLIN_ERR_PARAM : e[kErrNonfinite] ? QLIN_ERR_NONFINITE : QLIN_OK;
 }
 
 int qlin_quantize(int32_t rows, int32_t K, const void* A, int32_t a_dtype, int64_t lda, const float* gamma,
@@ -775,7 +775,7 @@ int run_gemv(qlin_workspace* ws, const qlin_weights* w, int rows, const void* A,
     p.ldc = ldc;
     p.c_kind = c_kind;
     p.flags = flags;
-    p.err = ws->err;
+    p.err = ws->err + kErrNonfinite;
     p.iw = g.iw;
     p.grid = g.grid;
     return launch_gemv(p, w->bits, g.waves, st) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
@@ -1167,7 +1167,7 @@ int run_impl(qlin_workspace* ws, const qlin_weights* w, int rows, const void* A,
     qp.ldq = w->Kp;
     qp.q = ws->q;
     qp.s = ws->s;
-    qp.err = ws->err;
+    qp.err = ws->err + kErrNonfinite;
     qp.gamma = gamma;
     qp.eps = eps;
     qp.flags = flags & ~kFlagErrOnHost;
@@ -1180,7 +1180,7 @@ int run_host_copies(qlin_workspace* ws, const qlin_weights* w, int rows, const f
                     uint32_t flags) {
     hipStream_t st = ws->stream;
     ws->err_used = true;
-    if (hipMemsetAsync(ws->err, 0, sizeof(uint32_t), st) != hipSuccess) return QLIN_ERR_DEVICE;
+    if (hipMemsetAsync(ws->err + kErrNonfinite, 0, sizeof(uint32_t), st) != hipSuccess) return QLIN_ERR_DEVICE;
     if (hipMemcpyAsync(ws->dA, A, (size_t)rows * w->K * sizeof(float), hipMemcpyHostToDevice, st) != hipSuccess)
         return QLIN_ERR_DEVICE;
     if (int rc = run_impl(ws, w, rows, ws->dA, QLIN_F32, w->K, nullptr, 0.0f, ws->dC, QLIN_F32, ncols, flags, st))
@@ -1188,7 +1188,7 @@ int run_host_copies(qlin_workspace* ws, const qlin_weights* w, int rows, const f
     if (hipMemcpyAsync(C, ws->dC, (size_t)rows * ncols * sizeof(float), hipMemcpyDeviceToHost, st) != hipSuccess)
         return QLIN_ERR_DEVICE;
     uint32_t e = 0;
-    if (hipMemcpyAsync(&e, ws->err, sizeof(e), hipMemcpyDeviceToHost, st) != hipSuccess ||
+    if (hipMemcpyAsync(&e, ws->err + kErrNonfinite, sizeof(e), hipMemcpyDeviceToHost, st) != hipSuccess ||
         hipStreamSynchronize(st) != hipSuccess)
         return QLIN_ERR_DEVICE;
     return e ? QLIN_ERR_NONFINITE : QLIN_OK;
@@ -1245,8 +1245,8 @@ int run_host(qlin_workspace* ws, const qlin_weights* w, int rows, const float* A
     *err_host = 0;
     const int step = (rows + blocks - 1) / blocks;
     int rc = QLIN_OK;
-    // the workspace's word reports this call, as every host-buffer call's
-    if (ws->err_used && hipMemsetAsync(ws->err, 0, sizeof(uint32_t), st) != hipSuccess) rc = QLIN_ERR_DEVICE;
+    // the workspace's word of non-finite rows reports this call, as every host-buffer call's
+    if (ws->err_used && hipMemsetAsync(ws->err + kErrNonfinite, 0, sizeof(uint32_t), st) != hipSuccess) rc = QLIN_ERR_DEVICE;
     auto rows_of = [&](int b) { return std::min(step, rows - b * step); };
     auto finish = [&](int b) {  // waits for block b and copies its rows out
         if (!rc && hipEventSynchronize(h->done[b % kSlots]) != hipSuccess) rc = QLIN_ERR_DEVICE;
@@ -1280,7 +1280,7 @@ int run_host(qlin_workspace* ws, const qlin_weights* w, int rows, const float* A
     } else if (*const_cast<volatile uint32_t*>(err_host)) {
         rc = QLIN_ERR_NONFINITE;
         ws->err_used = true;  // so that the next call clears it
-        if (hipMemcpyAsync(ws->err, err_host, sizeof(uint32_t), hipMemcpyHostToDevice, st) != hipSuccess ||
+        if (hipMemcpyAsync(ws->err + kErrNonfinite, err_host, sizeof(uint32_t), hipMemcpyHostToDevice, st) != hipSuccess ||
             hipStreamSynchronize(st) != hipSuccess)
             rc = QLIN_ERR_DEVICE;
     }

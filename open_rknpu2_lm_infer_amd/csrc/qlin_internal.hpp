@@ -133,7 +133,7 @@ struct WorkspaceParts {
     int cu_count;
     float* part;          // scratch for partial results, shared with the GEMM's split-K sums
     int64_t part_floats;
-    uint32_t* err;        // sticky error word
+    uint32_t* err;        // sticky error words
 };
 }  // namespace qlin
 struct qlin_workspace;
@@ -141,8 +141,9 @@ namespace qlin {
 int workspace_device(const qlin_workspace* ws);
 WorkspaceParts workspace_begin(qlin_workspace* ws, hipStream_t stream);
 
-// Bits of a workspace's sticky error word.
-enum : uint32_t { kErrNonfinite = 0x1u, kErrBatch = 0x2u };
+// A workspace's sticky error words, each zero or not: rows with Inf / NaN, which a host-buffer run clears and
+// reads for itself, and faults in the batch of a key/value cache call.
+enum : int { kErrNonfinite = 0, kErrBatch = 1, kErrWords = 2 };
 
 // Launchers (return hipError_t of the launch).
 hipError_t launch_quant(const QuantParams& p, int rows, hipStream_t stream);

@@ -94,8 +94,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
             finite &= fin;
         }
     }
-    const uint32_t e = (u.bad ? kErrBatch : 0u) | (finite ? 0u : kErrNonfinite);
-    if (e) atomicOr(p.err, e);
+    if (u.bad) atomicOr(p.err + kErrBatch, 1u);
+    if (!finite) atomicOr(p.err + kErrNonfinite, 1u);
 }
 
 template <int DP, typename T, bool VEC>
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     const int d0 = (threadIdx.x % LPU) * 8;
     int off;
     const int page = find_page(p, u, &off);
-    if (u.bad) atomicOr(p.err, kErrBatch);
+    if (u.bad) atomicOr(p.err + kErrBatch, 1u);
     if (!u.ok) return;
     const KvBlock<DP> blk(p.c, max(page, 0), u.h);
     uint2 w[2] = {make_uint2(0x80808080u, 0x80808080u), make_uint2(0x80808080u, 0x80808080u)};

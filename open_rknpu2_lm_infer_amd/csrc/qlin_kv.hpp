@@ -55,7 +55,7 @@ struct KvRows {
     int64_t ldk, ldv;
     int f16;
     int rne;
-    uint32_t* err;
+    uint32_t* err;  // [kErrWords]
     FastDiv by_blocks, by_heads;  // of workgroup and unit indexes
 };
 hipError_t launch_kv_append(const KvRows& p, hipStream_t stream);
@@ -85,7 +85,7 @@ struct AttendParams {
     FastDiv by_q_heads, by_join;                           // of the join's
     float* part_o;
     float* part_ml;
-    uint32_t* err;
+    uint32_t* err;  // [kErrWords]
 };
 // Tokens worked on at once by a workgroup of the attention kernel: chunks are multiples of it.
 constexpr int kAttendStep = 128;

@@ -6,6 +6,7 @@ import torch
 
 from open_rknpu2_lm_infer_amd import _lib
 from open_rknpu2_lm_infer_amd import qlinear as ql
+from open_rknpu2_lm_infer_amd import synth
 from tests.test_gpu_kv import DEV, F16, F32, Setup, i32
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,34 @@ def test_append_stores_nothing_for_a_sequence_at_fault(ws, dtype, starts, lens, 
     assert ws.status() == 0
     s.cache.close()
     ref.cache.close()
+
+
+def faulty_call(ws, nan=False):
+    """A call that finds a length past max_len; with nan, the rows of another sequence hold one."""
+    s = Setup(ws, [(40, 2)] * 2, 1, 64, 16, F16, seed=22)
+    k = s.rand(4, 64)
+    if nan:
+        k[3, 5] = float("nan")
+    ql.kv_append(ws, s.cache, s.batch(lens=[41, 40]), k.to(DEV), s.rand(4, 64).to(DEV))
+    torch.cuda.synchronize()
+    s.cache.close()
+
+
+@pytest.mark.parametrize("K", [256, 250])  # through pinned blocks, through copies
+def test_host_buffer_runs_leave_the_report_of_a_batch(K):
+    w = ql.Workspace(4, 256, 256)
+    packed, _, scales = synth.make_linear(128, K, 8, 5, device=DEV)
+    lin = ql.Weights.from_packed_device(8, K, 128, packed, scales)
+    A = synth.activations(4, K, 6).float().numpy()
+    want = ql.run_host_f32(w, lin, A)
+    faulty_call(w)
+    assert np.array_equal(ql.run_host_f32(w, lin, A), want)
+    assert w.status() == _lib.QLIN_ERR_PARAM and w.status() == 0
+    # its own report of a row is the call's, whatever a batch left
+    faulty_call(w)
+    A[2, 3] = np.inf
+    with pytest.raises(_lib.QlinError) as e:
+        ql.run_host_f32(w, lin, A)
+    assert e.value.rc == _lib.QLIN_ERR_NONFINITE
+    assert w.status() == _lib.QLIN_ERR_PARAM
+    w.close()
