@@ -154,7 +154,8 @@ int qlin_workspace_query(const qlin_workspace* ws, qlin_workspace_info* out);
 /* Sticky error word of asynchronous runs on this workspace: returns QLIN_OK or
  * QLIN_ERR_NONFINITE if any activation row seen since the last clear held Inf/NaN.
  * Synchronizes the workspace's last stream.  clear != 0 resets it.  QLIN_ERR_PARAM: a key/value cache
- * call found row starts, lengths or pages outside its batch's limits (see qlin_kv_batch).  A host-buffer run
+ * call found row starts, lengths or pages outside its batch's limits (see qlin_kv_batch).  Where there are both
+ * reports, this one comes first; what is cleared is the one returned, and the next call returns the other.  A host-buffer run
  * clears what was said of rows before it and leaves its own, and leaves what was said of batches. */
 int qlin_workspace_status(qlin_workspace* ws, int32_t clear);
 

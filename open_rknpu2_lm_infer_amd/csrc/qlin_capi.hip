@@ -639,8 +639,10 @@ int qlin_workspace_status(qlin_workspace* ws, int32_t clear) {
     uint32_t e[kErrWords] = {};
     if (hipStreamSynchronize(ws->last) != hipSuccess) return QLIN_ERR_DEVICE;
     if (hipMemcpy(e, ws->err, sizeof(e), hipMemcpyDeviceToHost) != hipSuccess) return QLIN_ERR_DEVICE;
-    if (clear && (e[kErrNonfinite] || e[kErrBatch]) && hipMemset(ws->err, 0, sizeof(e)) != hipSuccess) return QLIN_ERR_DEVICE;
-    return e[kErrBatch] ? QLIN_ERR_PARAM : e[kErrNonfinite] ? QLIN_ERR_NONFINITE : QLIN_OK;
+    const int word = e[kErrBatch] ? kErrBatch : kErrNonfinite;  // one report a call; the other one stays
+    if (!e[word]) return QLIN_OK;
+    if (clear && hipMemset(ws->err + word, 0, sizeof(uint32_t)) != hipSuccess) return QLIN_ERR_DEVICE;
+    return word == kErrBatch ? QLIN_ERR_PARAM : QLIN_ERR_NONFINITE;
 }
 
 int qlin_quantize(int32_t rows, int32_t K, const void* A, int32_t a_dtype, int64_t lda, const float* gamma,

@@ -99,3 +99,14 @@ def test_host_buffer_runs_leave_the_report_of_a_batch(K):
     assert e.value.rc == _lib.QLIN_ERR_NONFINITE
     assert w.status() == _lib.QLIN_ERR_PARAM
     w.close()
+
+
+def test_status_reports_one_fault_after_the_other():
+    w = ql.Workspace(1, 256, 256)
+    faulty_call(w, nan=True)
+    assert w.status(clear=False) == w.status(clear=False) == _lib.QLIN_ERR_PARAM
+    assert w.status() == _lib.QLIN_ERR_PARAM
+    assert w.status(clear=False) == _lib.QLIN_ERR_NONFINITE
+    assert w.status() == _lib.QLIN_ERR_NONFINITE
+    assert w.status() == 0
+    w.close()
