@@ -439,7 +439,8 @@ int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin
 /* The same for sequences that share their first prefix_tokens tokens (a multiple of page_tokens):
  * their pages are taken from prefix_pages (device, prefix_tokens / page_tokens ids) and read once
  * for all rows, and the tables' columns of the prefix are not read.  Lengths count the prefix; a
- * sequence shorter than it sees its first tokens. */
+ * sequence shorter than it sees its first tokens.  An id outside the cache among prefix_pages sets
+ * QLIN_ERR_PARAM in the workspace's error word and makes NaN of the rows that see tokens of that page. */
 int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
                              int32_t prefix_tokens, const int32_t* prefix_pages, int32_t q_heads,
                              const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,

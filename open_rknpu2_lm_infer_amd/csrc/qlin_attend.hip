@@ -132,28 +132,27 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     const const_ids table = (const_ids)(uintptr_t)(p.b.table + seq * p.b.table_ld);
     const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
-    bool bad_page = false, bad = false, bad_next = false;
+    bool bad_page = false, bad[2] = {false, false};  // of a tile: who sees none of its tokens keeps its result
     StepData<DP> d;
     Half16<DP> next[2];
     auto find_step = [&](int j) {  // end > 0
-        bad_next = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int jt = j + 16 * t, jj = min(jt, end - 1);
             const int id = (SHARED || jj < p.prefix ? prefix : table)[jj >> p.c.shift];
             next[t] = find_half<DP>(p.c, id, h, jt & off_mask, jt < end);
-            bad_next |= next[t].bad && jt < end;
+            next[t].bad = next[t].bad && jt < end;
+            bad_page |= next[t].bad;
         }
-        bad_page |= bad_next;
     };
     auto load_k = [&] {
 #pragma unroll
         for (int t = 0; t < 2; ++t) load_bytes<DP / 4, 64>(d.k[t], next[t].block, n * DP + 16 * g, next[t].k);
     };
     auto load_scales = [&] {
-        bad = bad_next;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            bad[t] = next[t].bad;
             d.ks[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].block, 16 * g, next[t].ks, 0));
             d.vs[t] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(next[t].block, 16 * g, next[t].vs, 0));
         }
@@ -239,7 +238,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                lv[4 * t + i] = bad ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
+                lv[4 * t + i] = bad[t] ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
                 iv[4 * t + i] = __builtin_amdgcn_rcpf(d.vs[t][i]);
             }
         half8v pf[R][LIMBS];

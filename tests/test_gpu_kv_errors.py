@@ -7,7 +7,7 @@ import torch
 from open_rknpu2_lm_infer_amd import _lib
 from open_rknpu2_lm_infer_amd import qlinear as ql
 from open_rknpu2_lm_infer_amd import synth
-from tests.test_gpu_kv import DEV, F16, F32, Setup, i32
+from tests.test_gpu_kv import DEV, F16, F32, Setup, check, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,38 @@ def test_status_reports_one_fault_after_the_other():
     assert w.status() == _lib.QLIN_ERR_NONFINITE
     assert w.status() == 0
     w.close()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("P", [16, 32])
+@pytest.mark.parametrize("new,hq", [(2, 4), (150, 8)])  # few vectors and many
+def test_bad_prefix_page_reaches_only_rows_that_see_it(ws, dtype, P, new, hq):
+    """The prefix's second page is outside the cache: sequences that end before it keep their results."""
+    seqs = [(P - 3, 2), (3 * P + new, new), (P, 1), (P + 1, 1), (5, 1)]
+    s = Setup(ws, seqs, 2, 64, P, dtype, seed=23 + P, q_heads=hq)
+    k, v = s.history()
+    at = 0
+    for n, _ in seqs:  # all begin with the longest sequence's tokens
+        m = min(n, 3 * P)
+        k[at:at + m], v[at:at + m] = k[P - 3:P - 3 + m].clone(), v[P - 3:P - 3 + m].clone()
+        at += n
+    s.fill(k, v)
+    q = s.rand(s.rows, hq * 64)
+    want, tol = s.expected(q, k, v, dtype)
+    pages = s.table[1, :3].copy()
+    kw = dict(prefix_tokens=3 * P, prefix_pages=i32(pages))
+    check(ql.kv_attention(ws, s.cache, s.batch(), q.to(DEV), **kw), want, tol)
+    assert ws.status() == 0
+    pages[1] = s.cache.pages
+    kw["prefix_pages"] = i32(pages)
+    out = ql.kv_attention(ws, s.cache, s.batch(), q.to(DEV), **kw)
+    assert ws.status() == _lib.QLIN_ERR_PARAM
+    r = 0
+    for n, m in seqs:
+        for t in range(m):
+            if n - m + t + 1 > P:
+                want[r] = np.nan
+            r += 1
+    assert np.isnan(want).any() and not np.isnan(want).all()
+    check(out, want, tol)
+    s.cache.close()
