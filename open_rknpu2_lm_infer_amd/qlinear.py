@@ -404,6 +404,8 @@ def kv_attention(ws: Workspace, cache: KVCache, batch: KVBatch, Q: torch.Tensor,
         out = torch.empty((Q.shape[0], cols), dtype=out_dtype or Q.dtype, device=Q.device)
     if scale is None:
         scale = D ** -0.5
+    # without prefix_tokens the table's columns would be read, which may hold anything for a prefix
+    assert prefix_tokens or prefix_pages is None or prefix_pages.numel() == 0, "prefix_pages without prefix_tokens"
     if prefix_tokens:
         assert prefix_pages is not None and prefix_pages.dtype == torch.int32 and prefix_pages.device == batch.device
         assert prefix_pages.is_contiguous() and prefix_pages.numel() * cache.page_tokens >= prefix_tokens
