@@ -326,6 +326,7 @@ class KVBatch:
                  max_len: int):
         assert row_start.dtype == length.dtype == page_table.dtype == torch.int32
         assert row_start.is_cuda and length.is_cuda and page_table.is_cuda
+        assert row_start.device == length.device == page_table.device, "the batch's arrays are on different devices"
         assert row_start.is_contiguous() and length.is_contiguous() and page_table.dim() == 2
         assert page_table.shape[1] <= 1 or page_table.stride(1) == 1
         seqs = length.numel()

@@ -72,3 +72,10 @@ def test_prefix_pages_and_tokens_come_together(reached):
     assert len(reached) == 2
     ql.kv_attention(WS, CACHE, batch(), q, out=out, prefix_pages=Tensor(0))  # a prefix of no pages
     assert reached[2] == "qlin_kv_attention"
+
+
+def test_batch_lies_on_one_device():
+    assert batch().device == torch.device("cuda:0")
+    for name in ("row_start", "length", "page_table"):
+        with pytest.raises(AssertionError, match="device"):
+            batch(**{name: "cuda:1"})
