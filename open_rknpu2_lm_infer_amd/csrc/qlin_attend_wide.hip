@@ -16,6 +16,7 @@
 // leave idle in turn.  For 16 matrix instructions of 32 x 32 x 16 a wave reads 16 KB of operands and 12 KB of scale
 // factors; the matrix instructions, their operands' reads and the barriers alone take 124 us.  64 vectors a wave would halve the reads, but their
 // registers leave one wave a SIMD (198 to 247 us).
+#include <atomic>
 #include <type_traits>
 
 #include "qlin_attend.hpp"
@@ -469,9 +470,17 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
 template <int DP, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_one(const AttendParams& p, hipStream_t st) {
     constexpr int bytes = 3 * TileLds<DP>::BYTES;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, Q16, SHARED>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (attr != hipSuccess) return attr;
+    // the LDS is asked for once on each device (those past 63: on every call), and again after a failure
+    static std::atomic<uint64_t> asked{0};
+    int device;
+    if (const hipError_t e = hipGetDevice(&device)) return e;
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if (!(asked.load(std::memory_order_relaxed) & bit)) {
+        if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, Q16, SHARED>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes))
+            return e;
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
     const int64_t tiles = SHARED ? p.by_prefix_tiles.d : p.by_tiles.d;
     const int64_t blocks = tiles * p.c.heads * (SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs);
     attend_wide_kernel<DP, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);

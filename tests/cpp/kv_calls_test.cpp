@@ -4,10 +4,13 @@
 //
 //   kv_calls_test index     row starts, lengths and page ids of any value stay inside the buffers
 //   kv_calls_test refusals  arguments outside the documented limits are refused before any launch
+//   kv_calls_test devices   each device that launches the kernel for many vectors has been asked for its LDS
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <limits>
+#include <set>
+#include <utility>
 #include <vector>
 
 #include <hip/hip_runtime_api.h>
@@ -17,6 +20,7 @@
 
 namespace {
 int g_launches = 0, g_device = 0, g_fail = 0;
+std::set<std::pair<const void*, int>> g_lds;  // functions whose dynamic LDS was raised, and on which device
 hipError_t alloc(void** p, size_t n) {
     if (g_fail > 0 && --g_fail == 0) return hipErrorOutOfMemory;
     *p = std::calloc(1, n ? n : 1);
@@ -40,7 +44,10 @@ hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) {
 }
 hipError_t hipStreamDestroy(hipStream_t s) { return std::free(s), hipSuccess; }
 hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
-hipError_t hipFuncSetAttribute(const void*, hipFuncAttribute, int) { return hipSuccess; }
+hipError_t hipFuncSetAttribute(const void* f, hipFuncAttribute a, int) {
+    if (a == hipFuncAttributeMaxDynamicSharedMemorySize) g_lds.insert({f, g_device});
+    return hipSuccess;
+}
 hipError_t hipThreadExchangeStreamCaptureMode(hipStreamCaptureMode*) { return hipSuccess; }
 hipError_t __hipPushCallConfiguration(dim3, dim3, size_t, hipStream_t) { return hipSuccess; }
 hipError_t __hipPopCallConfiguration(dim3* g, dim3* b, size_t* lds, hipStream_t* st) {
@@ -211,12 +218,30 @@ void refusals() {
     expect(prefix(0, nullptr) == QLIN_OK && prefix(16, table) == QLIN_OK, "prefix");
 }
 
+void devices() {
+    const int32_t starts[2] = {0, 600}, length[1] = {600}, table[38] = {};
+    const qlin_kv_batch b = {1, 600, 600, 600, starts, length, table, 38};
+    for (int dim : {64, 84, 256}) {
+        std::vector<float> q(600 * (size_t)dim), o(q.size());
+        for (int dev : {0, 1, 2}) {
+            g_device = dev;
+            Made m(1, dim, 16, 38);
+            const size_t before = g_lds.size();
+            for (int i = 0; i < 2; ++i)
+                expect(qlin_kv_attention(m.ws, m.c, &b, 1, q.data(), QLIN_F32, dim, 1.0f, o.data(), QLIN_F32, dim, nullptr) == QLIN_OK, "attention");
+            expect(g_lds.size() == before + 1, "the kernel's LDS is asked for on this device");
+        }
+    }
+    g_device = 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     const char* mode = argc > 1 ? argv[1] : "";
     if (!std::strcmp(mode, "index")) index();
     else if (!std::strcmp(mode, "refusals")) refusals();
+    else if (!std::strcmp(mode, "devices")) devices();
     else return 2;
     if (!g_bad) std::printf("PASS %s\n", mode);
     return g_bad != 0;

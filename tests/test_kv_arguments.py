@@ -1,11 +1,13 @@
-"""What the Python calls of the key/value cache refuse before they reach the library (no GPU: tensors and handles are
-stand-ins that say what they are)."""
+"""What the calls of the key/value cache do on the host: the Python ones (tensors and handles are stand-ins that say
+what they are) and those of tests/cpp/kv_calls_test.cpp."""
+import subprocess
 from types import SimpleNamespace
 
 import pytest
 import torch
 
 from open_rknpu2_lm_infer_amd import qlinear as ql
+from tests.test_kv import BIN
 
 
 class Tensor:
@@ -79,3 +81,8 @@ def test_batch_lies_on_one_device():
     for name in ("row_start", "length", "page_table"):
         with pytest.raises(AssertionError, match="device"):
             batch(**{name: "cuda:1"})
+
+
+def test_lds_of_many_vectors_is_asked_for_on_each_device():
+    r = subprocess.run([BIN, "devices"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "PASS devices" in r.stdout, r.stdout[-3000:] + r.stderr[-1000:]
