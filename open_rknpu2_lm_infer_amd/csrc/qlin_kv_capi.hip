@@ -97,7 +97,7 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     if (ldq < cols || ldo < cols) return QLIN_ERR_PARAM;
     AttendParams p{};
     WorkspaceParts wp;
-    if (q_heads > kKvMaxHeads || prefix > kKvMaxLen || (int64_t)batch->rows * q_heads > 1 << 30) return QLIN_ERR_UNSUPPORTED;
+    if (q_heads > kKvMaxHeads || std::fabs(scale) > kKvMaxScale || prefix > kKvMaxLen || (int64_t)batch->rows * q_heads > 1 << 30) return QLIN_ERR_UNSUPPORTED;
     if (int rc = begin(ws, cache, batch, stream, &p.b, &wp)) return rc;
     if (p.b.max_new == 0) return QLIN_OK;
     p.c = cache->c;

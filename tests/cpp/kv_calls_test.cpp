@@ -4,7 +4,9 @@
 //
 //   kv_calls_test index     row starts, lengths and page ids of any value stay inside the buffers
 //   kv_calls_test refusals  arguments outside the documented limits are refused before any launch
+//   kv_calls_test limits    the largest query heads and scales are taken, larger ones refused
 //   kv_calls_test devices   each device that launches the kernel for many vectors has been asked for its LDS
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -218,6 +220,21 @@ void refusals() {
     expect(prefix(0, nullptr) == QLIN_OK && prefix(16, table) == QLIN_OK, "prefix");
 }
 
+void limits() {
+    Made m(8, 16, 16, 8);
+    const int32_t starts[2] = {0, 1}, length[1] = {1}, table[1] = {0};
+    const qlin_kv_batch b = {1, 1, 1, 16, starts, length, table, 1};
+    std::vector<float> x(2048 * 16), y(x.size());
+    const auto attend = [&](int heads, float scale) {
+        return qlin_kv_attention(m.ws, m.c, &b, heads, x.data(), QLIN_F32, heads * 16, scale, y.data(), QLIN_F32, heads * 16, nullptr);
+    };
+    g_launches = 0;
+    expect(attend(1032, 1.0f) == QLIN_ERR_UNSUPPORTED && attend(2048, 1.0f) == QLIN_ERR_UNSUPPORTED, "too many query heads");
+    expect(attend(8, std::ldexp(1.01f, 64)) == QLIN_ERR_UNSUPPORTED && attend(8, -std::numeric_limits<float>::max()) == QLIN_ERR_UNSUPPORTED, "too large a scale");
+    expect(g_launches == 0, "nothing was launched");
+    expect(attend(1024, 1.0f) == QLIN_OK && attend(8, std::ldexp(1.0f, 64)) == QLIN_OK && attend(8, -1.0f) == QLIN_OK && attend(8, 0.0f) == QLIN_OK, "the limits");
+}
+
 void devices() {
     const int32_t starts[2] = {0, 600}, length[1] = {600}, table[38] = {};
     const qlin_kv_batch b = {1, 600, 600, 600, starts, length, table, 38};
@@ -241,6 +258,7 @@ int main(int argc, char** argv) {
     const char* mode = argc > 1 ? argv[1] : "";
     if (!std::strcmp(mode, "index")) index();
     else if (!std::strcmp(mode, "refusals")) refusals();
+    else if (!std::strcmp(mode, "limits")) limits();
     else if (!std::strcmp(mode, "devices")) devices();
     else return 2;
     if (!g_bad) std::printf("PASS %s\n", mode);

@@ -86,3 +86,8 @@ def test_batch_lies_on_one_device():
 def test_lds_of_many_vectors_is_asked_for_on_each_device():
     r = subprocess.run([BIN, "devices"], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and "PASS devices" in r.stdout, r.stdout[-3000:] + r.stderr[-1000:]
+
+
+def test_limits_of_query_heads_and_scale():
+    r = subprocess.run([BIN, "limits"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "PASS limits" in r.stdout, r.stdout[-3000:] + r.stderr[-1000:]
