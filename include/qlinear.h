@@ -428,10 +428,11 @@ int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_b
  * Q: device [rows, ldq] of q_dtype, query head h in columns h * head_dim ..; q_heads is a multiple of
  * kv_heads, and KV head h serves query heads h * q_heads / kv_heads ..  O: device [rows, ldo] of
  * o_dtype; it must not overlap Q.  scale: finite, up to 2^64 either way (else QLIN_ERR_UNSUPPORTED); where its product
- * with a row's largest |Q|, or with the largest |K| in sight, passes 2^110, results may be NaN.  Sums and the softmax are held in f32.  With fp16 rows in and
- * out, probabilities (scaled into fp16's range) are rounded to fp16 before they meet V; if either
- * is f32, queries and probabilities are kept to 22 bits.  The scales of the value rows that a row sees may lie
- * up to 2^96 apart (a row of zeros has 2^-64, so any values below 2^39 will do); past that,
+ * with a row's largest |Q|, or with the largest |K| in sight, passes 2^110, results may be NaN.
+ * Sums and the softmax are held in f32.  Queries and probabilities (scaled into fp16's range) are kept to 22 bits, fp16
+ * queries exactly; but with fp16 rows in and out, where max_new * q_heads / kv_heads (of the prefix: rows * q_heads /
+ * kv_heads) passes 256, probabilities are rounded to fp16 before they meet V, on top of the output's own
+ * rounding.  The scales of the value rows that a row sees may lie up to 2^96 apart (a row of zeros has 2^-64, so any values below 2^39 will do); past that,
  * tokens of the smallest values begin to lose their weight. */
 int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch,
                       int32_t q_heads, const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,

@@ -48,8 +48,10 @@ __device__ __forceinline__ float over_groups(float x) {
 // Workgroup: 4 waves, R tiles of 16 vectors of one KV head, one part of the tokens.  The waves take
 // steps of 32 tokens in turn, each with a running maximum, sum and output of its own, and join
 // them at the end: nothing is shared before that.
-// LIMBS = 2 (f32 rows in or out): queries and P as a sum of two fp16 values, 22 bits; fp16 queries are
-// exact with one, and P rounded to 11 bits is off by as much as an fp16 output.
+// P goes to the matrix core as a sum of two fp16 values, 22 bits, so that an fp16 output is off by its own rounding
+// alone, 2.1e-4 of it (2.6e-4 and 2.8e-4 with P rounded to one fp16 value, in 7.2, 56.4 and 24.4 us for one token at 300, 64
+// sequences of up to 4096 and a prefix of 8192 for 32 rows, against 7.4, 56.8 and 26.0).  f32 queries are such sums
+// too; fp16 ones are exact.
 // SHARED: the part of the prefix, for the rows of all sequences at once.
 template <int DP, int R>
 struct AttendLds {
@@ -57,11 +59,12 @@ struct AttendLds {
     float m[4][16 * R], l[4][16 * R];
     int seen[16 * R], most;  // SHARED: tokens that each vector sees, the most of them
 };
-template <int DP, int R, int LIMBS, bool Q16, bool SHARED>
+template <int DP, int R, bool Q16, bool SHARED>
 __device__ __forceinline__ void attend_part(const AttendParams& p, int block, AttendLds<DP, R>& lds) {
     constexpr int KS = DP / 32;   // matrix steps of a q . k
     constexpr int DT = DP / 16;   // tiles of 16 output columns
     constexpr int VT = 16 * R;    // vectors of the workgroup
+    constexpr int QL = Q16 ? 1 : 2, PL = 2;  // fp16 values of a query and of a P
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -170,7 +173,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     }
 
     // queries, as the B operand: lane (n, g) holds columns 64 c + 16 g .. + 15 of vector n, two matrix steps each
-    half8v qf[R][KS][LIMBS];
+    half8v qf[R][KS][QL];
     float unit[R];  // what the f16 operands were divided by, times scale2
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -178,7 +181,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         float x[DP / 4];
 #pragma unroll
         for (int i = 0; i < DP / 4; ++i) x[i] = query_at<KS, Q16>(qr[r], i / 8, i % 8);
-        if constexpr (LIMBS == 2) {
+        if constexpr (QL == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float m = 0.0f;
 #pragma unroll
@@ -194,10 +197,10 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                _Float16 y[LIMBS];
-                split_f16<LIMBS>(x[8 * k + i], y);
+                _Float16 y[QL];
+                split_f16<QL>(x[8 * k + i], y);
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) qf[r][k][q][i] = y[q];
+                for (int q = 0; q < QL; ++q) qf[r][k][q][i] = y[q];
             }
     }
 
@@ -227,7 +230,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int q = 0; q < LIMBS; ++q)
+                    for (int q = 0; q < QL; ++q)
                         sc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[r][k][q], sc[t][r], 0, 0, 0);
             }
         }
@@ -241,7 +244,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
                 lv[4 * t + i] = bad[t] ? kNan : __builtin_amdgcn_logf(d.vs[t][i]);
                 iv[4 * t + i] = __builtin_amdgcn_rcpf(d.vs[t][i]);
             }
-        half8v pf[R][LIMBS];
+        half8v pf[R][PL];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int left = min(seen[r], cap) - j - 4 * g;
@@ -267,13 +270,18 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
             }
             const float base = m[r] == kNegInf ? 0.0f : m[r] - kPShift;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = __builtin_amdgcn_exp2f(x[i] - base);
-                l[r] = 16 * (i / 4) + i % 4 < left ? __builtin_fmaf(e, iv[i], l[r]) : l[r];
-                _Float16 y[LIMBS];
-                split_f16<LIMBS>(e, y);
+            for (int i = 0; i < 8; i += 2) {
+                const float2v e = {__builtin_amdgcn_exp2f(x[i] - base), __builtin_amdgcn_exp2f(x[i + 1] - base)};
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) pf[r][q][i] = y[q];
+                for (int c = 0; c < 2; ++c)
+                    l[r] = 16 * (i / 4) + (i + c) % 4 < left ? __builtin_fmaf(e[c], iv[i + c], l[r]) : l[r];
+                const half2v y = __builtin_convertvector(e, half2v);
+                const half2v z = __builtin_convertvector(e - __builtin_convertvector(y, float2v), half2v);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    pf[r][0][i + c] = y[c];
+                    pf[r][1][i + c] = z[c];
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -288,7 +296,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q)
+                for (int q = 0; q < PL; ++q)
                     o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r][q], o[r][t], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -383,8 +391,8 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 
 // A launch: the first `shared` workgroups work on the prefix with RS tiles (0: there is none), the others on the
 // sequences' own tokens with RO.
-template <int DP, int RS, int RO, int LIMBS, bool Q16>
-__global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * LIMBS <= 64 ? 4 : DP * (RS > RO ? RS : RO) * LIMBS <= 128 ? 3 : 1)
+template <int DP, int RS, int RO, bool Q16>
+__global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 64 ? 4 : DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 128 ? 3 : 1)
 void attend_kernel(AttendParams p, int shared) {
     __shared__ union {
         AttendLds<DP, (RS > 0 ? RS : RO)> prefix;
@@ -392,11 +400,11 @@ void attend_kernel(AttendParams p, int shared) {
     } lds;
     if constexpr (RS > 0) {
         if ((int)blockIdx.x < shared) {
-            attend_part<DP, RS, LIMBS, Q16, true>(p, blockIdx.x, lds.prefix);
+            attend_part<DP, RS, Q16, true>(p, blockIdx.x, lds.prefix);
             return;
         }
     }
-    attend_part<DP, RO, LIMBS, Q16, false>(p, blockIdx.x - shared, lds.own);
+    attend_part<DP, RO, Q16, false>(p, blockIdx.x - shared, lds.own);
 }
 
 // Joins the parts of vectors: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes hold a vector's
@@ -482,7 +490,7 @@ int tile_of(const AttendParams& p, int64_t vectors) {
     return vectors <= 16 || p.c.dim_padded > 128 ? 16 : 32;
 }
 
-template <int DP, int LIMBS, bool Q16>
+template <int DP, bool Q16>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     const int own = attend_tile(p), shared = p.prefix_parts ? attend_tile_prefix(p) : 0;
     const uint32_t own_blocks = (uint32_t)((p.parts - p.prefix_parts) * (int64_t)p.b.seqs * p.c.heads * p.by_tiles.d);
@@ -495,27 +503,25 @@ hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     if (first == 0) {
         if constexpr (DP <= 128)
             if (own == 32) {
-                attend_kernel<DP, 0, 2, LIMBS, Q16><<<grid, 256, 0, st>>>(p, 0);
+                attend_kernel<DP, 0, 2, Q16><<<grid, 256, 0, st>>>(p, 0);
                 return hipGetLastError();
             }
-        attend_kernel<DP, 0, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, 0);
+        attend_kernel<DP, 0, 1, Q16><<<grid, 256, 0, st>>>(p, 0);
         return hipGetLastError();
     }
     if constexpr (DP <= 128) {  // the prefix's rows are those of all sequences: at least as many
-        if (own == 32) attend_kernel<DP, 2, 2, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
-        else if (shared == 32) attend_kernel<DP, 2, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
-        else attend_kernel<DP, 1, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+        if (own == 32) attend_kernel<DP, 2, 2, Q16><<<grid, 256, 0, st>>>(p, first);
+        else if (shared == 32) attend_kernel<DP, 2, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        else attend_kernel<DP, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
     } else {
-        attend_kernel<DP, 1, 1, LIMBS, Q16><<<grid, 256, 0, st>>>(p, first);
+        attend_kernel<DP, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
     }
     return hipGetLastError();
 }
 
 template <int DP>
 hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
-    const hipError_t e = !p.q_f16 ? launch_typed<DP, 2, false>(p, st)
-                         : p.o_f16 ? launch_typed<DP, 1, true>(p, st)
-                                   : launch_typed<DP, 2, true>(p, st);
+    const hipError_t e = p.q_f16 ? launch_typed<DP, true>(p, st) : launch_typed<DP, false>(p, st);
     if (e != hipSuccess || p.parts == 1) return e;
     // few parts: fewer than the groups of lanes a workgroup has for them
     AttendParams j = p;

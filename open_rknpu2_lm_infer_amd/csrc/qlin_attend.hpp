@@ -8,6 +8,7 @@ namespace qlin {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
@@ -38,7 +39,7 @@ __device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
 // steps leave the output as it is.  P stays at or below 2^(kPShift + kSlack), inside fp16.
 constexpr float kSlack = 5.0f;
 
-// fp16 high part, and the rest (exact in fp16 unless it underflows) where f32 is asked for.
+// fp16 high part, and with two limbs the rest (exact in fp16 unless it underflows).
 template <int LIMBS>
 __device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
     out[0] = (_Float16)x;

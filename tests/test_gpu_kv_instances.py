@@ -116,3 +116,20 @@ def test_captured_chunks(prefix, dtype):
         assert not torch.isnan(got).any() and (got[sum(news):] == 5).all()
     assert ws.status() == 0 and other.status() == 0
     del g
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("all_new", [False, True])  # tiles of 16 vectors, and of 32 (heads up to 128)
+def test_few_vectors_in_fp16_are_rounded_once(ws, all_new, D):
+    """fp16 rows in and out are held to the bound of probabilities of 22 bits and one rounding of the output.  Contexts are
+    short and queries small, so that the bound's other parts, 2^-15 of the values together, leave a probability's rounding
+    to 11 bits no room where values cancel."""
+    lens = [2 + i % 5 for i in range(40)]
+    s = Setup(ws, [(n, n if all_new else 1) for n in lens], 1, D, 16, F16, seed=D, q_heads=8)
+    k, v = s.history()
+    s.fill(k, v)
+    q = s.rand(s.rows, 8 * D, size=0.2)
+    out = ql.kv_attention(ws, s.cache, s.batch(), q.to(DEV))
+    s.dtype = F32  # the bound of two fp16 values a probability
+    check(out, *s.expected(q, k, v, F16))
+    s.cache.close()
