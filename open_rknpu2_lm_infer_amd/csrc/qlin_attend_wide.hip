@@ -49,11 +49,15 @@ struct Share {
     bool bad[SUBS];
 };
 
+// LIMBS fp16 values make a probability.  Two where rows are f32 in or out: 22 bits.  One where both are fp16: its
+// rounding to 11 bits adds to the output's own (2.6e-4 of the output against 64 bits, 2.1e-4 with two), and the second
+// value would cost half as many matrix instructions again (the prompt of 4096 tokens 177 us with one, 222 with two, a chunk
+// of 512 over 8192 102 and 122).  Queries of f32 are two values, those of fp16 one, exact.
 template <int DP, int LIMBS, bool Q16, bool SHARED>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
     using L = TileLds<DP>;
     using Sh = Share<DP>;
-    constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide;
+    constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide, QL = Q16 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -122,7 +126,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
 
     // queries, as the B operand: lane (n, hi) holds columns 16 s + 8 hi .. + 7 of its vector (vectors that
     // are none take the first row's)
-    half8v qf[KS][LIMBS];
+    half8v qf[KS][QL];
     float unit = 1.0f;
     const int64_t row = first_row + p.group.div(seen >= 0 ? v : 0);
     const int head = h * group + p.group.mod(seen >= 0 ? v : 0);
@@ -130,7 +134,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         QueryRow<KS, Q16> qr;
         load_query<KS, 16, false, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
         float up = 1.0f;
-        if constexpr (LIMBS == 2) {
+        if constexpr (QL == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
             float top = 0.0f;
 #pragma unroll
@@ -146,10 +150,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                _Float16 z[LIMBS];
-                split_f16<LIMBS>(query_at<KS, Q16>(qr, k, i) * up, z);
+                _Float16 z[QL];
+                split_f16<QL>(query_at<KS, Q16>(qr, k, i) * up, z);
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) qf[k][q][i] = z[q];
+                for (int q = 0; q < QL; ++q) qf[k][q][i] = z[q];
             }
     };
 
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
             sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].block, s, at[i].vs, 0));
         }
     };
-    const float key_unit = LIMBS == 2 ? 1.0f : p.scale2 * kCodeUnit;
+    const float key_unit = QL == 2 ? 1.0f : p.scale2 * kCodeUnit;
     // a share's way into the LDS, in pieces: 16 bytes of keys are two, four columns of values one each, then the scales
     constexpr int PIECES = 6 * Sh::SUBS;
     auto store_piece = [&](const Sh& sh, uint8_t* buf, int piece) {
@@ -242,7 +246,6 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
     // P of elements 2 i and 2 i + 1 of x
     auto exponents = [&](int i, float base, const float4v* iv) {
-        typedef float float2v __attribute__((ext_vector_type(2)));
         const float2v e = {__builtin_amdgcn_exp2f(x[2 * i] - base), __builtin_amdgcn_exp2f(x[2 * i + 1] - base)};
         l = __builtin_fmaf(e[0], iv[i / 2][2 * i % 4], l);
         l = __builtin_fmaf(e[1], iv[i / 2][2 * i % 4 + 1], l);
@@ -260,7 +263,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
 #pragma unroll
         for (int e = 2 * i; e < 2 * i + 2; ++e) {
             float z = s[e];
-            if constexpr (LIMBS == 2) z *= unit;
+            if constexpr (QL == 2) z *= unit;
             z = __builtin_fmaf(z, ks[e / 4][e % 4], lv[e / 4][e % 4]);
             // masked tokens are chosen away, whatever their scales hold
             if constexpr (decltype(mask)::value) z = 8 * (e / 4) + e % 4 < left ? z : kNegInf;
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
             }
             if constexpr (NEXT)
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[k][q], s, 0, 0, 0);
+                for (int q = 0; q < QL; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[k][q], s, 0, 0, 0);
 #pragma unroll
             for (int i = k * EP + 1; i < (k + 1) * EP + 1; ++i)
                 if (i < 8) exponents(i, base, iv);
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int q = 0; q < LIMBS; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(lds, k), qf[k][q], s, 0, 0, 0);
+                for (int q = 0; q < QL; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(lds, k), qf[k][q], s, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 8; ++i) scale(s, i, min(seen, cap) - j0 - 4 * hi, ks, lv, std::true_type{});
         }
