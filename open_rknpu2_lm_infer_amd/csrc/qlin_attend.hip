@@ -6,8 +6,9 @@
 // in one pass over the tokens with a running maximum.  Codes are exact in fp16, so q . k_j runs on
 // the matrix cores (f32 sums) without any rounding of the keys, and the value scale goes into the
 // probabilities: with l'_j = l_j log2 e + log2 s^V_j and m the running maximum of l',
-// P_j = 2^(l'_j - m) <= 1 multiplies the codes v_j, and the sum of e^(l_j) is sum_j P_j / s^V_j.
-// Taking the maximum over l' and not l keeps P inside fp16's range whatever the scales are.
+// P_j = 2^(l'_j - m) multiplies the codes v_j, and the sum of e^(l_j) is sum_j P_j / s^V_j.
+// Taking the maximum over l' and not l keeps P inside fp16's range whatever the scales are: m lags the largest l' by
+// at most kSlack, so P_j <= 2^kSlack, and 2^(kPShift + kSlack) as the matrix core gets it.
 //
 // A query row and head is a "vector"; the q_heads / kv_heads vectors of each row that share a KV
 // head, and the rows of a sequence, are worked on together, 16 to a tile.  Products are computed

@@ -38,6 +38,7 @@ __device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
 // The running maximum of a vector is raised only when a token passes it by more than this (bits): most
 // steps leave the output as it is.  P stays at or below 2^(kPShift + kSlack), inside fp16.
 constexpr float kSlack = 5.0f;
+static_assert(kPShift + kSlack < 16.0f, "P has to stay below fp16's 65504");
 
 // fp16 high part, and with two limbs the rest (exact in fp16 unless it underflows).
 template <int LIMBS>
