@@ -17,10 +17,11 @@
 // axis permuted, and P never leaves its lane.
 //
 // What bounds it, 8 KV heads of 128, 4 query heads each: with few rows a token's bytes, 2 * 128 + 8 a head (64
-// sequences of up to 4096 tokens, 263 MB: 64 us, 4.1 TB/s; one of 32768, 69 MB in 256 parts of 1024: 14.2 us,
-// 4.9 TB/s, and 4.2 us for the join), with one short sequence the chain of dependent loads, steps and the
-// waves' join (300 tokens: 7.5 us).  A prefix of 8192 tokens for 32 rows, 128 vectors a KV head in tiles of 32, takes 20 us
-// with the rows' own tokens: the vector units' exponents and byte permutes (28% of their time, waits for loads 48%).
+// sequences of up to 4096 tokens, 263 MB: 65 us, 4.1 TB/s; one of 32768, 69 MB in 32 parts of 1024, 256 workgroups: 13.9
+// us, 5 TB/s, and 4.6 us for the join), with one short sequence the chain of dependent loads, steps and the
+// waves' join (300 tokens: 7.8 us).  A prefix of 8192 tokens for 32 rows, 128 vectors a KV head in tiles of 32, takes 21.7 us
+// with the rows' own tokens: the vector units' exponents and byte permutes (31% of their time) and waits (42%), with
+// one wave a SIMD.
 #include "qlin_attend.hpp"
 
 namespace qlin {
@@ -483,9 +484,18 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 
 // Vectors of a workgroup, given how many share its tokens: one or two tiles here (two of 256 columns would
 // not fit the registers), or the wide kernel's.  That one reads a token's bytes once for 128 vectors but
-// waits at a barrier for every 32 tokens: with up to 256 vectors (512 in two limbs) more workgroups of this one
-// are faster.  (4096 tokens, 8 KV heads of 128, us here and there: fp16 64 vectors 15.5 / 17.8, 128 18.1 / 23.2,
-// 256 23.2 / 31.7, 512 33.9 / 37.8, a prefix for 512 45.2 / 44.3; f32 256 27.5 / 40.6, 512 41.3 / 51.1.)
+// waits at a barrier for every 32 tokens: with up to 256 vectors (512 where rows are f32 in or out) more workgroups of
+// this one are faster.  One sequence, 4096 tokens, 8 KV heads, us here and there:
+//   vectors           256          384          512          768         1024
+//   fp16, 64       17.0 / 23.5  25.5 / 24.3  24.4 / 27.9  33.6 / 32.1  34.4 / 32.9
+//   fp16, 128      21.6 / 32.3  34.1 / 34.7  30.9 / 37.8  45.7 / 46.9  48.4 / 46.5
+//   fp16, 256      30.6 / 43.8  51.5 / 60.3  53.2 / 68.6  75.5 / 80.4  96.2 / 93.1
+//   f32, 128       23.9 / 38.3  38.5 / 42.0  33.8 / 46.7  50.9 / 57.9  53.9 / 62.2
+//   prefix, fp16   24.9 / 35.7  36.3 / 41.2  35.4 / 47.6  48.4 / 54.5  57.3 / 65.1   (128 columns)
+//   prefix, f32    26.4 / 43.5  40.4 / 54.2  39.0 / 58.6  54.6 / 75.9  64.1 / 87.3
+// What a batch holds beside that moves the crossing, and the limit on vectors alone is a middle: of 257 to 512 fp16 vectors
+// in 36 random batches of 1 to 16 sequences this kernel takes 0.83 of the other's time on average, half of it for one
+// sequence of a few hundred tokens, 1.35 of it for one of 15000 tokens and up to 1.85 for 16 sequences.
 int tile_of(const AttendParams& p, int64_t vectors) {
     if (vectors > (p.q_f16 && p.o_f16 ? 256 : 512)) return kAttendWide;
     return vectors <= 16 || p.c.dim_padded > 128 ? 16 : 32;

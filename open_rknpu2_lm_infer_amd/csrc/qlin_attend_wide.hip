@@ -11,11 +11,12 @@
 // made, then O of tile u while the maximum of tile u + 1 is found.  Three tiles lie in the LDS: the values of u,
 // the keys of u + 1, and u + 2 on its way in.
 //
-// What bounds it (a prompt of 4096 tokens, 32 query and 8 KV heads of 128, 137 GFLOP: 167 to 178 us, 770 to 820 TFLOP/s):
+// What bounds it (a prompt of 4096 tokens, 32 query and 8 KV heads of 128, 137 GFLOP: 167 to 178 us a call, 770 to 820 TFLOP/s):
 // the LDS, busy 51% of the time, the vector units, 50%, and the matrix cores, 36%, each of which the two waves of a SIMD
 // leave idle in turn.  For 16 matrix instructions of 32 x 32 x 16 a wave reads 16 KB of operands and 12 KB of scale
 // factors; the matrix instructions, their operands' reads and the barriers alone take 124 us.  64 vectors a wave would halve the reads, but their
-// registers leave one wave a SIMD (198 to 247 us).
+// registers leave one wave a SIMD (198 to 247 us).  Heads of 64 take 141 us, of 256 412 (one wave a SIMD).  f32 queries of
+// 128 columns are two values of fp16 each and spill 23 to 25 registers: 305 us (f32 outputs of fp16 queries 224, no spill).
 #include <atomic>
 #include <type_traits>
 
