@@ -1,0 +1,680 @@
+"""Workloads of what a serving step needs between the qkv and the o projection, with inputs, plain forms, 64-bit results and costs.
+
+A case is one of these ways a program calls them:
+
+  rotate  the heads of rows turned by their positions (qlin_rope).
+  norm    the query and key heads of rows normalized and turned in one pass (qlin_norm_rope).
+  qkv     rows of the qkv projection: queries normalized and turned, keys normalized, turned and quantized into the cache,
+          values quantized into it (qlin_kv_append_qkv); the new rows are read back (qlin_kv_read).
+  step    a serving step's tables: row starts, lengths, pages and slots from the lengths of the requests (qlin_kv_step),
+          and the step that takes the same tokens back, as after drafted tokens that are all refused, or for requests that end.
+  store   key and value rows of new tokens into a 4-bit cache and back.
+  attend  query rows of new tokens over their sequences' tokens in a 4-bit cache: decoding, verification, prompts.
+  prefix  the same for a batch whose sequences begin with one shared prefix.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+_TORCH = {"f16": torch.float16, "f32": torch.float32}
+_BYTES = {"f16": 2, "f32": 4}
+SCALE_MIN = 2.0 ** -64
+GROUP = 32  # columns of a 4-bit row that share a unit
+EPS = 1e-6
+
+
+def listed():
+    # 32 query heads over 8 key/value heads of 128 are those of the 4096 + 1024 + 1024 columns of a Qwen3-4B qkv row
+    geo = {"q_heads": 32, "kv_heads": 8, "dim": 128, "page": 64, "in": "f16", "out": "f16"}
+    rot = {"rotary": 128, "first": 0, "layout": "half", "scaling": "plain", "base": 1e6, "factor": 1.0}
+    return [
+        # query and key heads of one decoded token, far into a conversation: the smallest call
+        {"name": "rotate_1", "kind": "rotate", "rows": 1, "far": 30000, **geo, **rot},
+        # a long prompt's rows in float32, neighbours turned, half of each head, wavelengths ramped for a 16 times longer context
+        {"name": "rotate_8192_f32", "kind": "rotate", "rows": 8192, "far": 500000, **geo, **rot, "in": "f32", "out": "f32",
+         "rotary": 64, "layout": "interleaved", "scaling": "ramp", "base": 1e4, "factor": 16.0},
+        # a ragged chunk with heads of an odd width, of which the middle is turned
+        {"name": "norm_700", "kind": "norm", "rows": 700, "far": 4000, **geo, **rot, "q_heads": 10, "kv_heads": 5, "dim": 84,
+         "rotary": 42, "first": 20, "scaling": "linear", "factor": 4.0},
+        # one decoded token from the qkv projection into the cache: latency
+        {"name": "qkv_1", "kind": "qkv", "seqs": 1, "len": 1000, "new": 1, "ragged": False, "idle": 0, **geo, **rot},
+        # a prompt of 4096 tokens from the qkv projection into the cache
+        {"name": "qkv_4096", "kind": "qkv", "seqs": 1, "len": 4096, "new": 4096, "ragged": False, "idle": 0, **geo, **rot},
+        # tables of 64 slots of which most decode, with drafted tokens
+        {"name": "step_64", "kind": "step", "seqs": 64, "len": 4096, "new": 4, "page": 64, "spare": 200},
+        # 3000 slots, prompts of up to 600 tokens among the decoded tokens, more asked for than there are pages
+        {"name": "step_3000", "kind": "step", "seqs": 3000, "len": 3000, "new": 600, "page": 16, "spare": 8000},
+        # a prompt of 4096 tokens stored in 4 bits and read back
+        {"name": "store_4096", "kind": "store", "seqs": 1, "len": 4096, "new": 4096, "ragged": False, "idle": 0, **geo},
+        # one token decoded at the reference's longest context
+        {"name": "decode_1x32768", "kind": "attend", "seqs": 1, "len": 32768, "new": 1, "ragged": False, "idle": 0, **geo},
+        # a serving step: 64 slots at lengths up to 4096, some idle
+        {"name": "decode_64x4096", "kind": "attend", "seqs": 64, "len": 4096, "new": 1, "ragged": True, "idle": 9, **geo},
+        # a chunk of 512 tokens at the end of a prompt of 8192
+        {"name": "chunk_512_of_8192", "kind": "attend", "seqs": 1, "len": 8192, "new": 512, "ragged": False, "idle": 0, **geo},
+        # samples of one prompt with drafted tokens, float32 rows, heads of 64
+        {"name": "prefix_8x2048_f32", "kind": "prefix", "seqs": 8, "len": 2300, "prefix": 2048, "new": 4, "ragged": True,
+         "idle": 0, "q_heads": 16, "kv_heads": 4, "dim": 64, "page": 32, "in": "f32", "out": "f32"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def _draw_rotation(rng, case):
+    half = rng.choice([case["dim"] // 2, case["dim"] // 4, rng.randint(1, max(case["dim"] // 2, 1))])
+    case["rotary"] = min(2 * max(half, 1), case["dim"] // 2 * 2)
+    case["first"] = rng.choice([0, 0, case["dim"] - case["rotary"], rng.randint(0, case["dim"] - case["rotary"])])
+    case["layout"] = rng.choice(["half", "half", "interleaved"])
+    case["scaling"] = rng.choice(["plain", "plain", "linear", "base", "bands", "ramp"])
+    case["base"] = rng.choice([1e4, 5e5, 1e6])
+    case["factor"] = 1.0 if case["scaling"] == "plain" else rng.choice([2.0, 4.0, 8.0, 32.0])
+
+
+def draw(rng):
+    kind = rng.choice(["rotate", "norm", "qkv", "qkv", "step", "step", "store", "attend", "attend", "attend", "prefix"])
+    if kind == "step":
+        seqs = _log_int(rng, 1, 3000)
+        new = rng.choice([1, 2, 4, 8, _log_int(rng, 16, 600)])
+        page = rng.choice([16, 32, 64, 128])
+        n = _log_int(rng, 16, 4096)
+        return {"kind": kind, "seqs": seqs, "len": max(n, new), "new": new, "page": page,
+                "spare": _log_int(rng, 1, 2 + seqs * -(-new // page) * 2)}
+    dim = rng.choice([64, 128, 128, 128, 256, rng.randint(2, 256)])
+    kv = rng.choice([1, 2, 4, 8, 8, rng.randint(1, 12)])
+    group = rng.choice([1, 2, 3, 4, 4, 5, 8])
+    while kv * group > 32:
+        group -= 1
+    t = rng.choice(["f16", "f16", "f32"])
+    case = {"kind": kind, "q_heads": kv * group, "kv_heads": kv, "dim": dim, "page": rng.choice([16, 32, 64, 64, 128]),
+            "in": t, "out": rng.choice([t, t, t, "f16", "f32"])}
+    if kind in ("rotate", "norm", "qkv"):
+        _draw_rotation(rng, case)
+    if kind in ("rotate", "norm"):
+        case["rows"], case["far"] = _log_int(rng, 1, 8192 if dim <= 128 else 4096), _log_int(rng, 1, 1000000)
+        return case
+    case["ragged"] = rng.random() < 0.7
+    if kind in ("store", "qkv"):
+        case["seqs"] = _log_int(rng, 1, 64)
+        case["new"] = _log_int(rng, 1, (4096 if dim <= 128 else 2048) // case["seqs"])
+        case["len"] = min(4096, case["new"] + _log_int(rng, 1, 1024))
+    elif kind == "prefix":
+        case["seqs"], case["new"] = rng.randint(2, 32), rng.choice([1, 1, 1, 2, 4])
+        case["prefix"] = max(1, _log_int(rng, 128, 8192) // case["page"]) * case["page"]
+        case["len"] = case["prefix"] + _log_int(rng, 1, 512)
+    elif rng.random() < 0.7:  # decoding, verification
+        case["seqs"], case["new"] = _log_int(rng, 1, 64), rng.choice([1, 1, 1, 2, 4, 7])
+        case["len"] = _log_int(rng, 1, 65536 // case["seqs"] if case["seqs"] > 2 else 32768)
+    else:  # prompts
+        case["seqs"], case["new"] = rng.choice([1, 1, 2, 4]), _log_int(rng, 16, 512)
+        case["len"] = case["new"] + _log_int(rng, 1, 3500)
+    case["new"] = min(case["new"], case["len"])
+    case["idle"] = rng.randint(2, 9) if case["seqs"] > 2 and rng.random() < 0.4 else 0
+    return case
+
+
+def _sequences(case):
+    """(length after the new rows, new rows) of every sequence."""
+    out = []
+    floor = case.get("prefix", 0)
+    for i in range(case["seqs"]):
+        n, new = case["len"], case["new"]
+        if case["ragged"] and i:  # the first keeps the full length
+            u = (i * 0.6180339887) % 1.0
+            new = 1 + int(u * new) if new > 4 else new
+            n = floor + max(1, int((n - floor) * (0.05 + 0.95 * ((i * 0.7548776662) % 1.0))))
+            new = min(new, n)
+        if case["idle"] and i % case["idle"] == case["idle"] - 1:
+            n = new = 0
+        out.append((n, new))
+    return out
+
+
+# ---- inputs, from the seed alone ---------------------------------------------------------
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _columns(case):
+    return -(-case["len"] // case["page"])
+
+
+def _table(case, seed):
+    """int32 [seqs, columns] page ids, scattered over the cache; the prefix's pages are every sequence's."""
+    cols, seqs = _columns(case), case["seqs"]
+    shared = case.get("prefix", 0) // case["page"]
+    perm = torch.randperm(shared + seqs * (cols - shared), generator=_gen(seed * 10 + 1), device="cuda").to(torch.int32)
+    return torch.cat([perm[:shared].expand(seqs, shared), perm[shared:].view(seqs, cols - shared)], 1).contiguous()
+
+
+def _pages(case):
+    shared = case.get("prefix", 0) // case["page"]
+    return shared + case["seqs"] * (_columns(case) - shared)
+
+
+def _history(case, seed):
+    """Key and value rows of every slot of the cache, [pages, page, kv_heads, dim]: channels of the keys differ in size
+    (a few are large, as in trained models), tokens differ in size."""
+    g = _gen(seed * 10 + 2)
+    shape = (_pages(case), case["page"], case["kv_heads"], case["dim"])
+    k = torch.randn(shape, generator=g, device="cuda")
+    k *= torch.where(torch.rand(shape[2:], generator=g, device="cuda") < 0.03, 6.0, 1.0)
+    v = torch.randn(shape, generator=g, device="cuda")
+    v *= torch.rand(shape[:3] + (1,), generator=g, device="cuda") + 0.25
+    t = _TORCH[case["in"]]
+    return k.to(t), v.to(t)
+
+
+def _heads(case):
+    return case["q_heads"] + case["kv_heads"] * (1 if case["kind"] in ("rotate", "norm") else 2)
+
+
+def _rows(case, seed):
+    """Rows of the qkv projection, [rows, heads * dim]; without its values where only queries and keys are worked on."""
+    rows = case["rows"] if "rows" in case else sum(n for _, n in _sequences(case))
+    g = _gen(seed * 10 + 3)
+    x = torch.randn((rows, _heads(case) * case["dim"]), generator=g, device="cuda")
+    if case["kind"] in ("norm", "qkv"):  # what is normalized differs in size from token to token
+        x *= 0.2 + 3.0 * torch.rand((rows, 1), generator=g, device="cuda")
+    return x.to(_TORCH[case["in"]])
+
+
+def _positions(case, seed):
+    """Ragged runs of consecutive positions that end before `far`, as the rows of a batch of chunks have them."""
+    rows, far = case["rows"], case["far"]
+    run = max(1, rows // 5)
+    g = _gen(seed * 10 + 4)
+    start = torch.randint(0, max(1, far), (-(-rows // run),), generator=g, device="cuda")
+    return (start.repeat_interleave(run)[:rows] + torch.arange(rows, device="cuda") % run).to(torch.int32)
+
+
+def _gammas(case, seed):
+    g = _gen(seed * 10 + 5)
+    out = []
+    for _ in range(2):
+        w = 1.0 + 0.2 * torch.randn((case["dim"],), generator=g, device="cuda")
+        out.append(w * torch.where(torch.rand((case["dim"],), generator=g, device="cuda") < 0.05, 3.0, 1.0))
+    return out
+
+
+def _requests(case, seed):
+    """Lengths, tokens asked for, page table and free list of a step's slots: some are idle, some have just come."""
+    seqs, P, g = case["seqs"], case["page"], _gen(seed * 10 + 6)
+    limit = case["len"] + case["new"]
+    u = torch.rand((4, seqs), generator=g, device="cuda")
+    length = (u[0] * case["len"]).to(torch.int32)
+    length = torch.where(u[1] < 0.1, 0, length)
+    add = torch.where(u[2] < 0.7, 1 + (u[3] * min(case["new"], 4)).to(torch.int32), 1 + (u[3] * case["new"]).to(torch.int32))
+    add = torch.where(u[2] > 0.95, 0, add).clamp(max=case["new"]).to(torch.int32)
+    cols = -(-limit // P)
+    held = (length + P - 1) // P
+    pages = seqs * -(-case["len"] // P) + case["spare"]
+    perm = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((seqs, cols), -1, dtype=torch.int32, device="cuda")
+    mine = torch.arange(cols, device="cuda") < held[:, None]
+    used = int(held.sum())
+    table[mine] = perm[:used]
+    free = torch.full((pages,), -1, dtype=torch.int32, device="cuda")
+    free[:case["spare"]] = perm[used:used + case["spare"]]  # the other pages are other requests'
+    count = torch.full((1,), case["spare"], dtype=torch.int32, device="cuda")
+    return length, add, table, free, count
+
+
+def _step_rows(case):
+    return case["seqs"] * min(case["new"], 4) + case["seqs"] * case["new"] // 4 + case["new"]
+
+
+def _split(case, x):
+    D, hq, hk = case["dim"], case["q_heads"], case["kv_heads"]
+    return x[:, :hq * D], x[:, hq * D:(hq + hk) * D], x[:, (hq + hk) * D:]
+
+
+# ---- the plain form -----------------------------------------------------------------------
+
+
+def _quantize8(x):
+    """Codes and scales of the last axis; the rounding in 64 bits, where a half is a half."""
+    s = (x.float().abs().amax(-1, keepdim=True) * torch.tensor(1.0 / 127.0, dtype=torch.float32, device=x.device)).clamp_min(SCALE_MIN)
+    y = (x.float() * (1.0 / s)).double()
+    return (torch.sign(y) * torch.floor(y.abs() + 0.5)).clamp(-127, 127).float(), s
+
+
+def _quantize4(x):
+    """Codes times units (whole numbers up to 7 * 255) and scales of the last axis."""
+    D = x.shape[-1]
+    f = torch.nn.functional.pad(x.float(), (0, -D % GROUP)).unflatten(-1, (-1, GROUP))
+    inv1785, inv7 = (torch.tensor(1.0 / n, dtype=torch.float32, device=x.device) for n in (1785, 7))
+    a = f.abs().amax(-1)
+    s = (a.amax(-1, keepdim=True) * inv1785).clamp_min(SCALE_MIN)
+    u = torch.ceil(a * (1.0 / s) * inv7).clamp(1, 255)
+    y = (f * (1.0 / (u * s))[..., None]).double()
+    c = (torch.sign(y) * torch.floor(y.abs() + 0.5)).clamp(-7, 7).float()
+    return (c * u[..., None]).flatten(-2)[..., :D], s
+
+
+def _turns(case):
+    """Turns a position adds to each pair, in 64 bits, and the amplitude."""
+    n, base, factor, how = case["rotary"], case["base"], case["factor"], case["scaling"]
+    i = torch.arange(0, n, 2, dtype=torch.float64, device="cuda")
+    if how == "base":
+        base = base * factor ** (n / (n - 2)) if n > 2 else base
+    w = base ** (-i / n)
+    if how == "linear":
+        w = w / factor
+    elif how == "bands":
+        whole = _ORIGINAL * w / (2 * math.pi)  # wavelengths that fit the original length
+        mix = ((whole - _BANDS[0]) / (_BANDS[1] - _BANDS[0])).clamp(0, 1)
+        w = w * (mix + (1 - mix) / factor)
+    elif how == "ramp":
+        lo, hi = (n * math.log(_ORIGINAL / (b * 2 * math.pi)) / (2 * math.log(base)) for b in (_RAMP[1], _RAMP[0]))
+        lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), n - 1)
+        mix = 1 - ((i / 2 - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        w = w * (mix + (1 - mix) / factor)
+    return w / (2 * math.pi), 0.1 * math.log(factor) + 1 if how == "ramp" else 1.0
+
+
+_ORIGINAL, _BANDS, _RAMP = 8192, (1.0, 4.0), (1.0, 32.0)
+
+
+def _plain_rotate(case, x, positions):
+    """x float32 [rows, heads, dim]; the angle in 64 bits, reduced to a turn, then 32."""
+    turns, amplitude = _turns(case)
+    t = positions.double()[:, None] * turns
+    angle = ((t - torch.round(t)) * (2 * math.pi)).float()[:, None]
+    c, s = torch.cos(angle) * amplitude, torch.sin(angle) * amplitude
+    lo, hi, out = case["first"], case["first"] + case["rotary"], x.clone()
+    if case["layout"] == "half":
+        mid = lo + case["rotary"] // 2
+        a, b = x[..., lo:mid], x[..., mid:hi]
+        out[..., lo:mid], out[..., mid:hi] = a * c - b * s, b * c + a * s
+    else:
+        a, b = x[..., lo:hi:2], x[..., lo + 1:hi:2]
+        out[..., lo:hi:2], out[..., lo + 1:hi:2] = a * c - b * s, b * c + a * s
+    return out
+
+
+def _plain_norm(x, gamma):
+    return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * gamma
+
+
+def _plain_heads(state):
+    """Queries and keys, normalized (but for `rotate`) and turned, float32 [rows, heads, dim]."""
+    case, D, hq, hk = state["case"], state["case"]["dim"], state["case"]["q_heads"], state["case"]["kv_heads"]
+    x = state["x"][:, :(hq + hk) * D].float().view(-1, hq + hk, D)
+    if case["kind"] != "rotate":
+        x = torch.cat([_plain_norm(x[:, :hq], state["gamma"][0]), _plain_norm(x[:, hq:], state["gamma"][1])], 1)
+    return _plain_rotate(case, x, state["positions"])
+
+
+def _plain_store(state, k, v, quantize):
+    """Quantizes rows k, v [rows, kv_heads, dim] into their pages and reads them back."""
+    case, at = state["case"], state["at"]
+    P = case["page"]
+    page = state["table"][at[:, 0], at[:, 2] // P].long()
+    out = []
+    for x, codes, scales in zip((k, v), (state["ck"], state["cv"]), (state["sk"], state["sv"])):
+        c, s = quantize(x)
+        codes[page, at[:, 2] % P], scales[page, at[:, 2] % P] = c, s
+        back = codes[page, at[:, 2] % P] * scales[page, at[:, 2] % P]
+        out.append(back.flatten(1).to(_TORCH["f16" if case["kind"] == "qkv" else case["out"]]))
+    return out
+
+
+def _plain_attend(state):
+    case, at = state["case"], state["at"]
+    B, T, hq, hk, D = case["seqs"], case["new"], case["q_heads"], case["kv_heads"], case["dim"]
+    G = hq // hk
+    pages = state["table"].long()
+
+    def dense(codes, scales):  # [B, kv_heads, tokens, dim]
+        x = codes[pages].float() * scales[pages]
+        return x.flatten(1, 2).transpose(1, 2)
+
+    q = torch.zeros((B, T, hq, D), device="cuda")
+    q[at[:, 0], at[:, 1]] = _split(case, state["x"])[0].float().reshape(-1, hq, D)
+    q = q.view(B, T, hk, G, D).permute(0, 2, 3, 1, 4).reshape(B, hk, G * T, D)
+    k = dense(state["ck"], state["sk"])
+    x = torch.matmul(q, k.transpose(2, 3).contiguous()) * (D ** -0.5)
+    del k
+    last = (state["length"] - state["new"])[:, None] + torch.arange(T, device="cuda")
+    unseen = torch.arange(x.shape[-1], device="cuda") > last[:, :, None]
+    x = x.view(B, hk, G, T, -1).masked_fill_(unseen[:, None, None], float("-inf"))
+    x = torch.exp(x - x.amax(-1, keepdim=True).clamp_min(-1e30))
+    o = torch.matmul(x.view(B, hk, G * T, -1), dense(state["cv"], state["sv"]))
+    o = o.view(B, hk, G, T, D) / x.sum(-1, keepdim=True).clamp_min(1e-30)
+    o = o.permute(0, 3, 1, 2, 4)[at[:, 0], at[:, 1]]
+    return [o.reshape(-1, hq * D).to(_TORCH[case["out"]])]
+
+
+def _owners(counts, total):
+    """For each of `total` things in order: whose it is, and its number there."""
+    who = torch.repeat_interleave(torch.arange(counts.numel(), device="cuda"), counts.long(), output_size=total)
+    return who, torch.arange(total, device="cuda") - (torch.cumsum(counts, 0) - counts)[who]
+
+
+def _plain_step(case, state, change, maps):
+    """One step on the state's lengths, table and free list; maps: row starts, row -> sequence, position, slot, refusals."""
+    P, limit = case["page"], case["len"] + case["new"]
+    n, c = state["length"].long(), change.long()
+    table, free, count = state["table"], state["free"], int(state["count"])
+    held = (n + P - 1) // P
+    # tokens taken back: pages behind the new length go on top of the free list
+    less = torch.clamp(n + c, min=0)
+    kept = (less + P - 1) // P
+    back = torch.where(c < 0, held - kept, 0)
+    total = int(back.sum())
+    who, j = _owners(back, total)
+    free[count:count + total] = table[who, kept[who] + j]
+    table[who, kept[who] + j] = -1
+    count += total
+    # tokens asked for: as long as rows, then pages last
+    want = torch.where((c > 0) & (c <= case["new"]) & (n + c <= limit), c, 0)
+    want = torch.where(torch.cumsum(want, 0) <= _step_rows(case), want, 0)
+    need = torch.where(want > 0, (n + want + P - 1) // P - held, 0)
+    want = torch.where((need == 0) | (torch.cumsum(need, 0) <= count), want, 0)
+    need = torch.where(want > 0, need, 0)
+    total = int(need.sum())
+    who, j = _owners(need, total)
+    table[who, held[who] + j] = free[count - 1 - torch.arange(total, device="cuda")]
+    count -= total
+    state["length"].copy_(torch.where(c < 0, less, n + want))
+    state["count"].fill_(count)
+    rows = int(want.sum())
+    maps["row_start"][0] = 0
+    maps["row_start"][1:] = torch.cumsum(want, 0)
+    who, j = _owners(want, rows)
+    at = n[who] + j
+    maps["row_seq"][:rows] = who.int()
+    maps["positions"][:rows] = at.int()
+    maps["slots"][:rows] = table[who, at // P].long() * P + at % P
+    maps["refused"].fill_(int(((c > 0) & (want == 0)).sum()))
+
+
+# ---- the program's side -------------------------------------------------------------------
+
+
+def _starts(seqs):
+    starts = [0]
+    for _, n in seqs:
+        starts.append(starts[-1] + n)
+    return starts
+
+
+def _own_rope(case):
+    from open_rknpu2_lm_infer_amd import qlinear as ql
+    low, high = _RAMP if case["scaling"] == "ramp" else _BANDS
+    return ql.Rope(case["dim"], case["rotary"], base=case["base"], first=case["first"], layout=case["layout"],
+                   scaling=case["scaling"], factor=case["factor"], original_len=_ORIGINAL, low=low, high=high)
+
+
+def _prepare_step(case, seed):
+    length, add, table, free, count = _requests(case, seed)
+    rows = _step_rows(case)
+    state = {"case": case, "length": length, "add": add, "less": torch.empty_like(add), "table": table, "free": free, "count": count}
+
+    def maps():
+        return {"row_start": torch.zeros((case["seqs"] + 1,), dtype=torch.int32, device="cuda"),
+                "row_seq": torch.full((rows,), -1, dtype=torch.int32, device="cuda"),
+                "positions": torch.full((rows,), -1, dtype=torch.int32, device="cuda"),
+                "slots": torch.full((rows,), -1, dtype=torch.int64, device="cuda"),
+                "refused": torch.zeros((1,), dtype=torch.int32, device="cuda")}
+
+    state["maps"] = [maps(), maps()]
+    if own:
+        from open_rknpu2_lm_infer_amd import qlinear as ql
+        state["ws"] = ql.Workspace(1, 256, 256)
+        state["cache"] = ql.KVCache(1, 64, free.numel(), case["page"], bits=4)
+        state["steps"] = [ql.KVStep(state["cache"], length, table, free, count, rows=rows, max_new=case["new"],
+                                    max_len=case["len"] + case["new"], **m) for m in state["maps"]]
+    return state
+
+
+def prepare(case, seed):
+    if case["kind"] == "step":
+        return _prepare_step(case, seed)
+    state = {"case": case, "x": _rows(case, seed)}
+    if case["kind"] in ("norm", "qkv"):
+        state["gamma"] = _gammas(case, seed)
+    if case["kind"] in ("rotate", "norm"):
+        state["positions"] = _positions(case, seed)
+        if own:
+            state["rope"] = _own_rope(case)
+            state["out"] = torch.empty(state["x"].shape, dtype=_TORCH[case["out"]], device="cuda")
+        return state
+    seqs, kind = _sequences(case), case["kind"]
+    starts = _starts(seqs)
+    state["table"] = _table(case, seed)
+    k, v = _history(case, seed)
+    length = torch.tensor([n for n, _ in seqs], dtype=torch.int32, device="cuda")
+    hk, D, out = case["kv_heads"], case["dim"], _TORCH[case["out"]]
+    if own:
+        from open_rknpu2_lm_infer_amd import qlinear as ql
+        pages, page = k.shape[:2]
+        cache = ql.KVCache(hk, D, pages, page, bits=8 if kind == "qkv" else 4)
+        ws = ql.Workspace(1, 256, 256)
+        # the history: every page as a full sequence of its own
+        ids = torch.arange(pages, dtype=torch.int32, device="cuda").view(pages, 1)
+        full = torch.full((pages,), page, dtype=torch.int32, device="cuda")
+        all_rows = torch.arange(pages + 1, dtype=torch.int32, device="cuda") * page
+        ql.kv_append(ws, cache, ql.KVBatch(all_rows, full, ids, pages * page, page, page),
+                     k.view(pages * page, hk * D), v.view(pages * page, hk * D))
+        start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        batch = ql.KVBatch(start, length, state["table"], starts[-1], max(n for _, n in seqs), case["len"])
+        state.update(ws=ws, cache=cache, batch=batch)
+        state["q"], state["k"], state["v"] = _split(case, state["x"])
+        if kind == "qkv":
+            state["rope"] = _own_rope(case)
+        if kind != "store":
+            state["out"] = torch.empty((starts[-1], case["q_heads"] * D), dtype=out, device="cuda")
+        if kind in ("store", "qkv"):
+            t = torch.float16 if kind == "qkv" else out
+            state["read"] = [torch.empty((starts[-1], hk * D), dtype=t, device="cuda") for _ in range(2)]
+        if kind == "prefix":
+            state["prefix"] = dict(prefix_tokens=case["prefix"], prefix_pages=state["table"][0, :case["prefix"] // page])
+        return state
+    # the plain form keeps whole numbers and scales as tensors, and where each new row of the batch goes
+    quantize = _quantize8 if kind == "qkv" else _quantize4
+    for name, x in (("k", k), ("v", v)):
+        c, state["s" + name] = quantize(x)
+        state["c" + name] = c.to(torch.int16) if kind in ("attend", "prefix") else c
+    state["length"] = length
+    state["new"] = torch.tensor([n for _, n in seqs], dtype=torch.int32, device="cuda")
+    at = [(i, t, n - m + t) for i, (n, m) in enumerate(seqs) for t in range(m)]
+    state["at"] = torch.tensor(at, dtype=torch.int64, device="cuda").view(-1, 3)
+    state["positions"] = state["at"][:, 2]
+    return state
+
+
+def run(state):
+    case = state["case"]
+    kind = case["kind"]
+    if own:
+        return _own_run(state, case, kind)
+    if kind == "step":
+        _plain_step(case, state, state["add"], state["maps"][0])
+        _plain_step(case, state, _granted_back(state), state["maps"][1])
+        return _step_outputs(state)
+    if kind in ("rotate", "norm"):
+        return [_plain_heads(state).flatten(1).to(_TORCH[case["out"]])]
+    if kind in ("attend", "prefix"):
+        return _plain_attend(state)
+    hk, D = case["kv_heads"], case["dim"]
+    if kind == "store":
+        _, k, v = _split(case, state["x"])
+        return _plain_store(state, k.reshape(-1, hk, D), v.reshape(-1, hk, D), _quantize4)
+    heads = _plain_heads(state)
+    q, k = heads[:, :case["q_heads"]], heads[:, case["q_heads"]:]
+    v = _split(case, state["x"])[2].reshape(-1, hk, D)
+    return [q.flatten(1).to(_TORCH[case["out"]])] + _plain_store(state, k, v, _quantize8)
+
+
+def _granted_back(state):
+    """The tokens that the first step granted, as a change that takes them back."""
+    starts = state["maps"][0]["row_start"]
+    return torch.sub(starts[:-1], starts[1:], out=state["less"])
+
+
+def _step_outputs(state):
+    return [state["length"], state["table"], state["free"], state["count"], *state["maps"]]
+
+
+def _own_run(state, case, kind):
+    from open_rknpu2_lm_infer_amd import qlinear as ql
+    if kind == "step":
+        ql.kv_step(state["ws"], state["steps"][0], state["add"])
+        ql.kv_step(state["ws"], state["steps"][1], _granted_back(state))
+        return _step_outputs(state)
+    if kind == "rotate":
+        return [ql.rope(state["rope"], state["x"], state["positions"], out=state["out"])]
+    if kind == "norm":
+        return [ql.norm_rope(state["rope"], state["x"], state["positions"], case["q_heads"], *state["gamma"], eps=EPS,
+                             out=state["out"])]
+    if kind == "qkv":
+        ql.kv_append_qkv(state["ws"], state["cache"], state["batch"], state["rope"], state["x"], case["q_heads"],
+                         *state["gamma"], eps=EPS, out=state["out"])
+        ql.kv_read(state["ws"], state["cache"], state["batch"], *state["read"])
+        return [state["out"], *state["read"]]
+    if kind == "store":
+        ql.kv_append(state["ws"], state["cache"], state["batch"], state["k"], state["v"])
+        ql.kv_read(state["ws"], state["cache"], state["batch"], *state["read"])
+        return state["read"]
+    ql.kv_attention(state["ws"], state["cache"], state["batch"], state["q"], out=state["out"], scale=case["dim"] ** -0.5,
+                    **state.get("prefix", {}))
+    return [state["out"]]
+
+
+# ---- costs and results ----------------------------------------------------------------------
+
+
+def work(case):
+    kind = case["kind"]
+    if kind == "step":  # a slot: change, length (in and out), row start, one table entry and one free page; a row's maps
+        rows = min(_step_rows(case), int(case["seqs"] * (0.7 * min(case["new"], 4) + 0.25 * case["new"]) / 2) + 1)
+        return {"bytes": 2 * 24 * case["seqs"] + 16 * rows, "flops": 2 * 20 * (case["seqs"] + rows)}
+    D, hk, hq, P = case["dim"], case["kv_heads"], case["q_heads"], case["page"]
+    size = {t: _BYTES[case[t]] for t in ("in", "out")}
+    if kind in ("rotate", "norm"):
+        rows = case["rows"]
+        return {"bytes": rows * ((hq + hk) * D * (size["in"] + size["out"]) + 4), "flops": rows * (hq + hk) * D * 8}
+    seqs = _sequences(case)
+    rows = sum(m for _, m in seqs)
+    # codes, units and scales of a key and a value
+    token = hk * (2 * D + 8) if kind == "qkv" else hk * (D + 2 * -(-D // GROUP) + 8)
+    if kind == "store":  # rows in, codes out and in again, rows out
+        return {"bytes": rows * (2 * hk * D * (size["in"] + size["out"]) + 2 * token), "flops": rows * 12 * hk * D}
+    if kind == "qkv":
+        return {"bytes": rows * ((hq + 2 * hk) * D * size["in"] + hq * D * size["out"] + 2 * token + 2 * hk * D * 2),
+                "flops": rows * (hq + 2 * hk) * D * 10}
+    shared = case.get("prefix", 0)
+    tokens = shared + sum(max(n - shared, 0) for n, _ in seqs)
+    flops = sum(4 * hq * D * (m * n - m * (m - 1) // 2) for n, m in seqs)
+    return {"bytes": tokens * token + rows * hq * D * (size["in"] + size["out"]) + 4 * (tokens // P + 1), "flops": flops}
+
+
+def _exact_angles(case):
+    """Radians a position adds to each pair, one by one."""
+    n, factor, how, out = case["rotary"], case["factor"], case["scaling"], []
+    for i in range(n // 2):
+        base = case["base"]
+        if how == "base" and n > 2:
+            base *= math.exp(math.log(factor) * n / (n - 2))
+        w = math.exp(-math.log(base) * 2 * i / n)
+        if how == "linear":
+            w /= factor
+        if how == "bands":
+            length = 2 * math.pi / w
+            if length > _ORIGINAL / _BANDS[0]:
+                w /= factor
+            elif length > _ORIGINAL / _BANDS[1]:
+                part = (_ORIGINAL / length - _BANDS[0]) / (_BANDS[1] - _BANDS[0])
+                w = (1 - part) * w / factor + part * w
+        if how == "ramp":
+            at = [n * math.log(_ORIGINAL / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in _RAMP]
+            first, last = max(math.floor(at[1]), 0), min(math.ceil(at[0]), n - 1)
+            part = min(max((i - first) / max(last - first, 0.001), 0.0), 1.0)
+            w = part * w / factor + (1 - part) * w
+        out.append(w)
+    return torch.tensor(out, dtype=torch.float64, device="cuda"), 1.0 + 0.1 * math.log(factor) if how == "ramp" else 1.0
+
+
+def _exact_heads(case, seed, x, positions):
+    """x float64 [rows, heads, dim]: as complex numbers times e^(i angle)."""
+    if case["kind"] != "rotate":
+        gq, gk = _gammas(case, seed)
+        g = torch.stack([gq] * case["q_heads"] + [gk] * case["kv_heads"]).double()
+        x = x / torch.sqrt(x.pow(2).sum(-1, keepdim=True) / case["dim"] + EPS) * g
+    w, amplitude = _exact_angles(case)
+    turn = torch.polar(torch.full_like(w, amplitude).expand(positions.numel(), -1).contiguous(),
+                       positions.double()[:, None] * w)[:, None]
+    lo, half, out = case["first"], case["rotary"] // 2, x.clone()
+    i = torch.arange(half, device="cuda")
+    left, right = (lo + i, lo + half + i) if case["layout"] == "half" else (lo + 2 * i, lo + 2 * i + 1)
+    z = torch.complex(x[..., left], x[..., right]) * turn
+    out[..., left], out[..., right] = z.real, z.imag
+    return out
+
+
+def _exact_stored(x, bits):
+    """What the cache holds of rows x: the definition's single precision scales, their products and the codes."""
+    x32 = x.to(torch.float32)
+    one = torch.ones((), dtype=torch.float32, device="cuda")
+    if bits == 8:
+        top = x32.abs().max(-1, keepdim=True).values * (one / 127)
+        s = torch.maximum(top, torch.full_like(top, SCALE_MIN))
+        y = torch.reciprocal(s) * x32
+        return torch.where(y < 0, torch.ceil(y.double() - 0.5), torch.floor(y.double() + 0.5)) * s.double()
+    top = x32.abs().max(-1, keepdim=True).values * (one / 1785)
+    s = torch.maximum(top, torch.full_like(top, SCALE_MIN))
+    out = []
+    for g in x32.split(GROUP, -1):
+        u = torch.ceil(g.abs().max(-1, keepdim=True).values * torch.reciprocal(s) * (one / 7))
+        u = torch.minimum(torch.maximum(u, one), 255 * one)
+        y = torch.reciprocal(u * s) * g
+        y = torch.where(y < 0, torch.ceil(y.double() - 0.5), torch.floor(y.double() + 0.5)).clamp(-7, 7)
+        out.append(y * u.double() * s.double())
+    return torch.cat(out, -1)
+
+
+def exact(case, seed):
+    kind = case["kind"]
+    if kind == "step":
+        return None
+    rows = _rows(case, seed)
+    hk, hq, D, P = case["kv_heads"], case["q_heads"], case["dim"], case["page"]
+    if kind in ("rotate", "norm"):
+        x = rows.double().view(rows.shape[0], hq + hk, D)
+        return [_exact_heads(case, seed, x, _positions(case, seed)).reshape(rows.shape)]
+    q, k, v = (t.reshape(rows.shape[0], -1, D) for t in _split(case, rows))
+    if kind == "store":
+        return [_exact_stored(t, 4).reshape(rows.shape[0], hk * D) for t in (k, v)]
+    if kind == "qkv":
+        at = torch.cat([torch.arange(n - m, n, device="cuda") for n, m in _sequences(case)])
+        y = _exact_heads(case, seed, torch.cat([q, k], 1).double(), at)
+        return [y[:, :hq].reshape(-1, hq * D), _exact_stored(y[:, hq:], 8).reshape(-1, hk * D),
+                _exact_stored(v, 8).reshape(-1, hk * D)]
+    table = _table(case, seed).cpu()
+    keys, values = _history(case, seed)
+    out, r = torch.zeros((rows.shape[0], hq, D), dtype=torch.float64, device="cuda"), 0
+    for i, (n, m) in enumerate(_sequences(case)):
+        if m == 0:
+            continue
+        ids = table[i, :-(-n // P)].long().cuda()
+        pos = torch.arange(n - m, n, device="cuda")
+        for h in range(hk):
+            kh = _exact_stored(keys[ids, :, h].reshape(-1, D)[:n], 4)
+            vh = _exact_stored(values[ids, :, h].reshape(-1, D)[:n], 4)
+            for g in range(h * (hq // hk), (h + 1) * (hq // hk)):
+                a = (q[r:r + m, g].double() @ kh.t()) / math.sqrt(D)
+                a[pos[:, None] < torch.arange(n, device="cuda")[None, :]] = -math.inf
+                out[r:r + m, g] = torch.softmax(a, 1) @ vh
+        r += m
+    return [out.reshape(-1, hq * D)]
