@@ -2,8 +2,8 @@
 
 A case is one of these ways a program calls them:
 
-  rotate  the heads of rows turned by their positions (qlin_rope).
-  norm    the query and key heads of rows normalized and turned in one pass (qlin_norm_rope).
+  rotate  the heads of rows turned by their positions (qlin_rope_run).
+  norm    the query and key heads of rows normalized and turned in one pass (qlin_rope_run_norm).
   qkv     rows of the qkv projection: queries normalized and turned, keys normalized, turned and quantized into the cache,
           values quantized into it (qlin_kv_append_qkv); the new rows are read back (qlin_kv_read).
   step    a serving step's tables: row starts, lengths, pages and slots from the lengths of the requests (qlin_kv_step),
