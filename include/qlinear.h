@@ -57,6 +57,7 @@ extern "C" {
 #define QLIN_SWIGLU 0x4u          /* fused SiLU(gate)*up epilogue, output [M, N/2] */
 #define QLIN_NO_FUSED_QUANT 0x8u  /* decode: quantize in a separate launch instead of in the GEMV */
 #define QLIN_RESIDUAL 0x10u       /* chain stage: add a residual row after the linear (see qlin_chain_stage) */
+#define QLIN_ROPE_INVERSE 0x20u   /* rotary positions: turn back (times the amplitude: the transposed map) */
 
 typedef struct qlin_weights qlin_weights;
 typedef struct qlin_workspace qlin_workspace;
@@ -352,7 +353,63 @@ int qlin_chain_stage_output(const qlin_chain* chain, int32_t stage, void** ptr, 
  * leaves no state behind: the next run is correct without any reset. */
 int qlin_chain_status(qlin_chain* chain, int32_t clear);
 
-/* ---- key/value cache in 8 bits, and attention over it ----
+/* ---- rotary positions, and the norms of query and key heads ----
+ * Replaces the CPU rope of the reference's decoder (Cpu::rope, src/model/cpu.rs) and its per-head norms of q and k: what lies
+ * between the qkv projection and the cache.  Pair i of rotary_dim / 2 columns (l, r) of every head of a row is turned by the
+ * angle t = position * w_i:
+ *   y[l] = a (x[l] cos t - x[r] sin t),   y[r] = a (x[r] cos t + x[l] sin t)
+ * with w_i = base^(-2 i / rotary_dim), scaled for contexts longer than the ones trained on.  The angle is reduced in 64
+ * bits, so far positions are turned as exactly as near ones (off by position * 2^-53 turns); all else is f32. */
+#define QLIN_ROPE_HALF 0        /* pair i: columns first + i and first + rotary_dim / 2 + i */
+#define QLIN_ROPE_INTERLEAVED 1 /* pair i: columns first + 2 i and first + 2 i + 1 */
+
+#define QLIN_ROPE_PLAIN 0  /* w_i */
+#define QLIN_ROPE_LINEAR 1 /* w_i / factor: positions interpolated */
+#define QLIN_ROPE_BASE 2   /* base * factor^(rotary_dim / (rotary_dim - 2)) in the place of base: the last pair as LINEAR, the first as it is */
+#define QLIN_ROPE_BANDS 3  /* by wavelength: w_i (k + (1 - k) / factor), k = (original_len w_i / 2 pi - low) / (high - low) within 0..1:
+                            * of `high` wavelengths in original_len and more kept, of `low` and fewer divided */
+#define QLIN_ROPE_RAMP 4   /* by pair: w_i (k + (1 - k) / factor), k = 1 - (i - lo) / (hi - lo) within 0..1 (hi - lo at least 0.001), where
+                            * pair(t) = rotary_dim ln(original_len / (2 pi t)) / (2 ln base), lo = max(floor(pair(high)), 0),
+                            * hi = min(ceil(pair(low)), rotary_dim - 1); the amplitude defaults to 0.1 ln factor + 1 */
+typedef struct qlin_rope qlin_rope;
+
+typedef struct qlin_rope_config {
+    int32_t head_dim;   /* 1..256 */
+    int32_t rotary_dim; /* columns that are turned, even, 2..head_dim */
+    int32_t first;      /* the first of them; the others stay as they are */
+    int32_t layout;     /* QLIN_ROPE_HALF, QLIN_ROPE_INTERLEAVED */
+    int32_t scaling;    /* QLIN_ROPE_PLAIN .. QLIN_ROPE_RAMP */
+    int32_t reserved;
+    double base;         /* above 1 */
+    double factor;       /* at least 1 (not read for PLAIN) */
+    double original_len; /* tokens, positive (BANDS, RAMP) */
+    double low, high;    /* 0 < low < high (BANDS, RAMP) */
+    double amplitude;    /* a; 0: 1, with RAMP 0.1 ln factor + 1 */
+} qlin_rope_config;
+
+/* The handle belongs to the device that is current here, which has to be the current one in every call with it. */
+int qlin_rope_create(const qlin_rope_config* config, qlin_rope** out);
+void qlin_rope_free(qlin_rope* rope);
+/* w_i in radians a position, [rotary_dim / 2], and the amplitude (host pointers). */
+int qlin_rope_query(const qlin_rope* rope, double* radians, double* amplitude);
+
+/* Turns `heads` heads (1..1024) of head_dim columns of every row: X device [rows, ldx] of x_dtype, head h in columns
+ * h * head_dim ..; positions device int32 [rows], any value; Y device [rows, ldy] of y_dtype gets the whole heads.  Y may be X
+ * with the same type and stride (in place); else they must not overlap.  flags: QLIN_ROPE_INVERSE.  Up to 2^24 - 1
+ * rows; 0 do nothing.  Inf and NaN reach the pair they are in. */
+int qlin_rope_run(const qlin_rope* rope, int32_t rows, int32_t heads, const void* X, int32_t x_dtype, int64_t ldx,
+                  const int32_t* positions, void* Y, int32_t y_dtype, int64_t ldy, uint32_t flags, void* stream);
+
+/* RMSNorm of every head and the rotation in one pass: rows hold q_heads heads, then k_heads (either may be 0), as the first
+ * columns of qkv rows do.
+ *   n[d] = x[d] / sqrt(mean_d x^2 + eps) * gamma[d],  then as above
+ * q_gamma, k_gamma: device f32 [head_dim], NULL: that kind is not normalized; eps > 0.  rope NULL: norms alone, positions
+ * are not read.  Sums are f32: values up to 2^59.  A head with Inf or NaN is NaN where it had them (with NaN, everywhere). */
+int qlin_rope_run_norm(const qlin_rope* rope, int32_t rows, int32_t head_dim, int32_t q_heads, int32_t k_heads,
+                       const float* q_gamma, const float* k_gamma, float eps, const void* X, int32_t x_dtype, int64_t ldx,
+                       const int32_t* positions, void* Y, int32_t y_dtype, int64_t ldy, uint32_t flags, void* stream);
+
+/* ---- key/value cache in 8 or 4 bits, and attention over it ----
  * The reference keeps its keys and values in FP16 and runs attention as a unit of the native
  * library (src/npu/attention.rs); these calls keep a decoder layer on the device between its qkv
  * and o projections.  Keys and values are quantized like the activations, one scale per token and KV head:
@@ -360,6 +417,9 @@ int qlin_chain_status(qlin_chain* chain, int32_t clear);
  * each operation one f32 rounding and 1/127 the nearest f32 (the scale is within one f32 step of the quotient).
  * A row with Inf or NaN gets the scale NaN (whoever reads it gets NaN) and sets
  * QLIN_ERR_NONFINITE in the workspace's error word.
+ * In 4 bits every 32 columns g of a row have a unit of their own, a whole number, beside the row's scale:
+ *   s = max(absmax_d |x[d]| * (1/1785), 2^-64),  u[g] = clamp(ceil(absmax_{d in g} |x[d]| * (1/s) * (1/7)), 1, 255)
+ *   code[d] = clamp(round(x[d] * (1/(u[g] * s))), -7, 7),  read as code[d] * u[g] * s
  *
  * Tokens lie in pages of page_tokens; a sequence's tokens p .. p + page_tokens - 1 are the page named
  * by column p / page_tokens of its row of the page table.  Who owns which page is the caller's
@@ -410,6 +470,10 @@ typedef struct qlin_kv_batch {
 
 /* Geometry outside the limits above: QLIN_ERR_UNSUPPORTED.  Rows never written read as zeros. */
 int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out);
+/* The same in 8 or 4 bits (else QLIN_ERR_PARAM).  A token and KV head of 128 columns take 264 bytes in 8 bits, 144 in 4.  All
+ * calls below take either. */
+int qlin_kv_create_bits(const qlin_kv_config* config, int32_t bits, qlin_kv_cache** out);
+int32_t qlin_kv_bits(const qlin_kv_cache* cache); /* 8 or 4 */
 void qlin_kv_free(qlin_kv_cache* cache);
 int qlin_kv_query(const qlin_kv_cache* cache, qlin_kv_info* out);
 
@@ -419,7 +483,17 @@ int qlin_kv_query(const qlin_kv_cache* cache, qlin_kv_info* out);
 int qlin_kv_append(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const void* K,
                    int64_t ldk, const void* V, int64_t ldv, int32_t dtype, uint32_t flags, void* stream);
 
-/* Reads the same rows back: x[d] = code[d] * s, one f32 rounding, then dtype. */
+/* From the rows of the qkv projection into the cache in one pass: what qlin_rope_run_norm makes of queries and keys, each row
+ * at its token's place, and qlin_kv_append of the keys (not rounded in between) and of the values.  QKV: device [rows, ld] of dtype,
+ * q_heads (1..1024) query heads of head_dim columns, then the cache's key heads, then as many value heads.  Q: device
+ * [rows, ldq] of q_dtype gets the query heads; it may be QKV with the same type and stride, else they must not overlap.
+ * rope NULL: nothing is turned; q_gamma, k_gamma NULL: not normalized.  flags: QLIN_ROUND_HALF_EVEN.  At most 2^24 - 1
+ * seqs * max_new.  Where row starts at fault give two sequences a row, its queries are either's. */
+int qlin_kv_append_qkv(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const qlin_rope* rope,
+                       int32_t q_heads, const float* q_gamma, const float* k_gamma, float eps, const void* QKV,
+                       int32_t dtype, int64_t ld, void* Q, int32_t q_dtype, int64_t ldq, uint32_t flags, void* stream);
+
+/* Reads the same rows back: x[d] = code[d] * s (code[d] * u[g] * s), one f32 rounding, then dtype. */
 int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K,
                  int64_t ldk, void* V, int64_t ldv, int32_t dtype, void* stream);
 
@@ -429,7 +503,7 @@ int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_b
  * Q: device [rows, ldq] of q_dtype, query head h in columns h * head_dim ..; q_heads is a multiple of
  * kv_heads, and KV head h serves query heads h * q_heads / kv_heads ..  O: device [rows, ldo] of
  * o_dtype; it must not overlap Q.  scale: finite, up to 2^64 either way (else QLIN_ERR_UNSUPPORTED); where its product
- * with a row's largest |Q|, or with the largest |K| in sight, passes 2^110, results may be NaN.
+ * with a row's largest |Q|, or with the largest |K| in sight, passes 2^110 (4 bits: 2^106), results may be NaN.
  * Sums and the softmax are held in f32.  Queries and probabilities (scaled into fp16's range) are kept to 22 bits, fp16
  * queries exactly; but with fp16 rows in and out, where max_new * q_heads / kv_heads (of the prefix: rows * q_heads /
  * kv_heads) passes 256, probabilities are rounded to fp16 before they meet V, on top of the output's own
@@ -451,6 +525,45 @@ int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, con
                              int32_t prefix_tokens, const int32_t* prefix_pages, int32_t q_heads,
                              const void* Q, int32_t q_dtype, int64_t ldq, float scale, void* O,
                              int32_t o_dtype, int64_t ldo, void* stream);
+
+/* ---- tables of a serving step, on the device ----
+ * From what the requests of a step ask for to the arrays of its qlin_kv_batch, with pages from a free list, without the host:
+ * a captured step can be replayed while lengths, tables and list live on the device.  Slot i holds length[i] tokens;
+ *   change[i] > 0: so many more (the new rows), change[i] < 0: so many fewer, from the end (drafted tokens that were refused; at
+ *   least length[i] ends the request), 0: an idle slot.
+ * First pages that no token is left on go back on top of the free list, slot after slot, columns rising, and their table
+ * entries become -1.  Then slots are served in their order, each wholly or not at all: one is refused where change[i] > max_new,
+ * its length would pass max_len, the rows asked for by the slots up to it pass `rows`, or it needs pages and those needed by the slots up to it
+ * (of those not refused before) pass the list.  A refused slot stays as it is and has no rows.  Pages come from the top of the
+ * list (what they leave there stays), slot after slot, columns rising.
+ * The arrays must not overlap each other.  The call takes the cache's page size and number of pages only; it is a
+ * workspace call like the others, which allocates nothing and can be captured.
+ * A length below 0 or above max_len (that slot is left alone), a free count outside 0 .. pages (taken as the nearer of
+ * the two), more pages given back than there are, or an id outside the cache set QLIN_ERR_PARAM in the workspace's error
+ * word; no such value is followed out of a buffer, but which pages belong to whom is then unspecified.  That no page is
+ * in the list or the tables twice is the caller's business. */
+typedef struct qlin_kv_tables {
+    int32_t seqs;          /* slots, 1..2^20; seqs * ceil(max_len / page_tokens) up to 2^30 */
+    int32_t rows;          /* rows there is room for, 0..2^24 */
+    int32_t max_new;       /* of one slot; what a later qlin_kv_batch is given */
+    int32_t max_len;       /* up to 2^30 */
+    int32_t prefix_tokens; /* a multiple of page_tokens, up to max_len: pages of these first tokens are shared, neither taken
+                            * nor given back, and their columns not written */
+    int32_t reserved;
+    const int32_t* change; /* device [seqs] */
+    int32_t* length;       /* device [seqs], in and out */
+    int32_t* page_table;   /* device [seqs, page_ld], in and out */
+    int64_t page_ld;       /* at least ceil(max_len / page_tokens) */
+    int32_t* free_pages;   /* device [pages of the cache], the first free_count of them free */
+    int32_t* free_count;   /* device [1], in and out */
+    int32_t* row_start;    /* device [seqs + 1], out */
+    /* out, each may be NULL.  Entries of rows behind the last are left as they are. */
+    int32_t* row_seq;   /* device [rows]: whose row it is */
+    int32_t* positions; /* device [rows]: its token's place */
+    int64_t* slots;     /* device [rows]: page * page_tokens + the place in it */
+    int32_t* refused;   /* device [1]: slots that asked for rows and have none */
+} qlin_kv_tables;
+int qlin_kv_step(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_tables* tables, void* stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,15 @@ QLIN_NORM_SEQUENTIAL = 0x2
 QLIN_SWIGLU = 0x4
 QLIN_NO_FUSED_QUANT = 0x8
 QLIN_RESIDUAL = 0x10
+QLIN_ROPE_INVERSE = 0x20
+
+QLIN_ROPE_HALF = 0
+QLIN_ROPE_INTERLEAVED = 1
+QLIN_ROPE_PLAIN = 0
+QLIN_ROPE_LINEAR = 1
+QLIN_ROPE_BASE = 2
+QLIN_ROPE_BANDS = 3
+QLIN_ROPE_RAMP = 4
 
 QLIN_PATH_GEMV_FUSED = 0
 QLIN_PATH_GEMV = 1
@@ -79,7 +88,17 @@ SIGNATURES = {
     "qlin_run_noalloc": (ctypes.c_int, [_P, _I32, _P, _I32, _I64, _P, _F, _P, _I32, _I64, _U32, _P, _P]),
     "qlin_swiglu": (ctypes.c_int, [_I32, _I32, _P, _I32, _I64, _P, _I32, _I64, _P]),
     "qlin_run_plan": (ctypes.c_int, [_P, _P, _I32, _P, _I64, _P, _U32, _P]),
+    "qlin_rope_create": (ctypes.c_int, [_P, _P]),
+    "qlin_rope_free": (None, [_P]),
+    "qlin_rope_query": (ctypes.c_int, [_P, _P, _P]),
+    "qlin_rope_run": (ctypes.c_int, [_P, _I32, _I32, _P, _I32, _I64, _P, _P, _I32, _I64, _U32, _P]),
+    "qlin_rope_run_norm": (ctypes.c_int, [_P, _I32, _I32, _I32, _I32, _P, _P, _F, _P, _I32, _I64, _P, _P, _I32, _I64, _U32,
+                                          _P]),
     "qlin_kv_create": (ctypes.c_int, [_P, _P]),
+    "qlin_kv_create_bits": (ctypes.c_int, [_P, _I32, _P]),
+    "qlin_kv_bits": (_I32, [_P]),
+    "qlin_kv_append_qkv": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _F, _P, _I32, _I64, _P, _I32, _I64, _U32, _P]),
+    "qlin_kv_step": (ctypes.c_int, [_P, _P, _P, _P]),
     "qlin_kv_free": (None, [_P]),
     "qlin_kv_query": (ctypes.c_int, [_P, _P]),
     "qlin_kv_append": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _I64, _I32, _U32, _P]),
@@ -131,6 +150,20 @@ class KVInfo(ctypes.Structure):
 class KVBatch(ctypes.Structure):
     _fields_ = [("seqs", _I32), ("rows", _I32), ("max_new", _I32), ("max_len", _I32), ("row_start", _P),
                 ("length", _P), ("page_table", _P), ("page_ld", _I64)]
+
+
+class KVTables(ctypes.Structure):
+    _fields_ = [("seqs", _I32), ("rows", _I32), ("max_new", _I32), ("max_len", _I32), ("prefix_tokens", _I32),
+                ("reserved", _I32), ("change", _P), ("length", _P), ("page_table", _P), ("page_ld", _I64),
+                ("free_pages", _P), ("free_count", _P), ("row_start", _P), ("row_seq", _P), ("positions", _P),
+                ("slots", _P), ("refused", _P)]
+
+
+class RopeConfig(ctypes.Structure):
+    _fields_ = [("head_dim", _I32), ("rotary_dim", _I32), ("first", _I32), ("layout", _I32), ("scaling", _I32),
+                ("reserved", _I32), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("original_len", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("amplitude", ctypes.c_double)]
 
 
 class QlinError(RuntimeError):

@@ -48,7 +48,8 @@ COMMON = [
 FILE_FLAGS = {"qlin_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "qlin_gemm_ks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "qlin_gemm_pp.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-              "qlin_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+              "qlin_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "qlin_attend4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 ROOT = os.path.dirname(HERE)
 TEST_SRC = os.path.join(ROOT, "tests", "cpp", "npu_backend_test.cpp")
@@ -58,6 +59,8 @@ HOST_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "host_calls_test.cpp")
 HOST_TEST_BIN = os.path.join(TEST_BUILD, "host_calls_test")
 KV_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "kv_calls_test.cpp")
 KV_TEST_BIN = os.path.join(TEST_BUILD, "kv_calls_test")
+STEP_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "step_calls_test.cpp")
+STEP_TEST_BIN = os.path.join(TEST_BUILD, "step_calls_test")
 STATIC_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "static_link_test.c")
 STATIC_TEST_BIN = os.path.join(TEST_BUILD, "static_link_test")
 
@@ -118,7 +121,7 @@ def build_calib() -> str:
 
 def build_tests() -> str:
     """Native tests: the npu mirror (its checker, the CPU oracle, is compiled in), the host side
-    of the host-buffer and key/value cache calls and the static archive."""
+    of the host-buffer, key/value cache and serving step calls and the static archive."""
     os.makedirs(TEST_BUILD, exist_ok=True)
     oracle_obj = os.path.join(TEST_BUILD, "qlin_oracle.o")
     subprocess.run(["gcc", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-std=c11", "-c",
@@ -126,7 +129,7 @@ def build_tests() -> str:
     subprocess.run(["g++", "-O2", "-std=c++17", "-ffp-contract=off", TEST_SRC, oracle_obj, "-o", TEST_BIN,
                     f"-L{HERE}", "-lqlinear", "-Wl,-rpath,$ORIGIN/../../../open_rknpu2_lm_infer_amd", "-lm"], check=True)
     # their own definitions of the HIP calls take the place of the runtime's
-    for src, exe in ((HOST_TEST_SRC, HOST_TEST_BIN), (KV_TEST_SRC, KV_TEST_BIN)):
+    for src, exe in ((HOST_TEST_SRC, HOST_TEST_BIN), (KV_TEST_SRC, KV_TEST_BIN), (STEP_TEST_SRC, STEP_TEST_BIN)):
         subprocess.run(["g++", "-O1", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", src, "-o", exe,
                         "-rdynamic", "-pthread", f"-L{HERE}", "-lqlinear",
                         "-Wl,-rpath,$ORIGIN/../../../open_rknpu2_lm_infer_amd"], check=True)

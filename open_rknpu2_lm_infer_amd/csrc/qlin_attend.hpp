@@ -1,4 +1,4 @@
-// Parts that the attention kernels share: exact fp16 codes from the cache's bytes, query rows, output rows.
+// Parts that the attention kernels share: exact fp16 codes from the cache's bytes or nibbles, query rows, output rows.
 #pragma once
 
 #include "qlin_kv.hpp"
@@ -26,13 +26,43 @@ __device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t se
     const half2v m = {(_Float16)32768.0f, (_Float16)32768.0f}, a = {(_Float16)-0.25f, (_Float16)-0.25f};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, m, a));
 }
-constexpr float kCodeUnit = 512.0f;  // 1 / 2^-9
+// What codes are worth in the matrix core's operands: 2^-9 in 8 bits, and 2^-13 for a code times its unit in 4.
+template <int BITS>
+constexpr float kCodeUnit = BITS == 8 ? 512.0f : 8192.0f;
 
 // Eight codes of consecutive columns, bytes of (w0, w1).
 __device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
     const uint4v r = {codes2(w0, w0, 0x0c010c00u), codes2(w0, w0, 0x0c030c02u), codes2(w1, w1, 0x0c010c00u),
                       codes2(w1, w1, 0x0c030c02u)};
     return __builtin_bit_cast(half8v, r);
+}
+
+// 4 bits: a nibble (code + 8) in bits 4..7 of a half is n * 2^-20, times unit * 2^7 less unit * 2^-10 it is
+// code * unit * 2^-13.  Both factors and the result (up to 7 * 255, 11 bits, at least 2^-13) are exact in fp16, so a unit
+// costs nothing but these factors of it.
+struct Unit2 {
+    half2v m, a;
+};
+// Units of bytes i and j of w that sel (0x04000400 | j << 16 | i with 4 for the constant's bytes) picks: 0x6400 | u is 1024 + u.
+__device__ __forceinline__ Unit2 units2(uint32_t w, int i, int j) {
+    const half2v k = {(_Float16)1024.0f, (_Float16)1024.0f}, up = {(_Float16)128.0f, (_Float16)128.0f},
+                 down = {(_Float16)-0x1p-10f, (_Float16)-0x1p-10f};
+    const half2v u = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04000400u | (uint32_t)j << 16 | (uint32_t)i)) - k;
+    return {u * up, u * down};
+}
+__device__ __forceinline__ uint32_t nibbles2(uint32_t at4, const Unit2& u) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, at4 & 0x00f000f0u), u.m, u.a));
+}
+// Eight codes of consecutive columns, nibbles of w, in the order that the halves of a word give them: columns
+// 0 4 1 5 2 6 3 7.  Queries are laid out alike (operand_column).
+__device__ __forceinline__ half8v nibbles8(uint32_t w, const Unit2& u) {
+    const uint4v r = {nibbles2(w << 4, u), nibbles2(w, u), nibbles2(w >> 4, u), nibbles2(w >> 8, u)};
+    return __builtin_bit_cast(half8v, r);
+}
+// Which of eight consecutive columns is element i of a key's operand.
+template <int BITS>
+__host__ __device__ constexpr int operand_column(int i) {
+    return BITS == 8 ? i : i % 2 * 4 + i / 2;
 }
 
 // The running maximum of a vector is raised only when a token passes it by more than this (bits): most
@@ -47,17 +77,17 @@ __device__ __forceinline__ void split_f16(float x, _Float16 out[LIMBS]) {
     if constexpr (LIMBS == 2) out[1] = (_Float16)(x - (float)out[0]);
 }
 
-// Columns of a query row on their way to the matrix core: KS groups of eight as they lie in memory, two
-// (PAIR: one 16-byte chunk of a key's bytes) or one at column first and every STEP columns; columns past the
+// Columns of a query row on their way to the matrix core: KS groups of eight as they lie in memory, RUN of them side by
+// side (one load of a key's bytes) at column first and every STEP columns; columns past the
 // head's are zeros.  All loads are issued before any is used.
 template <int KS, bool Q16>
 struct QueryRow {
     uint4v w[KS][Q16 ? 1 : 2];
 };
-template <int KS, int STEP, bool PAIR, bool Q16>
+template <int KS, int STEP, int RUN, bool Q16>
 __device__ __forceinline__ void load_query(const AttendParams& p, QueryRow<KS, Q16>& r, int64_t at, int first) {
     constexpr int W = Q16 ? 1 : 2;
-    auto column = [](int k) { return PAIR ? k / 2 * STEP + k % 2 * 8 : k * STEP; };
+    auto column = [](int k) { return k / RUN * STEP + k % RUN * 8; };
     if (p.q_vec) {  // heads of whole groups of 8, 16-byte aligned
         const uint8_t* q = reinterpret_cast<const uint8_t*>(p.q) + (at + first) * (2 * W);
 #pragma unroll
@@ -121,39 +151,44 @@ __device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int
 
 template <int N>
 struct Bytes {
-    uint32_t w[N / 4];
+    uint32_t w[(N + 3) / 4];
 };
 
 typedef const __attribute__((address_space(4))) int32_t* const_ids;
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
 // Where a wave finds 16 tokens: the block of their page and head as a buffer, and the offsets of their keys,
-// values and scales.  An id outside the cache leads to page 0 (bad); a group that is not there is a
+// values, scales and, in 4 bits, of the units of their columns' first group (the next one's are a page's tokens
+// further).  An id outside the cache leads to page 0 (bad); a group that is not there is a
 // buffer of no bytes, which reads without an access.
-template <int DP>
+template <int DP, int BITS>
 struct Half16 {
     __amdgpu_buffer_rsrc_t block;
-    int k, v, ks, vs;
+    int k, v, ks, vs, ku, vu;
     bool bad;
 };
-template <int DP>
-__device__ __forceinline__ Half16<DP> find_half(const KvCache& c, int id, int head, int off, bool there) {
-    Half16<DP> x;
+template <int DP, int BITS>
+__device__ __forceinline__ Half16<DP, BITS> find_half(const KvCache& c, int id, int head, int off, bool there) {
+    constexpr int ROW = DP * BITS / 8;
+    Half16<DP, BITS> x;
     x.bad = false;
-    const int page = kv_page(id, c.pages, &x.bad), values = DP << c.shift, bytes = (2 * DP + 8) << c.shift;
+    const int page = kv_page(id, c.pages, &x.bad), values = ROW << c.shift, bytes = (int)kv_block_bytes(BITS, DP, c.shift);
     x.block = __builtin_amdgcn_make_buffer_rsrc(c.data + ((int64_t)page * c.heads + head) * bytes, (short)0,
                                                 there ? bytes : 0, 0x00027000);  // raw, 32-bit elements
-    x.k = off * DP;
-    x.v = values + off * DP;
+    x.k = off * ROW;
+    x.v = values + off * ROW;
     x.ks = 2 * values + 4 * off;
     x.vs = x.ks + (4 << c.shift);
+    x.ku = 2 * values + (8 << c.shift) + off;
+    x.vu = x.ku + (DP / kKvGroup << c.shift);
     return x;
 }
 
-// N bytes of a buffer, at a lane's offset from `from` on: up to 16 of them, or 16 every STEP.
+// N bytes of a buffer, at a lane's offset from `from` on: up to 16 of them, or 16 every STEP.  Two are the low ones of a word.
 template <int N, int STEP>
 __device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at, int from) {
-    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
+    if constexpr (N == 2) r.w[0] = __builtin_amdgcn_raw_buffer_load_b16(b, at, from, 0);
+    else if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
     else if constexpr (N == 8) {
         const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, from, 0));
         r.w[0] = x[0];

@@ -1,4 +1,5 @@
-// Attention of new rows over the 8-bit key/value cache.
+// Attention of new rows over the key/value cache: the kernel for few vectors and the joins, for one width of the cache
+// (qlin_attend.hip: 8 bits, qlin_attend4.hip: 4).
 //
 //   l_j = scale * s^K_j * (q . k_j)          j = the tokens a row sees (itself and before)
 //   o   = sum_j e^(l_j) s^V_j v_j / sum_j e^(l_j),   no token: 0
@@ -22,19 +23,28 @@
 // waves' join (300 tokens: 7.8 us).  A prefix of 8192 tokens for 32 rows, 128 vectors a KV head in tiles of 32, takes 21.7 us
 // with the rows' own tokens: the vector units' exponents and byte permutes (31% of their time) and waits (42%), with
 // one wave a SIMD.
+//
+// In 4 bits a code times its group's unit takes the code's place; it is as exact, and all else is the same.
+#pragma once
+
 #include "qlin_attend.hpp"
 
 namespace qlin {
 namespace {
 
 // What a wave loads for one step of 32 tokens: two tiles of 16.  Lane l (n = l % 16, g = l / 16)
-// holds, as the matrix core's A operand, columns 64 c + 16 g .. + 15 of key n of each tile (a load covers 64
-// bytes of each of 16 keys), and columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
-template <int DP>
+// holds, as the matrix core's A operand, columns of key n of each tile, RUN groups of eight side by side (8 bits: columns
+// 64 c + 16 g .. + 15, a load covers 64 bytes of each of 16 keys; 4 bits: 128 c + 32 g .. + 31 in as many bytes, or
+// 16 g .. + 15 of heads of 64), and columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
+template <int DP, int BITS>
 struct StepData {
-    Bytes<DP / 4> k[2];
-    Bytes<DP / 16> v[8];
+    static constexpr int KB = DP / 4 * BITS / 8, VB = DP / 16 * BITS / 8;  // bytes
+    static constexpr int RUN = KB < 16 ? DP / 32 : 16 / BITS;
+    static constexpr int KU = DP == 256 ? 2 : 1;  // groups of 32 columns that a lane's keys lie in
+    Bytes<KB> k[2];
+    Bytes<VB> v[8];
     float4v ks[2], vs[2];  // scales of tokens 4g .. 4g + 3
+    uint32_t ku[2][KU], vu[2];  // 4 bits: units of key n, and of values 4g .. 4g + 3, a byte each
 };
 
 // Sum and maximum over the four lanes n, n + 16, n + 32, n + 48.
@@ -61,8 +71,10 @@ struct AttendLds {
     float m[4][16 * R], l[4][16 * R];
     int seen[16 * R], most;  // SHARED: tokens that each vector sees, the most of them
 };
-template <int DP, int R, bool Q16, bool SHARED>
+template <int DP, int BITS, int R, bool Q16, bool SHARED>
 __device__ __forceinline__ void attend_part(const AttendParams& p, int block, AttendLds<DP, R>& lds) {
+    using Step = StepData<DP, BITS>;
+    constexpr int ROW = DP * BITS / 8;  // bytes of a key
     constexpr int KS = DP / 32;   // matrix steps of a q . k
     constexpr int DT = DP / 16;   // tiles of 16 output columns
     constexpr int VT = 16 * R;    // vectors of the workgroup
@@ -130,7 +142,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         const int v = seen[r] >= 0 ? v0 + 16 * r + n : 0;
         out_row[r] = first_row + p.group.div(v);
         head[r] = h * group + p.group.mod(v);
-        load_query<KS, 64, true, Q16>(p, qr[r], out_row[r] * p.ldq + (int64_t)head[r] * p.c.dim, 16 * g);
+        load_query<KS, 32 * Step::RUN, Step::RUN, Q16>(p, qr[r], out_row[r] * p.ldq + (int64_t)head[r] * p.c.dim, 8 * Step::RUN * g);
     }
 
     // page ids through the scalar cache: nothing writes them while the kernel runs
@@ -138,21 +150,27 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false, bad[2] = {false, false};  // of a tile: who sees none of its tokens keeps its result
-    StepData<DP> d;
-    Half16<DP> next[2];
+    Step d;
+    Half16<DP, BITS> next[2];
     auto find_step = [&](int j) {  // end > 0
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int jt = j + 16 * t, jj = min(jt, end - 1);
             const int id = (SHARED || jj < p.prefix ? prefix : table)[jj >> p.c.shift];
-            next[t] = find_half<DP>(p.c, id, h, jt & off_mask, jt < end);
+            next[t] = find_half<DP, BITS>(p.c, id, h, jt & off_mask, jt < end);
             next[t].bad = next[t].bad && jt < end;
             bad_page |= next[t].bad;
         }
     };
     auto load_k = [&] {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) load_bytes<DP / 4, 64>(d.k[t], next[t].block, n * DP + 16 * g, next[t].k);
+        for (int t = 0; t < 2; ++t) {
+            load_bytes<Step::KB, 64>(d.k[t], next[t].block, n * ROW + (Step::KB < 16 ? Step::KB : 16) * g, next[t].k);
+            if constexpr (BITS == 4)
+#pragma unroll
+                for (int c = 0; c < Step::KU; ++c)
+                    d.ku[t][c] = __builtin_amdgcn_raw_buffer_load_b8(next[t].block, n + (((DP == 64 ? g / 2 : g) + 4 * c) << p.c.shift), next[t].ku, 0);
+        }
     };
     auto load_scales = [&] {
 #pragma unroll
@@ -164,7 +182,11 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     };
     auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_bytes<DP / 16, 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * DP + n * (DP / 16), next[i / 4].v);
+        for (int i = 0; i < 8; ++i) load_bytes<Step::VB, 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * ROW + n * Step::VB, next[i / 4].v);
+        if constexpr (BITS == 4)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                d.vu[t] = __builtin_amdgcn_raw_buffer_load_b32(next[t].block, 4 * g + (n * (DP / 16) / kKvGroup << p.c.shift), next[t].vu, 0);
     };
     int j = j0 + 32 * wave;
     if (end > 0) {
@@ -174,12 +196,12 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         load_v();
     }
 
-    // queries, as the B operand: lane (n, g) holds columns 64 c + 16 g .. + 15 of vector n, two matrix steps each
+    // queries, as the B operand: lane (n, g) holds the columns of vector n that it holds of a key, eight a matrix step
     half8v qf[R][KS][QL];
     float unit[R];  // what the f16 operands were divided by, times scale2
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        unit[r] = p.scale2 * kCodeUnit;
+        unit[r] = p.scale2 * kCodeUnit<BITS>;
         float x[DP / 4];
 #pragma unroll
         for (int i = 0; i < DP / 4; ++i) x[i] = query_at<KS, Q16>(qr[r], i / 8, i % 8);
@@ -200,7 +222,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 _Float16 y[QL];
-                split_f16<QL>(x[8 * k + i], y);
+                split_f16<QL>(x[8 * k + operand_column<BITS>(i)], y);
 #pragma unroll
                 for (int q = 0; q < QL; ++q) qf[r][k][q][i] = y[q];
             }
@@ -228,7 +250,9 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
             for (int r = 0; r < R; ++r) sc[t][r] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const half8v a = codes8(d.k[t].w[2 * k], d.k[t].w[2 * k + 1]);
+                half8v a;
+                if constexpr (BITS == 8) a = codes8(d.k[t].w[2 * k], d.k[t].w[2 * k + 1]);
+                else a = nibbles8(d.k[t].w[k], units2(d.ku[t][k / 4], 0, 0));
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -289,11 +313,26 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
         __builtin_amdgcn_sched_barrier(0);
         load_scales();
         // O^T: columns n * DP/16 + t (row n of the operand) over tokens 4g + i of both tiles
+        Unit2 vu[4];
+        if constexpr (BITS == 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vu[i] = units2(d.vu[i / 2], i % 2 * 2, i % 2 * 2 + 1);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            const uint32_t lo = t & 3, sel = 0x0c000c00u | (4 + lo) << 16 | lo;
-            const uint4v w = {codes2(d.v[1].w[t / 4], d.v[0].w[t / 4], sel), codes2(d.v[3].w[t / 4], d.v[2].w[t / 4], sel),
-                              codes2(d.v[5].w[t / 4], d.v[4].w[t / 4], sel), codes2(d.v[7].w[t / 4], d.v[6].w[t / 4], sel)};
+            uint4v w;
+            if constexpr (BITS == 8) {
+                const uint32_t lo = t & 3, sel = 0x0c000c00u | (4 + lo) << 16 | lo;
+                w = uint4v{codes2(d.v[1].w[t / 4], d.v[0].w[t / 4], sel), codes2(d.v[3].w[t / 4], d.v[2].w[t / 4], sel),
+                           codes2(d.v[5].w[t / 4], d.v[4].w[t / 4], sel), codes2(d.v[7].w[t / 4], d.v[6].w[t / 4], sel)};
+            } else {
+                // the byte of columns t and t ^ 1 of two tokens, then its lower or upper nibble
+                const uint32_t at = t / 2 % 4, sel = 0x0c000c00u | (4 + at) << 16 | at;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t y = __builtin_amdgcn_perm(d.v[2 * i + 1].w[t / 8], d.v[2 * i].w[t / 8], sel);
+                    w[i] = nibbles2(t % 2 ? y : y << 4, vu[i]);
+                }
+            }
             const half8v a = __builtin_bit_cast(half8v, w);
 #pragma unroll
             for (int r = 0; r < R; ++r)
@@ -367,7 +406,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     for (int r = 0; r < R; ++r) {
         if (seen[r] < 0) continue;
         if (p.parts == 1) {
-            const float f = l_all[r] == 0.0f ? 0.0f : kCodeUnit / l_all[r];
+            const float f = l_all[r] == 0.0f ? 0.0f : kCodeUnit<BITS> / l_all[r];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -393,7 +432,7 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 
 // A launch: the first `shared` workgroups work on the prefix with RS tiles (0: there is none), the others on the
 // sequences' own tokens with RO.
-template <int DP, int RS, int RO, bool Q16>
+template <int DP, int BITS, int RS, int RO, bool Q16>
 __global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 64 ? 4 : DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 128 ? 3 : 1)
 void attend_kernel(AttendParams p, int shared) {
     __shared__ union {
@@ -402,18 +441,18 @@ void attend_kernel(AttendParams p, int shared) {
     } lds;
     if constexpr (RS > 0) {
         if ((int)blockIdx.x < shared) {
-            attend_part<DP, RS, Q16, true>(p, blockIdx.x, lds.prefix);
+            attend_part<DP, BITS, RS, Q16, true>(p, blockIdx.x, lds.prefix);
             return;
         }
     }
-    attend_part<DP, RO, Q16, false>(p, blockIdx.x - shared, lds.own);
+    attend_part<DP, BITS, RO, Q16, false>(p, blockIdx.x - shared, lds.own);
 }
 
 // Joins the parts of vectors: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes hold a vector's
 // columns, four each.  MANY parts: a workgroup per vector, its groups of lanes take the parts in turn
 // and are joined in the LDS.  Few: a group per vector.  Maxima and outputs of four parts are loaded together
 // and the maximum runs along: what is short here is the chain of loads (sequence, parts), not their bytes.
-template <int DP, bool MANY>
+template <int DP, int BITS, bool MANY>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     constexpr int LPV = DP / 4, GROUPS = 256 / LPV, STEP = MANY ? GROUPS : 1;
     __shared__ __align__(16) float lds_o[MANY ? GROUPS : 1][DP];
@@ -477,62 +516,43 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
             for (int c = 0; c < 4; ++c) o[c] = __builtin_fmaf(f, z[c], o[c]);
         }
     }
-    const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
+    const float f = l == 0.0f ? 0.0f : kCodeUnit<BITS> / l;
     const float y[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
     store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, d, y);
 }
 
-// Vectors of a workgroup, given how many share its tokens: one or two tiles here (two of 256 columns would
-// not fit the registers), or the wide kernel's.  That one reads a token's bytes once for 128 vectors but
-// waits at a barrier for every 32 tokens: with up to 256 vectors (512 where rows are f32 in or out) more workgroups of
-// this one are faster.  One sequence, 4096 tokens, 8 KV heads, us here and there:
-//   vectors           256          384          512          768         1024
-//   fp16, 64       17.0 / 23.5  25.5 / 24.3  24.4 / 27.9  33.6 / 32.1  34.4 / 32.9
-//   fp16, 128      21.6 / 32.3  34.1 / 34.7  30.9 / 37.8  45.7 / 46.9  48.4 / 46.5
-//   fp16, 256      30.6 / 43.8  51.5 / 60.3  53.2 / 68.6  75.5 / 80.4  96.2 / 93.1
-//   f32, 128       23.9 / 38.3  38.5 / 42.0  33.8 / 46.7  50.9 / 57.9  53.9 / 62.2
-//   prefix, fp16   24.9 / 35.7  36.3 / 41.2  35.4 / 47.6  48.4 / 54.5  57.3 / 65.1   (128 columns)
-//   prefix, f32    26.4 / 43.5  40.4 / 54.2  39.0 / 58.6  54.6 / 75.9  64.1 / 87.3
-// What a batch holds beside that moves the crossing, and the limit on vectors alone is a middle: of 257 to 512 fp16 vectors
-// in 36 random batches of 1 to 16 sequences this kernel takes 0.83 of the other's time on average, half of it for one
-// sequence of a few hundred tokens, 1.35 of it for one of 15000 tokens and up to 1.85 for 16 sequences.
-int tile_of(const AttendParams& p, int64_t vectors) {
-    if (vectors > (p.q_f16 && p.o_f16 ? 256 : 512)) return kAttendWide;
-    return vectors <= 16 || p.c.dim_padded > 128 ? 16 : 32;
-}
-
-template <int DP, bool Q16>
+template <int DP, int BITS, bool Q16>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     const int own = attend_tile(p), shared = p.prefix_parts ? attend_tile_prefix(p) : 0;
     const uint32_t own_blocks = (uint32_t)((p.parts - p.prefix_parts) * (int64_t)p.b.seqs * p.c.heads * p.by_tiles.d);
     const uint32_t shared_blocks = (uint32_t)(p.prefix_parts * (int64_t)p.c.heads * p.by_prefix_tiles.d);
     if (shared >= kAttendWide)
-        if (hipError_t e = launch_attend_wide(p, true, st)) return e;
-    if (own >= kAttendWide) return launch_attend_wide(p, false, st);
+        if (hipError_t e = launch_attend_wide<BITS>(p, true, st)) return e;
+    if (own >= kAttendWide) return launch_attend_wide<BITS>(p, false, st);
     const uint32_t first = shared >= kAttendWide ? 0 : shared_blocks;
     const dim3 grid(first + own_blocks);
     if (first == 0) {
         if constexpr (DP <= 128)
             if (own == 32) {
-                attend_kernel<DP, 0, 2, Q16><<<grid, 256, 0, st>>>(p, 0);
+                attend_kernel<DP, BITS, 0, 2, Q16><<<grid, 256, 0, st>>>(p, 0);
                 return hipGetLastError();
             }
-        attend_kernel<DP, 0, 1, Q16><<<grid, 256, 0, st>>>(p, 0);
+        attend_kernel<DP, BITS, 0, 1, Q16><<<grid, 256, 0, st>>>(p, 0);
         return hipGetLastError();
     }
     if constexpr (DP <= 128) {  // the prefix's rows are those of all sequences: at least as many
-        if (own == 32) attend_kernel<DP, 2, 2, Q16><<<grid, 256, 0, st>>>(p, first);
-        else if (shared == 32) attend_kernel<DP, 2, 1, Q16><<<grid, 256, 0, st>>>(p, first);
-        else attend_kernel<DP, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        if (own == 32) attend_kernel<DP, BITS, 2, 2, Q16><<<grid, 256, 0, st>>>(p, first);
+        else if (shared == 32) attend_kernel<DP, BITS, 2, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        else attend_kernel<DP, BITS, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
     } else {
-        attend_kernel<DP, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        attend_kernel<DP, BITS, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
     }
     return hipGetLastError();
 }
 
-template <int DP>
+template <int DP, int BITS>
 hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
-    const hipError_t e = p.q_f16 ? launch_typed<DP, true>(p, st) : launch_typed<DP, false>(p, st);
+    const hipError_t e = p.q_f16 ? launch_typed<DP, BITS, true>(p, st) : launch_typed<DP, BITS, false>(p, st);
     if (e != hipSuccess || p.parts == 1) return e;
     // few parts: fewer than the groups of lanes a workgroup has for them
     AttendParams j = p;
@@ -540,21 +560,19 @@ hipError_t launch_dp(const AttendParams& p, hipStream_t st) {
     const bool many = p.parts >= groups;
     const int64_t blocks = many ? vectors : (vectors + groups - 1) / groups;
     j.by_join = fast_div((int)blocks);
-    if (many) attend_join_kernel<DP, true><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
-    else attend_join_kernel<DP, false><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
+    if (many) attend_join_kernel<DP, BITS, true><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
+    else attend_join_kernel<DP, BITS, false><<<dim3((uint32_t)(blocks * p.b.seqs)), 256, 0, st>>>(j);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int attend_tile(const AttendParams& p) { return tile_of(p, (int64_t)p.b.max_new * p.group.d); }
-int attend_tile_prefix(const AttendParams& p) { return tile_of(p, (int64_t)p.b.rows * p.group.d); }
-
-hipError_t launch_attend(const AttendParams& p, hipStream_t st) {
+template <int BITS>
+hipError_t launch_attend_bits(const AttendParams& p, hipStream_t st) {
     switch (p.c.dim_padded) {
-        case 64: return launch_dp<64>(p, st);
-        case 128: return launch_dp<128>(p, st);
-        default: return launch_dp<256>(p, st);
+        case 64: return launch_dp<64, BITS>(p, st);
+        case 128: return launch_dp<128, BITS>(p, st);
+        default: return launch_dp<256, BITS>(p, st);
     }
 }
 

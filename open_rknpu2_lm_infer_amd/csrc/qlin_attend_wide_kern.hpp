@@ -1,5 +1,6 @@
-// Attention of many rows over the 8-bit key/value cache: prompts, chunks of prompts, and the shared
-// prefix of a batch.  The formulas are those of qlin_attend.hip.
+// Attention of many rows over the key/value cache: prompts, chunks of prompts, and the shared
+// prefix of a batch, for one width of the cache (qlin_attend_wide.hip: 8 bits, qlin_attend_wide4.hip: 4).  The formulas are
+// those of qlin_attend_kern.hpp.
 //
 // A workgroup holds 128 vectors, 32 a wave, and walks over its tokens 32 at a time.  The
 // bytes of a tile are loaded two tiles ahead, made into fp16 codes once for the four waves and laid down
@@ -17,6 +18,8 @@
 // factors; the matrix instructions, their operands' reads and the barriers alone take 124 us.  64 vectors a wave would halve the reads, but their
 // registers leave one wave a SIMD (198 to 247 us).  Heads of 64 take 141 us, of 256 412 (one wave a SIMD).  f32 queries of
 // 128 columns are two values of fp16 each and spill 23 to 25 registers: 305 us (f32 outputs of fp16 queries 224, no spill).
+#pragma once
+
 #include <atomic>
 #include <type_traits>
 
@@ -38,15 +41,17 @@ struct TileLds {
     static constexpr int V = kTokens * KROW, S = V + DP * VROW, BYTES = S + 3 * kTokens * 4;
 };
 
-// A thread's share of a tile on its way from the cache to the LDS: 16 bytes of a key, and four columns
+// A thread's share of a tile on its way from the cache to the LDS: 16 columns of a key, and four columns
 // of four tokens' values; SUBS of each.  A wave's share i lies in one 16-token half of the tile.
-template <int DP>
+template <int DP, int BITS>
 struct Share {
     static constexpr int SUBS = DP == 256 ? 2 : 1;
     static constexpr int KCOLS = DP / 16, VCOLS = DP / 4;  // lanes across a row
-    uint4v k[SUBS];
-    uint32_t v[SUBS][4];
+    static constexpr int KB = 16 * BITS / 8, VB = 4 * BITS / 8;  // bytes
+    Bytes<KB> k[SUBS];
+    Bytes<VB> v[SUBS][4];
     float ks[SUBS], vs[SUBS];
+    uint32_t ku[SUBS], vu[SUBS];  // 4 bits: the key's unit, the four values' units, a byte each
     bool bad[SUBS];
 };
 
@@ -54,10 +59,11 @@ struct Share {
 // rounding to 11 bits adds to the output's own (2.6e-4 of the output against 64 bits, 2.1e-4 with two), and the second
 // value would cost half as many matrix instructions again (the prompt of 4096 tokens 177 us with one, 222 with two, a chunk
 // of 512 over 8192 102 and 122).  Queries of f32 are two values, those of fp16 one, exact.
-template <int DP, int LIMBS, bool Q16, bool SHARED>
+template <int DP, int BITS, int LIMBS, bool Q16, bool SHARED>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kernel(AttendParams p) {
     using L = TileLds<DP>;
-    using Sh = Share<DP>;
+    using Sh = Share<DP, BITS>;
+    constexpr int ROW = DP * BITS / 8;  // bytes of a key
     constexpr int KS = DP / 16, ND = DP / 32, VT = kAttendWide, QL = Q16 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hi = lane >> 5;
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     const int head = h * group + p.group.mod(seen >= 0 ? v : 0);
     auto load_queries = [&] {
         QueryRow<KS, Q16> qr;
-        load_query<KS, 16, false, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
+        load_query<KS, 16, 1, Q16>(p, qr, row * p.ldq + (int64_t)head * p.c.dim, 8 * hi);
         float up = 1.0f;
         if constexpr (QL == 2) {
             // the row's largest value goes to [2^13, 2^14): the low parts stay normal, f32 rows of any size fit
@@ -145,14 +151,14 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const int e = kv_clamp((int)((__float_as_uint(top) >> 23) & 0xff) - 127, -100, 126);
             up = __uint_as_float((uint32_t)(13 - e + 127) << 23);  // 2^(13 - e)
-            unit = p.scale2 * kCodeUnit * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+            unit = p.scale2 * kCodeUnit<BITS> * __uint_as_float((uint32_t)(e - 13 + 127) << 23);
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 _Float16 z[QL];
-                split_f16<QL>(query_at<KS, Q16>(qr, k, i) * up, z);
+                split_f16<QL>(query_at<KS, Q16>(qr, k, operand_column<BITS>(i)) * up, z);
 #pragma unroll
                 for (int q = 0; q < QL; ++q) qf[k][q][i] = z[q];
             }
@@ -166,8 +172,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false;
-    const int k_row = DP == 256 ? tid / 16 : tid % 128 / Sh::KCOLS % 16, k_at = k_row * DP + tid % Sh::KCOLS * 16;
-    const int v_quad = DP == 256 ? wave : tid / Sh::VCOLS % 4, v_at = 4 * v_quad * DP + tid % Sh::VCOLS * 4;
+    const int k_row = DP == 256 ? tid / 16 : tid % 128 / Sh::KCOLS % 16, k_at = k_row * ROW + tid % Sh::KCOLS * Sh::KB;
+    const int v_quad = DP == 256 ? wave : tid / Sh::VCOLS % 4, v_at = 4 * v_quad * ROW + tid % Sh::VCOLS * Sh::VB;
+    const int ku_at = k_row + (tid % Sh::KCOLS * 16 / kKvGroup << p.c.shift), vu_at = 4 * v_quad + (tid % Sh::VCOLS * 4 / kKvGroup << p.c.shift);
     // A tile on its way: the page ids (loaded a step ahead of their use), the buffers, the bytes.
     int ids[Sh::SUBS];
     auto load_ids = [&](int j) {
@@ -179,12 +186,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     };
     // Past the end the last page is read again, an id outside the cache reads page 0: all of that is masked or
     // made NaN.
-    Half16<DP> at[Sh::SUBS];
+    Half16<DP, BITS> at[Sh::SUBS];
     auto find = [&](int j) {
 #pragma unroll
         for (int i = 0; i < Sh::SUBS; ++i) {
             const int jt = j + 16 * half(i);
-            at[i] = find_half<DP>(p.c, ids[i], h, jt & off_mask, true);
+            at[i] = find_half<DP, BITS>(p.c, ids[i], h, jt & off_mask, true);
             at[i].bad = at[i].bad && jt < end;
             bad_page |= at[i].bad;
         }
@@ -194,16 +201,19 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
 #pragma unroll
         for (int i = 0; i < Sh::SUBS; ++i) {
             sh.bad[i] = at[i].bad;
-            sh.k[i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(at[i].block, k_at, at[i].k, 0));
+            load_bytes<Sh::KB, 16>(sh.k[i], at[i].block, k_at, at[i].k);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(at[i].block, v_at + x * DP, at[i].v, 0);
+            for (int x = 0; x < 4; ++x) load_bytes<Sh::VB, 16>(sh.v[i][x], at[i].block, v_at + x * ROW, at[i].v);
+            if constexpr (BITS == 4) {
+                sh.ku[i] = __builtin_amdgcn_raw_buffer_load_b8(at[i].block, ku_at, at[i].ku, 0);
+                sh.vu[i] = __builtin_amdgcn_raw_buffer_load_b32(at[i].block, vu_at, at[i].vu, 0);
+            }
             const int s = 4 * (lane & 15);
             sh.ks[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].block, s, at[i].ks, 0));
             sh.vs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at[i].block, s, at[i].vs, 0));
         }
     };
-    const float key_unit = QL == 2 ? 1.0f : p.scale2 * kCodeUnit;
+    const float key_unit = QL == 2 ? 1.0f : p.scale2 * kCodeUnit<BITS>;
     // a share's way into the LDS, in pieces: 16 bytes of keys are two, four columns of values one each, then the scales
     constexpr int PIECES = 6 * Sh::SUBS;
     auto store_piece = [&](const Sh& sh, uint8_t* buf, int piece) {
@@ -211,12 +221,23 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         const int i = piece / 6, x = piece % 6 - 2;
         if (x < 0) {
             uint8_t* to = buf + (16 * half(i) + k_row) * L::KROW + tid % Sh::KCOLS * 32 + 16 * (x + 2);
-            *reinterpret_cast<half8v*>(to) = codes8(sh.k[i][2 * (x + 2)], sh.k[i][2 * (x + 2) + 1]);
+            if constexpr (BITS == 8) *reinterpret_cast<half8v*>(to) = codes8(sh.k[i].w[2 * (x + 2)], sh.k[i].w[2 * (x + 2) + 1]);
+            else *reinterpret_cast<half8v*>(to) = nibbles8(sh.k[i].w[x + 2], units2(sh.ku[i], 0, 0));
         } else {
             // tokens 4 quad + 0..3 of the half: quad 2 b + h goes to place 8 h + 4 b of 16
             const int place = 16 * half(i) + 8 * (v_quad & 1) + 4 * (v_quad >> 1);
-            const uint32_t sel = 0x0c000c00u | (4 + x) << 16 | x;
-            const uint2v w = {codes2(sh.v[i][1], sh.v[i][0], sel), codes2(sh.v[i][3], sh.v[i][2], sel)};
+            const uint32_t byte = BITS == 8 ? x : x / 2, sel = 0x0c000c00u | (4 + byte) << 16 | byte;
+            uint2v w;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t v0 = sh.v[i][2 * y].w[0], v1 = sh.v[i][2 * y + 1].w[0];
+                if constexpr (BITS == 8) {
+                    w[y] = codes2(v1, v0, sel);
+                } else {
+                    const uint32_t z = __builtin_amdgcn_perm(v1, v0, sel);
+                    w[y] = nibbles2(x % 2 ? z : z << 4, units2(sh.vu[i], 2 * y, 2 * y + 1));
+                }
+            }
             // column d is row d / ND of tile d % ND: a lane's columns of all tiles are neighbours
             const int d = tid % Sh::VCOLS * 4 + x;
             *reinterpret_cast<uint2v*>(buf + L::V + (d % ND * 32 + d / ND) * L::VROW + 2 * place) = w;
@@ -450,7 +471,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     l += __shfl_xor(l, 32, 64);
     if (seen < 0) return;
     if (p.parts == 1) {
-        const float f = l == 0.0f ? 0.0f : kCodeUnit / l;
+        const float f = l == 0.0f ? 0.0f : kCodeUnit<BITS> / l;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float z[ND];
@@ -471,7 +492,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     }
 }
 
-template <int DP, int LIMBS, bool Q16, bool SHARED>
+template <int DP, int BITS, int LIMBS, bool Q16, bool SHARED>
 hipError_t launch_one(const AttendParams& p, hipStream_t st) {
     constexpr int bytes = 3 * TileLds<DP>::BYTES;
     // the LDS is asked for once on each device (those past 63: on every call), and again after a failure
@@ -480,35 +501,36 @@ hipError_t launch_one(const AttendParams& p, hipStream_t st) {
     if (const hipError_t e = hipGetDevice(&device)) return e;
     const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
     if (!(asked.load(std::memory_order_relaxed) & bit)) {
-        if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, LIMBS, Q16, SHARED>),
+        if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_wide_kernel<DP, BITS, LIMBS, Q16, SHARED>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes))
             return e;
         asked.fetch_or(bit, std::memory_order_relaxed);
     }
     const int64_t tiles = SHARED ? p.by_prefix_tiles.d : p.by_tiles.d;
     const int64_t blocks = tiles * p.c.heads * (SHARED ? p.prefix_parts : (p.parts - p.prefix_parts) * (int64_t)p.b.seqs);
-    attend_wide_kernel<DP, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
+    attend_wide_kernel<DP, BITS, LIMBS, Q16, SHARED><<<dim3((uint32_t)blocks), kThreads, bytes, st>>>(p);
     return hipGetLastError();
 }
 
-template <int DP, bool SHARED>
+template <int DP, int BITS, bool SHARED>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
-    if (!p.q_f16) return launch_one<DP, 2, false, SHARED>(p, st);
-    return p.o_f16 ? launch_one<DP, 1, true, SHARED>(p, st) : launch_one<DP, 2, true, SHARED>(p, st);
+    if (!p.q_f16) return launch_one<DP, BITS, 2, false, SHARED>(p, st);
+    return p.o_f16 ? launch_one<DP, BITS, 1, true, SHARED>(p, st) : launch_one<DP, BITS, 2, true, SHARED>(p, st);
 }
 
-template <int DP>
+template <int DP, int BITS>
 hipError_t launch_dp(const AttendParams& p, bool prefix, hipStream_t st) {
-    return prefix ? launch_typed<DP, true>(p, st) : launch_typed<DP, false>(p, st);
+    return prefix ? launch_typed<DP, BITS, true>(p, st) : launch_typed<DP, BITS, false>(p, st);
 }
 
 }  // namespace
 
+template <int BITS>
 hipError_t launch_attend_wide(const AttendParams& p, bool prefix, hipStream_t st) {
     switch (p.c.dim_padded) {
-        case 64: return launch_dp<64>(p, prefix, st);
-        case 128: return launch_dp<128>(p, prefix, st);
-        default: return launch_dp<256>(p, prefix, st);
+        case 64: return launch_dp<64, BITS>(p, prefix, st);
+        case 128: return launch_dp<128, BITS>(p, prefix, st);
+        default: return launch_dp<256, BITS>(p, prefix, st);
     }
 }
 

@@ -1,0 +1,274 @@
+// Heads of query and key rows normalized and turned by their positions, and the same on the way into the cache.
+//
+//   n = x / sqrt(mean x^2 + eps) * gamma        a head's columns; without gamma n = x
+//   y_l = a (n_l cos t - n_r sin t),  y_r = a (n_r cos t + n_l sin t)      t = position * w_i for pair i = (l, r)
+//
+// The angle is position * w_i quarter turns in 64 bits less the nearest whole number: what is left, at most half a
+// quarter turn, is exact to 2^-26 of a quarter in f32 however far the position is, and the whole number's last two
+// bits say which of (c, s), (-s, c), (-c, -s), (s, -c) it is.  sin and cos of up to an eighth of a turn are their
+// series to the 9th and 10th power, the next terms being 2e-9 and 5e-10.  No table of positions is read: a lane has
+// four pairs, whose factors it computes once a row for all heads it works on.
+//
+// A group of dim_padded / 8 lanes holds a head, 8 values a lane: four pairs, or eight of the columns that are not
+// turned.  Every value is read by the lane that writes it, so rows may be worked on in place.  Keys on their way into
+// the cache are laid down in the LDS and taken up again in the order of their columns, 8 a lane, which is what
+// quantize_row wants.
+#include "qlin_kv_rows.hpp"
+#include "qlin_rope.hpp"
+
+namespace qlin {
+namespace {
+
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void turn(double quarters, float& c, float& s) {
+    const double whole = __builtin_rint(quarters);
+    const float f = (float)(quarters - whole), z = f * f;
+    const int k = (int)whole;  // positions below 2^31 and at most a radian each: below 2^31
+    // (pi/2)^n / n! with alternating signs
+    float a = __builtin_fmaf(z, 1.6044118478735982e-4f, -4.681754135318687e-3f);
+    a = __builtin_fmaf(z, a, 7.969262624616704e-2f);
+    a = __builtin_fmaf(z, a, -6.4596409750624626e-1f);
+    a = __builtin_fmaf(z, a, 1.5707963267948966f) * f;
+    float b = __builtin_fmaf(z, -2.5202042373060605e-5f, 9.192602748394264e-4f);
+    b = __builtin_fmaf(z, b, -2.0863480763352961e-2f);
+    b = __builtin_fmaf(z, b, 2.5366950790104803e-1f);
+    b = __builtin_fmaf(z, b, -1.2337005501361697f);
+    b = __builtin_fmaf(z, b, 1.0f);
+    c = k & 1 ? a : b;
+    s = k & 1 ? b : a;
+    c = (k + 1) & 2 ? -c : c;
+    s = k & 2 ? -s : s;
+}
+
+// Columns of a lane's eight values: blocks of four at a and b.
+struct Blocks {
+    int a, b;
+    bool has_a, has_b;
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+    if constexpr (sizeof(T) == 2) {
+        const half4v h = *reinterpret_cast<const half4v*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (float)h[i];
+    } else {
+        const float4v f = *reinterpret_cast<const float4v*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = f[i];
+    }
+}
+
+// BITS 0: rows with positions.  8, 4: rows of a batch, into a cache of that width.  VEC: blocks of four columns are whole
+// and aligned.  WIDE: twice the lanes a head.
+template <int DP, bool WIDE, typename T, bool VEC, int BITS>
+__global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
+    constexpr int LPH = DP / 8 * (WIDE ? 2 : 1), GROUPS = 256 / LPH;
+    __shared__ __align__(16) float lds[BITS ? GROUPS : 1][BITS ? DP + 4 : 4];
+    const int lane = threadIdx.x % LPH, group = threadIdx.x / LPH;
+    int64_t row;
+    int pos = 0, off = 0, page = -1;
+    bool bad = false;
+    const int unit = p.by_splits.div(blockIdx.x), split = p.by_splits.mod(blockIdx.x);
+    if constexpr (BITS == 0) {
+        row = unit;
+        if (p.rope.rotary) pos = p.positions[row];
+    } else {
+        const int i = p.by_new.div(unit), t = p.by_new.mod(unit);
+        const KvSeq s = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
+        bad = s.bad;
+        if (t >= s.rows) {
+            if (bad && threadIdx.x == 0) atomicOr(p.err + kErrBatch, 1u);
+            return;
+        }
+        row = s.row0 + t;
+        pos = s.len - s.rows + t;
+        off = pos & ((1 << p.c.shift) - 1);
+        // nothing is stored of a sequence whose row starts or length are at fault
+        if (!bad && pos >= 0) {
+            const int id = kv_page(p.b.table[i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
+            page = bad ? -1 : id;
+        }
+    }
+
+    // the columns of queries and keys: pairs first, then those that are not turned
+    const int pairs = p.rope.rotary / 2, turned = (pairs + 3) / 4, first = p.rope.first;
+    const bool turns = lane < turned;
+    const int e0 = 8 * (lane - turned), rest = p.dim - p.rope.rotary;
+    auto column = [&](int j) {  // of value j, -1: none
+        if (turns) {
+            if (p.rope.interleaved) return 8 * lane + j < p.rope.rotary ? first + 8 * lane + j : -1;
+            const int i = 4 * lane + j % 4;
+            return i < pairs ? first + i + (j < 4 ? 0 : pairs) : -1;
+        }
+        const int e = e0 + j;
+        return e < rest ? (e < first ? e : e + p.rope.rotary) : -1;
+    };
+    const Blocks qk = {max(column(0), 0), max(column(4), 0), column(0) >= 0, column(4) >= 0};
+    const Blocks straight = {8 * lane, 8 * lane + 4, 8 * lane < p.dim, 8 * lane + 4 < p.dim};
+
+    const int heads = p.q_heads + (BITS ? 2 : 1) * p.k_heads, step = p.splits * GROUPS;
+    auto load = [&](int h, float* x) {
+        const T* at = reinterpret_cast<const T*>(p.x) + row * p.ldx + (int64_t)h * p.dim;
+        const bool value = BITS && h >= p.q_heads + p.k_heads;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+        if constexpr (VEC) {
+            const Blocks b = value ? straight : qk;
+            if (b.has_a) load4<T>(at + b.a, x);
+            if (b.has_b) load4<T>(at + b.b, x + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = value ? (8 * lane + j < p.dim ? 8 * lane + j : -1) : column(j);
+                if (c >= 0) x[j] = ld1<T>(at, c);
+            }
+        }
+    };
+
+    int h = split * GROUPS + group;
+    float x[8];
+    if (h < heads) load(h, x);
+    float g[2][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int c = column(j);
+        g[0][j] = p.q_gamma && c >= 0 ? p.q_gamma[c] : 0.0f;
+        g[1][j] = p.k_gamma && c >= 0 ? p.k_gamma[c] : 0.0f;
+    }
+    float co[4] = {}, si[4] = {};
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            turn(pos * p.rope.quarters[min(4 * lane + i, pairs - 1)], co[i], si[i]);
+            co[i] *= p.rope.amplitude;
+            si[i] *= p.inverse ? -p.rope.amplitude : p.rope.amplitude;
+        }
+    }
+
+    bool finite = true;
+    while (h < heads) {
+        float next[8];
+        if (h + step < heads) load(h + step, next);
+        const bool query = h < p.q_heads, value = BITS && h >= p.q_heads + p.k_heads;
+        if (!value) {
+            if (query ? p.q_gamma != nullptr : p.k_gamma != nullptr) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
+#pragma unroll
+                for (int o = 1; o < LPH; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                // at least the smallest normal number: what v_rsq_f32 gives for less is no number to scale zeros by.  (A
+                // NaN stays one.)
+                const float m = __builtin_fmaf(sum, p.inv_dim, p.eps), r = __builtin_amdgcn_rsqf(m < 0x1p-126f ? 0x1p-126f : m);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = (x[j] * r) * (query ? g[0][j] : g[1][j]);
+            }
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float l = p.rope.interleaved ? x[2 * i] : x[i], r = p.rope.interleaved ? x[2 * i + 1] : x[4 + i];
+                    const float yl = __builtin_fmaf(l, co[i], -(r * si[i])), yr = __builtin_fmaf(r, co[i], l * si[i]);
+                    if (p.rope.interleaved) {
+                        x[2 * i] = yl;
+                        x[2 * i + 1] = yr;
+                    } else {
+                        x[i] = yl;
+                        x[4 + i] = yr;
+                    }
+                }
+            }
+        }
+        if (BITS == 0 || query) {
+            const int64_t at = row * p.ldy + (int64_t)h * p.dim;
+            if (VEC && p.y_vec) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (!(k ? qk.has_b : qk.has_a)) continue;
+                    const int64_t c = at + (k ? qk.b : qk.a);
+                    const float* y = x + 4 * k;
+                    if (p.y_f16)
+                        *reinterpret_cast<half4v*>(reinterpret_cast<_Float16*>(p.y) + c) =
+                            half4v{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+                    else
+                        *reinterpret_cast<float4v*>(reinterpret_cast<float*>(p.y) + c) = float4v{y[0], y[1], y[2], y[3]};
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int c = column(j);
+                    if (c < 0) continue;
+                    if (p.y_f16) reinterpret_cast<_Float16*>(p.y)[at + c] = (_Float16)x[j];
+                    else reinterpret_cast<float*>(p.y)[at + c] = x[j];
+                }
+            }
+        } else if constexpr (BITS != 0) {
+            const KvBlock<DP, BITS> blk(p.c, max(page, 0), h - p.q_heads - (value ? p.k_heads : 0));
+            const int d0 = 8 * lane;
+            if (!value) {
+                // a head's lanes are of one wave, whose accesses to the LDS are done in their order
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (const int c = column(j); c >= 0) lds[group][c] = x[j];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = d0 + j < p.dim ? lds[group][min(d0 + j, DP - 1)] : 0.0f;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+            if (d0 < DP) {
+                const bool fin = value ? quantize_row<DP, BITS, true>(blk, off, d0, x, p.rne, page >= 0)
+                                       : quantize_row<DP, BITS, false>(blk, off, d0, x, p.rne, page >= 0);
+                finite &= fin || page < 0;
+            }
+        }
+        h += step;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = next[j];
+    }
+    if constexpr (BITS != 0) {
+        if (bad && threadIdx.x == 0) atomicOr(p.err + kErrBatch, 1u);
+        if (!finite) atomicOr(p.err + kErrNonfinite, 1u);
+    }
+}
+
+template <int DP, int BITS, typename T>
+hipError_t launch_typed(const HeadsParams& p, dim3 grid, hipStream_t st) {
+    // four columns side by side: pairs and the others are groups of eight, heads and rows of four
+    const bool vec = p.x_vec && p.dim % 4 == 0 && p.rope.rotary % 8 == 0 && p.rope.first % 4 == 0;
+    if (vec) heads_kernel<DP, false, T, true, BITS><<<grid, 256, 0, st>>>(p);
+    else if (heads_wide(p)) heads_kernel<DP, true, T, false, BITS><<<grid, 256, 0, st>>>(p);
+    else heads_kernel<DP, false, T, false, BITS><<<grid, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int BITS>
+hipError_t launch_bits(const HeadsParams& p, dim3 grid, hipStream_t st) {
+    switch (p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256) {
+        case 64: return p.x_f16 ? launch_typed<64, BITS, __half>(p, grid, st) : launch_typed<64, BITS, float>(p, grid, st);
+        case 128: return p.x_f16 ? launch_typed<128, BITS, __half>(p, grid, st) : launch_typed<128, BITS, float>(p, grid, st);
+        default: return p.x_f16 ? launch_typed<256, BITS, __half>(p, grid, st) : launch_typed<256, BITS, float>(p, grid, st);
+    }
+}
+
+int lanes(const HeadsParams& p) { return p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 32; }
+
+}  // namespace
+
+bool heads_wide(const HeadsParams& p) {
+    return (p.rope.rotary / 2 + 3) / 4 + (p.dim - p.rope.rotary + 7) / 8 > lanes(p);
+}
+int heads_at_once(const HeadsParams& p) { return 256 / (lanes(p) * (heads_wide(p) ? 2 : 1)); }
+
+hipError_t launch_heads(const HeadsParams& p, hipStream_t st) {
+    return launch_bits<0>(p, dim3((uint32_t)((int64_t)p.rows * p.splits)), st);
+}
+hipError_t launch_heads_append(const HeadsParams& p, hipStream_t st) {
+    const dim3 grid((uint32_t)((int64_t)p.b.seqs * p.b.max_new * p.splits));
+    return p.c.bits == 4 ? launch_bits<4>(p, grid, st) : launch_bits<8>(p, grid, st);
+}
+
+}  // namespace qlin

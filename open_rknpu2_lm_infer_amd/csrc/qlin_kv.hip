@@ -1,6 +1,6 @@
-// Key/value cache in 8 bits: new rows quantized into their pages, and read back.
+// Key/value cache in 8 and 4 bits: new rows quantized into their pages, and read back.
 //
-// A row is the key (or value) of one token and one head, dim values x:
+// A row is the key (or value) of one token and one head, dim values x; the rules are at quantize_row.  In 8 bits it is
 //   s = max(absmax |x| * (1/127), 2^-64),  code = clamp(round(x * (1/s)), -127, 127),
 // every operation one f32 rounding, 1/127 the f32 nearest to it.  That is the rule of the per-token
 // activation quantization but for its division by 127, whose place a multiplication takes: the
@@ -14,8 +14,7 @@
 // 4096 tokens of 8 heads of 128: 15.9 us with one, 16.3 with two, 19.2 with four).  At that size the
 // append moves 25 MB in 9.3 us (2.7 TB/s) and the read as much in 6.7 (3.8 TB/s); one token takes them
 // 3.1 and 2.6 us, most of it the dependent loads of its place in the batch and in the page table.
-#include "qlin_kv.hpp"
-#include "qlin_rows.hpp"
+#include "qlin_kv_rows.hpp"
 
 namespace qlin {
 namespace {
@@ -53,7 +52,7 @@ __device__ __forceinline__ int find_page(const KvRows& p, Unit& u, int* off) {
     return bad ? -1 : page;
 }
 
-template <int DP, typename T, bool VEC>
+template <int DP, int BITS, typename T, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
     constexpr int LPU = DP / 8;
     Unit u = find_unit<LPU>(p);
@@ -69,36 +68,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
     // on pages that other sequences may read: nothing of it is stored
     int off = 0;
     const int page = u.bad ? -1 : find_page(p, u, &off);
-    const KvBlock<DP> blk(p.c, max(page, 0), u.h);
-    bool finite = true;
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        uint32_t m = 0;  // largest bit pattern of |x|: for non-negative floats their order, Inf and NaN on top
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[y][i]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = LPU / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-        const bool fin = m < 0x7f800000u;
-        const float s = fin ? fmaxf(__uint_as_float(m) * (1.0f / 127.0f), kKvScaleMin) : __uint_as_float(0x7fc00000u);
-        const float inv = fin ? 1.0f / s : 0.0f;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = fin ? x[y][i] : 0.0f;
-            const int c = p.rne ? quant_finite<true>(v, inv) : quant_finite<false>(v, inv);
-            w[i / 4] |= (uint32_t)(c + 128) << (8 * (i % 4));
-        }
-        if (page >= 0) {
-            *reinterpret_cast<uint2*>((y ? blk.v(off) : blk.k(off)) + d0) = make_uint2(w[0], w[1]);
-            if (d0 == 0) *(y ? blk.vs(off) : blk.ks(off)) = s;
-            finite &= fin;
-        }
-    }
+    const KvBlock<DP, BITS> blk(p.c, max(page, 0), u.h);
+    const bool k = quantize_row<DP, BITS, false>(blk, off, d0, x[0], p.rne, page >= 0);
+    const bool v = quantize_row<DP, BITS, true>(blk, off, d0, x[1], p.rne, page >= 0);
+    const bool finite = page < 0 || (k && v);
     if (u.bad) atomicOr(p.err + kErrBatch, 1u);
     if (!finite) atomicOr(p.err + kErrNonfinite, 1u);
 }
 
-template <int DP, typename T, bool VEC>
+template <int DP, int BITS, typename T, bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     constexpr int LPU = DP / 8;
     Unit u = find_unit<LPU>(p);
@@ -107,14 +85,23 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     const int page = find_page(p, u, &off);
     if (u.bad) atomicOr(p.err + kErrBatch, 1u);
     if (!u.ok) return;
-    const KvBlock<DP> blk(p.c, max(page, 0), u.h);
-    uint2 w[2] = {make_uint2(0x80808080u, 0x80808080u), make_uint2(0x80808080u, 0x80808080u)};
+    const KvBlock<DP, BITS> blk(p.c, max(page, 0), u.h);
+    constexpr uint32_t zero = BITS == 8 ? 0x80808080u : 0x88888888u;
+    uint2 w[2] = {make_uint2(zero, zero), make_uint2(zero, zero)};
     // no such token: zeros; a page outside the cache: NaN
     const float none = u.s.len - u.s.rows + u.t < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
     float s[2] = {none, none};
+    int unit[2] = {1, 1};
     if (page >= 0) {
-        w[0] = *reinterpret_cast<const uint2*>(blk.k(off) + d0);
-        w[1] = *reinterpret_cast<const uint2*>(blk.v(off) + d0);
+        if constexpr (BITS == 8) {
+            w[0] = *reinterpret_cast<const uint2*>(blk.k(off) + d0);
+            w[1] = *reinterpret_cast<const uint2*>(blk.v(off) + d0);
+        } else {
+            w[0].x = *reinterpret_cast<const uint32_t*>(blk.k(off) + d0 / 2);
+            w[1].x = *reinterpret_cast<const uint32_t*>(blk.v(off) + d0 / 2);
+            unit[0] = *blk.ku(d0 / kKvGroup, off);
+            unit[1] = *blk.vu(d0 / kKvGroup, off);
+        }
         s[0] = *blk.ks(off);
         s[1] = *blk.vs(off);
     }
@@ -124,7 +111,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
         alignas(16) T y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float x = (float)((int)(((i < 4 ? w[z].x : w[z].y) >> (8 * (i % 4))) & 0xffu) - 128) * s[z];
+            int c;
+            if constexpr (BITS == 8) c = (int)(((i < 4 ? w[z].x : w[z].y) >> (8 * (i % 4))) & 0xffu) - 128;
+            else c = ((int)((w[z].x >> (4 * i)) & 0xfu) - 8) * unit[z];
+            const float x = (float)c * s[z];
             if constexpr (sizeof(T) == 2) y[i] = __builtin_bit_cast(T, f16_of_f32(x));
             else y[i] = x;
         }
@@ -142,48 +132,58 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     }
 }
 
-__global__ __launch_bounds__(256) void kv_clear_kernel(uint32_t* data, int64_t words, int64_t block_words, int64_t code_words) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256)
-        data[i] = i % block_words < code_words ? 0x80808080u : __float_as_uint(kKvScaleMin);
+// Words of a block: codes, then scales, then (4 bits) units.
+__global__ __launch_bounds__(256) void kv_clear_kernel(uint32_t* data, int64_t words, int64_t block_words, int64_t code_words,
+                                                       int64_t scale_words, uint32_t zero) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+        const int64_t at = i % block_words;
+        data[i] = at < code_words ? zero : at < code_words + scale_words ? __float_as_uint(kKvScaleMin) : 0x01010101u;
+    }
 }
 
-template <int DP, typename T, bool VEC>
+template <int DP, int BITS, typename T, bool VEC>
 hipError_t launch_rows(KvRows p, bool append, hipStream_t st) {
     const int64_t per_seq = (int64_t)p.b.max_new * p.c.heads, upb = 256 / (DP / 8);
     p.by_blocks = fast_div((int)((per_seq + upb - 1) / upb));
     p.by_heads = fast_div(p.c.heads);
     const dim3 grid((uint32_t)(p.by_blocks.d * (int64_t)p.b.seqs));
-    if (append) kv_append_kernel<DP, T, VEC><<<grid, 256, 0, st>>>(p);
-    else kv_read_kernel<DP, T, VEC><<<grid, 256, 0, st>>>(p);
+    if (append) kv_append_kernel<DP, BITS, T, VEC><<<grid, 256, 0, st>>>(p);
+    else kv_read_kernel<DP, BITS, T, VEC><<<grid, 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
-template <int DP>
+template <int DP, int BITS>
 hipError_t launch_dp(const KvRows& p, bool append, hipStream_t st) {
     // 16-byte accesses: every row and head 16-byte aligned, heads of whole groups of 8
     const int per16 = p.f16 ? 8 : 4;
     const bool vec = p.c.dim % 8 == 0 && p.ldk % per16 == 0 && p.ldv % per16 == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
     if (p.f16) {
-        return vec ? launch_rows<DP, __half, true>(p, append, st) : launch_rows<DP, __half, false>(p, append, st);
+        return vec ? launch_rows<DP, BITS, __half, true>(p, append, st) : launch_rows<DP, BITS, __half, false>(p, append, st);
     }
-    return vec ? launch_rows<DP, float, true>(p, append, st) : launch_rows<DP, float, false>(p, append, st);
+    return vec ? launch_rows<DP, BITS, float, true>(p, append, st) : launch_rows<DP, BITS, float, false>(p, append, st);
+}
+
+template <int BITS>
+hipError_t launch_bits(const KvRows& p, bool append, hipStream_t st) {
+    switch (p.c.dim_padded) {
+        case 64: return launch_dp<64, BITS>(p, append, st);
+        case 128: return launch_dp<128, BITS>(p, append, st);
+        default: return launch_dp<256, BITS>(p, append, st);
+    }
 }
 
 hipError_t launch_any(const KvRows& p, bool append, hipStream_t st) {
-    switch (p.c.dim_padded) {
-        case 64: return launch_dp<64>(p, append, st);
-        case 128: return launch_dp<128>(p, append, st);
-        default: return launch_dp<256>(p, append, st);
-    }
+    return p.c.bits == 4 ? launch_bits<4>(p, append, st) : launch_bits<8>(p, append, st);
 }
 
 }  // namespace
 
 hipError_t launch_kv_clear(const KvCache& c, hipStream_t st) {
-    const int64_t block = kv_block_bytes(c.dim_padded, c.shift) / 4;
+    const int64_t block = kv_block_bytes(c.bits, c.dim_padded, c.shift) / 4;
     kv_clear_kernel<<<dim3(4096), 256, 0, st>>>(reinterpret_cast<uint32_t*>(c.data), block * c.heads * c.pages, block,
-                                                 ((int64_t)c.dim_padded << c.shift) / 2);
+                                                ((int64_t)c.dim_padded * c.bits << c.shift) / 16, (int64_t)2 << c.shift,
+                                                c.bits == 4 ? 0x88888888u : 0x80808080u);
     return hipGetLastError();
 }
 hipError_t launch_kv_append(const KvRows& p, hipStream_t st) { return launch_any(p, true, st); }

@@ -18,29 +18,40 @@ constexpr float kKvMaxScale = 0x1p64f;
 constexpr int kKvMaxSeqs = 1 << 20, kKvMaxRows = 1 << 24, kKvMaxLen = 1 << 30;
 constexpr int64_t kKvMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads of one launch
 
-// The cache in device memory.  Codes are stored as code + 128, one byte each: a byte b between two
+// Columns of a 4-bit row that share a unit.  Units and row scales: x = code * unit * scale with codes -7 .. 7 and units 1 ..
+// 255, whole numbers: a code times a unit has 11 bits, what fp16 holds.
+constexpr int kKvGroup = 32;
+
+// The cache in device memory.  Codes of 8 bits are stored as code + 128, one byte each: a byte b between two
 // zero bytes is the fp16 subnormal b * 2^-24, so one byte permute and one packed FMA make two exact
-// fp16 codes of two bytes.  Columns dim .. dim_padded - 1 hold code 0.
+// fp16 codes of two bytes.  Codes of 4 bits are stored as code + 8, the lower nibble of a byte the even column.
+// Columns dim .. dim_padded - 1 hold code 0.
 //
 // A block of a page and head is contiguous: keys [page tokens][dim_padded], values alike, then the
-// key scales f32 [page tokens] and the value scales.  One address leads to all of it.
+// key scales f32 [page tokens] and the value scales, and in 4 bits the units of keys, a byte each,
+// [dim_padded / 32][page tokens], and of values.  One address leads to all of it.
 struct KvCache {
     uint8_t* data;  // [pages][heads] blocks
     int pages, heads, dim, dim_padded, shift;  // 1 << shift tokens a page
+    int bits;                                  // 8 or 4
 };
-__host__ __device__ __forceinline__ int64_t kv_block_bytes(int dim_padded, int shift) {
-    return (int64_t)(2 * dim_padded + 8) << shift;
+__host__ __device__ __forceinline__ int64_t kv_block_bytes(int bits, int dim_padded, int shift) {
+    return (int64_t)(bits == 8 ? 2 * dim_padded + 8 : dim_padded + 8 + 2 * (dim_padded / kKvGroup)) << shift;
 }
-template <int DP>
+template <int DP, int BITS>
 struct KvBlock {
+    static constexpr int ROW = DP * BITS / 8;
     uint8_t* base;
     int shift;
     __device__ KvBlock(const KvCache& c, int page, int head)
-        : base(c.data + ((int64_t)page * c.heads + head) * kv_block_bytes(DP, c.shift)), shift(c.shift) {}
-    __device__ uint8_t* k(int off) const { return base + off * DP; }
-    __device__ uint8_t* v(int off) const { return base + (((int64_t)DP << shift) + off * DP); }
-    __device__ float* ks(int off) const { return reinterpret_cast<float*>(base + ((int64_t)(2 * DP) << shift)) + off; }
+        : base(c.data + ((int64_t)page * c.heads + head) * kv_block_bytes(BITS, DP, c.shift)), shift(c.shift) {}
+    __device__ uint8_t* k(int off) const { return base + off * ROW; }
+    __device__ uint8_t* v(int off) const { return base + (((int64_t)ROW << shift) + off * ROW); }
+    __device__ float* ks(int off) const { return reinterpret_cast<float*>(base + ((int64_t)(2 * ROW) << shift)) + off; }
     __device__ float* vs(int off) const { return ks(off + (1 << shift)); }
+    // unit of group g (4 bits)
+    __device__ uint8_t* ku(int g, int off) const { return base + ((int64_t)(2 * ROW + 8 + g) << shift) + off; }
+    __device__ uint8_t* vu(int g, int off) const { return ku(g + DP / kKvGroup, off); }
 };
 
 struct KvBatch {
@@ -97,6 +108,12 @@ int attend_tile(const AttendParams& p);
 int attend_tile_prefix(const AttendParams& p);
 constexpr int kAttendWide = 128;  // of the kernel for many vectors
 hipError_t launch_attend(const AttendParams& p, hipStream_t stream);
+template <int BITS>
+hipError_t launch_attend_bits(const AttendParams& p, hipStream_t stream);
+extern template hipError_t launch_attend_bits<4>(const AttendParams& p, hipStream_t stream);
+template <int BITS>
 hipError_t launch_attend_wide(const AttendParams& p, bool prefix, hipStream_t stream);
+extern template hipError_t launch_attend_wide<8>(const AttendParams& p, bool prefix, hipStream_t stream);
+extern template hipError_t launch_attend_wide<4>(const AttendParams& p, bool prefix, hipStream_t stream);
 
 }  // namespace qlin

@@ -1,5 +1,5 @@
 // C ABI of the key/value cache: its handle, the argument checks, and how an attention call is cut
-// into parts.
+// into parts; the pass from the qkv projection into it, and the tables of a serving step.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -8,6 +8,8 @@
 
 #include "../../include/qlinear.h"
 #include "qlin_kv.hpp"
+#include "qlin_kv_step.hpp"
+#include "qlin_rope_handle.hpp"
 
 using namespace qlin;
 
@@ -151,11 +153,19 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
 
 }  // namespace
 
+namespace qlin {
+int64_t kv_step_scratch(int seqs);  // ints
+hipError_t launch_kv_step(StepParams p, int32_t* scratch, hipStream_t stream);
+}  // namespace qlin
+
 extern "C" {
 
-int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) {
+int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) { return qlin_kv_create_bits(config, 8, out); }
+
+int qlin_kv_create_bits(const qlin_kv_config* config, int32_t bits, qlin_kv_cache** out) {
     if (!out) return QLIN_ERR_PARAM;
     *out = nullptr;
+    if (bits != 8 && bits != 4) return QLIN_ERR_PARAM;
     if (!config || config->kv_heads <= 0 || config->head_dim <= 0 || config->pages <= 0 ||
         !power_of_two(config->page_tokens))
         return QLIN_ERR_PARAM;
@@ -167,13 +177,14 @@ int qlin_kv_create(const qlin_kv_config* config, qlin_kv_cache** out) {
     auto* x = new (std::nothrow) qlin_kv_cache();
     if (!x) return QLIN_ERR_NOMEM;
     KvCache& c = x->c;
+    c.bits = bits;
     c.pages = config->pages;
     c.heads = config->kv_heads;
     c.dim = config->head_dim;
     c.dim_padded = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     while ((1 << c.shift) < config->page_tokens) ++c.shift;
     x->device = dev;
-    x->device_bytes = (uint64_t)c.pages * c.heads * kv_block_bytes(c.dim_padded, c.shift);
+    x->device_bytes = (uint64_t)c.pages * c.heads * kv_block_bytes(c.bits, c.dim_padded, c.shift);
     if (hipMalloc(&c.data, x->device_bytes) != hipSuccess) {
         (void)hipGetLastError();
         delete x;
@@ -205,6 +216,8 @@ int qlin_kv_query(const qlin_kv_cache* x, qlin_kv_info* out) {
     return QLIN_OK;
 }
 
+int32_t qlin_kv_bits(const qlin_kv_cache* x) { return x ? x->c.bits : QLIN_ERR_PARAM; }
+
 int qlin_kv_append(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const void* K, int64_t ldk,
                    const void* V, int64_t ldv, int32_t dtype, uint32_t flags, void* stream) {
     return rows_call(ws, cache, batch, const_cast<void*>(K), ldk, const_cast<void*>(V), ldv, dtype, flags, stream, true);
@@ -213,6 +226,69 @@ int qlin_kv_append(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch
 int qlin_kv_read(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, void* K, int64_t ldk, void* V,
                  int64_t ldv, int32_t dtype, void* stream) {
     return rows_call(ws, cache, batch, K, ldk, V, ldv, dtype, 0, stream, false);
+}
+
+int qlin_kv_append_qkv(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_batch* batch, const qlin_rope* rope,
+                       int32_t q_heads, const float* q_gamma, const float* k_gamma, float eps, const void* QKV, int32_t dtype,
+                       int64_t ld, void* Q, int32_t q_dtype, int64_t ldq, uint32_t flags, void* stream) {
+    if (!cache || !batch || (batch->rows > 0 && (!QKV || !Q)) || !is_dtype(dtype) || !is_dtype(q_dtype) ||
+        (flags & ~QLIN_ROUND_HALF_EVEN) || q_heads <= 0 || (rope && (rope->dim != cache->c.dim || rope->device != cache->device)))
+        return QLIN_ERR_PARAM;
+    if ((q_gamma || k_gamma) && !(eps > 0.0f && std::isfinite(eps))) return QLIN_ERR_PARAM;
+    const int64_t heads = (int64_t)q_heads + 2 * cache->c.heads, D = cache->c.dim;
+    if (ld < heads * D || ldq < q_heads * D) return QLIN_ERR_PARAM;
+    if (q_heads > kKvMaxHeads) return QLIN_ERR_UNSUPPORTED;
+    HeadsParams p{};
+    WorkspaceParts parts;
+    if (int rc = begin(ws, cache, batch, stream, &p.b, &parts)) return rc;
+    if (p.b.max_new == 0) return QLIN_OK;
+    if ((int64_t)p.b.seqs * p.b.max_new > kKvMaxGrid) return QLIN_ERR_UNSUPPORTED;
+    heads_common(&p, rope, cache->c.dim, q_heads, cache->c.heads, q_gamma, k_gamma, eps, QKV, dtype == QLIN_F16, ld, Q,
+                 q_dtype == QLIN_F16, ldq);
+    p.c = cache->c;
+    p.by_new = fast_div(p.b.max_new);
+    p.rne = (flags & QLIN_ROUND_HALF_EVEN) != 0;
+    p.err = parts.err;
+    heads_split(&p, (int64_t)p.b.seqs * p.b.max_new, (int)heads);
+    return launch_heads_append(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
+}
+
+int qlin_kv_step(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_tables* t, void* stream) {
+    if (!ws || !cache || !t || t->seqs <= 0 || t->rows < 0 || t->max_new < 0 || t->max_len < 0 || t->prefix_tokens < 0 ||
+        t->prefix_tokens > t->max_len || (t->prefix_tokens & ((1 << cache->c.shift) - 1)) || !t->change || !t->length ||
+        !t->free_pages || !t->free_count || !t->row_start || (t->max_len > 0 && !t->page_table))
+        return QLIN_ERR_PARAM;
+    const int64_t columns = ceil_div(t->max_len, (int64_t)1 << cache->c.shift);
+    if (t->page_ld < columns) return QLIN_ERR_PARAM;
+    if (t->seqs > kKvMaxSeqs || t->rows > kKvMaxRows || t->max_len > kKvMaxLen || t->seqs * columns > kStepMost)
+        return QLIN_ERR_UNSUPPORTED;
+    if (workspace_device(ws) != cache->device) return QLIN_ERR_PARAM;
+    int dev;
+    if (hipGetDevice(&dev) != hipSuccess) return QLIN_ERR_NODEVICE;
+    if (dev != cache->device) return QLIN_ERR_PARAM;
+    const WorkspaceParts parts = workspace_begin(ws, (hipStream_t)stream);
+    if (kv_step_scratch(t->seqs) > parts.part_floats) return QLIN_ERR_UNSUPPORTED;
+    StepParams p{};
+    p.seqs = t->seqs;
+    p.rows = t->rows;
+    p.max_new = t->max_new;
+    p.max_len = t->max_len;
+    p.shared = t->prefix_tokens >> cache->c.shift;
+    p.pages = cache->c.pages;
+    p.shift = cache->c.shift;
+    p.change = t->change;
+    p.length = t->length;
+    p.table = t->page_table;
+    p.table_ld = t->page_ld;
+    p.free_pages = t->free_pages;
+    p.free_count = t->free_count;
+    p.row_start = t->row_start;
+    p.row_seq = t->row_seq;
+    p.positions = t->positions;
+    p.slots = t->slots;
+    p.refused = t->refused;
+    p.err = parts.err;
+    return launch_kv_step(p, reinterpret_cast<int32_t*>(parts.part), (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
 }
 
 int qlin_kv_attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batch* batch, int32_t q_heads,

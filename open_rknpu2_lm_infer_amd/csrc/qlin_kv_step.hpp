@@ -1,0 +1,80 @@
+// Tables of a serving step: what the C entry point hands to the kernels of qlin_kv_step.hip, and the rules for one slot,
+// plain integer functions, the same on the device and in host tests.
+#pragma once
+
+#include "qlin_kv_index.hpp"
+
+namespace qlin {
+
+// What one slot asks for.  Its own pages are the columns from `shared` (those of the prefix) on.
+struct StepSlot {
+    int len;   // tokens after what it gives back, before what it is given
+    int from;  // first column that is given back (back > 0) or given
+    int back;  // pages given back
+    int want;  // tokens asked for, as far as the slot's own limits allow them
+    int need;  // pages for them
+    bool asks, bad;
+};
+
+// Columns that n tokens take, those of the prefix among them in any case.  n is 0 .. 2^30.
+QLIN_HD int step_columns(int n, int shift, int shared) {
+    const int c = (n + (1 << shift) - 1) >> shift;
+    return c > shared ? c : shared;
+}
+
+QLIN_HD StepSlot step_slot(int n, int change, int shift, int shared, int rows, int max_new, int max_len) {
+    StepSlot s{n, 0, 0, 0, 0, change > 0, n < 0 || n > max_len};
+    if (s.bad || change == 0) return s;
+    const int held = step_columns(n, shift, shared);
+    if (change < 0) {
+        s.len = change < -n ? 0 : n + change;
+        s.from = step_columns(s.len, shift, shared);
+        s.back = held - s.from;
+        return s;
+    }
+    if (change > max_new || change > rows || change > max_len - n) return s;
+    s.want = change;
+    s.from = held;
+    s.need = step_columns(n + change, shift, shared) - held;
+    return s;
+}
+
+// Last i of start[0 .. n] (not decreasing, start[0] = 0) with start[i] <= k: whose the k-th thing is, for k < start[n].
+template <typename P>
+QLIN_HD int step_owner(P start, int n, int k) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= k) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Sums that stay at kStepMost once they reach it: above everything that can be granted.
+constexpr int kStepMost = 1 << 30;
+QLIN_HD int step_add(int a, int b) {
+    const uint32_t c = static_cast<uint32_t>(a) + static_cast<uint32_t>(b);
+    return c > static_cast<uint32_t>(kStepMost) ? kStepMost : static_cast<int>(c);
+}
+
+struct StepParams {
+    int seqs, rows, max_new, max_len, shared, pages, shift;
+    const int32_t* change;
+    int32_t* length;
+    int32_t* table;
+    int64_t table_ld;
+    int32_t* free_pages;
+    int32_t* free_count;
+    int32_t* row_start;
+    int32_t* row_seq;
+    int32_t* positions;
+    int64_t* slots;
+    int32_t* refused;
+    // scratch: totals, then [seqs + 1] first pages given and given back
+    int32_t* totals;
+    int32_t *need_start, *back_start;
+    uint32_t* err;
+};
+
+}  // namespace qlin

@@ -12,8 +12,8 @@ import torch
 
 from . import _lib
 from ._lib import (QLIN_F16, QLIN_F32, QLIN_NO_FUSED_QUANT, QLIN_NORM_SEQUENTIAL,  # noqa: F401
-                   QLIN_PATH_GEMM, QLIN_PATH_GEMV, QLIN_PATH_GEMV_FUSED, QLIN_RESIDUAL, QLIN_ROUND_HALF_EVEN,
-                   QLIN_SWIGLU, check)
+                   QLIN_PATH_GEMM, QLIN_PATH_GEMV, QLIN_PATH_GEMV_FUSED, QLIN_RESIDUAL, QLIN_ROPE_INVERSE,
+                   QLIN_ROUND_HALF_EVEN, QLIN_SWIGLU, check)
 
 _DT = {torch.float32: QLIN_F32, torch.float16: QLIN_F16}
 
@@ -293,13 +293,106 @@ def run_quantized(ws: Workspace, w: Weights, q: torch.Tensor, s: torch.Tensor, o
     return out
 
 
-class KVCache:
-    """Keys and values of kv_heads heads of head_dim in 8 bits, in `pages` pages of page_tokens tokens (qlin_kv_cache)."""
+class Rope:
+    """Rotary positions (qlin_rope): which columns of a head are turned, in which layout and by how much a position.
+    layout: "half" or "interleaved"; scaling: "plain", "linear", "base", "bands" (by wavelength, low and high in
+    wavelengths of original_len) or "ramp" (by pair, low and high likewise); amplitude 0: the scaling's own."""
 
-    def __init__(self, kv_heads: int, head_dim: int, pages: int, page_tokens: int = 64):
+    LAYOUTS = {"half": _lib.QLIN_ROPE_HALF, "interleaved": _lib.QLIN_ROPE_INTERLEAVED}
+    SCALINGS = {"plain": _lib.QLIN_ROPE_PLAIN, "linear": _lib.QLIN_ROPE_LINEAR, "base": _lib.QLIN_ROPE_BASE,
+                "bands": _lib.QLIN_ROPE_BANDS, "ramp": _lib.QLIN_ROPE_RAMP}
+
+    def __init__(self, head_dim: int, rotary_dim: int | None = None, base: float = 10000.0, first: int = 0,
+                 layout: str = "half", scaling: str = "plain", factor: float = 1.0, original_len: float = 0.0,
+                 low: float = 0.0, high: float = 0.0, amplitude: float = 0.0):
+        self.handle = ctypes.c_void_p()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        cfg = _lib.RopeConfig(head_dim, rotary_dim, first, self.LAYOUTS[layout], self.SCALINGS[scaling], 0, base, factor,
+                              original_len, low, high, amplitude)
+        check(_lib.load().qlin_rope_create(ctypes.byref(cfg), ctypes.byref(self.handle)), "qlin_rope_create")
+        self.head_dim, self.rotary_dim = head_dim, rotary_dim
+        w, a = (ctypes.c_double * (rotary_dim // 2))(), ctypes.c_double()
+        check(_lib.load().qlin_rope_query(self.handle, w, ctypes.byref(a)), "qlin_rope_query")
+        self.radians, self.amplitude = list(w), a.value
+
+    def close(self):
+        if self.handle:
+            _lib.load().qlin_rope_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _rope_rows(X: torch.Tensor, positions: torch.Tensor | None, out: torch.Tensor | None, out_dtype) -> torch.Tensor:
+    """Checks rows, positions and the output of a rotary call; the output."""
+    rows, cols = X.shape
+    assert X.is_cuda and (X.stride(1) == 1 or cols == 1)
+    assert positions is None or (positions.dtype == torch.int32 and positions.device == X.device
+                                 and positions.is_contiguous() and positions.numel() == rows)
+    if out is None:
+        out = torch.empty((rows, cols), dtype=out_dtype or X.dtype, device=X.device)
+    assert out.shape == X.shape and out.device == X.device and (out.stride(1) == 1 or cols == 1)
+    return out
+
+
+def _row_ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # one row has no stride of its own
+
+
+def rope(rope: Rope, X: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None,
+         flags: int = 0) -> torch.Tensor:
+    """The heads of rows X [rows, heads * head_dim] turned by their rows' positions, int32 [rows] (qlin_rope_run); out may
+    be X.  flags: QLIN_ROPE_INVERSE."""
+    assert positions is not None
+    out = _rope_rows(X, positions, out, out_dtype)
+    heads = X.shape[1] // rope.head_dim
+    assert heads * rope.head_dim == X.shape[1]
+    rc = _lib.load().qlin_rope_run(rope.handle, X.shape[0], heads, X.data_ptr(), _DT[X.dtype], _row_ld(X), positions.data_ptr(),
+                                   out.data_ptr(), _DT[out.dtype], _row_ld(out), flags, _raw_stream(X.device))
+    if rc:
+        check(rc, "qlin_rope_run")
+    return out
+
+
+def _gamma_ptr(gamma: torch.Tensor | None, dim: int, device: torch.device) -> int | None:
+    if gamma is None:
+        return None
+    assert gamma.dtype == torch.float32 and gamma.device == device and gamma.is_contiguous() and gamma.numel() == dim
+    return gamma.data_ptr()
+
+
+def norm_rope(rope: Rope | None, X: torch.Tensor, positions: torch.Tensor | None, q_heads: int,
+              q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None, eps: float = 1e-6,
+              out: torch.Tensor | None = None, out_dtype=None, flags: int = 0, head_dim: int | None = None) -> torch.Tensor:
+    """RMSNorm of every head of rows X [rows, (q_heads + key heads) * head_dim], then the rotation (qlin_rope_run_norm); out
+    may be X.  Without rope: norms alone, of heads of head_dim."""
+    assert (rope is None) == (positions is None) and (rope is None or head_dim in (None, rope.head_dim))
+    out = _rope_rows(X, positions, out, out_dtype)
+    D = head_dim if rope is None else rope.head_dim
+    heads = X.shape[1] // D
+    assert heads * D == X.shape[1] and 0 <= q_heads <= heads
+    rc = _lib.load().qlin_rope_run_norm(
+        rope.handle if rope else None, X.shape[0], D, q_heads, heads - q_heads, _gamma_ptr(q_gamma, D, X.device),
+        _gamma_ptr(k_gamma, D, X.device), eps, X.data_ptr(), _DT[X.dtype], _row_ld(X),
+        positions.data_ptr() if rope else None, out.data_ptr(), _DT[out.dtype], _row_ld(out), flags, _raw_stream(X.device))
+    if rc:
+        check(rc, "qlin_rope_run_norm")
+    return out
+
+
+class KVCache:
+    """Keys and values of kv_heads heads of head_dim in 8 or 4 bits, in `pages` pages of page_tokens tokens
+    (qlin_kv_cache)."""
+
+    def __init__(self, kv_heads: int, head_dim: int, pages: int, page_tokens: int = 64, bits: int = 8):
         self.handle = ctypes.c_void_p()
         cfg = _lib.KVConfig(kv_heads, head_dim, page_tokens, pages)
-        check(_lib.load().qlin_kv_create(ctypes.byref(cfg), ctypes.byref(self.handle)), "qlin_kv_create")
+        check(_lib.load().qlin_kv_create_bits(ctypes.byref(cfg), bits, ctypes.byref(self.handle)), "qlin_kv_create_bits")
+        self.bits = _lib.load().qlin_kv_bits(self.handle)
         info = _lib.KVInfo()
         check(_lib.load().qlin_kv_query(self.handle, ctypes.byref(info)), "qlin_kv_query")
         self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
@@ -371,6 +464,72 @@ def kv_append(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor, V:
                                     _raw_stream(batch.device))
     if rc:
         check(rc, "qlin_kv_append")
+
+
+def kv_append_qkv(ws: Workspace, cache: KVCache, batch: KVBatch, rope: Rope | None, QKV: torch.Tensor, q_heads: int,
+                  q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                  out: torch.Tensor | None = None, out_dtype=None, flags: int = 0) -> torch.Tensor:
+    """Rows of the qkv projection, [rows, (q_heads + 2 * kv_heads) * head_dim], into the cache in one pass: queries and keys
+    normalized and turned by their tokens' places, keys and values quantized into their pages (qlin_kv_append_qkv).
+    Returns the queries [rows, q_heads * head_dim]; out may be those columns of QKV."""
+    _kv_check(cache, batch)
+    D = cache.head_dim
+    assert rope is None or rope.head_dim == D
+    if out is None:
+        out = torch.empty((QKV.shape[0], q_heads * D), dtype=out_dtype or QKV.dtype, device=QKV.device)
+    rc = _lib.load().qlin_kv_append_qkv(
+        ws.handle, cache.handle, batch.ref, rope.handle if rope else None, q_heads, _gamma_ptr(q_gamma, D, batch.device),
+        _gamma_ptr(k_gamma, D, batch.device), eps, QKV.data_ptr(), _DT[QKV.dtype],
+        _kv_ld(batch, QKV, q_heads * D + 2 * cache.columns), out.data_ptr(), _DT[out.dtype], _kv_ld(batch, out, q_heads * D),
+        flags, _raw_stream(batch.device))
+    if rc:
+        check(rc, "qlin_kv_append_qkv")
+    return out
+
+
+class KVStep:
+    """Device arrays of a serving step's slots (qlin_kv_tables): what a step reads and changes, length [seqs], page_table
+    [seqs, columns], free_pages [cache.pages] and free_count [1], and what it makes, row_start [seqs + 1], row_seq, positions (int32)
+    and slots (int64) [rows] and refused [1], each made here unless given (row_seq, positions, slots and refused:
+    maps=False for none).  batch: the KVBatch of the rows that a step granted."""
+
+    def __init__(self, cache: KVCache, length: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, rows: int, max_new: int, max_len: int, prefix_tokens: int = 0,
+                 row_start: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                 refused: torch.Tensor | None = None, maps: bool = True):
+        seqs, device = length.numel(), length.device
+
+        def array(t, n, dtype=torch.int32, made=True):
+            if t is None and made:
+                t = torch.zeros((n,), dtype=dtype, device=device)
+            assert t is None or (t.dtype == dtype and t.device == device and t.is_contiguous() and t.numel() == n)
+            return t
+
+        self.length, self.free_pages = array(length, seqs), array(free_pages, cache.pages)
+        self.free_count, self.row_start = array(free_count, 1), array(row_start, seqs + 1)
+        self.row_seq, self.positions = array(row_seq, rows, made=maps), array(positions, rows, made=maps)
+        self.slots, self.refused = array(slots, rows, torch.int64, maps), array(refused, 1, made=maps)
+        self.page_table, self.cache, self.seqs, self.rows, self.device = page_table, cache, seqs, rows, device
+        # checks the table too; a batch's max_new is at most its rows
+        self.batch = KVBatch(self.row_start, length, page_table, rows, min(max_new, rows), max_len)
+        assert self.batch.columns * cache.page_tokens >= max_len, "the page table is too narrow for max_len"
+        assert device.index == cache.device, "the slots and the cache are on different devices"
+        ptr = [t.data_ptr() if t is not None else None for t in
+               (self.free_pages, self.free_count, self.row_start, self.row_seq, self.positions, self.slots, self.refused)]
+        self.c = _lib.KVTables(seqs, rows, max_new, max_len, prefix_tokens, 0, None, length.data_ptr(), page_table.data_ptr(),
+                               self.batch.c.page_ld, *ptr)
+        self.ref = ctypes.byref(self.c)
+
+
+def kv_step(ws: Workspace, step: KVStep, change: torch.Tensor) -> KVBatch:
+    """Grants and takes back tokens, int32 [seqs], and makes the step's tables (qlin_kv_step); its batch."""
+    assert change.dtype == torch.int32 and change.device == step.device and change.is_contiguous() and change.numel() == step.seqs
+    step.c.change = change.data_ptr()
+    rc = _lib.load().qlin_kv_step(ws.handle, step.cache.handle, step.ref, _raw_stream(step.device))
+    if rc:
+        check(rc, "qlin_kv_step")
+    return step.batch
 
 
 def kv_read(ws: Workspace, cache: KVCache, batch: KVBatch, K: torch.Tensor | None = None, V: torch.Tensor | None = None,
