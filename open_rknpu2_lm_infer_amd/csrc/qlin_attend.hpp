@@ -26,9 +26,9 @@ __device__ __forceinline__ uint32_t codes2(uint32_t hi, uint32_t lo, uint32_t se
     const half2v m = {(_Float16)32768.0f, (_Float16)32768.0f}, a = {(_Float16)-0.25f, (_Float16)-0.25f};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, m, a));
 }
-// What codes are worth in the matrix core's operands: 2^-9 in 8 bits, and 2^-13 for a code times its unit in 4.
+// What codes are worth in the matrix core's operands: 2^-9 in 8 bits, and 2^-16 for a code times its unit in 4.
 template <int BITS>
-constexpr float kCodeUnit = BITS == 8 ? 512.0f : 8192.0f;
+constexpr float kCodeUnit = BITS == 8 ? 512.0f : 65536.0f;
 
 // Eight codes of consecutive columns, bytes of (w0, w1).
 __device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
@@ -37,26 +37,30 @@ __device__ __forceinline__ half8v codes8(uint32_t w0, uint32_t w1) {
     return __builtin_bit_cast(half8v, r);
 }
 
-// 4 bits: a nibble (code + 8) in bits 4..7 of a half is n * 2^-20, times unit * 2^7 less unit * 2^-10 it is
-// code * unit * 2^-13.  Both factors and the result (up to 7 * 255, 11 bits, at least 2^-13) are exact in fp16, so a unit
-// costs nothing but these factors of it.
+// 4 bits: a nibble (code + 8) in the lowest bits of a half is n * 2^-24, in the next four n * 2^-20.  Times unit * 2^8 or
+// unit * 2^4, less unit * 2^-13, either is code * unit * 2^-16: factors and result (up to 7 * 255, 11 bits) are exact in fp16, small
+// results as subnormals, which the matrix core takes as they are.  So a unit costs nothing but its factors, and two of the
+// four nibbles of a half no shift.
 struct Unit2 {
-    half2v m, a;
+    half2v lo, hi, less;
 };
-// Units of bytes i and j of w that sel (0x04000400 | j << 16 | i with 4 for the constant's bytes) picks: 0x6400 | u is 1024 + u.
+// Units of bytes i and j of w: 0x6400 | u is 1024 + u.
 __device__ __forceinline__ Unit2 units2(uint32_t w, int i, int j) {
-    const half2v k = {(_Float16)1024.0f, (_Float16)1024.0f}, up = {(_Float16)128.0f, (_Float16)128.0f},
-                 down = {(_Float16)-0x1p-10f, (_Float16)-0x1p-10f};
+    const half2v k = {(_Float16)1024.0f, (_Float16)1024.0f}, lo = {(_Float16)256.0f, (_Float16)256.0f},
+                 hi = {(_Float16)16.0f, (_Float16)16.0f}, less = {(_Float16)-0x1p-13f, (_Float16)-0x1p-13f};
     const half2v u = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04000400u | (uint32_t)j << 16 | (uint32_t)i)) - k;
-    return {u * up, u * down};
+    return {u * lo, u * hi, u * less};
 }
-__device__ __forceinline__ uint32_t nibbles2(uint32_t at4, const Unit2& u) {
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, at4 & 0x00f000f0u), u.m, u.a));
+// Nibbles x of both halves of w.
+__device__ __forceinline__ uint32_t nibbles2(uint32_t w, int x, const Unit2& u) {
+    const uint32_t y = x < 2 ? w : w >> 8;
+    return __builtin_bit_cast(uint32_t, x % 2 ? __builtin_elementwise_fma(__builtin_bit_cast(half2v, y & 0x00f000f0u), u.hi, u.less)
+                                              : __builtin_elementwise_fma(__builtin_bit_cast(half2v, y & 0x000f000fu), u.lo, u.less));
 }
-// Eight codes of consecutive columns, nibbles of w, in the order that the halves of a word give them: columns
-// 0 4 1 5 2 6 3 7.  Queries are laid out alike (operand_column).
+// Eight codes of consecutive columns of a key, in the order that the halves of a word give them: columns 0 4 1 5 2 6 3 7.
+// Queries are laid out alike (operand_column).
 __device__ __forceinline__ half8v nibbles8(uint32_t w, const Unit2& u) {
-    const uint4v r = {nibbles2(w << 4, u), nibbles2(w, u), nibbles2(w >> 4, u), nibbles2(w >> 8, u)};
+    const uint4v r = {nibbles2(w, 0, u), nibbles2(w, 1, u), nibbles2(w, 2, u), nibbles2(w, 3, u)};
     return __builtin_bit_cast(half8v, r);
 }
 // Which of eight consecutive columns is element i of a key's operand.
@@ -151,7 +155,7 @@ __device__ __forceinline__ void store_out(const AttendParams& p, int64_t at, int
 
 template <int N>
 struct Bytes {
-    uint32_t w[(N + 3) / 4];
+    uint32_t w[N / 4];
 };
 
 typedef const __attribute__((address_space(4))) int32_t* const_ids;
@@ -184,11 +188,10 @@ __device__ __forceinline__ Half16<DP, BITS> find_half(const KvCache& c, int id, 
     return x;
 }
 
-// N bytes of a buffer, at a lane's offset from `from` on: up to 16 of them, or 16 every STEP.  Two are the low ones of a word.
+// N bytes of a buffer, at a lane's offset from `from` on: up to 16 of them, or 16 every STEP.
 template <int N, int STEP>
 __device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b, int at, int from) {
-    if constexpr (N == 2) r.w[0] = __builtin_amdgcn_raw_buffer_load_b16(b, at, from, 0);
-    else if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
+    if constexpr (N == 4) r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, from, 0);
     else if constexpr (N == 8) {
         const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(b, at, from, 0));
         r.w[0] = x[0];
@@ -203,4 +206,21 @@ __device__ __forceinline__ void load_bytes(Bytes<N>& r, __amdgpu_buffer_rsrc_t b
     }
 }
 
+// Sum and maximum over the four lanes n, n + 16, n + 32, n + 48.
+template <bool MAX>
+__device__ __forceinline__ float over_groups(float x) {
+    typedef unsigned int pair __attribute__((ext_vector_type(2)));
+    pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// What the waves of a workgroup join in: 16 vectors a tile.
+template <int DP, int R>
+struct AttendLds {
+    alignas(16) float o[2][16 * R][DP + 4];  // rows padded: 16 lanes' rows start in different banks
+    float m[4][16 * R], l[4][16 * R];
+    int seen[16 * R], most;  // SHARED: tokens that each vector sees, the most of them
+};
 }  // namespace qlin

@@ -27,7 +27,9 @@
 // In 4 bits a code times its group's unit takes the code's place; it is as exact, and all else is the same.
 #pragma once
 
-#include "qlin_attend.hpp"
+#include <type_traits>
+
+#include "qlin_attend_classes.hpp"
 
 namespace qlin {
 namespace {
@@ -38,24 +40,15 @@ namespace {
 // 16 g .. + 15 of heads of 64), and columns n * DP/16 .. + DP/16 - 1 of values 4g .. 4g + 3 of each tile.
 template <int DP, int BITS>
 struct StepData {
-    static constexpr int KB = DP / 4 * BITS / 8, VB = DP / 16 * BITS / 8;  // bytes
+    // Bytes of a key, and of a value (8 bits) or of two tokens' values (4 bits)
+    static constexpr int KB = DP / 4 * BITS / 8, VB = DP / 16, VL = BITS == 8 ? 4 : 2;
     static constexpr int RUN = KB < 16 ? DP / 32 : 16 / BITS;
     static constexpr int KU = DP == 256 ? 2 : 1;  // groups of 32 columns that a lane's keys lie in
     Bytes<KB> k[2];
-    Bytes<VB> v[8];
+    Bytes<VB> v[2 * VL];
     float4v ks[2], vs[2];  // scales of tokens 4g .. 4g + 3
     uint32_t ku[2][KU], vu[2];  // 4 bits: units of key n, and of values 4g .. 4g + 3, a byte each
 };
-
-// Sum and maximum over the four lanes n, n + 16, n + 32, n + 48.
-template <bool MAX>
-__device__ __forceinline__ float over_groups(float x) {
-    typedef unsigned int pair __attribute__((ext_vector_type(2)));
-    pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
-    x = MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
-    return MAX ? fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) : __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 // Workgroup: 4 waves, R tiles of 16 vectors of one KV head, one part of the tokens.  The waves take
 // steps of 32 tokens in turn, each with a running maximum, sum and output of its own, and join
@@ -65,12 +58,6 @@ __device__ __forceinline__ float over_groups(float x) {
 // sequences of up to 4096 and a prefix of 8192 for 32 rows, against 7.4, 56.8 and 26.0).  f32 queries are such sums
 // too; fp16 ones are exact.
 // SHARED: the part of the prefix, for the rows of all sequences at once.
-template <int DP, int R>
-struct AttendLds {
-    alignas(16) float o[2][16 * R][DP + 4];  // rows padded: 16 lanes' rows start in different banks
-    float m[4][16 * R], l[4][16 * R];
-    int seen[16 * R], most;  // SHARED: tokens that each vector sees, the most of them
-};
 template <int DP, int BITS, int R, bool Q16, bool SHARED>
 __device__ __forceinline__ void attend_part(const AttendParams& p, int block, AttendLds<DP, R>& lds) {
     using Step = StepData<DP, BITS>;
@@ -182,7 +169,9 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
     };
     auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_bytes<Step::VB, 16>(d.v[i], next[i / 4].block, (4 * g + i % 4) * ROW + n * Step::VB, next[i / 4].v);
+        for (int i = 0; i < 2 * Step::VL; ++i)
+            load_bytes<Step::VB, 16>(d.v[i], next[i / Step::VL].block, (4 / Step::VL) * ((Step::VL * g + i % Step::VL) * ROW) + n * Step::VB,
+                                     next[i / Step::VL].v);
         if constexpr (BITS == 4)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -325,13 +314,8 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
                 w = uint4v{codes2(d.v[1].w[t / 4], d.v[0].w[t / 4], sel), codes2(d.v[3].w[t / 4], d.v[2].w[t / 4], sel),
                            codes2(d.v[5].w[t / 4], d.v[4].w[t / 4], sel), codes2(d.v[7].w[t / 4], d.v[6].w[t / 4], sel)};
             } else {
-                // the byte of columns t and t ^ 1 of two tokens, then its lower or upper nibble
-                const uint32_t at = t / 2 % 4, sel = 0x0c000c00u | (4 + at) << 16 | at;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t y = __builtin_amdgcn_perm(d.v[2 * i + 1].w[t / 8], d.v[2 * i].w[t / 8], sel);
-                    w[i] = nibbles2(t % 2 ? y : y << 4, vu[i]);
-                }
+                for (int i = 0; i < 4; ++i) w[i] = nibbles2(d.v[i].w[t / 4], t % 4, vu[i]);
             }
             const half8v a = __builtin_bit_cast(half8v, w);
 #pragma unroll
@@ -431,8 +415,8 @@ __device__ __forceinline__ void attend_part(const AttendParams& p, int block, At
 }
 
 // A launch: the first `shared` workgroups work on the prefix with RS tiles (0: there is none), the others on the
-// sequences' own tokens with RO.
-template <int DP, int BITS, int RS, int RO, bool Q16>
+// sequences' own tokens with RO, or CO classes of tokens for up to 16 / CO vectors.
+template <int DP, int BITS, int RS, int RO, bool Q16, int CO = 1>
 __global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 64 ? 4 : DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 128 ? 3 : 1)
 void attend_kernel(AttendParams p, int shared) {
     __shared__ union {
@@ -445,7 +429,8 @@ void attend_kernel(AttendParams p, int shared) {
             return;
         }
     }
-    attend_part<DP, BITS, RO, Q16, false>(p, blockIdx.x - shared, lds.own);
+    if constexpr (CO > 1) attend_classes<DP, CO, Q16>(p, blockIdx.x - shared, lds.own);
+    else attend_part<DP, BITS, RO, Q16, false>(p, blockIdx.x - shared, lds.own);
 }
 
 // Joins the parts of vectors: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  DP / 4 lanes hold a vector's
@@ -521,6 +506,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     store_out<4>(p, row * p.ldo + (int64_t)head * p.c.dim, d, y);
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 template <int DP, int BITS, bool Q16>
 hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     const int own = attend_tile(p), shared = p.prefix_parts ? attend_tile_prefix(p) : 0;
@@ -531,21 +519,29 @@ hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     if (own >= kAttendWide) return launch_attend_wide<BITS>(p, false, st);
     const uint32_t first = shared >= kAttendWide ? 0 : shared_blocks;
     const dim3 grid(first + own_blocks);
-    if (first == 0) {
-        if constexpr (DP <= 128)
-            if (own == 32) {
-                attend_kernel<DP, BITS, 0, 2, Q16><<<grid, 256, 0, st>>>(p, 0);
-                return hipGetLastError();
-            }
-        attend_kernel<DP, BITS, 0, 1, Q16><<<grid, 256, 0, st>>>(p, 0);
-        return hipGetLastError();
-    }
+    auto launch = [&](auto shared_tiles, auto own_tiles, auto classes) {
+        attend_kernel<DP, BITS, decltype(shared_tiles)::value, decltype(own_tiles)::value, Q16, decltype(classes)::value>
+            <<<grid, 256, 0, st>>>(p, first);
+    };
+    // one tile of vectors; in 4 bits of few of them with classes of tokens, whose steps lie in one page
+    auto launch_small = [&](auto shared_tiles) {
+        if constexpr (BITS == 4) {
+            const int64_t vectors = (int64_t)p.b.max_new * p.group.d;
+            if (vectors <= 4 && p.c.shift >= 6) return launch(shared_tiles, Int<1>{}, Int<4>{});
+            if (vectors <= 8 && p.c.shift >= 5) return launch(shared_tiles, Int<1>{}, Int<2>{});
+        }
+        launch(shared_tiles, Int<1>{}, Int<1>{});
+    };
     if constexpr (DP <= 128) {  // the prefix's rows are those of all sequences: at least as many
-        if (own == 32) attend_kernel<DP, BITS, 2, 2, Q16><<<grid, 256, 0, st>>>(p, first);
-        else if (shared == 32) attend_kernel<DP, BITS, 2, 1, Q16><<<grid, 256, 0, st>>>(p, first);
-        else attend_kernel<DP, BITS, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        if (own == 32 && first) launch(Int<2>{}, Int<2>{}, Int<1>{});
+        else if (own == 32) launch(Int<0>{}, Int<2>{}, Int<1>{});
+        else if (!first) launch_small(Int<0>{});
+        else if (shared == 32) launch_small(Int<2>{});
+        else launch_small(Int<1>{});
+    } else if (first) {
+        launch_small(Int<1>{});
     } else {
-        attend_kernel<DP, BITS, 1, 1, Q16><<<grid, 256, 0, st>>>(p, first);
+        launch_small(Int<0>{});
     }
     return hipGetLastError();
 }

@@ -47,9 +47,9 @@ template <int DP, int BITS>
 struct Share {
     static constexpr int SUBS = DP == 256 ? 2 : 1;
     static constexpr int KCOLS = DP / 16, VCOLS = DP / 4;  // lanes across a row
-    static constexpr int KB = 16 * BITS / 8, VB = 4 * BITS / 8;  // bytes
+    static constexpr int KB = 16 * BITS / 8, VL = BITS == 8 ? 4 : 2;  // bytes of a key; loads of values, of a token or of two
     Bytes<KB> k[SUBS];
-    Bytes<VB> v[SUBS][4];
+    uint32_t v[SUBS][VL];
     float ks[SUBS], vs[SUBS];
     uint32_t ku[SUBS], vu[SUBS];  // 4 bits: the key's unit, the four values' units, a byte each
     bool bad[SUBS];
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false;
     const int k_row = DP == 256 ? tid / 16 : tid % 128 / Sh::KCOLS % 16, k_at = k_row * ROW + tid % Sh::KCOLS * Sh::KB;
-    const int v_quad = DP == 256 ? wave : tid / Sh::VCOLS % 4, v_at = 4 * v_quad * ROW + tid % Sh::VCOLS * Sh::VB;
+    const int v_quad = DP == 256 ? wave : tid / Sh::VCOLS % 4, v_at = 4 * v_quad * ROW + tid % Sh::VCOLS * 4;
     const int ku_at = k_row + (tid % Sh::KCOLS * 16 / kKvGroup << p.c.shift), vu_at = 4 * v_quad + (tid % Sh::VCOLS * 4 / kKvGroup << p.c.shift);
     // A tile on its way: the page ids (loaded a step ahead of their use), the buffers, the bytes.
     int ids[Sh::SUBS];
@@ -203,7 +203,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
             sh.bad[i] = at[i].bad;
             load_bytes<Sh::KB, 16>(sh.k[i], at[i].block, k_at, at[i].k);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) load_bytes<Sh::VB, 16>(sh.v[i][x], at[i].block, v_at + x * ROW, at[i].v);
+            for (int x = 0; x < Sh::VL; ++x)
+                sh.v[i][x] = __builtin_amdgcn_raw_buffer_load_b32(at[i].block, v_at + x * (4 / Sh::VL * ROW), at[i].v, 0);
             if constexpr (BITS == 4) {
                 sh.ku[i] = __builtin_amdgcn_raw_buffer_load_b8(at[i].block, ku_at, at[i].ku, 0);
                 sh.vu[i] = __builtin_amdgcn_raw_buffer_load_b32(at[i].block, vu_at, at[i].vu, 0);
@@ -226,17 +227,13 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_wide_kerne
         } else {
             // tokens 4 quad + 0..3 of the half: quad 2 b + h goes to place 8 h + 4 b of 16
             const int place = 16 * half(i) + 8 * (v_quad & 1) + 4 * (v_quad >> 1);
-            const uint32_t byte = BITS == 8 ? x : x / 2, sel = 0x0c000c00u | (4 + byte) << 16 | byte;
             uint2v w;
+            if constexpr (BITS == 8) {
+                const uint32_t sel = 0x0c000c00u | (4 + x) << 16 | x;
+                w = uint2v{codes2(sh.v[i][1], sh.v[i][0], sel), codes2(sh.v[i][3], sh.v[i][2], sel)};
+            } else {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const uint32_t v0 = sh.v[i][2 * y].w[0], v1 = sh.v[i][2 * y + 1].w[0];
-                if constexpr (BITS == 8) {
-                    w[y] = codes2(v1, v0, sel);
-                } else {
-                    const uint32_t z = __builtin_amdgcn_perm(v1, v0, sel);
-                    w[y] = nibbles2(x % 2 ? z : z << 4, units2(sh.vu[i], 2 * y, 2 * y + 1));
-                }
+                for (int y = 0; y < 2; ++y) w[y] = nibbles2(sh.v[i][y], x, units2(sh.vu[i], 2 * y, 2 * y + 1));
             }
             // column d is row d / ND of tile d % ND: a lane's columns of all tiles are neighbours
             const int d = tid % Sh::VCOLS * 4 + x;

@@ -98,7 +98,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
             w[1] = *reinterpret_cast<const uint2*>(blk.v(off) + d0);
         } else {
             w[0].x = *reinterpret_cast<const uint32_t*>(blk.k(off) + d0 / 2);
-            w[1].x = *reinterpret_cast<const uint32_t*>(blk.v(off) + d0 / 2);
+            const uint16_t* v = blk.v4(d0 / 4, off);
+            w[1].x = v[0] | (uint32_t)v[2] << 16;
             unit[0] = *blk.ku(d0 / kKvGroup, off);
             unit[1] = *blk.vu(d0 / kKvGroup, off);
         }

@@ -24,7 +24,8 @@ constexpr int kKvGroup = 32;
 
 // The cache in device memory.  Codes of 8 bits are stored as code + 128, one byte each: a byte b between two
 // zero bytes is the fp16 subnormal b * 2^-24, so one byte permute and one packed FMA make two exact
-// fp16 codes of two bytes.  Codes of 4 bits are stored as code + 8, the lower nibble of a byte the even column.
+// fp16 codes of two bytes.  Codes of 4 bits are stored as code + 8, nibble c % 8 of a word column c; of values, which the
+// matrix core takes two tokens at a time, a word holds four columns of tokens 2 i and 2 i + 1, a half each.
 // Columns dim .. dim_padded - 1 hold code 0.
 //
 // A block of a page and head is contiguous: keys [page tokens][dim_padded], values alike, then the
@@ -47,6 +48,10 @@ struct KvBlock {
         : base(c.data + ((int64_t)page * c.heads + head) * kv_block_bytes(BITS, DP, c.shift)), shift(c.shift) {}
     __device__ uint8_t* k(int off) const { return base + off * ROW; }
     __device__ uint8_t* v(int off) const { return base + (((int64_t)ROW << shift) + off * ROW); }
+    // columns 4 q .. 4 q + 3 of a value (4 bits); the next four columns lie two halves further
+    __device__ uint16_t* v4(int q, int off) const {
+        return reinterpret_cast<uint16_t*>(base + (((int64_t)ROW << shift) + (off >> 1) * 2 * ROW)) + 2 * q + (off & 1);
+    }
     __device__ float* ks(int off) const { return reinterpret_cast<float*>(base + ((int64_t)(2 * ROW) << shift)) + off; }
     __device__ float* vs(int off) const { return ks(off + (1 << shift)); }
     // unit of group g (4 bits)

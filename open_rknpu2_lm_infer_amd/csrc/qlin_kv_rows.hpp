@@ -56,7 +56,13 @@ __device__ __forceinline__ bool quantize_row(const KvBlock<DP, BITS>& blk, int o
         if constexpr (BITS == 8) {
             *reinterpret_cast<uint2*>(row + d0) = make_uint2(w[0], w[1]);
         } else {
-            *reinterpret_cast<uint32_t*>(row + d0 / 2) = w[0];
+            if constexpr (VALUE) {
+                uint16_t* v = blk.v4(d0 / 4, off);
+                v[0] = (uint16_t)w[0];
+                v[2] = (uint16_t)(w[0] >> 16);
+            } else {
+                *reinterpret_cast<uint32_t*>(row + d0 / 2) = w[0];
+            }
             if (d0 % kKvGroup == 0) *(VALUE ? blk.vu(d0 / kKvGroup, off) : blk.ku(d0 / kKvGroup, off)) = (uint8_t)u;
         }
         if (d0 == 0) *(VALUE ? blk.vs(off) : blk.ks(off)) = s;
