@@ -27,6 +27,11 @@ int tile_of(const AttendParams& p, int64_t vectors) {
 
 int attend_tile(const AttendParams& p) { return tile_of(p, (int64_t)p.b.max_new * p.group.d); }
 int attend_tile_prefix(const AttendParams& p) { return tile_of(p, (int64_t)p.b.rows * p.group.d); }
+int attend_classes_of(const AttendParams& p) {
+    const int64_t vectors = (int64_t)p.b.max_new * p.group.d;
+    if (p.c.bits != 4) return 1;
+    return vectors <= 4 && p.c.shift >= 6 ? 4 : vectors <= 8 && p.c.shift >= 5 ? 2 : 1;
+}
 
 hipError_t launch_attend(const AttendParams& p, hipStream_t st) {
     return p.c.bits == 4 ? launch_attend_bits<4>(p, st) : launch_attend_bits<8>(p, st);

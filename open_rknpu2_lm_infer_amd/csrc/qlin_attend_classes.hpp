@@ -5,9 +5,16 @@
 // vectors times C classes of tokens: column n is vector n % (16 / C), and of the C tiles of 16 tokens that a step
 // has, it takes tile n / (16 / C).  The logits of all tiles are computed for all columns and each lane keeps its own
 // tile's; a column has a running maximum, sum and output over its tokens, P of a column is zero for the others' tokens, and
-// classes are joined as waves are.  Half of what is left is making fp16 of the nibbles.
+// classes are joined as waves are.  Two thirds of what is left for the vector units is making fp16 of the nibbles.
 //
 // A step's tokens lie in one page (pages of at least 16 C tokens): one id, one buffer, and a lane's scales in one load.
+//
+// What bounds it, 8 KV heads of 128, 4 query heads each (us, as graph nodes): HBM where there is much to read, 64 sequences of
+// 4096 tokens, 302 MB, 62, 4.9 TB/s; below that some 6 a workgroup that are no work of a step but the chain of loads
+// before the first (length, page id, bytes) and the join behind the last, and 1.4 a step and wave (one token over 300 tokens 6.7, over
+// 32768 in 256 workgroups 12.6 and 3.9 for the join's launch).  64 sequences of up to 4096 tokens 48 where all
+// columns' exponents are computed took 61.  Workgroups of 8 waves take 9% longer over 54 batches of 1 to 64 sequences of
+// 300 to 32768 tokens, and twice the parts 6%.
 #pragma once
 
 #include "qlin_attend.hpp"
@@ -38,27 +45,35 @@ __device__ __forceinline__ float4v own_class(const float4v (&x)[C], int cls) {
     return y;
 }
 
-// Largest (sum) over the lanes of a vector's classes.
+// Largest (sum) over the lanes of a vector's classes: rotations of a row of 16 lanes by 8, then by 4.
 template <int C, bool MAX>
 __device__ __forceinline__ float over_classes(float x) {
-#pragma unroll
-    for (int o = 16 / C; o < 16; o <<= 1) {
-        const float y = __shfl_xor(x, o, 64);
-        x = MAX ? fmaxf(x, y) : x + y;
+    const float y = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, true));  // row_ror:8
+    x = MAX ? fmaxf(x, y) : x + y;
+    if constexpr (C == 4) {
+        const float z = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, true));  // row_ror:4
+        x = MAX ? fmaxf(x, z) : x + z;
     }
     return x;
 }
 
+// What the waves of a workgroup join in.
+template <int DP, int C>
+struct ClassLds {
+    alignas(16) float o[4][16 / C][DP + 4];
+    float m[4][16 / C], l[4][16 / C];
+};
 template <int DP, int C, bool Q16>
-__device__ __forceinline__ void attend_classes(const AttendParams& p, int block, AttendLds<DP, 1>& lds) {
+__device__ __forceinline__ void attend_classes(const AttendParams& p, int block, ClassLds<DP, C>& lds) {
     using Step = ClassStep<DP, C>;
     constexpr int ROW = DP / 2, KS = DP / 32, DT = DP / 16, V = 16 / C, TOKENS = 16 * C, QL = Q16 ? 1 : 2, PL = 2;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, cls = n / V;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // heads fastest, parts slowest (see attend_part); one tile of vectors
+    // heads fastest, parts slowest (see attend_part), the last ones first: those of long sequences do not come to an end
+    // after all others, and those that are empty end at once; one tile of vectors
     const int h = p.by_heads.mod(block);
     const int b = p.by_heads.div(block);
-    const int seq = p.by_seqs.mod(b), part = p.by_seqs.div(b);
+    const int seq = p.by_seqs.mod(b), part = p.parts - p.prefix_parts - 1 - p.by_seqs.div(b);
     const int group = p.group.d;
 
     const int j0 = p.own_from + part * p.chunk;
@@ -235,75 +250,64 @@ __device__ __forceinline__ void attend_classes(const AttendParams& p, int block,
     }
     if (bad_page && lane == 0) atomicOr(p.err + kErrBatch, 1u);
 
-    // join the waves and classes: a common maximum, then waves 3 -> 1 and 2 -> 0, 1 -> 0, then the classes' lanes
+    // Join: the classes in the lanes of a row of 16, then the waves in the LDS, where a thread takes NC columns of a vector.
     l = over_groups<false>(l);
-    if (g == 0) {
-        lds.m[wave][n] = m;
-        lds.l[wave][n] = l;
-    }
-    __syncthreads();
-    const float m_all = over_classes<C, true>(fmaxf(fmaxf(lds.m[0][n], lds.m[1][n]), fmaxf(lds.m[2][n], lds.m[3][n])));
-    const float base = m_all == kNegInf ? 0.0f : m_all;
-    float l_all = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) l_all += lds.l[w][n] * __builtin_amdgcn_exp2f(lds.m[w][n] - base);
-    l_all = over_classes<C, false>(l_all);
-    const float fade = __builtin_amdgcn_exp2f(m - base);
-#pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] *= fade;
-    // columns (4 g + i) * DT + t of a vector, t = 4 u .. 4 u + 3
-    auto four = [&](int i, int u) -> float4v { return {o[4 * u][i], o[4 * u + 1][i], o[4 * u + 2][i], o[4 * u + 3][i]}; };
-    auto put = [&](int slot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int u = 0; u < DT / 4; ++u) *reinterpret_cast<float4v*>(&lds.o[slot][n][(4 * g + i) * DT + 4 * u]) = four(i, u);
-    };
-    auto add = [&](int slot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int u = 0; u < DT / 4; ++u) {
-                const float4v y = *reinterpret_cast<const float4v*>(&lds.o[slot][n][(4 * g + i) * DT + 4 * u]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[4 * u + c][i] += y[c];
-            }
-    };
-    if (wave >= 2) put(wave - 2);
-    __syncthreads();
-    if (wave < 2) add(wave);
-    __syncthreads();
-    if (wave == 1) put(0);
-    __syncthreads();
-    if (wave != 0) return;
-    add(0);
+    const float m_wave = over_classes<C, true>(m);
+    const float fade = m_wave == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_wave);
+    l = over_classes<C, false>(l * fade);
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][i] = over_classes<C, false>(o[t][i]);
-    if (seen < 0 || cls != 0) return;
+        for (int i = 0; i < 4; ++i) o[t][i] = over_classes<C, false>(o[t][i] * fade);
+    if (cls == 0) {
+        // columns (4 g + i) * DT + t of a vector
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < DT; u += 4)
+                *reinterpret_cast<float4v*>(&lds.o[wave][v][(4 * g + i) * DT + u]) = float4v{o[u][i], o[u + 1][i], o[u + 2][i], o[u + 3][i]};
+        if (g == 0) {
+            lds.m[wave][v] = m_wave;
+            lds.l[wave][v] = l;
+        }
+    }
+    __syncthreads();
+    constexpr int NC = V * DP / 256;
+    const int vec = tid / (DP / NC), d0 = tid % (DP / NC) * NC;
+    if (vec >= vectors) return;
+    float w[4], m_all = kNegInf, l_all = 0.0f, y[NC] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m_all = fmaxf(m_all, lds.m[i][vec]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = m_all == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(lds.m[i][vec] - m_all);
+        l_all = __builtin_fmaf(w[i], lds.l[i][vec], l_all);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) y[c] = __builtin_fmaf(w[i], lds.o[i][vec][d0 + c], y[c]);
+    }
+    const int64_t row = s.row0 + p.group.div(vec);
+    const int at = h * group + p.group.mod(vec);
     if (p.parts == 1) {
         const float f = l_all == 0.0f ? 0.0f : kCodeUnit<4> / l_all;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int u = 0; u < DT / 4; ++u) {
-                const float4v y = four(i, u) * f;
-                const float z[4] = {y[0], y[1], y[2], y[3]};
-                store_out<4>(p, out_row * p.ldo + (int64_t)head * p.c.dim, (4 * g + i) * DT + 4 * u, z);
-            }
+        for (int c = 0; c < NC; ++c) y[c] *= f;
+        store_out<NC>(p, row * p.ldo + (int64_t)at * p.c.dim, d0, y);
     } else {
-        const int64_t slot = (out_row * p.q_heads + head) * p.parts + p.prefix_parts + part;
+        const int64_t slot = (row * p.q_heads + at) * p.parts + p.prefix_parts + part;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int u = 0; u < DT / 4; ++u)
-                *reinterpret_cast<float4v*>(p.part_o + slot * DP + (4 * g + i) * DT + 4 * u) = four(i, u);
-        if (g == 0) {
+        for (int c = 0; c < NC; ++c) p.part_o[slot * DP + d0 + c] = y[c];
+        if (d0 == 0) {
             p.part_ml[2 * slot] = m_all;
             p.part_ml[2 * slot + 1] = l_all;
         }
     }
+}
+
+// A launch of them without a prefix.
+template <int DP, int C, bool Q16>
+__global__ __launch_bounds__(256) void attend_classes_kernel(AttendParams p) {
+    __shared__ ClassLds<DP, C> lds;
+    attend_classes<DP, C, Q16>(p, blockIdx.x, lds);
 }
 
 }  // namespace

@@ -420,8 +420,8 @@ template <int DP, int BITS, int RS, int RO, bool Q16, int CO = 1>
 __global__ __launch_bounds__(256, DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 64 ? 4 : DP * (RS > RO ? RS : RO) * (Q16 ? 1 : 2) <= 128 ? 3 : 1)
 void attend_kernel(AttendParams p, int shared) {
     __shared__ union {
-        AttendLds<DP, (RS > 0 ? RS : RO)> prefix;
-        AttendLds<DP, RO> own;
+        AttendLds<DP, (RS > 0 ? RS : 1)> prefix;
+        std::conditional_t<(CO > 1), ClassLds<DP, (CO > 1 ? CO : 2)>, AttendLds<DP, RO>> own;
     } lds;
     if constexpr (RS > 0) {
         if ((int)blockIdx.x < shared) {
@@ -520,15 +520,15 @@ hipError_t launch_typed(const AttendParams& p, hipStream_t st) {
     const uint32_t first = shared >= kAttendWide ? 0 : shared_blocks;
     const dim3 grid(first + own_blocks);
     auto launch = [&](auto shared_tiles, auto own_tiles, auto classes) {
-        attend_kernel<DP, BITS, decltype(shared_tiles)::value, decltype(own_tiles)::value, Q16, decltype(classes)::value>
-            <<<grid, 256, 0, st>>>(p, first);
+        constexpr int RS = decltype(shared_tiles)::value, RO = decltype(own_tiles)::value, C = decltype(classes)::value;
+        if constexpr (RS == 0 && C > 1) attend_classes_kernel<DP, C, Q16><<<grid, 256, 0, st>>>(p);
+        else attend_kernel<DP, BITS, RS, RO, Q16, C><<<grid, 256, 0, st>>>(p, first);
     };
-    // one tile of vectors; in 4 bits of few of them with classes of tokens, whose steps lie in one page
+    // one tile of vectors, or part of one with classes of tokens
     auto launch_small = [&](auto shared_tiles) {
         if constexpr (BITS == 4) {
-            const int64_t vectors = (int64_t)p.b.max_new * p.group.d;
-            if (vectors <= 4 && p.c.shift >= 6) return launch(shared_tiles, Int<1>{}, Int<4>{});
-            if (vectors <= 8 && p.c.shift >= 5) return launch(shared_tiles, Int<1>{}, Int<2>{});
+            if (attend_classes_of(p) == 4) return launch(shared_tiles, Int<1>{}, Int<4>{});
+            if (attend_classes_of(p) == 2) return launch(shared_tiles, Int<1>{}, Int<2>{});
         }
         launch(shared_tiles, Int<1>{}, Int<1>{});
     };

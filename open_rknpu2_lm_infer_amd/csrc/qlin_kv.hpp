@@ -111,6 +111,9 @@ constexpr int kAttendStep = 128;
 // Vectors of a workgroup: over a sequence's own tokens, over the prefix.
 int attend_tile(const AttendParams& p);
 int attend_tile_prefix(const AttendParams& p);
+// Classes of tokens that the kernel for few vectors gives the matrix core's columns to (4 bits; 1: vectors have them all).  A
+// step's tokens, 16 a class, have to lie in one page.
+int attend_classes_of(const AttendParams& p);
 constexpr int kAttendWide = 128;  // of the kernel for many vectors
 hipError_t launch_attend(const AttendParams& p, hipStream_t stream);
 template <int BITS>

@@ -133,11 +133,12 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.own_from = apart ? prefix : 0;
     // The kernel for few vectors runs best with one workgroup a CU (64 sequences of up to 4096 tokens: 73 us
     // uncut, 76 and 80 us in parts of 1024 and 512); parts of 2048 tokens bound what a single long sequence of a
-    // ragged batch costs.  The one for many vectors has two workgroups a CU, of which the second hides the first's
+    // ragged batch costs (4 bits and very few vectors: of 4096 tokens; 64 sequences of 4096 tokens 64 us, of up to 4096 52,
+    // with parts of 1024 74 and 51, of 2048 74 and 52).  The one for many vectors has two workgroups a CU, of which the second hides the first's
     // waits; the prefix, whose results are all joined, one.
     const bool few = attend_tile(p) < kAttendWide;
     int parts = 1;
-    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, few ? wp.cu_count : 2 * wp.cu_count, few ? 2048 : kKvMaxLen,
+    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, few ? wp.cu_count : 2 * wp.cu_count, !few ? kKvMaxLen : attend_classes_of(p) > 1 ? 4096 : 2048,
         apart ? cap / 2 : cap, &parts, &p.chunk);
     if (apart) cut(prefix, prefix_blocks, wp.cu_count, kKvMaxLen, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
