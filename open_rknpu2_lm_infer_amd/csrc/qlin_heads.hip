@@ -6,8 +6,8 @@
 // The angle is position * w_i quarter turns in 64 bits less the nearest whole number: what is left, at most half a
 // quarter turn, is exact to 2^-26 of a quarter in f32 however far the position is, and the whole number's last two
 // bits say which of (c, s), (-s, c), (-c, -s), (s, -c) it is.  sin and cos of up to an eighth of a turn are their
-// series to the 9th and 10th power, the next terms being 2e-9 and 5e-10.  No table of positions is read: a lane has
-// four pairs, whose factors it computes once a row for all heads it works on.
+// series to the 9th and 10th power, the next terms being 2e-9 and 5e-10.  No table of positions is read: a workgroup
+// computes its rows' factors, one a thread, into the LDS, from where the lanes of all their heads have them.
 //
 // A group of dim_padded / 8 lanes holds a head, 8 values a lane: four pairs, or eight of the columns that are not
 // turned.  Every value is read by the lane that writes it, so rows may be worked on in place.  Keys on their way into
@@ -66,35 +66,46 @@ __device__ __forceinline__ void load4(const T* p, float* x) {
 template <int DP, bool WIDE, typename T, bool VEC, int BITS>
 __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
     constexpr int LPH = DP / 8 * (WIDE ? 2 : 1), GROUPS = 256 / LPH;
-    __shared__ __align__(16) float lds[BITS ? GROUPS : 1][BITS ? DP + 4 : 4];
+    __shared__ __align__(16) float angles[4][DP];  // cosine and sine of the pairs of a row
+    __shared__ __align__(16) float keys[BITS ? GROUPS : 1][BITS ? DP + 4 : 4];
     const int lane = threadIdx.x % LPH, group = threadIdx.x / LPH;
-    int64_t row;
-    int pos = 0, off = 0, page = -1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // rows row0 .. row0 + rows - 1, at positions pos0 .. (batch)
+    int block = blockIdx.x;
+    if constexpr (BITS != 0) {
+        // workgroups go to the 8 XCDs in turn: those of neighbouring rows to one of them, in whose L2 the scales of a page's
+        // tokens come together
+        const int xcd = block % 8, all = gridDim.x;
+        block = xcd * (all / 8) + min(xcd, all % 8) + block / 8;
+    }
+    const int unit = p.by_splits.div(block), split = p.by_splits.mod(block);
+    int64_t row0;
+    int rows, pos0 = 0, seq = 0;
     bool bad = false;
-    const int unit = p.by_splits.div(blockIdx.x), split = p.by_splits.mod(blockIdx.x);
     if constexpr (BITS == 0) {
-        row = unit;
-        if (p.rope.rotary) pos = p.positions[row];
+        row0 = (int64_t)unit * p.block_rows;
+        rows = (int)min((int64_t)p.block_rows, p.rows - row0);
     } else {
-        const int i = p.by_new.div(unit), t = p.by_new.mod(unit);
-        const KvSeq s = kv_seq(p.b.row_start, p.b.length, i, p.b.rows, p.b.max_new, p.b.max_len);
+        seq = p.by_new.div(unit);
+        const int t = p.by_new.mod(unit) * p.block_rows;
+        const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
         bad = s.bad;
         if (t >= s.rows) {
             if (bad && threadIdx.x == 0) atomicOr(p.err + kErrBatch, 1u);
             return;
         }
-        row = s.row0 + t;
-        pos = s.len - s.rows + t;
-        off = pos & ((1 << p.c.shift) - 1);
-        // nothing is stored of a sequence whose row starts or length are at fault
-        if (!bad && pos >= 0) {
-            const int id = kv_page(p.b.table[i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
-            page = bad ? -1 : id;
-        }
+        row0 = s.row0 + t;
+        rows = min(p.block_rows, s.rows - t);
+        pos0 = s.len - s.rows + t;
     }
+    const bool by_wave = p.block_rows > 1;
+    const int r = by_wave ? wave : 0;  // this group's row
+    const bool works = r < rows;
+    const int64_t row = row0 + r;
 
     // the columns of queries and keys: pairs first, then those that are not turned
-    const int pairs = p.rope.rotary / 2, turned = (pairs + 3) / 4, first = p.rope.first;
+    const int pairs = p.rope.rotary / 2, first = p.rope.first;
+    const int turned = (pairs + 3) / 4;
     const bool turns = lane < turned;
     const int e0 = 8 * (lane - turned), rest = p.dim - p.rope.rotary;
     auto column = [&](int j) {  // of value j, -1: none
@@ -106,10 +117,12 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
         const int e = e0 + j;
         return e < rest ? (e < first ? e : e + p.rope.rotary) : -1;
     };
-    const Blocks qk = {max(column(0), 0), max(column(4), 0), column(0) >= 0, column(4) >= 0};
     const Blocks straight = {8 * lane, 8 * lane + 4, 8 * lane < p.dim, 8 * lane + 4 < p.dim};
+    const Blocks qk = VEC ? Blocks{max(column(0), 0), max(column(4), 0), column(0) >= 0, column(4) >= 0} : straight;
 
-    const int heads = p.q_heads + (BITS ? 2 : 1) * p.k_heads, step = p.splits * GROUPS;
+    constexpr int PER_WAVE = 64 / LPH;
+    const int heads = p.q_heads + (BITS ? 2 : 1) * p.k_heads;
+    const int step = p.splits * (by_wave ? PER_WAVE : GROUPS);
     auto load = [&](int h, float* x) {
         const T* at = reinterpret_cast<const T*>(p.x) + row * p.ldx + (int64_t)h * p.dim;
         const bool value = BITS && h >= p.q_heads + p.k_heads;
@@ -123,34 +136,62 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int c = value ? (8 * lane + j < p.dim ? 8 * lane + j : -1) : column(j);
-                if (c >= 0) x[j] = ld1<T>(at, c);
+                const float y = ld1<T>(at, max(c, 0));  // loads without branches: none waits for another
+                x[j] = c >= 0 ? y : 0.0f;
             }
         }
     };
 
-    int h = split * GROUPS + group;
-    float x[8];
-    if (h < heads) load(h, x);
-    float g[2][8];
+    // the first head's values and the norms' factors do not wait for the angles
+    int h = by_wave ? split * PER_WAVE + group % PER_WAVE : split * GROUPS + group;
+    float x[8] = {};
+    if (works && h < heads) load(h, x);
+    float g[2][8] = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int c = column(j);
-        g[0][j] = p.q_gamma && c >= 0 ? p.q_gamma[c] : 0.0f;
-        g[1][j] = p.k_gamma && c >= 0 ? p.k_gamma[c] : 0.0f;
+    for (int k = 0; k < 2; ++k) {
+        const float* gamma = k ? p.k_gamma : p.q_gamma;
+        if (!gamma) continue;
+        if constexpr (VEC) {
+            if (qk.has_a) load4<float>(gamma + qk.a, g[k]);
+            if (qk.has_b) load4<float>(gamma + qk.b, g[k] + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[k][j] = gamma[max(column(j), 0)];
+        }
     }
+    for (int k = threadIdx.x; k < rows * pairs; k += 256) {
+        const int y = p.by_pairs.div(k), i = p.by_pairs.mod(k);
+        int pos = pos0 + y;
+        if constexpr (BITS == 0) pos = p.positions[row0 + y];
+        float c, s;
+        turn(pos * p.rope.quarters[i], c, s);
+        angles[y][2 * i] = c * p.rope.amplitude;
+        angles[y][2 * i + 1] = s * (p.inverse ? -p.rope.amplitude : p.rope.amplitude);
+    }
+    int off = 0, page = -1;
+    if constexpr (BITS != 0) {
+        const int pos = pos0 + r;
+        off = pos & ((1 << p.c.shift) - 1);
+        // nothing is stored of a sequence whose row starts or length are at fault
+        if (!bad && works && pos >= 0) {
+            const int id = kv_page(p.b.table[seq * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
+            page = bad ? -1 : id;
+        }
+    }
+    __syncthreads();
     float co[4] = {}, si[4] = {};
-    if (turns) {
+    if (turns && works) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            turn(pos * p.rope.quarters[min(4 * lane + i, pairs - 1)], co[i], si[i]);
-            co[i] *= p.rope.amplitude;
-            si[i] *= p.inverse ? -p.rope.amplitude : p.rope.amplitude;
+            const int at = 2 * (VEC ? 4 * lane + i : min(4 * lane + i, pairs - 1));
+            co[i] = angles[r][at];
+            si[i] = angles[r][at + 1];
         }
     }
 
     bool finite = true;
-    while (h < heads) {
-        float next[8];
+    while (works && h < heads) {
+        float next[8] = {};
         if (h + step < heads) load(h + step, next);
         const bool query = h < p.q_heads, value = BITS && h >= p.q_heads + p.k_heads;
         if (!value) {
@@ -158,32 +199,31 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-#pragma unroll
-                for (int o = 1; o < LPH; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                sum = lanes_sum<LPH>(sum);
                 // at least the smallest normal number: what v_rsq_f32 gives for less is no number to scale zeros by.  (A
                 // NaN stays one.)
-                const float m = __builtin_fmaf(sum, p.inv_dim, p.eps), r = __builtin_amdgcn_rsqf(m < 0x1p-126f ? 0x1p-126f : m);
+                const float m = __builtin_fmaf(sum, p.inv_dim, p.eps), f = __builtin_amdgcn_rsqf(m < 0x1p-126f ? 0x1p-126f : m);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = (x[j] * r) * (query ? g[0][j] : g[1][j]);
+                for (int j = 0; j < 8; ++j) x[j] = (x[j] * f) * (query ? g[0][j] : g[1][j]);
             }
             if (turns) {
+                auto rotate = [&](float& l, float& r, int i) {
+                    const float y = __builtin_fmaf(l, co[i], -(r * si[i]));
+                    r = __builtin_fmaf(r, co[i], l * si[i]);
+                    l = y;
+                };
+                if (p.rope.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float l = p.rope.interleaved ? x[2 * i] : x[i], r = p.rope.interleaved ? x[2 * i + 1] : x[4 + i];
-                    const float yl = __builtin_fmaf(l, co[i], -(r * si[i])), yr = __builtin_fmaf(r, co[i], l * si[i]);
-                    if (p.rope.interleaved) {
-                        x[2 * i] = yl;
-                        x[2 * i + 1] = yr;
-                    } else {
-                        x[i] = yl;
-                        x[4 + i] = yr;
-                    }
+                    for (int i = 0; i < 4; ++i) rotate(x[2 * i], x[2 * i + 1], i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) rotate(x[i], x[4 + i], i);
                 }
             }
         }
         if (BITS == 0 || query) {
             const int64_t at = row * p.ldy + (int64_t)h * p.dim;
-            if (VEC && p.y_vec) {
+            if constexpr (VEC) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     if (!(k ? qk.has_b : qk.has_a)) continue;
@@ -209,13 +249,28 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
             const int d0 = 8 * lane;
             if (!value) {
                 // a head's lanes are of one wave, whose accesses to the LDS are done in their order
+                float* to = keys[group];
+                if constexpr (VEC) {
+                    if (qk.has_a) *reinterpret_cast<float4v*>(to + qk.a) = float4v{x[0], x[1], x[2], x[3]};
+                    if (qk.has_b) *reinterpret_cast<float4v*>(to + qk.b) = float4v{x[4], x[5], x[6], x[7]};
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (const int c = column(j); c >= 0) lds[group][c] = x[j];
+                    for (int j = 0; j < 8; ++j)
+                        if (const int c = column(j); c >= 0) to[c] = x[j];
+                }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
+                if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = d0 + j < p.dim ? lds[group][min(d0 + j, DP - 1)] : 0.0f;
+                    for (int k = 0; k < 2; ++k) {
+                        const float4v y = *reinterpret_cast<const float4v*>(to + d0 + 4 * k);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[4 * k + j] = d0 + 4 * k < p.dim ? y[j] : 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = d0 + j < p.dim ? to[min(d0 + j, DP - 1)] : 0.0f;
+                }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
             }
@@ -230,7 +285,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
         for (int j = 0; j < 8; ++j) x[j] = next[j];
     }
     if constexpr (BITS != 0) {
-        if (bad && threadIdx.x == 0) atomicOr(p.err + kErrBatch, 1u);
+        if (bad && threadIdx.x % 64 == 0) atomicOr(p.err + kErrBatch, 1u);
         if (!finite) atomicOr(p.err + kErrNonfinite, 1u);
     }
 }
@@ -238,7 +293,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
 template <int DP, int BITS, typename T>
 hipError_t launch_typed(const HeadsParams& p, dim3 grid, hipStream_t st) {
     // four columns side by side: pairs and the others are groups of eight, heads and rows of four
-    const bool vec = p.x_vec && p.dim % 4 == 0 && p.rope.rotary % 8 == 0 && p.rope.first % 4 == 0;
+    const bool vec = p.vec && p.dim % 4 == 0 && p.rope.rotary % 8 == 0 && p.rope.first % 4 == 0;
     if (vec) heads_kernel<DP, false, T, true, BITS><<<grid, 256, 0, st>>>(p);
     else if (heads_wide(p)) heads_kernel<DP, true, T, false, BITS><<<grid, 256, 0, st>>>(p);
     else heads_kernel<DP, false, T, false, BITS><<<grid, 256, 0, st>>>(p);
@@ -261,13 +316,13 @@ int lanes(const HeadsParams& p) { return p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 3
 bool heads_wide(const HeadsParams& p) {
     return (p.rope.rotary / 2 + 3) / 4 + (p.dim - p.rope.rotary + 7) / 8 > lanes(p);
 }
-int heads_at_once(const HeadsParams& p) { return 256 / (lanes(p) * (heads_wide(p) ? 2 : 1)); }
+int heads_at_once(const HeadsParams& p) { return 64 / (lanes(p) * (heads_wide(p) ? 2 : 1)); }
 
 hipError_t launch_heads(const HeadsParams& p, hipStream_t st) {
-    return launch_bits<0>(p, dim3((uint32_t)((int64_t)p.rows * p.splits)), st);
+    return launch_bits<0>(p, dim3((uint32_t)(((int64_t)p.rows + p.block_rows - 1) / p.block_rows * p.splits)), st);
 }
 hipError_t launch_heads_append(const HeadsParams& p, hipStream_t st) {
-    const dim3 grid((uint32_t)((int64_t)p.b.seqs * p.b.max_new * p.splits));
+    const dim3 grid((uint32_t)((int64_t)p.b.seqs * p.by_new.d * p.splits));
     return p.c.bits == 4 ? launch_bits<4>(p, grid, st) : launch_bits<8>(p, grid, st);
 }
 

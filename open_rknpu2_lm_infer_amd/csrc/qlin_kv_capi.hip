@@ -247,10 +247,9 @@ int qlin_kv_append_qkv(qlin_workspace* ws, qlin_kv_cache* cache, const qlin_kv_b
     heads_common(&p, rope, cache->c.dim, q_heads, cache->c.heads, q_gamma, k_gamma, eps, QKV, dtype == QLIN_F16, ld, Q,
                  q_dtype == QLIN_F16, ldq);
     p.c = cache->c;
-    p.by_new = fast_div(p.b.max_new);
     p.rne = (flags & QLIN_ROUND_HALF_EVEN) != 0;
     p.err = parts.err;
-    heads_split(&p, (int64_t)p.b.seqs * p.b.max_new, (int)heads);
+    heads_split(&p, p.b.seqs, p.b.max_new, (int)heads);
     return launch_heads_append(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
 }
 

@@ -1,18 +1,42 @@
 // Rows on their way into the key/value cache and back: what append, read and the pass from the qkv projection share.
 #pragma once
 
+#include <type_traits>
+
 #include "qlin_kv.hpp"
 #include "qlin_rows.hpp"
 
 namespace qlin {
 
-// Largest of a value over the 2, 4 .. N lanes of a group.
+// f over the N lanes of a group (2 .. 64, aligned), each step joining halves of twice the lanes: exchanges within four lanes, mirrors of
+// eight and of sixteen, then swaps of rows and halves of the wave.  FROM: lanes that agree already.
+template <int N, int FROM = 1, typename F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x, F f) {
+    auto dpp = [&](auto ctrl) { return f(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true)); };
+    if constexpr (N > 1 && FROM <= 1) x = dpp(std::integral_constant<int, 0xb1>{});   // quad_perm 1 0 3 2
+    if constexpr (N > 2 && FROM <= 2) x = dpp(std::integral_constant<int, 0x4e>{});   // quad_perm 2 3 0 1
+    if constexpr (N > 4 && FROM <= 4) x = dpp(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    if constexpr (N > 8 && FROM <= 8) x = dpp(std::integral_constant<int, 0x140>{});  // row_mirror
+    typedef unsigned int pair __attribute__((ext_vector_type(2)));
+    if constexpr (N > 16 && FROM <= 16) {
+        const pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(x, x, false, false));
+        x = f(r[0], r[1]);
+    }
+    if constexpr (N > 32 && FROM <= 32) {
+        const pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(x, x, false, false));
+        x = f(r[0], r[1]);
+    }
+    return x;
+}
+template <int N, int FROM = 1>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+    return over_lanes<N, FROM>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
 template <int N>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t m, int from = 1) {
-#pragma unroll
-    for (int o = 1; o < N; o <<= 1)
-        if (o >= from) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    return m;
+__device__ __forceinline__ float lanes_sum(float x) {
+    return __uint_as_float(over_lanes<N>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
 }
 
 // Quantizes columns d0 .. d0 + 7 of a row, x (zeros past the head), of which DP / 8 lanes hold the rest, and stores
@@ -30,7 +54,7 @@ __device__ __forceinline__ bool quantize_row(const KvBlock<DP, BITS>& blk, int o
     uint32_t a = 0;
     if constexpr (BITS == 4) {
         a = lanes_max<kKvGroup / 8>(m);
-        m = lanes_max<DP / 8>(a, kKvGroup / 8);
+        m = lanes_max<DP / 8, kKvGroup / 8>(a);
     } else {
         m = lanes_max<DP / 8>(m);
     }
@@ -43,14 +67,19 @@ __device__ __forceinline__ bool quantize_row(const KvBlock<DP, BITS>& blk, int o
             inv = 1.0f / (u * s);
         }
     }
-    uint32_t w[BITS / 4] = {};
+    // codes side by side, sums of shifted ones: each is above zero with what is added to all of them
+    uint32_t w[BITS / 4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = fin ? x[i] : 0.0f;
-        const int c = rne ? quant_finite<true>(v, inv) : quant_finite<false>(v, inv);
-        if constexpr (BITS == 8) w[i / 4] |= (uint32_t)(c + 128) << (8 * (i % 4));
-        else w[0] |= (uint32_t)(c + 8) << (4 * i);
-    }
+    for (int i = 0; i < BITS / 4; ++i) w[i] = BITS == 8 ? 0x80808080u : 0x88888888u;
+    auto pack = [&](auto even) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = quant_finite<decltype(even)::value>(fin ? x[i] : 0.0f, inv);
+            w[BITS == 8 ? i / 4 : 0] += (uint32_t)c << (BITS * (BITS == 8 ? i % 4 : i));
+        }
+    };
+    if (rne) pack(std::true_type{});
+    else pack(std::false_type{});
     if (store) {
         uint8_t* row = VALUE ? blk.v(off) : blk.k(off);
         if constexpr (BITS == 8) {

@@ -7,10 +7,13 @@
 // Every sum is a scan, so that nothing depends on the order in which threads run.  Sums grow along the slots: who is
 // refused for want of rows (or pages) is followed by none that is granted some, and what the granted take is the sum itself.
 //
-// One workgroup scans, 1024 slots at a time.  Whose the k-th row, page taken or page given back is, is found by a binary
-// search in the scanned starts.  With few rows the same workgroup does that too, with the starts in the LDS: one launch;
-// with more, two more launches do: the pages given back have to lie in the list before any is taken.
+// One workgroup scans, up to 4096 slots at a time, and gives pages back; whose the k-th row, page taken or page given back is,
+// is found by a binary search in the scanned starts, which lie in the LDS up to 4096 slots.  With few rows the same
+// workgroup takes pages and writes the rows' maps too: one launch.  With more a second launch does, the first having laid
+// down its starts.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "qlin_kv.hpp"
 #include "qlin_kv_step.hpp"
@@ -19,7 +22,24 @@ namespace qlin {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-enum : int { kCount = 0, kAvail = 1, kNeed = 2, kBack = 3, kRows = 4, kTotals = 8 };
+enum : int { kAvail = 0, kNeed = 1, kRows = 2, kTotals = 4 };
+
+// Sum over the lanes up to this one of its wave, or of its row of 16.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_from(int x) {
+    return step_add(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, ROWS == 0xf));
+}
+__device__ __forceinline__ int row_scan(int x) {
+    x = add_from<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+    x = add_from<0x112, 0xf>(x);
+    x = add_from<0x114, 0xf>(x);
+    return add_from<0x118, 0xf>(x);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x = row_scan(x);
+    x = add_from<0x142, 0xa>(x);     // the last lane of rows 0 and 2 to rows 1 and 3
+    return add_from<0x143, 0xc>(x);  // lane 31 to the upper half
+}
 
 // Inclusive sums of N values over the workgroup, and their totals.
 template <int N>
@@ -28,17 +48,10 @@ struct Scan {
 };
 template <int N>
 __device__ __forceinline__ Scan<N> scan(const int (&v)[N], int (*lds)[kWaves]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Scan<N> s;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s.at[k] = v[k];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int y = __shfl_up(s.at[k], o, 64);
-            s.at[k] = step_add(s.at[k], lane >= o ? y : 0);
-        }
+    for (int k = 0; k < N; ++k) s.at[k] = wave_scan(v[k]);
     __syncthreads();  // who still reads an earlier scan's
     if (lane == 63)
 #pragma unroll
@@ -46,162 +59,228 @@ __device__ __forceinline__ Scan<N> scan(const int (&v)[N], int (*lds)[kWaves]) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        int before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const int x = lds[k][w];
-            before = w < wave ? step_add(before, x) : before;
-            all = step_add(all, x);
-        }
-        s.at[k] = step_add(s.at[k], before);
-        s.total[k] = all;
+        const int all = row_scan(lds[k][lane % kWaves]);
+        s.total[k] = __builtin_amdgcn_readlane(all, kWaves - 1);
+        s.at[k] = step_add(s.at[k], wave == 0 ? 0 : __builtin_amdgcn_readlane(all, max(wave - 1, 0)));
     }
     return s;
 }
 
-// Pages given back: from the table to the free list, from thread `first` on every `stride`.
+// Pages given back: from the table to the free list, from thread `first` on every `stride`, four at a time.
 template <typename P>
 __device__ __forceinline__ void give_back(const StepParams& p, P back_start, int count, int total, int first, int stride) {
-    for (int k = first; k < total; k += stride) {
-        const int i = step_owner(back_start, p.seqs, k);
-        const int column = step_columns(p.length[i], p.shift, p.shared) + k - back_start[i];
-        int32_t* at = p.table + i * p.table_ld + column;
-        const int id = *at;
-        *at = -1;
-        bool bad = count + k >= p.pages;  // more pages than there are: some were in the list already
-        if (!bad) p.free_pages[count + k] = id;
-        kv_page(id, p.pages, &bad);
-        if (bad) atomicOr(p.err + kErrBatch, 1u);
-    }
-}
-
-// Pages taken and the rows' maps.  What the list holds is not written here, and of the table only what a slot is given.
-template <typename P>
-__device__ __forceinline__ void take(const StepParams& p, P need_start, P row_start, int avail, int need, int rows, int first, int stride) {
-    for (int k = first; k < need; k += stride) {
-        const int i = step_owner(need_start, p.seqs, k);
-        const int old = p.length[i] - (row_start[i + 1] - row_start[i]);
-        const int id = p.free_pages[avail - 1 - k];
-        p.table[i * p.table_ld + step_columns(old, p.shift, p.shared) + k - need_start[i]] = id;
-        bool bad = false;
-        kv_page(id, p.pages, &bad);
-        if (bad) atomicOr(p.err + kErrBatch, 1u);
-    }
-    if (!p.row_seq && !p.positions && !p.slots) return;
-    for (int r = first; r < rows; r += stride) {
-        const int i = step_owner(row_start, p.seqs, r);
-        const int begin = row_start[i], old = p.length[i] - (row_start[i + 1] - begin), pos = old + r - begin;
-        if (p.row_seq) p.row_seq[r] = i;
-        if (p.positions) p.positions[r] = pos;
-        if (p.slots) {
-            // a page taken in this step comes from the list, as its table entry is being written
-            const int column = pos >> p.shift, fresh = column - step_columns(old, p.shift, p.shared);
-            const int id = fresh >= 0 ? p.free_pages[avail - 1 - (need_start[i] + fresh)] : p.table[i * p.table_ld + column];
-            p.slots[r] = ((int64_t)id << p.shift) + (pos & ((1 << p.shift) - 1));
+    constexpr int U = 4;
+    for (int k0 = first; k0 < total; k0 += U * stride) {
+        int k[U], i[U], id[U];
+        int32_t* at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = min(k0 + u * stride, total - 1);  // the last one again, which is stored once
+        step_owners<U>(back_start, p.seqs, k, i);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            at[u] = p.table + i[u] * p.table_ld + step_columns(p.length[i[u]], p.shift, p.shared) + k[u] - back_start[i[u]];
+            id[u] = *at[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * stride >= total) continue;
+            *at[u] = -1;
+            bool bad = count + k[u] >= p.pages;  // more pages than there are: some were in the list already
+            if (!bad) p.free_pages[count + k[u]] = id[u];
+            kv_page(id[u], p.pages, &bad);
+            if (bad) atomicOr(p.err + kErrBatch, 1u);
         }
     }
 }
 
-// ALL: up to 1024 slots, and the rows and pages too.
-template <bool ALL>
-__global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p) {
+// Pages taken and the rows' maps, U at a time.  What the list holds is not written here, and of the table only what a slot is given.
+template <int U, typename P>
+__device__ __forceinline__ void take(const StepParams& p, P need_start, P row_start, int avail, int need, int rows, int first, int stride) {
+    const int items = p.row_seq || p.positions || p.slots ? rows : 0;
+    for (int k0 = first; k0 < max(need, items); k0 += U * stride) {
+        int k[U], i[U], old[U];
+        if (k0 < need) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = min(k0 + u * stride, need - 1);
+            step_owners<U>(need_start, p.seqs, k, i);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u * stride >= need) continue;
+                old[u] = p.length[i[u]] - (row_start[i[u] + 1] - row_start[i[u]]);
+                const int id = p.free_pages[avail - 1 - k[u]];
+                p.table[i[u] * p.table_ld + step_columns(old[u], p.shift, p.shared) + k[u] - need_start[i[u]]] = id;
+                bool bad = false;
+                kv_page(id, p.pages, &bad);
+                if (bad) atomicOr(p.err + kErrBatch, 1u);
+            }
+        }
+        if (k0 < items) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = min(k0 + u * stride, items - 1);
+            step_owners<U>(row_start, p.seqs, k, i);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u * stride >= items) continue;
+                const int r = k[u], begin = row_start[i[u]], next = row_start[i[u] + 1];
+                old[u] = p.length[i[u]] - (next - begin);
+                const int pos = old[u] + r - begin;
+                if (p.row_seq) p.row_seq[r] = i[u];
+                if (p.positions) p.positions[r] = pos;
+                if (p.slots) {
+                    // a page taken in this step comes from the list, as its table entry is being written
+                    const int column = pos >> p.shift, fresh = column - step_columns(old[u], p.shift, p.shared);
+                    const int id = fresh >= 0 ? p.free_pages[avail - 1 - (need_start[i[u]] + fresh)] : p.table[i[u] * p.table_ld + column];
+                    p.slots[r] = ((int64_t)id << p.shift) + (pos & ((1 << p.shift) - 1));
+                }
+            }
+        }
+    }
+}
+
+// A thread has ITEMS slots of each 1024 * ITEMS.  ONE: there are no more, and their starts lie in the LDS.  rows_too: pages
+// are taken and the rows' maps written here, not by the second launch.
+template <int ITEMS, bool ONE>
+__global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p, int rows_too) {
+    constexpr int CAP = kThreads * ITEMS;
     __shared__ int sums[3][kWaves];
-    __shared__ int lds[ALL ? 3 : 1][ALL ? kThreads + 1 : 1];
+    __shared__ int starts[ONE ? 3 : 1][ONE ? CAP + 1 : 1];  // of rows, pages taken, pages given back
     const int tid = threadIdx.x;
     int count = *p.free_count;
-    bool bad = count < 0 || count > p.pages;
-    count = kv_clamp(count, 0, p.pages);
-    auto slot = [&](int i) {
-        StepSlot s{};
-        if (i < p.seqs) s = step_slot(p.length[i], p.change[i], p.shift, p.shared, p.rows, p.max_new, p.max_len);
-        bad |= s.bad;
-        return s;
+    bool bad = false;
+    StepSlot s[ITEMS];
+    auto load = [&](int i0) {  // slots i0 + ITEMS tid ..
+        int n[ITEMS], c[ITEMS];
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = min(i0 + ITEMS * tid + k, p.seqs - 1);
+            n[k] = p.length[i];
+            c[k] = p.change[i];
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            s[k] = i0 + ITEMS * tid + k < p.seqs ? step_slot(n[k], c[k], p.shift, p.shared, p.rows, p.max_new, p.max_len) : StepSlot{};
+            bad |= s[k].bad;
+        }
     };
+    auto sum = [&](auto member) {
+        int x = 0;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) x = step_add(x, s[k].*member);
+        return x;
+    };
+    // pages given back by all slots, before any is granted some
     int back = 0;
-    if constexpr (!ALL) {
-        for (int i0 = 0; i0 < p.seqs; i0 += kThreads) {
-            const int v[1] = {slot(i0 + tid).back};
-            const Scan<1> s = scan<1>(v, sums);
-            if (i0 + tid < p.seqs) p.back_start[i0 + tid] = back + s.at[0] - v[0];
-            back += s.total[0];
+    if constexpr (!ONE) {
+        for (int i0 = 0; i0 < p.seqs; i0 += CAP) {
+            load(i0);
+            const int v[1] = {sum(&StepSlot::back)};
+            const Scan<1> t = scan<1>(v, sums);
+            int at = back + t.at[0] - v[0];
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (i0 + ITEMS * tid + k < p.seqs) p.back_start[i0 + ITEMS * tid + k] = at;
+                at += s[k].back;
+            }
+            back += t.total[0];
         }
         if (tid == 0) p.back_start[p.seqs] = back;
     }
+    bad |= count < 0 || count > p.pages;
+    count = kv_clamp(count, 0, p.pages);
     int rows_sum = 0, need_sum = 0, rows = 0, need = 0, refused = 0, avail = 0;
-    for (int i0 = 0; i0 < p.seqs; i0 += kThreads) {
-        const int i = i0 + tid;
-        StepSlot s = slot(i);
-        const int all[3] = {s.want, s.need, ALL ? s.back : 0};
+    for (int i0 = 0; i0 < p.seqs; i0 += CAP) {
+        load(i0);
+        const int all[3] = {sum(&StepSlot::want), sum(&StepSlot::need), ONE ? sum(&StepSlot::back) : 0};
         const Scan<3> t = scan<3>(all, sums);
-        if constexpr (ALL) back = t.total[2];
+        if constexpr (ONE) back = t.total[2];
         avail = min(count + back, p.pages);
-        int row_at = rows + t.at[0], need_at = need + t.at[1], row_total = t.total[0], need_total = t.total[1];
-        const bool short_of = step_add(rows_sum, t.total[0]) > p.rows || step_add(need_sum, t.total[1]) > avail;
-        if (!short_of) {
-            rows_sum += t.total[0];
-            need_sum += t.total[1];
+        int row_at = t.at[0] - all[0], need_at = t.at[1] - all[1], back_at = t.at[2] - all[2];  // before this thread's slots
+        int row_total = t.total[0], need_total = t.total[1];
+        if (step_add(rows_sum, row_total) <= p.rows && step_add(need_sum, need_total) <= avail) {
+            rows_sum += row_total;
+            need_sum += need_total;
         } else {
             // some are refused: rows first, then pages, then what is left
-            if (step_add(rows_sum, t.at[0]) > p.rows) s.want = s.need = 0;
-            rows_sum = step_add(rows_sum, t.total[0]);
-            const int v[1] = {s.need};
+            int upto = step_add(rows_sum, row_at);
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                upto = step_add(upto, s[k].want);
+                if (upto > p.rows) s[k].want = s[k].need = 0;
+            }
+            rows_sum = step_add(rows_sum, row_total);
+            const int v[1] = {sum(&StepSlot::need)};
             const Scan<1> u = scan<1>(v, sums);
-            if (s.need > 0 && step_add(need_sum, u.at[0]) > avail) s.want = s.need = 0;
+            upto = step_add(need_sum, u.at[0] - v[0]);
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                upto = step_add(upto, s[k].need);
+                if (s[k].need > 0 && upto > avail) s[k].want = s[k].need = 0;
+            }
             need_sum = step_add(need_sum, u.total[0]);
-            const int w[2] = {s.want, s.need};
+            const int w[2] = {sum(&StepSlot::want), sum(&StepSlot::need)};
             const Scan<2> x = scan<2>(w, sums);
-            row_at = rows + x.at[0];
-            need_at = need + x.at[1];
+            row_at = x.at[0] - w[0];
+            need_at = x.at[1] - w[1];
             row_total = x.total[0];
             need_total = x.total[1];
         }
-        if (i < p.seqs) {
-            p.row_start[i] = row_at - s.want;
-            if (s.len + s.want != p.length[i]) p.length[i] = s.len + s.want;
-            if constexpr (ALL) {
-                lds[0][i] = row_at - s.want;
-                lds[1][i] = need_at - s.need;
-                lds[2][i] = t.at[2] - s.back;
-            } else {
-                p.need_start[i] = need_at - s.need;
+        row_at += rows;
+        need_at += need;
+        int none = 0;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = i0 + ITEMS * tid + k;
+            if (i >= p.seqs) continue;
+            p.row_start[i] = row_at;
+            if constexpr (ONE) {
+                starts[0][i] = row_at;
+                starts[1][i] = need_at;
+                starts[2][i] = back_at;
             }
+            if (!ONE || !rows_too) p.need_start[i] = need_at;
+            if (s[k].asks || s[k].back > 0 || s[k].shrinks) p.length[i] = s[k].len + s[k].want;
+            row_at += s[k].want;
+            need_at += s[k].need;
+            back_at += s[k].back;
+            none += s[k].asks && s[k].want == 0;
         }
         rows += row_total;
         need += need_total;
-        refused += __syncthreads_count(s.asks && s.want == 0);
+        if (p.refused) {
+            const int v[1] = {none};
+            refused += scan<1>(v, sums).total[0];
+        }
     }
+    if (count + back > p.pages) bad = true;  // more pages than there are: some were in the list already
     if (bad) atomicOr(p.err + kErrBatch, 1u);
     if (tid == 0) {
         p.row_start[p.seqs] = rows;
         *p.free_count = avail - need;
         if (p.refused) *p.refused = refused;
-        if (count + back > p.pages) atomicOr(p.err + kErrBatch, 1u);
-        if constexpr (ALL) {
-            lds[0][p.seqs] = rows;
-            lds[1][p.seqs] = need;
-            lds[2][p.seqs] = back;
-        } else {
+        if constexpr (ONE) {
+            starts[0][p.seqs] = rows;
+            starts[1][p.seqs] = need;
+            starts[2][p.seqs] = back;
+        }
+        if (!ONE || !rows_too) {
             p.need_start[p.seqs] = need;
-            p.totals[kCount] = count;
             p.totals[kAvail] = avail;
             p.totals[kNeed] = need;
-            p.totals[kBack] = back;
             p.totals[kRows] = rows;
         }
     }
-    if constexpr (ALL) {
-        __syncthreads();  // lengths and starts
-        give_back(p, lds[2], count, back, tid, kThreads);
+    __syncthreads();  // lengths and starts
+    if constexpr (ONE) give_back(p, starts[2], count, back, tid, kThreads);
+    else give_back(p, p.back_start, count, back, tid, kThreads);
+    if constexpr (ONE) {
+        if (!rows_too) return;
         __syncthreads();
-        take(p, lds[1], lds[0], avail, need, rows, tid, kThreads);
+        take<2>(p, starts[1], starts[0], avail, need, rows, tid, kThreads);
     }
 }
 
-__global__ __launch_bounds__(256) void kv_step_back_kernel(StepParams p) {
-    give_back(p, p.back_start, p.totals[kCount], p.totals[kBack], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
-}
 __global__ __launch_bounds__(256) void kv_step_take_kernel(StepParams p) {
-    take(p, p.need_start, p.row_start, p.totals[kAvail], p.totals[kNeed], p.totals[kRows], blockIdx.x * 256 + threadIdx.x,
+    take<1>(p, p.need_start, p.row_start, p.totals[kAvail], p.totals[kNeed], p.totals[kRows], blockIdx.x * 256 + threadIdx.x,
          gridDim.x * 256);
 }
 
@@ -216,17 +295,14 @@ hipError_t launch_kv_step(StepParams p, int32_t* scratch, hipStream_t st) {
     p.totals = scratch;
     p.need_start = scratch + kTotals;
     p.back_start = p.need_start + p.seqs + 1;
-    if (p.seqs <= kThreads && p.rows <= kOneRows) {
-        kv_step_kernel<true><<<1, kThreads, 0, st>>>(p);
-        return hipGetLastError();
-    }
-    kv_step_kernel<false><<<1, kThreads, 0, st>>>(p);
-    if (const hipError_t e = hipGetLastError()) return e;
-    kv_step_back_kernel<<<256, 256, 0, st>>>(p);
-    if (const hipError_t e = hipGetLastError()) return e;
-    const int64_t items = p.rows;
-    const int grid = (int)((items + 255) / 256 < 128 ? 128 : (items + 255) / 256 > 2048 ? 2048 : (items + 255) / 256);
-    kv_step_take_kernel<<<grid, 256, 0, st>>>(p);
+    const bool rows_too = p.seqs <= 4 * kThreads && p.rows <= kOneRows;
+    if (p.seqs <= kThreads) kv_step_kernel<1, true><<<1, kThreads, 0, st>>>(p, rows_too);
+    else if (p.seqs <= 4 * kThreads) kv_step_kernel<4, true><<<1, kThreads, 0, st>>>(p, rows_too);
+    else kv_step_kernel<4, false><<<1, kThreads, 0, st>>>(p, 0);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || rows_too) return e;
+    const int blocks = (p.rows + 255) / 256;
+    kv_step_take_kernel<<<std::clamp(blocks, 128, 2048), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 

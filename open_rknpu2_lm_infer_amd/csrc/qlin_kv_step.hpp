@@ -13,7 +13,7 @@ struct StepSlot {
     int back;  // pages given back
     int want;  // tokens asked for, as far as the slot's own limits allow them
     int need;  // pages for them
-    bool asks, bad;
+    bool asks, shrinks, bad;
 };
 
 // Columns that n tokens take, those of the prefix among them in any case.  n is 0 .. 2^30.
@@ -23,7 +23,7 @@ QLIN_HD int step_columns(int n, int shift, int shared) {
 }
 
 QLIN_HD StepSlot step_slot(int n, int change, int shift, int shared, int rows, int max_new, int max_len) {
-    StepSlot s{n, 0, 0, 0, 0, change > 0, n < 0 || n > max_len};
+    StepSlot s{n, 0, 0, 0, 0, change > 0, change < 0, n < 0 || n > max_len};
     if (s.bad || change == 0) return s;
     const int held = step_columns(n, shift, shared);
     if (change < 0) {
@@ -39,16 +39,23 @@ QLIN_HD StepSlot step_slot(int n, int change, int shift, int shared, int rows, i
     return s;
 }
 
-// Last i of start[0 .. n] (not decreasing, start[0] = 0) with start[i] <= k: whose the k-th thing is, for k < start[n].
+// Last i of start[0 .. n] (not decreasing, start[0] = 0) with start[i] <= k, for U values of k below start[n]: whose the
+// k-th things are.  The searches go step by step beside each other.
+template <int U, typename P>
+QLIN_HD void step_owners(P start, int n, const int (&k)[U], int (&i)[U]) {
+    for (int u = 0; u < U; ++u) i[u] = 0;
+    for (int left = n; left > 1;) {
+        const int half = left >> 1;
+        for (int u = 0; u < U; ++u) i[u] += start[i[u] + half] <= k[u] ? half : 0;
+        left -= half;
+    }
+}
 template <typename P>
 QLIN_HD int step_owner(P start, int n, int k) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= k) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+    const int one[1] = {k};
+    int i[1];
+    step_owners<1>(start, n, one, i);
+    return i[0];
 }
 
 // Sums that stay at kStepMost once they reach it: above everything that can be granted.

@@ -67,7 +67,7 @@ int run(const qlin_rope* rope, int32_t rows, int32_t dim, int32_t q_heads, int32
     p.inverse = (flags & QLIN_ROPE_INVERSE) != 0;
     p.rows = rows;
     p.positions = positions;
-    heads_split(&p, rows, (int)heads);
+    heads_split(&p, 1, rows, (int)heads);
     return launch_heads(p, (hipStream_t)stream) == hipSuccess ? QLIN_OK : QLIN_ERR_DEVICE;
 }
 
@@ -85,24 +85,28 @@ void heads_common(HeadsParams* p, const qlin_rope* rope, int dim, int q_heads, i
     p->x = x;
     p->ldx = ldx;
     p->x_f16 = x_f16;
-    p->x_vec = aligned(x, x_f16, ldx);
     p->dim = dim;
     p->q_heads = q_heads;
     p->k_heads = k_heads;
     p->q_gamma = q_gamma;
     p->k_gamma = k_gamma;
+    p->vec = aligned(x, x_f16, ldx) && aligned(y, y_f16, ldy) &&
+             (reinterpret_cast<uintptr_t>(q_gamma) | reinterpret_cast<uintptr_t>(k_gamma)) % 16 == 0;
     p->eps = eps;
     p->inv_dim = 1.0f / (float)dim;
     p->y = y;
     p->ldy = ldy;
     p->y_f16 = y_f16;
-    p->y_vec = aligned(y, y_f16, ldy);
 }
 
-void heads_split(HeadsParams* p, int64_t rows, int heads) {
-    const int64_t once = heads_at_once(*p), passes = (heads + once - 1) / once;
-    p->splits = (int)std::clamp<int64_t>(2048 / std::max<int64_t>(rows, 1), 1, passes);
+void heads_split(HeadsParams* p, int64_t seqs, int64_t rows, int heads) {
+    p->block_rows = p->x_f16 && seqs * rows >= 2048 ? 4 : 1;
+    const int64_t once = heads_at_once(*p) * (4 / p->block_rows), passes = (heads + once - 1) / once;
+    const int64_t blocks = (rows + p->block_rows - 1) / p->block_rows;
+    p->splits = (int)std::clamp<int64_t>(1024 / std::max<int64_t>(seqs * blocks, 1), 1, passes);
     p->by_splits = fast_div(p->splits);
+    p->by_new = fast_div((int)blocks);
+    p->by_pairs = fast_div(std::max(p->rope.rotary / 2, 1));
 }
 
 }  // namespace qlin

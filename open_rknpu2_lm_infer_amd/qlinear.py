@@ -327,20 +327,19 @@ class Rope:
             pass
 
 
-def _rope_rows(X: torch.Tensor, positions: torch.Tensor | None, out: torch.Tensor | None, out_dtype) -> torch.Tensor:
-    """Checks rows, positions and the output of a rotary call; the output."""
-    rows, cols = X.shape
-    assert X.is_cuda and (X.stride(1) == 1 or cols == 1)
-    assert positions is None or (positions.dtype == torch.int32 and positions.device == X.device
-                                 and positions.is_contiguous() and positions.numel() == rows)
+def _rope_rows(X: torch.Tensor, positions: torch.Tensor | None, out: torch.Tensor | None, out_dtype):
+    """Checks rows, positions and the output of a rotary call: rows, columns, row stride, the output and its row stride."""
+    (rows, cols), (ldx, step), device = X.shape, X.stride(), X.get_device()
+    assert device >= 0 and (step == 1 or cols == 1)
+    if positions is not None:
+        assert positions.dtype == torch.int32 and positions.get_device() == device
+        assert positions.is_contiguous() and positions.numel() == rows
     if out is None:
         out = torch.empty((rows, cols), dtype=out_dtype or X.dtype, device=X.device)
-    assert out.shape == X.shape and out.device == X.device and (out.stride(1) == 1 or cols == 1)
-    return out
-
-
-def _row_ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # one row has no stride of its own
+    (out_rows, out_cols), (ldo, step) = out.shape, out.stride()
+    assert out_rows == rows and out_cols == cols and out.get_device() == device and (step == 1 or cols == 1)
+    # one row has no stride of its own
+    return (rows, cols, ldx, out, ldo) if rows > 1 else (rows, cols, cols, out, cols)
 
 
 def rope(rope: Rope, X: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None,
@@ -348,20 +347,21 @@ def rope(rope: Rope, X: torch.Tensor, positions: torch.Tensor, out: torch.Tensor
     """The heads of rows X [rows, heads * head_dim] turned by their rows' positions, int32 [rows] (qlin_rope_run); out may
     be X.  flags: QLIN_ROPE_INVERSE."""
     assert positions is not None
-    out = _rope_rows(X, positions, out, out_dtype)
-    heads = X.shape[1] // rope.head_dim
-    assert heads * rope.head_dim == X.shape[1]
-    rc = _lib.load().qlin_rope_run(rope.handle, X.shape[0], heads, X.data_ptr(), _DT[X.dtype], _row_ld(X), positions.data_ptr(),
-                                   out.data_ptr(), _DT[out.dtype], _row_ld(out), flags, _raw_stream(X.device))
+    rows, cols, ldx, out, ldo = _rope_rows(X, positions, out, out_dtype)
+    D = rope.head_dim
+    heads = cols // D
+    assert heads * D == cols
+    rc = _lib.load().qlin_rope_run(rope.handle, rows, heads, X.data_ptr(), _DT[X.dtype], ldx, positions.data_ptr(), out.data_ptr(),
+                                   _DT[out.dtype], ldo, flags, _raw_stream(X.device))
     if rc:
         check(rc, "qlin_rope_run")
     return out
 
 
-def _gamma_ptr(gamma: torch.Tensor | None, dim: int, device: torch.device) -> int | None:
+def _gamma_ptr(gamma: torch.Tensor | None, dim: int, device: int) -> int | None:
     if gamma is None:
         return None
-    assert gamma.dtype == torch.float32 and gamma.device == device and gamma.is_contiguous() and gamma.numel() == dim
+    assert gamma.dtype == torch.float32 and gamma.get_device() == device and gamma.is_contiguous() and gamma.numel() == dim
     return gamma.data_ptr()
 
 
@@ -371,14 +371,14 @@ def norm_rope(rope: Rope | None, X: torch.Tensor, positions: torch.Tensor | None
     """RMSNorm of every head of rows X [rows, (q_heads + key heads) * head_dim], then the rotation (qlin_rope_run_norm); out
     may be X.  Without rope: norms alone, of heads of head_dim."""
     assert (rope is None) == (positions is None) and (rope is None or head_dim in (None, rope.head_dim))
-    out = _rope_rows(X, positions, out, out_dtype)
+    rows, cols, ldx, out, ldo = _rope_rows(X, positions, out, out_dtype)
     D = head_dim if rope is None else rope.head_dim
-    heads = X.shape[1] // D
-    assert heads * D == X.shape[1] and 0 <= q_heads <= heads
+    heads, device = cols // D, X.get_device()
+    assert heads * D == cols and 0 <= q_heads <= heads
     rc = _lib.load().qlin_rope_run_norm(
-        rope.handle if rope else None, X.shape[0], D, q_heads, heads - q_heads, _gamma_ptr(q_gamma, D, X.device),
-        _gamma_ptr(k_gamma, D, X.device), eps, X.data_ptr(), _DT[X.dtype], _row_ld(X),
-        positions.data_ptr() if rope else None, out.data_ptr(), _DT[out.dtype], _row_ld(out), flags, _raw_stream(X.device))
+        rope.handle if rope else None, rows, D, q_heads, heads - q_heads, _gamma_ptr(q_gamma, D, device),
+        _gamma_ptr(k_gamma, D, device), eps, X.data_ptr(), _DT[X.dtype], ldx, positions.data_ptr() if rope else None,
+        out.data_ptr(), _DT[out.dtype], ldo, flags, _raw_stream(X.device))
     if rc:
         check(rc, "qlin_rope_run_norm")
     return out
@@ -473,15 +473,19 @@ def kv_append_qkv(ws: Workspace, cache: KVCache, batch: KVBatch, rope: Rope | No
     normalized and turned by their tokens' places, keys and values quantized into their pages (qlin_kv_append_qkv).
     Returns the queries [rows, q_heads * head_dim]; out may be those columns of QKV."""
     _kv_check(cache, batch)
-    D = cache.head_dim
+    D, device = cache.head_dim, cache.device
+    q_cols, cols = q_heads * D, q_heads * D + 2 * cache.columns
+    (rows, n), (ld, step) = QKV.shape, QKV.stride()
+    assert n == cols and rows >= batch.rows and (step == 1 or n == 1) and QKV.get_device() == device
     assert rope is None or rope.head_dim == D
     if out is None:
-        out = torch.empty((QKV.shape[0], q_heads * D), dtype=out_dtype or QKV.dtype, device=QKV.device)
+        out = torch.empty((rows, q_cols), dtype=out_dtype or QKV.dtype, device=QKV.device)
+    (out_rows, n), (ldo, step) = out.shape, out.stride()
+    assert n == q_cols and out_rows >= batch.rows and (step == 1 or n == 1) and out.get_device() == device
     rc = _lib.load().qlin_kv_append_qkv(
-        ws.handle, cache.handle, batch.ref, rope.handle if rope else None, q_heads, _gamma_ptr(q_gamma, D, batch.device),
-        _gamma_ptr(k_gamma, D, batch.device), eps, QKV.data_ptr(), _DT[QKV.dtype],
-        _kv_ld(batch, QKV, q_heads * D + 2 * cache.columns), out.data_ptr(), _DT[out.dtype], _kv_ld(batch, out, q_heads * D),
-        flags, _raw_stream(batch.device))
+        ws.handle, cache.handle, batch.ref, rope.handle if rope else None, q_heads, _gamma_ptr(q_gamma, D, device),
+        _gamma_ptr(k_gamma, D, device), eps, QKV.data_ptr(), _DT[QKV.dtype], ld if rows > 1 else cols, out.data_ptr(),
+        _DT[out.dtype], ldo if out_rows > 1 else q_cols, flags, _raw_stream(batch.device))
     if rc:
         check(rc, "qlin_kv_append_qkv")
     return out
@@ -524,7 +528,8 @@ class KVStep:
 
 def kv_step(ws: Workspace, step: KVStep, change: torch.Tensor) -> KVBatch:
     """Grants and takes back tokens, int32 [seqs], and makes the step's tables (qlin_kv_step); its batch."""
-    assert change.dtype == torch.int32 and change.device == step.device and change.is_contiguous() and change.numel() == step.seqs
+    assert change.dtype == torch.int32 and change.get_device() == step.device.index and change.is_contiguous()
+    assert change.numel() == step.seqs
     step.c.change = change.data_ptr()
     rc = _lib.load().qlin_kv_step(ws.handle, step.cache.handle, step.ref, _raw_stream(step.device))
     if rc:

@@ -13,7 +13,8 @@ import torch
 from open_rknpu2_lm_infer_amd import _lib
 from open_rknpu2_lm_infer_amd import qlinear as ql
 from tests import headref
-from tests.test_kv_arguments import Tensor, reached  # noqa: F401
+from tests import test_kv_arguments
+from tests.test_kv_arguments import reached  # noqa: F401
 
 BIN = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build", "step_calls_test")
 
@@ -27,6 +28,11 @@ def test_step_calls(mode):
 def test_structs_match_header_sizes():
     assert ctypes.sizeof(_lib.RopeConfig) == 72
     assert ctypes.sizeof(_lib.KVTables) == 112
+
+
+class Tensor(test_kv_arguments.Tensor):
+    def get_device(self):
+        return self.device.index
 
 
 ROPE = SimpleNamespace(handle=1, head_dim=64)
