@@ -155,7 +155,7 @@ int qlin_workspace_query(const qlin_workspace* ws, qlin_workspace_info* out);
 /* Sticky error word of asynchronous runs on this workspace: returns QLIN_OK or
  * QLIN_ERR_NONFINITE if any activation row seen since the last clear held Inf/NaN.
  * Synchronizes the workspace's last stream.  clear != 0 resets it.  QLIN_ERR_PARAM: a key/value cache
- * call found row starts, lengths or pages outside its batch's limits (see qlin_kv_batch).  Where there are both
+ * call found row starts, lengths or pages outside its batch's limits (see qlin_kv_batch, qlin_kv_tables).  Where there are both
  * reports, this one comes first; what is cleared is the one returned, and the next call returns the other.  A host-buffer run
  * clears what was said of rows before it and leaves its own, and leaves what was said of batches. */
 int qlin_workspace_status(qlin_workspace* ws, int32_t clear);
@@ -548,7 +548,7 @@ typedef struct qlin_kv_tables {
     int32_t max_new;       /* of one slot; what a later qlin_kv_batch is given */
     int32_t max_len;       /* up to 2^30 */
     int32_t prefix_tokens; /* a multiple of page_tokens, up to max_len: pages of these first tokens are shared, neither taken
-                            * nor given back, and their columns not written */
+                            * nor given back, and their columns not written (slots of rows among them are read from them) */
     int32_t reserved;
     const int32_t* change; /* device [seqs] */
     int32_t* length;       /* device [seqs], in and out */

@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <new>
 
 #include "../../include/qlinear.h"
@@ -37,8 +38,8 @@ double frequency(const qlin_rope_config& g, int i) {
 bool good(const qlin_rope_config& g) {
     if (g.head_dim <= 0 || g.rotary_dim <= 0 || g.rotary_dim % 2 || g.first < 0 || g.first > g.head_dim - g.rotary_dim ||
         (g.layout != QLIN_ROPE_HALF && g.layout != QLIN_ROPE_INTERLEAVED) || g.scaling < QLIN_ROPE_PLAIN ||
-        g.scaling > QLIN_ROPE_RAMP || !std::isfinite(g.base) || !(g.base > 1.0) || !std::isfinite(g.amplitude) ||
-        g.amplitude < 0.0)
+        g.scaling > QLIN_ROPE_RAMP || !std::isfinite(g.base) || !(g.base > 1.0) || !(g.amplitude >= 0.0) ||
+        g.amplitude > (double)std::numeric_limits<float>::max())
         return false;
     if (g.scaling == QLIN_ROPE_PLAIN) return true;
     if (!std::isfinite(g.factor) || !(g.factor >= 1.0)) return false;

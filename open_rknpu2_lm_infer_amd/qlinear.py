@@ -310,7 +310,7 @@ class Rope:
         cfg = _lib.RopeConfig(head_dim, rotary_dim, first, self.LAYOUTS[layout], self.SCALINGS[scaling], 0, base, factor,
                               original_len, low, high, amplitude)
         check(_lib.load().qlin_rope_create(ctypes.byref(cfg), ctypes.byref(self.handle)), "qlin_rope_create")
-        self.head_dim, self.rotary_dim = head_dim, rotary_dim
+        self.head_dim, self.rotary_dim, self.device = head_dim, rotary_dim, torch.cuda.current_device()
         w, a = (ctypes.c_double * (rotary_dim // 2))(), ctypes.c_double()
         check(_lib.load().qlin_rope_query(self.handle, w, ctypes.byref(a)), "qlin_rope_query")
         self.radians, self.amplitude = list(w), a.value
@@ -327,10 +327,10 @@ class Rope:
             pass
 
 
-def _rope_rows(X: torch.Tensor, positions: torch.Tensor | None, out: torch.Tensor | None, out_dtype):
+def _rope_rows(device: int, X: torch.Tensor, positions: torch.Tensor | None, out: torch.Tensor | None, out_dtype):
     """Checks rows, positions and the output of a rotary call: rows, columns, row stride, the output and its row stride."""
-    (rows, cols), (ldx, step), device = X.shape, X.stride(), X.get_device()
-    assert device >= 0 and (step == 1 or cols == 1)
+    (rows, cols), (ldx, step) = X.shape, X.stride()
+    assert X.get_device() == device and (step == 1 or cols == 1)
     if positions is not None:
         assert positions.dtype == torch.int32 and positions.get_device() == device
         assert positions.is_contiguous() and positions.numel() == rows
@@ -347,7 +347,7 @@ def rope(rope: Rope, X: torch.Tensor, positions: torch.Tensor, out: torch.Tensor
     """The heads of rows X [rows, heads * head_dim] turned by their rows' positions, int32 [rows] (qlin_rope_run); out may
     be X.  flags: QLIN_ROPE_INVERSE."""
     assert positions is not None
-    rows, cols, ldx, out, ldo = _rope_rows(X, positions, out, out_dtype)
+    rows, cols, ldx, out, ldo = _rope_rows(rope.device, X, positions, out, out_dtype)
     D = rope.head_dim
     heads = cols // D
     assert heads * D == cols
@@ -371,9 +371,10 @@ def norm_rope(rope: Rope | None, X: torch.Tensor, positions: torch.Tensor | None
     """RMSNorm of every head of rows X [rows, (q_heads + key heads) * head_dim], then the rotation (qlin_rope_run_norm); out
     may be X.  Without rope: norms alone, of heads of head_dim."""
     assert (rope is None) == (positions is None) and (rope is None or head_dim in (None, rope.head_dim))
-    rows, cols, ldx, out, ldo = _rope_rows(X, positions, out, out_dtype)
+    device = torch.cuda.current_device() if rope is None else rope.device
+    rows, cols, ldx, out, ldo = _rope_rows(device, X, positions, out, out_dtype)
     D = head_dim if rope is None else rope.head_dim
-    heads, device = cols // D, X.get_device()
+    heads = cols // D
     assert heads * D == cols and 0 <= q_heads <= heads
     rc = _lib.load().qlin_rope_run_norm(
         rope.handle if rope else None, rows, D, q_heads, heads - q_heads, _gamma_ptr(q_gamma, D, device),
@@ -477,7 +478,7 @@ def kv_append_qkv(ws: Workspace, cache: KVCache, batch: KVBatch, rope: Rope | No
     q_cols, cols = q_heads * D, q_heads * D + 2 * cache.columns
     (rows, n), (ld, step) = QKV.shape, QKV.stride()
     assert n == cols and rows >= batch.rows and (step == 1 or n == 1) and QKV.get_device() == device
-    assert rope is None or rope.head_dim == D
+    assert rope is None or (rope.head_dim == D and rope.device == device)
     if out is None:
         out = torch.empty((rows, q_cols), dtype=out_dtype or QKV.dtype, device=QKV.device)
     (out_rows, n), (ldo, step) = out.shape, out.stride()

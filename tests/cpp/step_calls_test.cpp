@@ -172,7 +172,7 @@ void refusals() {
     const qlin_rope_config good = {128, 64, 0, QLIN_ROPE_HALF, QLIN_ROPE_PLAIN, 0, 1e4, 0.0, 0.0, 0.0, 0.0, 0.0};
     qlin_rope* r = nullptr;
     const double nan = std::nan(""), inf = std::numeric_limits<double>::infinity();
-    for (int i = 0; i < 28; ++i) {
+    for (int i = 0; i < 30; ++i) {
         qlin_rope_config g = good;
         g.factor = 4.0;
         g.original_len = 8192;
@@ -207,6 +207,8 @@ void refusals() {
             case 25: g.rotary_dim = kLow; break;
             case 26: g.head_dim = 64, g.first = 2; break;
             case 27: g.scaling = QLIN_ROPE_LINEAR, g.factor = inf; break;
+            case 28: g.amplitude = 1e39; break;
+            case 29: g.amplitude = inf; break;
         }
         r = reinterpret_cast<qlin_rope*>(1);
         expect(qlin_rope_create(&g, &r) == QLIN_ERR_PARAM && !r, "a configuration that makes no sense");

@@ -84,6 +84,10 @@ STEPS = [  # slots, page, max_len, rows, max_new, spare pages, prefix
     (3000, 16, 200, 9000, 40, 500, 0),
     (300, 16, 600, 20000, 600, 4000, 0),  # prompts
     (5, 4096, 9000, 10, 3, 1, 4096),
+    (4096, 16, 64, 4096, 9, 900, 0),      # the most of one scan, one launch
+    (4097, 16, 64, 4096, 9, 900, 0),      # two scans
+    (9001, 16, 100, 5000, 20, 3000, 16),  # rows and pages run out in the second or third
+    (9001, 16, 100, 200000, 20, 2000, 0),
 ]
 
 

@@ -226,6 +226,20 @@ def test_any_number_of_rows(rows):
         check(out[rows - 2:rows], want, tol)
 
 
+@pytest.mark.parametrize("D,n,first,layout,heads", [s for s in SHAPES if s[4] <= 8])
+@pytest.mark.parametrize("rows", [2050, 2303])
+def test_many_rows_of_every_shape(D, n, first, layout, heads, rows):
+    """Four fp16 rows a workgroup, the last one with fewer: a row's result is that of the row alone."""
+    rope = ql.Rope(D, n, first=first, layout=layout)
+    g = (rand((D,), F32, seed=1) + 2.0).to(DEV)
+    x, pos = rand((rows, heads * D), F16, seed=rows).to(DEV), torch.arange(rows, dtype=torch.int32, device=DEV) * 3
+    out = torch.full((rows + 1, heads * D), 5.0, dtype=F16, device=DEV)
+    ql.norm_rope(rope, x, pos, heads // 2, g, None, out=out[:rows])
+    assert (out[rows:] == 5).all()
+    for r in (0, 1, 2, 3, 4, 1030, rows - 3, rows - 2, rows - 1):
+        assert torch.equal(ql.norm_rope(rope, x[r:r + 1], pos[r:r + 1], heads // 2, g, None)[0], out[r]), r
+
+
 def test_streams_and_captured_rows():
     """On a stream of its own and in a graph, replayed with other rows and positions and eager calls in between."""
     D, heads, rows = 64, 6, 33

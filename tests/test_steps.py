@@ -35,12 +35,13 @@ class Tensor(test_kv_arguments.Tensor):
         return self.device.index
 
 
-ROPE = SimpleNamespace(handle=1, head_dim=64)
+ROPE = SimpleNamespace(handle=1, head_dim=64, device=0)
 WS = SimpleNamespace(handle=1)
 F16 = torch.float16
 
 
-def test_rope_arguments(reached):  # noqa: F811
+def test_rope_arguments(reached, monkeypatch):  # noqa: F811
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     x, pos = Tensor(5, 256, dtype=F16), Tensor(5)
     ql.rope(ROPE, x, pos, out=Tensor(5, 256, dtype=F16))
     ql.norm_rope(ROPE, x, pos, 3, None, Tensor(64, dtype=torch.float32), out=Tensor(5, 256, dtype=torch.float32))
@@ -54,6 +55,9 @@ def test_rope_arguments(reached):  # noqa: F811
         lambda: ql.rope(ROPE, x, pos, out=Tensor(5, 192, dtype=F16)),
         lambda: ql.rope(ROPE, x, pos, out=Tensor(5, 256, dtype=F16, device="cuda:1")),
         lambda: ql.rope(ROPE, x, None, out=x),
+        lambda: ql.rope(SimpleNamespace(handle=1, head_dim=64, device=1), x, pos, out=x),
+        lambda: ql.norm_rope(None, Tensor(5, 256, dtype=F16, device="cuda:1"), None, 1, None, None, head_dim=64,
+                             out=Tensor(5, 256, dtype=F16, device="cuda:1")),
         lambda: ql.norm_rope(ROPE, x, pos, 5, None, None, out=x),  # more query heads than heads
         lambda: ql.norm_rope(ROPE, x, pos, 3, Tensor(128, dtype=torch.float32), None, out=x),
         lambda: ql.norm_rope(ROPE, x, pos, 3, Tensor(64, dtype=F16), None, out=x),
@@ -81,7 +85,9 @@ def test_append_qkv_arguments(reached):  # noqa: F811
         lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, Tensor(4, 512, dtype=F16), 4, out=Tensor(5, 256, dtype=F16)),
         lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, x, 4, out=Tensor(4, 256, dtype=F16)),
         lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, x, 4, out=Tensor(5, 512, dtype=F16)),
-        lambda: ql.kv_append_qkv(WS, cache, batch, SimpleNamespace(handle=1, head_dim=128), x, 4, out=Tensor(5, 256, dtype=F16)),
+        lambda: ql.kv_append_qkv(WS, cache, batch, SimpleNamespace(handle=1, head_dim=128, device=0), x, 4, out=Tensor(5, 256, dtype=F16)),
+        lambda: ql.kv_append_qkv(WS, cache, batch, SimpleNamespace(handle=1, head_dim=64, device=1), x, 4, out=Tensor(5, 256, dtype=F16)),
+        lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, Tensor(5, 512, dtype=F16, device="cuda:1"), 4, out=Tensor(5, 256, dtype=F16)),
         lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, x, 4, Tensor(32, dtype=torch.float32), out=Tensor(5, 256, dtype=F16)),
         lambda: ql.kv_append_qkv(WS, cache, batch, ROPE, x, 4, Tensor(64, dtype=torch.float32, device="cuda:1"), out=Tensor(5, 256, dtype=F16)),
     ]
