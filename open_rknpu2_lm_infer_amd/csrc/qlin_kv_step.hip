@@ -11,6 +11,11 @@
 // is found by a binary search in the scanned starts, which lie in the LDS up to 4096 slots.  With few rows the same
 // workgroup takes pages and writes the rows' maps too: one launch.  With more a second launch does, the first having laid
 // down its starts.
+//
+// What bounds it: the chain of loads, scans and stores of one workgroup, 4.7 us for 64 slots of which 60 get up to 4 rows
+// each (2 of them the launch), as much to take the rows back; 3000 slots that are granted 14000 pages and 230000 rows 8.4 us
+// and 7.6 for the second launch's searches, and 12.9 to give those pages back, whose table entries one CU reads and writes
+// one by one.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -66,10 +71,10 @@ __device__ __forceinline__ Scan<N> scan(const int (&v)[N], int (*lds)[kWaves]) {
     return s;
 }
 
-// Pages given back: from the table to the free list, from thread `first` on every `stride`, four at a time.
-template <typename P>
-__device__ __forceinline__ void give_back(const StepParams& p, P back_start, int count, int total, int first, int stride) {
-    constexpr int U = 4;
+// Pages given back: from the table to the free list, from thread `first` on every `stride`, U at a time.  from: the first
+// column that a slot gives back.
+template <int U, typename P, typename F>
+__device__ __forceinline__ void give_back(const StepParams& p, P back_start, F from, int count, int total, int first, int stride) {
     for (int k0 = first; k0 < total; k0 += U * stride) {
         int k[U], i[U], id[U];
         int32_t* at[U];
@@ -78,7 +83,7 @@ __device__ __forceinline__ void give_back(const StepParams& p, P back_start, int
         step_owners<U>(back_start, p.seqs, k, i);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            at[u] = p.table + i[u] * p.table_ld + step_columns(p.length[i[u]], p.shift, p.shared) + k[u] - back_start[i[u]];
+            at[u] = p.table + i[u] * p.table_ld + from(i[u]) + k[u] - back_start[i[u]];
             id[u] = *at[u];
         }
 #pragma unroll
@@ -143,7 +148,8 @@ template <int ITEMS, bool ONE>
 __global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p, int rows_too) {
     constexpr int CAP = kThreads * ITEMS;
     __shared__ int sums[3][kWaves];
-    __shared__ int starts[ONE ? 3 : 1][ONE ? CAP + 1 : 1];  // of rows, pages taken, pages given back
+    // of pages given back and taken; of rows, or (not rows_too) the first columns given back
+    __shared__ int starts[ONE ? 3 : 1][ONE ? CAP + 1 : 1];
     const int tid = threadIdx.x;
     int count = *p.free_count;
     bool bad = false;
@@ -233,9 +239,9 @@ __global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p, int row
             if (i >= p.seqs) continue;
             p.row_start[i] = row_at;
             if constexpr (ONE) {
-                starts[0][i] = row_at;
+                starts[0][i] = back_at;
                 starts[1][i] = need_at;
-                starts[2][i] = back_at;
+                starts[2][i] = rows_too ? row_at : s[k].from;
             }
             if (!ONE || !rows_too) p.need_start[i] = need_at;
             if (s[k].asks || s[k].back > 0 || s[k].shrinks) p.length[i] = s[k].len + s[k].want;
@@ -258,9 +264,9 @@ __global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p, int row
         *p.free_count = avail - need;
         if (p.refused) *p.refused = refused;
         if constexpr (ONE) {
-            starts[0][p.seqs] = rows;
+            starts[0][p.seqs] = back;
             starts[1][p.seqs] = need;
-            starts[2][p.seqs] = back;
+            starts[2][p.seqs] = rows;
         }
         if (!ONE || !rows_too) {
             p.need_start[p.seqs] = need;
@@ -270,12 +276,17 @@ __global__ __launch_bounds__(kThreads) void kv_step_kernel(StepParams p, int row
         }
     }
     __syncthreads();  // lengths and starts
-    if constexpr (ONE) give_back(p, starts[2], count, back, tid, kThreads);
-    else give_back(p, p.back_start, count, back, tid, kThreads);
+    auto from_length = [&](int i) { return step_columns(p.length[i], p.shift, p.shared); };
     if constexpr (ONE) {
-        if (!rows_too) return;
+        if (!rows_too) {
+            give_back<4>(p, starts[0], [&](int i) { return starts[2][i]; }, count, back, tid, kThreads);
+            return;
+        }
+        give_back<2>(p, starts[0], from_length, count, back, tid, kThreads);
         __syncthreads();
-        take<2>(p, starts[1], starts[0], avail, need, rows, tid, kThreads);
+        take<2>(p, starts[1], starts[2], avail, need, rows, tid, kThreads);
+    } else {
+        give_back<4>(p, p.back_start, from_length, count, back, tid, kThreads);
     }
 }
 
@@ -284,8 +295,9 @@ __global__ __launch_bounds__(256) void kv_step_take_kernel(StepParams p) {
          gridDim.x * 256);
 }
 
-// Rows up to which one workgroup does it all.
-constexpr int kOneRows = 4096;
+// Rows up to which one workgroup does it all (us a step there and in two launches, half the steps taking as much back:
+// 256 rows 3.5 and 4.9, 4096 4.6 and 5.7, 8192 5.3 and 5.4, 16384 8.1 and 5.6).
+constexpr int kOneRows = 8192;
 
 }  // namespace
 
