@@ -77,6 +77,12 @@ __device__ __forceinline__ void attend_classes(const AttendParams& p, int block,
     const int group = p.group.d;
 
     const int j0 = p.own_from + part * p.chunk;
+    // page ids through the scalar cache: nothing writes them while the kernel runs.  The first step's, where the table has a
+    // column for it, does not wait for the sequence's length
+    const const_ids table = (const_ids)(uintptr_t)(p.b.table + seq * p.b.table_ld);
+    const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
+    const int first = j0 + TOKENS * wave;
+    const int first_id = first < p.b.max_len ? (first < p.prefix ? prefix : table)[first >> p.c.shift] : 0;
     const KvSeq s = kv_seq(p.b.row_start, p.b.length, seq, p.b.rows, p.b.max_new, p.b.max_len);
     if (s.bad && tid == 0) atomicOr(p.err + kErrBatch, 1u);
     const int vectors = s.rows * group;
@@ -92,15 +98,16 @@ __device__ __forceinline__ void attend_classes(const AttendParams& p, int block,
     QueryRow<KS, Q16> qr;
     load_query<KS, 32 * Step::RUN, Step::RUN, Q16>(p, qr, out_row * p.ldq + (int64_t)head * p.c.dim, 8 * Step::RUN * g);
 
-    const const_ids table = (const_ids)(uintptr_t)(p.b.table + seq * p.b.table_ld);
-    const const_ids prefix = (const_ids)(uintptr_t)p.prefix_pages;
     const int off_mask = (1 << p.c.shift) - 1;
     bool bad_page = false, bad = false;  // who sees none of a bad step's tokens keeps its result
     Step d;
     Half16<DP, 4> next;
-    auto find_step = [&](int j) {  // end > 0
+    auto page_of = [&](int j) {  // end > 0
         const int jj = min(j, end - 1);
-        next = find_half<DP, 4>(p.c, (jj < p.prefix ? prefix : table)[jj >> p.c.shift], h, j & off_mask, j < end);
+        return (jj < p.prefix ? prefix : table)[jj >> p.c.shift];
+    };
+    auto find_step = [&](int j, int id) {
+        next = find_half<DP, 4>(p.c, id, h, j & off_mask, j < end);
         next.bad = next.bad && j < end;
         bad_page |= next.bad;
     };
@@ -128,9 +135,9 @@ __device__ __forceinline__ void attend_classes(const AttendParams& p, int block,
             d.vu[t] = __builtin_amdgcn_raw_buffer_load_b32(next.block, 4 * g + (n * DT / kKvGroup << p.c.shift), next.vu + 16 * t, 0);
         }
     };
-    int j = j0 + TOKENS * wave;
+    int j = first;
     if (end > 0) {
-        find_step(j);
+        find_step(j, first_id);
         load_k();
         load_scales();
         load_v();
@@ -171,7 +178,7 @@ __device__ __forceinline__ void attend_classes(const AttendParams& p, int block,
 
     // The next step's bytes are loaded over this one's as those are used (see attend_part).
     for (; j < end; j += 4 * TOKENS) {
-        find_step(j + 4 * TOKENS);
+        find_step(j + 4 * TOKENS, page_of(j + 4 * TOKENS));
         float4v sc[C];
 #pragma unroll
         for (int t = 0; t < C; ++t) {
