@@ -13,6 +13,11 @@
 // turned.  Every value is read by the lane that writes it, so rows may be worked on in place.  Keys on their way into
 // the cache are laid down in the LDS and taken up again in the order of their columns, 8 a lane, which is what
 // quantize_row wants.
+//
+// What bounds it (us, heads of 128, as graph nodes): memory for many f32 rows, 8192 of 40 heads, 336 MB, 63, 5.3 TB/s, what a
+// copy reaches; as many fp16 rows take 48, their accesses being 8 bytes a lane; 4096 fp16 rows of 32 + 8 + 8 heads into the cache 24, 93 MB, with
+// vector instructions issuing half of that time.  One row is latency: 3.0, and 4.2 into the cache (lengths, page id, values, angles one
+// after the other).
 #include "qlin_kv_rows.hpp"
 #include "qlin_rope.hpp"
 

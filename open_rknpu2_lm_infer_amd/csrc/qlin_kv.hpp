@@ -1,4 +1,4 @@
-// Key/value cache: what the C entry points hand to the kernels of qlin_kv.hip and qlin_attend.hip.
+// Key/value cache: what the C entry points hand to the kernels of qlin_kv.hip and qlin_attend*.hip.
 #pragma once
 
 #include "qlin_internal.hpp"
