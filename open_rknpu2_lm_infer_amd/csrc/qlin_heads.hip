@@ -53,17 +53,16 @@ struct Blocks {
     bool has_a, has_b;
 };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* x) {
-    if constexpr (sizeof(T) == 2) {
-        const half4v h = *reinterpret_cast<const half4v*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)h[i];
-    } else {
-        const float4v f = *reinterpret_cast<const float4v*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = f[i];
-    }
+// A lane's eight values on their way, as they lie in memory: what converts them waits for them.
+template <typename T, bool VEC>
+struct Raw {
+    uint32_t w[VEC ? 2 * sizeof(T) : 8];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ float raw_at(const Raw<T, VEC>& r, int j) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[j]);
+    else if constexpr (VEC) return f32_of_f16_bits(r.w[j / 2] >> (16 * (j % 2)));
+    else return f32_of_f16_bits(r.w[j]);
 }
 
 // BITS 0: rows with positions.  8, 4: rows of a batch, into a cache of that width.  VEC: blocks of four columns are whole
@@ -71,6 +70,7 @@ __device__ __forceinline__ void load4(const T* p, float* x) {
 template <int DP, bool WIDE, typename T, bool VEC, int BITS>
 __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
     constexpr int LPH = DP / 8 * (WIDE ? 2 : 1), GROUPS = 256 / LPH;
+    constexpr int AHEAD = VEC ? 2 : 1;  // heads of a group that are on their way
     __shared__ __align__(16) float angles[4][DP];  // cosine and sine of the pairs of a row
     __shared__ __align__(16) float keys[BITS ? GROUPS : 1][BITS ? DP + 4 : 4];
     const int lane = threadIdx.x % LPH, group = threadIdx.x / LPH;
@@ -128,39 +128,50 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
     constexpr int PER_WAVE = 64 / LPH;
     const int heads = p.q_heads + (BITS ? 2 : 1) * p.k_heads;
     const int step = p.splits * (by_wave ? PER_WAVE : GROUPS);
-    auto load = [&](int h, float* x) {
-        const T* at = reinterpret_cast<const T*>(p.x) + row * p.ldx + (int64_t)h * p.dim;
+    // Without a branch, of a head and columns that are there: no load waits for another.
+    const int64_t from = (row0 + min(r, rows - 1)) * p.ldx;
+    auto load = [&](int h, Raw<T, VEC>& x) {
+        h = min(h, heads - 1);
+        const T* at = reinterpret_cast<const T*>(p.x) + from + (int64_t)h * p.dim;
         const bool value = BITS && h >= p.q_heads + p.k_heads;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.0f;
         if constexpr (VEC) {
+            constexpr int N = sizeof(T);  // words of a block
+            typedef uint32_t block_t __attribute__((ext_vector_type(N)));
             const Blocks b = value ? straight : qk;
-            if (b.has_a) load4<T>(at + b.a, x);
-            if (b.has_b) load4<T>(at + b.b, x + 4);
+            const block_t y = *reinterpret_cast<const block_t*>(at + (b.has_a ? b.a : 0));
+            const block_t z = *reinterpret_cast<const block_t*>(at + (b.has_b ? b.b : 0));
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x.w[i] = y[i];
+                x.w[N + i] = z[i];
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int c = value ? (8 * lane + j < p.dim ? 8 * lane + j : -1) : column(j);
-                const float y = ld1<T>(at, max(c, 0));  // loads without branches: none waits for another
-                x[j] = c >= 0 ? y : 0.0f;
+                const int c = value ? min(8 * lane + j, p.dim - 1) : max(column(j), 0);
+                if constexpr (sizeof(T) == 2) x.w[j] = reinterpret_cast<const uint16_t*>(at)[c];
+                else x.w[j] = reinterpret_cast<const uint32_t*>(at)[c];
             }
         }
     };
 
-    // the first head's values and the norms' factors do not wait for the angles
+    // the first heads' values and the norms' factors do not wait for the angles
     int h = by_wave ? split * PER_WAVE + group % PER_WAVE : split * GROUPS + group;
-    // (two heads are on their way, one in a cache's pass: 8192 f32 rows turned 65.9 -> 63.4 us, fp16 52 -> 48; the pass 31.7 and 32.3)
-    float x[8] = {}, next[8] = {};
-    if (works && h < heads) load(h, x);
-    if (BITS == 0 && works && h + step < heads) load(h + step, next);
+    Raw<T, VEC> raw[AHEAD + 1];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(h + i * step, raw[i]);
     float g[2][8] = {};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const float* gamma = k ? p.k_gamma : p.q_gamma;
         if (!gamma) continue;
         if constexpr (VEC) {
-            if (qk.has_a) load4<float>(gamma + qk.a, g[k]);
-            if (qk.has_b) load4<float>(gamma + qk.b, g[k] + 4);
+            const float4v y = *reinterpret_cast<const float4v*>(gamma + qk.a), z = *reinterpret_cast<const float4v*>(gamma + qk.b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                g[k][j] = y[j];
+                g[k][4 + j] = z[j];
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[k][j] = gamma[max(column(j), 0)];
@@ -197,11 +208,24 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
     }
 
     bool finite = true;
-    while (works && h < heads) {
-        float after[8] = {};
-        if (BITS == 0 && h + 2 * step < heads) load(h + 2 * step, after);
-        if (BITS != 0 && h + step < heads) load(h + step, next);
+    for (int done = 0; done < heads; done += step) {
+        // (past the end the last head again: a branch here makes every load be waited for at once, the prompt's pass 37 us and
+        // not 32; single columns, which are eight loads, have it)
+        if (VEC || done + AHEAD * step < heads) load(h + AHEAD * step, raw[AHEAD]);
         const bool query = h < p.q_heads, value = BITS && h >= p.q_heads + p.k_heads;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            bool there;
+            if constexpr (VEC) there = value ? (j < 4 ? straight.has_a : straight.has_b) : (j < 4 ? qk.has_a : qk.has_b);
+            else there = value ? 8 * lane + j < p.dim : column(j) >= 0;
+            x[j] = there ? raw_at<T, VEC>(raw[0], j) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) raw[i] = raw[i + 1];
+        const int head = h;
+        h += step;
+        if (!works || head >= heads) continue;
         if (!value) {
             if (query ? p.q_gamma != nullptr : p.k_gamma != nullptr) {
                 float sum = 0.0f;
@@ -230,7 +254,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
             }
         }
         if (BITS == 0 || query) {
-            const int64_t at = row * p.ldy + (int64_t)h * p.dim;
+            const int64_t at = row * p.ldy + (int64_t)head * p.dim;
             if constexpr (VEC) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -253,7 +277,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
                 }
             }
         } else if constexpr (BITS != 0) {
-            const KvBlock<DP, BITS> blk(p.c, max(page, 0), h - p.q_heads - (value ? p.k_heads : 0));
+            const KvBlock<DP, BITS> blk(p.c, max(page, 0), head - p.q_heads - (value ? p.k_heads : 0));
             const int d0 = 8 * lane;
             if (!value) {
                 // a head's lanes are of one wave, whose accesses to the LDS are done in their order
@@ -287,12 +311,6 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
                                        : quantize_row<DP, BITS, false>(blk, off, d0, x, p.rne, page >= 0);
                 finite &= fin || page < 0;
             }
-        }
-        h += step;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = next[j];
-            if constexpr (BITS == 0) next[j] = after[j];
         }
     }
     if constexpr (BITS != 0) {
