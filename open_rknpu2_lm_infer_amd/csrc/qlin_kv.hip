@@ -41,15 +41,56 @@ __device__ __forceinline__ Unit find_unit(const KvRows& p) {
     return r;
 }
 
+// The table's entry for a unit's token (of none: some entry, or a length where the table may have none).
+__device__ __forceinline__ int load_id(const KvRows& p, const Unit& u) {
+    const int pos = kv_clamp(u.s.len - u.s.rows + u.t, 0, max(p.b.max_len - 1, 0));
+    const int32_t* at = p.b.max_len > 0 ? p.b.table + (u.i * p.b.table_ld + (pos >> p.c.shift)) : p.b.length;
+    return *at;
+}
 // The slot of a unit's token: its page (-1: no such token, or a page outside the cache) and place in it.
-__device__ __forceinline__ int find_page(const KvRows& p, Unit& u, int* off) {
+__device__ __forceinline__ int find_page(const KvRows& p, Unit& u, int id, int* off) {
     const int pos = u.s.len - u.s.rows + u.t;
     *off = pos & ((1 << p.c.shift) - 1);
     if (!u.ok || pos < 0) return -1;
     bool bad = false;
-    const int page = kv_page(p.b.table[u.i * p.b.table_ld + (pos >> p.c.shift)], p.c.pages, &bad);
+    const int page = kv_page(id, p.c.pages, &bad);
     u.bad |= bad;
     return bad ? -1 : page;
+}
+
+// Columns d0 .. d0 + 7 of a row as they lie in memory (past the head: of its last columns).
+template <typename T, bool VEC>
+struct RawRow {
+    uint4 w[sizeof(T) / 2];  // VEC
+    uint32_t x[VEC ? 1 : 8];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_raw(RawRow<T, VEC>& r, const T* row, int d0, int dim) {
+    if constexpr (VEC) {
+        const uint4* at = reinterpret_cast<const uint4*>(row + (d0 < dim ? d0 : 0));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = at[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = min(d0 + i, dim - 1);
+            if constexpr (sizeof(T) == 2) r.x[i] = reinterpret_cast<const uint16_t*>(row)[d];
+            else r.x[i] = reinterpret_cast<const uint32_t*>(row)[d];
+        }
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ float raw_value(const RawRow<T, VEC>& r, int i) {
+    if constexpr (!VEC) {
+        if constexpr (sizeof(T) == 2) return f32_of_f16_bits(r.x[i]);
+        else return __uint_as_float(r.x[i]);
+    } else {
+        const uint4& w = r.w[sizeof(T) == 2 ? 0 : i / 4];
+        const int word = sizeof(T) == 2 ? i / 2 : i % 4;
+        const uint32_t y = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+        if constexpr (sizeof(T) == 2) return f32_of_f16_bits(y >> (16 * (i % 2)));
+        else return __uint_as_float(y);
+    }
 }
 
 template <int DP, int BITS, typename T, bool VEC>
@@ -57,17 +98,22 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows p) {
     constexpr int LPU = DP / 8;
     Unit u = find_unit<LPU>(p);
     const int d0 = (threadIdx.x % LPU) * 8;
-    // the rows' loads do not wait for the page's
-    float x[2][8] = {};
-    if (u.ok) {
-        const int64_t row = u.s.row0 + u.t, col = (int64_t)u.h * p.c.dim;
-        load8<T, VEC>(reinterpret_cast<const T*>(p.k) + row * p.ldk + col, d0, p.c.dim, x[0]);
-        load8<T, VEC>(reinterpret_cast<const T*>(p.v) + row * p.ldv + col, d0, p.c.dim, x[1]);
-    }
+    // the page's id, the key and the value are on their way together: no branch before any is there.  (One after the other
+    // 4096 tokens of 8 heads of 128 took 9.6 us in 4 bits.)
+    const int id = load_id(p, u);
+    const int64_t row = u.ok ? u.s.row0 + u.t : 0, col = (int64_t)u.h * p.c.dim;
+    RawRow<T, VEC> raw[2];
+    load_raw<T, VEC>(raw[0], reinterpret_cast<const T*>(p.k) + row * p.ldk + col, d0, p.c.dim);
+    load_raw<T, VEC>(raw[1], reinterpret_cast<const T*>(p.v) + row * p.ldv + col, d0, p.c.dim);
+    float x[2][8];
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[y][i] = u.ok && d0 + i < p.c.dim ? raw_value<T, VEC>(raw[y], i) : 0.0f;
     // the positions of a sequence whose row starts or length are out of bounds are clamped ones, other tokens' slots
     // on pages that other sequences may read: nothing of it is stored
     int off = 0;
-    const int page = u.bad ? -1 : find_page(p, u, &off);
+    const int page = u.bad ? -1 : find_page(p, u, id, &off);
     const KvBlock<DP, BITS> blk(p.c, max(page, 0), u.h);
     const bool k = quantize_row<DP, BITS, false>(blk, off, d0, x[0], p.rne, page >= 0);
     const bool v = quantize_row<DP, BITS, true>(blk, off, d0, x[1], p.rne, page >= 0);
@@ -82,7 +128,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRows p) {
     Unit u = find_unit<LPU>(p);
     const int d0 = (threadIdx.x % LPU) * 8;
     int off;
-    const int page = find_page(p, u, &off);
+    const int page = find_page(p, u, load_id(p, u), &off);
     if (u.bad) atomicOr(p.err + kErrBatch, 1u);
     if (!u.ok) return;
     const KvBlock<DP, BITS> blk(p.c, max(page, 0), u.h);
