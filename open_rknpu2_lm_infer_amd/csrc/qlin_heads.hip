@@ -14,10 +14,10 @@
 // the cache are laid down in the LDS and taken up again in the order of their columns, 8 a lane, which is what
 // quantize_row wants.
 //
-// What bounds it (us, heads of 128, as graph nodes): memory for many f32 rows, 8192 of 40 heads, 336 MB, 63, 5.3 TB/s, what a
-// copy reaches; as many fp16 rows take 48, their accesses being 8 bytes a lane; 4096 fp16 rows of 32 + 8 + 8 heads into the cache 24, 93 MB, with
-// vector instructions issuing half of that time.  One row is latency: 3.0, and 4.2 into the cache (lengths, page id, values, angles one
-// after the other).
+// What bounds it (us, heads of 128, as graph nodes): memory for many f32 rows, 8192 of 40 heads, 336 MB, 63.6, 5.3 TB/s, what a
+// copy reaches; as many fp16 rows take 38, 4.4 TB/s, their accesses being 8 bytes a lane; 4096 fp16 rows of 32 + 8 + 8 heads
+// into the cache 20.4, 93 MB, with vector instructions issuing half of that time.  One row is latency: 2.8, and 3.8 into the
+// cache (lengths, page id, values, angles one after the other).
 #include "qlin_kv_rows.hpp"
 #include "qlin_rope.hpp"
 

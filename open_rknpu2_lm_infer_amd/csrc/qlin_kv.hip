@@ -12,7 +12,7 @@
 // fp16 in, 8 bytes of codes out, and the absmax is a few lane exchanges.  One row a group and many
 // workgroups: two or four rows a group, their loads in flight together, are slower (both kernels over
 // 4096 tokens of 8 heads of 128: 15.9 us with one, 16.3 with two, 19.2 with four).  At that size the
-// append moves 25 MB in 9.3 us (2.7 TB/s) and the read as much in 6.7 (3.8 TB/s); one token takes them
+// append moves 25 MB in 8.8 us (2.9 TB/s) and the read as much in 6.7 (3.8 TB/s); one token takes them
 // 3.1 and 2.6 us, most of it the dependent loads of its place in the batch and in the page table.
 #include "qlin_kv_rows.hpp"
 

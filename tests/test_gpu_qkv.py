@@ -105,15 +105,28 @@ def test_pass_equals_its_parts(ws, bits, dtype, out_dtype, seqs, hq, hk, D, P, n
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("D,n,first,hq,hk", [(128, 128, 0, 6, 2), (64, 32, 16, 3, 3), (84, 42, 20, 2, 1), (250, 244, 3, 1, 1)])
-def test_many_rows(ws, bits, D, n, first, hq, hk):
-    """Four fp16 rows a workgroup: ragged sequences whose rows are no multiples of four, idle ones, rows without a token."""
+def test_many_rows(ws, bits, dtype, D, n, first, hq, hk):
+    """Four rows a workgroup: ragged sequences whose rows are no multiples of four, idle ones, rows without a token."""
     b = Batch([(700, 700), (650, 301), (0, 0), (5, 3), (2, 6), (1, 1)], hk, D, 32, bits, seed=D)
     rope, g = ql.Rope(D, n, first=first), (rand((D,), F32, 1, 0.3) + 1).to(DEV)
-    x = rand((b.rows, (hq + 2 * hk) * D), F16, seed=D).to(DEV)
-    want = apart(ws, b, rope, x, hq, hk, D, g, g, F16)
+    x = rand((b.rows, (hq + 2 * hk) * D), dtype, seed=D).to(DEV)
+    want = apart(ws, b, rope, x, hq, hk, D, g, g, dtype)
     got = ql.kv_append_qkv(ws, b.caches[0], b.batch, rope, x, hq, g, g)
     assert torch.equal(got, want)
+    one, two = b.contents(ws)
+    assert torch.equal(one, two) and one.any() and ws.status() == 0
+    b.close()
+
+
+@pytest.mark.parametrize("new", [1, 2, 3, 5])
+def test_many_sequences_of_few_rows(ws, new):
+    """More than 2048 rows, of which a sequence has fewer than a workgroup's four, or one more."""
+    b = Batch([(new + i % 3, new - (i % 5 == 4)) for i in range(2200)], 1, 64, 16, 8, seed=new)
+    rope, x = ql.Rope(64), rand((b.rows, 6 * 64), F16, seed=new).to(DEV)
+    want = apart(ws, b, rope, x, 4, 1, 64, None, None, F16)
+    assert torch.equal(ql.kv_append_qkv(ws, b.caches[0], b.batch, rope, x, 4), want)
     one, two = b.contents(ws)
     assert torch.equal(one, two) and one.any() and ws.status() == 0
     b.close()

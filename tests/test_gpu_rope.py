@@ -227,17 +227,30 @@ def test_any_number_of_rows(rows):
 
 
 @pytest.mark.parametrize("D,n,first,layout,heads", [s for s in SHAPES if s[4] <= 8])
-@pytest.mark.parametrize("rows", [2050, 2303])
-def test_many_rows_of_every_shape(D, n, first, layout, heads, rows):
-    """Four fp16 rows a workgroup, the last one with fewer: a row's result is that of the row alone."""
+@pytest.mark.parametrize("rows", [1025, 2050, 2303])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_many_rows_of_every_shape(D, n, first, layout, heads, rows, dtype):
+    """Four rows a workgroup, the last one with fewer: a row's result is that of the row alone."""
     rope = ql.Rope(D, n, first=first, layout=layout)
     g = (rand((D,), F32, seed=1) + 2.0).to(DEV)
-    x, pos = rand((rows, heads * D), F16, seed=rows).to(DEV), torch.arange(rows, dtype=torch.int32, device=DEV) * 3
-    out = torch.full((rows + 1, heads * D), 5.0, dtype=F16, device=DEV)
+    x, pos = rand((rows, heads * D), dtype, seed=rows).to(DEV), torch.arange(rows, dtype=torch.int32, device=DEV) * 3
+    out = torch.full((rows + 1, heads * D), 5.0, dtype=dtype, device=DEV)
     ql.norm_rope(rope, x, pos, heads // 2, g, None, out=out[:rows])
     assert (out[rows:] == 5).all()
-    for r in (0, 1, 2, 3, 4, 1030, rows - 3, rows - 2, rows - 1):
+    for r in (0, 1, 2, 3, 4, rows // 2, rows - 3, rows - 2, rows - 1):
         assert torch.equal(ql.norm_rope(rope, x[r:r + 1], pos[r:r + 1], heads // 2, g, None)[0], out[r]), r
+
+
+def test_f32_rows_past_what_the_caches_hold():
+    """40 million columns and a few: one row a workgroup again, results those of a few rows."""
+    D, heads, rows = 128, 40, 7830
+    rope, x = ql.Rope(D, layout="interleaved"), rand((rows, heads * D), F32, seed=3).to(DEV)
+    pos = torch.arange(rows, dtype=torch.int32, device=DEV)
+    out = torch.full((rows + 1, heads * D), 5.0, dtype=F32, device=DEV)
+    ql.rope(rope, x, pos, out=out[:rows])
+    assert (out[rows:] == 5).all()
+    for a in range(0, rows, 700):
+        assert torch.equal(ql.rope(rope, x[a:a + 700], pos[a:a + 700]), out[a:min(a + 700, rows)]), a
 
 
 def test_streams_and_captured_rows():
