@@ -404,8 +404,8 @@ int qlin_rope_run(const qlin_rope* rope, int32_t rows, int32_t heads, const void
  * columns of qkv rows do.
  *   n[d] = x[d] / sqrt(mean_d x^2 + eps) * gamma[d],  then as above
  * q_gamma, k_gamma: device f32 [head_dim], NULL: that kind is not normalized; eps > 0.  rope NULL: norms alone, positions
- * are not read.  Sums are f32: values up to 2^59.  A head with Inf is NaN where it had them and
- * in their pairs, one with NaN everywhere. */
+ * are not read.  Sums are f32: values up to 2^59.  A head with Inf is NaN where it had them and in their pairs, one with NaN
+ * everywhere. */
 int qlin_rope_run_norm(const qlin_rope* rope, int32_t rows, int32_t head_dim, int32_t q_heads, int32_t k_heads,
                        const float* q_gamma, const float* k_gamma, float eps, const void* X, int32_t x_dtype, int64_t ldx,
                        const int32_t* positions, void* Y, int32_t y_dtype, int64_t ldy, uint32_t flags, void* stream);

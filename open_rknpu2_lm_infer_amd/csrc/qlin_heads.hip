@@ -321,9 +321,7 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsParams p) {
 
 template <int DP, int BITS, typename T>
 hipError_t launch_typed(const HeadsParams& p, dim3 grid, hipStream_t st) {
-    // four columns side by side: pairs and the others are groups of eight, heads and rows of four
-    const bool vec = p.vec && p.dim % 4 == 0 && p.rope.rotary % 8 == 0 && p.rope.first % 4 == 0;
-    if (vec) heads_kernel<DP, false, T, true, BITS><<<grid, 256, 0, st>>>(p);
+    if (heads_vec(p)) heads_kernel<DP, false, T, true, BITS><<<grid, 256, 0, st>>>(p);
     else if (heads_wide(p)) heads_kernel<DP, true, T, false, BITS><<<grid, 256, 0, st>>>(p);
     else heads_kernel<DP, false, T, false, BITS><<<grid, 256, 0, st>>>(p);
     return hipGetLastError();
@@ -342,6 +340,7 @@ int lanes(const HeadsParams& p) { return p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 3
 
 }  // namespace
 
+bool heads_vec(const HeadsParams& p) { return p.vec && p.dim % 4 == 0 && p.rope.rotary % 8 == 0 && p.rope.first % 4 == 0; }
 bool heads_wide(const HeadsParams& p) {
     return (p.rope.rotary / 2 + 3) / 4 + (p.dim - p.rope.rotary + 7) / 8 > lanes(p);
 }

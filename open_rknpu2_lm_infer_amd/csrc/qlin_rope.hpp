@@ -39,6 +39,8 @@ struct HeadsParams {
     int rne;
     uint32_t* err;
 };
+// Four columns side by side: pairs and the others are groups of eight, heads and rows of four.
+bool heads_vec(const HeadsParams& p);
 // Lanes a head takes beside its columns' eighth: twice as many where the pairs and the other columns are no groups of eight.
 bool heads_wide(const HeadsParams& p);
 int heads_at_once(const HeadsParams& p);  // of a wave

@@ -102,7 +102,7 @@ void heads_common(HeadsParams* p, const qlin_rope* rope, int dim, int q_heads, i
 
 void heads_split(HeadsParams* p, int64_t seqs, int64_t rows, int heads) {
     const int64_t all = seqs * rows, wave = heads_at_once(*p);
-    const bool streamed = !p->x_f16 && p->vec && heads >= 4 * wave && all * heads * p->dim >= 40000000;
+    const bool streamed = !p->x_f16 && heads_vec(*p) && heads >= 4 * wave && all * heads * p->dim >= 40000000;
     p->block_rows = rows > 2 && all >= (heads <= 2 * wave ? 1024 : 2048) && !streamed ? 4 : 1;
     const int64_t once = wave * (4 / p->block_rows), passes = (heads + once - 1) / once;
     const int64_t blocks = (rows + p->block_rows - 1) / p->block_rows;

@@ -17,9 +17,9 @@ void heads_common(HeadsParams* p, const qlin_rope* rope, int dim, int q_heads, i
                   float eps, const void* x, bool x_f16, int64_t ldx, void* y, bool y_f16, int64_t ldy);
 // How rows are shared out: one a workgroup and, while they are few, its heads over several workgroups; of many rows four a
 // workgroup, one a wave, which then shares what is computed once among more heads, and has no wave without one.  Many are
-// 2048, and 1024 where a row's heads are work for two waves at most; f32 rows that fill a workgroup stay alone from 160 MB on, which
-// memory takes better in long pieces, and so do sequences of one or two rows, whose blocks of four would be empty.  With one and
-// four rows a workgroup, us as graph nodes:
+// 2048, and 1024 where a row's heads are work for two waves at most.  f32 rows in blocks of four columns that fill a
+// workgroup stay alone from 160 MB on, which memory takes better in long pieces, and so do sequences of one or two rows, whose
+// blocks of four would be empty.  With one and four rows a workgroup, us as graph nodes:
 //   heads of 128, f32, turned: 6 heads, 1024 rows 3.9 and 3.6, 8192 rows 16.1 and 11.2, 65536 rows 129 and 75; 16 heads, 1024 rows
 //     4.7 and 5.0, 8192 rows 22.2 and 21.6; 40 heads, 1024 rows 9.0 and 9.0, 2048 15.0 and 14.1, 6000 (122 MB) 42.1 and 42.5,
 //     8192 (168 MB) 63.4 and 68.5; 24 heads, 16384 rows (201 MB) 74 and 79
