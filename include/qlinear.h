@@ -540,16 +540,18 @@ int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, con
  * The arrays must not overlap each other.  The call takes the cache's page size and number of pages only; it is a
  * workspace call like the others, which allocates nothing and can be captured.
  * A length below 0 or above max_len (that slot is left alone), a free count outside 0 .. pages (taken as the nearer of
- * the two), more pages given back than there are, or an id outside the cache set QLIN_ERR_PARAM in the workspace's error
- * word; no such value is followed out of a buffer, but which pages belong to whom is then unspecified.  That no page is
- * in the list or the tables twice is the caller's business. */
+ * the two), more pages given back than there are, or an id outside the cache (of a page taken, given back, or of the slot's
+ * own that a row lies on, where slots are asked for) set QLIN_ERR_PARAM in the workspace's error
+ * word; no such value is followed out of a buffer, the slots of rows on such a page are -1, but which pages belong to
+ * whom is then unspecified.  That no page is in the list or the tables twice is the caller's business. */
 typedef struct qlin_kv_tables {
     int32_t seqs;          /* slots, 1..2^20; seqs * ceil(max_len / page_tokens) up to 2^30 */
     int32_t rows;          /* rows there is room for, 0..2^24 */
     int32_t max_new;       /* of one slot; what a later qlin_kv_batch is given */
     int32_t max_len;       /* up to 2^30 */
     int32_t prefix_tokens; /* a multiple of page_tokens, up to max_len: pages of these first tokens are shared, neither taken
-                            * nor given back, and their columns not written (slots of rows among them are read from them) */
+                            * nor given back, and their columns not written (slots of rows among them are made of what they
+                            * hold, whatever it is) */
     int32_t reserved;
     const int32_t* change; /* device [seqs] */
     int32_t* length;       /* device [seqs], in and out */
@@ -561,7 +563,7 @@ typedef struct qlin_kv_tables {
     /* out, each may be NULL.  Entries of rows behind the last are left as they are. */
     int32_t* row_seq;   /* device [rows]: whose row it is */
     int32_t* positions; /* device [rows]: its token's place */
-    int64_t* slots;     /* device [rows]: page * page_tokens + the place in it */
+    int64_t* slots;     /* device [rows]: page * page_tokens + the place in it; -1: the page is none of the cache's */
     int32_t* refused;   /* device [1]: slots that asked for rows and have none */
 } qlin_kv_tables;
 int qlin_kv_step(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_tables* tables, void* stream);

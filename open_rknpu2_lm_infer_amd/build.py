@@ -61,6 +61,8 @@ KV_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "kv_calls_test.cpp")
 KV_TEST_BIN = os.path.join(TEST_BUILD, "kv_calls_test")
 STEP_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "step_calls_test.cpp")
 STEP_TEST_BIN = os.path.join(TEST_BUILD, "step_calls_test")
+LIMITS_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "step_limits_test.cpp")
+LIMITS_TEST_BIN = os.path.join(TEST_BUILD, "step_limits_test")
 STATIC_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "static_link_test.c")
 STATIC_TEST_BIN = os.path.join(TEST_BUILD, "static_link_test")
 
@@ -129,7 +131,8 @@ def build_tests() -> str:
     subprocess.run(["g++", "-O2", "-std=c++17", "-ffp-contract=off", TEST_SRC, oracle_obj, "-o", TEST_BIN,
                     f"-L{HERE}", "-lqlinear", "-Wl,-rpath,$ORIGIN/../../../open_rknpu2_lm_infer_amd", "-lm"], check=True)
     # their own definitions of the HIP calls take the place of the runtime's
-    for src, exe in ((HOST_TEST_SRC, HOST_TEST_BIN), (KV_TEST_SRC, KV_TEST_BIN), (STEP_TEST_SRC, STEP_TEST_BIN)):
+    for src, exe in ((HOST_TEST_SRC, HOST_TEST_BIN), (KV_TEST_SRC, KV_TEST_BIN), (STEP_TEST_SRC, STEP_TEST_BIN),
+                     (LIMITS_TEST_SRC, LIMITS_TEST_BIN)):
         subprocess.run(["g++", "-O1", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", src, "-o", exe,
                         "-rdynamic", "-pthread", f"-L{HERE}", "-lqlinear",
                         "-Wl,-rpath,$ORIGIN/../../../open_rknpu2_lm_infer_amd"], check=True)

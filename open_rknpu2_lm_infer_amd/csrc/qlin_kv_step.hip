@@ -135,7 +135,9 @@ __device__ __forceinline__ void take(const StepParams& p, P need_start, P row_st
                     // a page taken in this step comes from the list, as its table entry is being written
                     const int column = pos >> p.shift, fresh = column - step_columns(old[u], p.shift, p.shared);
                     const int id = fresh >= 0 ? p.free_pages[avail - 1 - (need_start[i[u]] + fresh)] : p.table[i[u] * p.table_ld + column];
-                    p.slots[r] = ((int64_t)id << p.shift) + (pos & ((1 << p.shift) - 1));
+                    bool bad = false;
+                    p.slots[r] = step_place(id, pos, p.shift, p.shared, p.pages, &bad);
+                    if (bad) atomicOr(p.err + kErrBatch, 1u);
                 }
             }
         }

@@ -65,6 +65,16 @@ QLIN_HD int step_add(int a, int b) {
     return c > static_cast<uint32_t>(kStepMost) ? kStepMost : static_cast<int>(c);
 }
 
+// Slot of the token at place pos, whose page is `id`.  Of a page of the slot's own outside the cache (bad): -1, so that whoever
+// stores by slots is led nowhere.  A prefix's pages are not the tables' business: their ids are taken as they are.
+QLIN_HD int64_t step_place(int id, int pos, int shift, int shared, int pages, bool* bad) {
+    bool outside = false;
+    kv_page(id, pages, &outside);
+    outside = outside && (pos >> shift) >= shared;
+    *bad |= outside;
+    return outside ? -1 : static_cast<int64_t>(id) * (1 << shift) + (pos & ((1 << shift) - 1));
+}
+
 struct StepParams {
     int seqs, rows, max_new, max_len, shared, pages, shift;
     const int32_t* change;
