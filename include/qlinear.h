@@ -533,10 +533,13 @@ int qlin_kv_attention_prefix(qlin_workspace* ws, const qlin_kv_cache* cache, con
  *   change[i] > 0: so many more (the new rows), change[i] < 0: so many fewer, from the end (drafted tokens that were refused; at
  *   least length[i] ends the request), 0: an idle slot.
  * First pages that no token is left on go back on top of the free list, slot after slot, columns rising, and their table
- * entries become -1.  Then slots are served in their order, each wholly or not at all: one is refused where change[i] > max_new,
- * its length would pass max_len, the rows asked for by the slots up to it pass `rows`, or it needs pages and those needed by the slots up to it
- * (of those not refused before) pass the list.  A refused slot stays as it is and has no rows.  Pages come from the top of the
- * list (what they leave there stays), slot after slot, columns rising.
+ * entries become -1.  Then slots are served in their order, each wholly or not at all.  One is refused, in this order,
+ *   where it can never be served: change[i] above max_new or above `rows`, or a length that would pass max_len;
+ *   where the rows asked for by the slots up to it, but for those refused by the first rule, pass `rows`;
+ *   where it needs pages, and those needed by the slots up to it, but for those refused by the first two rules, pass the list.
+ * So a slot that is too large stands in nobody's way, but one that came too late for rows (pages) keeps all behind it from
+ * rows (pages).  A refused slot stays as it is and has no rows.  Pages come from the top of the list (what they leave there
+ * stays), slot after slot, columns rising.
  * The arrays must not overlap each other.  The call takes the cache's page size and number of pages only; it is a
  * workspace call like the others, which allocates nothing and can be captured.
  * A length below 0 or above max_len (that slot is left alone), a free count outside 0 .. pages (taken as the nearer of

@@ -2,10 +2,11 @@
 //
 // Slot i holds n_i tokens and asks for c_i more, or gives -c_i back.  Pages given back go on top of the free list in the
 // order of the slots, then those asked for are taken from its top in the same order:
-//   wanted   w_i = c_i where the slot's own limits allow it,  and sum_{j <= i} w_j <= rows
+//   wanted   w_i = c_i where c_i <= max_new, c_i <= rows and n_i + c_i <= max_len, else 0;  then sum_{j <= i} w_j <= rows
 //   granted  p_i = pages that n_i + w_i tokens take beyond those of n_i;  p_i = 0 or sum_{j <= i} p_j <= free pages
-// Every sum is a scan, so that nothing depends on the order in which threads run.  Sums grow along the slots: who is
-// refused for want of rows (or pages) is followed by none that is granted some, and what the granted take is the sum itself.
+// Every sum is a scan, so that nothing depends on the order in which threads run.  Sums grow along the slots: who comes too
+// late for rows (or pages) is followed by none that is granted rows (pages), and what the granted take is the sum itself.  Who is
+// too large to be served at all is in no sum.
 //
 // One workgroup scans, up to 4096 slots at a time, and gives pages back; whose the k-th row, page taken or page given back is,
 // is found by a binary search in the scanned starts, which lie in the LDS up to 4096 slots.  With few rows the same

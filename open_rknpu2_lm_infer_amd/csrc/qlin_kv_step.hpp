@@ -11,7 +11,7 @@ struct StepSlot {
     int len;   // tokens after what it gives back, before what it is given
     int from;  // first column that is given back (back > 0) or given
     int back;  // pages given back
-    int want;  // tokens asked for, as far as the slot's own limits allow them
+    int want;  // tokens asked for; 0 where they are more than can ever be granted
     int need;  // pages for them
     bool asks, shrinks, bad;
 };

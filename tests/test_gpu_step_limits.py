@@ -1,10 +1,12 @@
-"""The tables of a serving step at their limits on the GPU: ids of no page under rows, with few rows (one launch) and many (two)."""
+"""The tables of a serving step at their limits on the GPU: ids of no page under rows, with few rows (one launch) and many (two), and
+which slots are refused."""
 import numpy as np
 import pytest
 import torch
 
 from open_rknpu2_lm_infer_amd import _lib
 from open_rknpu2_lm_infer_amd import qlinear as ql
+from tests.test_step_limits import REFUSED
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +107,21 @@ def test_without_slots_held_pages_are_not_read(ws, seqs, rows):
     ql.kv_step(ws, s.step, i32([2] * 5 + [0] * (seqs - 5)))
     assert ws.status() == 0 and s.step.length[:5].tolist() == [20] * 5
     s.close()
+
+
+@pytest.mark.parametrize("slots", [3, 1500, 5000])
+@pytest.mark.parametrize("change,max_new,max_len,spare,rows", REFUSED)
+def test_who_is_refused(ws, slots, change, max_new, max_len, spare, rows):
+    """The same slots alone, and among idle ones; those of the list are the last, so that sums come from all before."""
+    n = len(change)
+    cols = max(-(-min(max_len, 1024) // 16), 2)
+    cache = ql.KVCache(1, 64, slots + 9, 16)
+    table = torch.full((slots, cols), -1, dtype=torch.int32, device=DEV)
+    table[:, 0] = torch.arange(slots, device=DEV)
+    free = torch.arange(slots, 2 * slots + 9, dtype=torch.int32, device=DEV)[:slots + 9].clamp(max=slots + 8)
+    step = ql.KVStep(cache, i32([10] * slots), table, free, i32([spare]), 8, max_new, min(max_len, 1024))
+    ql.kv_step(ws, step, i32([0] * (slots - n) + change))
+    assert step.length.tolist() == [10] * (slots - n) + [10 + r for r in rows]
+    assert step.row_start[slots - n:].tolist() == [sum(rows[:i]) for i in range(n + 1)]
+    assert step.refused.item() == sum(c > 0 and r == 0 for c, r in zip(change, rows)) and ws.status() == 0
+    cache.close()
