@@ -175,7 +175,6 @@ void count_workspace(int d) {
 
 namespace {
 
-constexpr int64_t kGemmPartInts = 16 << 20;  // split-K partial buffer: 64 MiB of int32
 constexpr int kGemmTileM = 128, kGemmTileK = 128;
 
 int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }

@@ -127,6 +127,9 @@ __device__ __forceinline__ float residual_add(const void* R, int64_t ldr, int r_
     return h + p;
 }
 
+// Scratch for partial results of every workspace that a caller makes: 64 MiB of int32.
+constexpr int64_t kGemmPartInts = 16 << 20;
+
 // What entry points outside qlin_capi.hip take from a workspace, and the begin of a run on it (the
 // stream is remembered for qlin_workspace_status).
 struct WorkspaceParts {

@@ -155,7 +155,6 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
 }  // namespace
 
 namespace qlin {
-int64_t kv_step_scratch(int seqs);  // ints
 hipError_t launch_kv_step(StepParams p, int32_t* scratch, hipStream_t stream);
 }  // namespace qlin
 
@@ -266,8 +265,8 @@ int qlin_kv_step(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_t
     int dev;
     if (hipGetDevice(&dev) != hipSuccess) return QLIN_ERR_NODEVICE;
     if (dev != cache->device) return QLIN_ERR_PARAM;
+    static_assert(kv_step_scratch(kKvMaxSeqs) <= kGemmPartInts, "every workspace has room for the most slots");
     const WorkspaceParts parts = workspace_begin(ws, (hipStream_t)stream);
-    if (kv_step_scratch(t->seqs) > parts.part_floats) return QLIN_ERR_UNSUPPORTED;
     StepParams p{};
     p.seqs = t->seqs;
     p.rows = t->rows;

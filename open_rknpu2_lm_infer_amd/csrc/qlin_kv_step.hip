@@ -28,7 +28,7 @@ namespace qlin {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-enum : int { kAvail = 0, kNeed = 1, kRows = 2, kTotals = 4 };
+enum : int { kAvail = 0, kNeed = 1, kRows = 2 };  // of the scratch's totals
 
 // Sum over the lanes up to this one of its wave, or of its row of 16.
 template <int CTRL, int ROWS>
@@ -304,11 +304,9 @@ constexpr int kOneRows = 8192;
 
 }  // namespace
 
-int64_t kv_step_scratch(int seqs) { return kTotals + 2 * ((int64_t)seqs + 1); }
-
 hipError_t launch_kv_step(StepParams p, int32_t* scratch, hipStream_t st) {
     p.totals = scratch;
-    p.need_start = scratch + kTotals;
+    p.need_start = scratch + kStepTotals;
     p.back_start = p.need_start + p.seqs + 1;
     const bool rows_too = p.seqs <= 4 * kThreads && p.rows <= kOneRows;
     if (p.seqs <= kThreads) kv_step_kernel<1, true><<<1, kThreads, 0, st>>>(p, rows_too);

@@ -75,6 +75,10 @@ QLIN_HD int64_t step_place(int id, int pos, int shift, int shared, int pages, bo
     return outside ? -1 : static_cast<int64_t>(id) * (1 << shift) + (pos & ((1 << shift) - 1));
 }
 
+// Scratch of a call, int32: totals, then [seqs + 1] first pages given and given back.
+constexpr int kStepTotals = 4;
+constexpr int64_t kv_step_scratch(int seqs) { return kStepTotals + 2 * (static_cast<int64_t>(seqs) + 1); }
+
 struct StepParams {
     int seqs, rows, max_new, max_len, shared, pages, shift;
     const int32_t* change;
@@ -88,8 +92,7 @@ struct StepParams {
     int32_t* positions;
     int64_t* slots;
     int32_t* refused;
-    // scratch: totals, then [seqs + 1] first pages given and given back
-    int32_t* totals;
+    int32_t* totals;  // scratch
     int32_t *need_start, *back_start;
     uint32_t* err;
 };

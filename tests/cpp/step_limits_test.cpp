@@ -1,6 +1,7 @@
 // The tables of a serving step at their limits, without a GPU.
 //
 //   step_limits_test places   slots of rows: pages inside and outside the cache, a prefix's among them
+//   step_limits_test room     the most slots find room in every workspace's scratch
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -36,11 +37,18 @@ void places() {
                             }
 }
 
+void room() {
+    expect(qlin::kv_step_scratch(1 << 20) * (int64_t)sizeof(int32_t) <= (int64_t)64 << 20, "64 MiB of scratch");
+    for (int seqs : {1, 2, 4096, 4097, 1 << 20})
+        expect(qlin::kv_step_scratch(seqs) >= qlin::kStepTotals + 2 * ((int64_t)seqs + 1), "totals and two arrays of starts");
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     const char* mode = argc > 1 ? argv[1] : "";
     if (!std::strcmp(mode, "places")) places();
+    else if (!std::strcmp(mode, "room")) room();
     else return 2;
     if (!g_bad) std::printf("PASS %s\n", mode);
     return g_bad != 0;
