@@ -133,12 +133,16 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     p.own_from = apart ? prefix : 0;
     // The kernel for few vectors runs best with one workgroup a CU (64 sequences of up to 4096 tokens: 73 us
     // uncut, 76 and 80 us in parts of 1024 and 512); parts of 2048 tokens bound what a single long sequence of a
-    // ragged batch costs (4 bits and very few vectors: of 4096 tokens; 64 sequences of 4096 tokens 64 us, of up to 4096 52,
-    // with parts of 1024 74 and 51, of 2048 74 and 52).  The one for many vectors has two workgroups a CU, of which the second hides the first's
+    // ragged batch costs.  In 4 bits with four classes of tokens they are of 4096 where the sequences make two workgroups a CU
+    // uncut: 64 sequences of 4096 tokens, and of up to 4096, us with parts of 4096 and of 2048, for 8 KV heads of 128 with 4 query
+    // heads each 55 / 62 and 44 / 44, of 64 columns 32 / 33 and 29 / 30; but with fewer workgroups, 4 KV heads, 34 / 31 and 33 / 29,
+    // 32 sequences of up to 8192, 8 KV heads, 48 / 43; and with two classes, 8 query heads, 67 / 62 and 52 / 48, 4 KV heads 44 / 34
+    // and 43 / 33.  The kernel for many vectors has two workgroups a CU, of which the second hides the first's
     // waits; the prefix, whose results are all joined, one.
     const bool few = attend_tile(p) < kAttendWide;
+    const int most = !few ? kKvMaxLen : attend_classes_of(p) == 4 && own_blocks >= 2 * wp.cu_count ? 4096 : 2048;
     int parts = 1;
-    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, few ? wp.cu_count : 2 * wp.cu_count, !few ? kKvMaxLen : attend_classes_of(p) > 1 ? 4096 : 2048,
+    cut(std::max(p.b.max_len - p.own_from, 0), own_blocks, few ? wp.cu_count : 2 * wp.cu_count, most,
         apart ? cap / 2 : cap, &parts, &p.chunk);
     if (apart) cut(prefix, prefix_blocks, wp.cu_count, kKvMaxLen, cap - parts, &p.prefix_parts, &p.prefix_chunk);
     p.parts = parts + p.prefix_parts;
