@@ -4,7 +4,8 @@
 //   y_l = a (n_l cos t - n_r sin t),  y_r = a (n_r cos t + n_l sin t)      t = position * w_i for pair i = (l, r)
 //
 // The angle is position * w_i quarter turns in 64 bits less the nearest whole number: what is left, at most half a
-// quarter turn, is exact to 2^-26 of a quarter in f32 however far the position is, and the whole number's last two
+// quarter turn, is rounded to f32, off by 2^-26 of a quarter, and by position * 2^-51 more for the roundings of w_i and of the
+// product in 64 bits, which pass the former from position 2^25 on (near 2^31 they are 2^-20).  The whole number's last two
 // bits say which of (c, s), (-s, c), (-c, -s), (s, -c) it is.  sin and cos of up to an eighth of a turn are their
 // series to the 9th and 10th power, the next terms being 2e-9 and 5e-10.  No table of positions is read: a workgroup
 // computes its rows' factors, one a thread, into the LDS, from where the lanes of all their heads have them.
