@@ -12,8 +12,9 @@ constexpr float kKvScaleMin = 0x1p-64f;
 constexpr int kKvMaxDim = 256;
 constexpr int kKvMinPage = 16, kKvMaxPage = 4096;  // tokens, powers of two
 constexpr int kKvMaxHeads = 1024;
-// Of the softmax's scale.  The kernels multiply it, log2 e and 2^9 by a row's power of two (f32 rows) before they
-// multiply by a key's scale: finite up to here for queries below 2^47, so that a key of zeros has the exponent 0 and not 0 * inf.
+// Of the softmax's scale.  The kernels multiply it, log2 e and what a code is worth (2^9 in 8 bits, 2^16 in 4) by a row's power of two,
+// 2^(e - 13) for a largest query of 2^e (f32 rows), and that by the products' sum (up to 2^20 in 8 bits, 2^17 in 4) before they
+// multiply by a key's scale: finite up to here for queries below 2^47 (2^43), and a key of zeros has the exponent 0 and not 0 * inf.
 constexpr float kKvMaxScale = 0x1p64f;
 constexpr int kKvMaxSeqs = 1 << 20, kKvMaxRows = 1 << 24, kKvMaxLen = 1 << 30;
 constexpr int64_t kKvMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads of one launch
