@@ -414,13 +414,13 @@ int qlin_rope_run_norm(const qlin_rope* rope, int32_t rows, int32_t head_dim, in
  * The reference keeps its keys and values in FP16 and runs attention as a unit of the native
  * library (src/npu/attention.rs); these calls keep a decoder layer on the device between its qkv
  * and o projections.  Keys and values are quantized like the activations, one scale per token and KV head:
- *   s = max(absmax_d |x[d]| * (1/127), 2^-64),  code[d] = clamp(round(x[d] * (1/s)), -127, 127)
+ *   s = max(absmax_d |x[d]| * (1/127), 2^-64),  code[d] = round(x[d] * (1/s)), which is within -127 .. 127
  * each operation one f32 rounding and 1/127 the nearest f32 (the scale is within one f32 step of the quotient).
  * A row with Inf or NaN gets the scale NaN (whoever reads it gets NaN) and sets
  * QLIN_ERR_NONFINITE in the workspace's error word.
  * In 4 bits every 32 columns g of a row have a unit of their own, a whole number, beside the row's scale:
  *   s = max(absmax_d |x[d]| * (1/1785), 2^-64),  u[g] = clamp(ceil(absmax_{d in g} |x[d]| * (1/s) * (1/7)), 1, 255)
- *   code[d] = clamp(round(x[d] * (1/(u[g] * s))), -7, 7),  read as code[d] * u[g] * s
+ *   code[d] = round(x[d] * (1/(u[g] * s))), which is within -7 .. 7;  read as code[d] * u[g] * s
  *
  * Tokens lie in pages of page_tokens; a sequence's tokens p .. p + page_tokens - 1 are the page named
  * by column p / page_tokens of its row of the page table.  Who owns which page is the caller's

@@ -1,7 +1,7 @@
 // Key/value cache in 8 and 4 bits: new rows quantized into their pages, and read back.
 //
 // A row is the key (or value) of one token and one head, dim values x; the rules are at quantize_row.  In 8 bits it is
-//   s = max(absmax |x| * (1/127), 2^-64),  code = clamp(round(x * (1/s)), -127, 127),
+//   s = max(absmax |x| * (1/127), 2^-64),  code = round(x * (1/s)),
 // every operation one f32 rounding, 1/127 the f32 nearest to it.  That is the rule of the per-token
 // activation quantization but for its division by 127, whose place a multiplication takes: the
 // scales agree to one step of f32.  A row that holds
