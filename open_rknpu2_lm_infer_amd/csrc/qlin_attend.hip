@@ -33,7 +33,7 @@ int tile_of(const AttendParams& p, int64_t vectors) {
 
 int attend_tile(const AttendParams& p) { return tile_of(p, (int64_t)p.b.max_new * p.group.d); }
 int attend_tile_prefix(const AttendParams& p) { return tile_of(p, (int64_t)p.b.rows * p.group.d); }
-// Two classes against none, fp16, us, 4 KV heads with 8 query heads each, pages of 32 (of 150 batches of 4 to 8 vectors on pages of 32
+// Two classes against none, fp16, us (one cache over and over), 4 KV heads with 8 query heads each, pages of 32 (of 150 batches of 4 to 8 vectors on pages of 32
 // and 64, fp16 and f32, two take longer in none):
 //                     64            128           256
 //   1 x 300           4.9 / 6.0     6.0 / 7.6     8.3 / 10.8

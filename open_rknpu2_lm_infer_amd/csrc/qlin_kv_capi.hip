@@ -134,7 +134,7 @@ int attention(qlin_workspace* ws, const qlin_kv_cache* cache, const qlin_kv_batc
     // The kernel for few vectors runs best with one workgroup a CU (64 sequences of up to 4096 tokens: 73 us
     // uncut, 76 and 80 us in parts of 1024 and 512); parts of 2048 tokens bound what a single long sequence of a
     // ragged batch costs.  In 4 bits with four classes of tokens they are of 4096 where the sequences make two workgroups a CU
-    // uncut: 64 sequences of 4096 tokens, and of up to 4096, us with parts of 4096 and of 2048, for 8 KV heads of 128 with 4 query
+    // uncut: 64 sequences of 4096 tokens, and of up to 4096, us (one cache over and over) with parts of 4096 and of 2048, for 8 KV heads of 128 with 4 query
     // heads each 55 / 62 and 44 / 44, of 64 columns 32 / 33 and 29 / 30; but with fewer workgroups, 4 KV heads, 34 / 31 and 33 / 29,
     // 32 sequences of up to 8192, 8 KV heads, 48 / 43; and with two classes, 8 query heads, 67 / 62 and 52 / 48, 4 KV heads 44 / 34
     // and 43 / 33.  The kernel for many vectors has two workgroups a CU, of which the second hides the first's
